@@ -1,0 +1,394 @@
+"""The calls of a recurrent layer with 8-bit projections that are timed, through the public entry points.
+
+Three operators: the gated linear recurrence (training, prompts and its one-token update), the RMS norm
+of the residual stream (training, tokens, and with an 8-bit output that the next projection reads) and
+the matrix product in 8-bit integers with a scale for each token and each output channel.  They are the
+parts of one layer: norm -> 8-bit projection -> recurrence -> 8-bit projection -> residual stream.
+
+A case is a dict: ``op`` and its sizes, the activations' ``dtype`` ("bf16", "f16" or "f32").  With ``own``
+false ``run`` computes the operators with elementary torch operations in 32 bits; with it true it calls
+the library.  ``exact`` computes the definitions in 64 bits.
+"""
+
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+SCALE = 8.0  # of the recurrence's log decay
+EPS = 1e-5
+
+
+def listed():
+    return [
+        # Training one layer on four sequences of 4096 tokens, 2560 channels: the recurrence's benchmark shape.
+        recurrence("recurrence_train", 4, 4096, 2560, "bf16", True),
+        # Float32 training on packed documents: a ragged length, resets, a state carried in.
+        recurrence("recurrence_train_packed_f32", 3, 1003, 1536, "f32", True, True, True),
+        # A long prompt of one user: one sequence of 32768 tokens, no gradients.
+        recurrence("recurrence_prompt_long", 1, 32768, 2560, "bf16", False),
+        # A user's next turn: a short ragged prompt with the state carried in.
+        recurrence("recurrence_prompt_short", 1, 333, 2048, "f16", False, True),
+        # One token of one sequence: the smallest call, all latency.
+        update("recurrence_token", 1, 2560, "bf16"),
+        # One token of a full serving batch.
+        update("recurrence_token_batch", 256, 5120, "bf16"),
+        # The norm ahead of a layer in training: 8192 tokens, bf16 stream.
+        norm("norm_train", 8192, 2560, "bf16", "bf16"),
+        # The same with the stream kept in float32, as mixed-precision training does; a ragged batch.
+        norm("norm_train_f32_stream", 1003, 5120, "bf16", "f32"),
+        # One token through the norm and the 8-bit input projection (2560 -> 2 x 5120): weights' bytes.
+        project("project_token", 1, 2560, 10240, "bf16"),
+        # A prompt of 1999 tokens through the same: the ordinary matrix product, ragged rows.
+        project("project_prompt", 1999, 2560, 10240, "bf16"),
+        # The output projection of a batch of prompts: activations quantised, then 8192 x 2560 x 5120.
+        linear("linear_prompts", 8192, 5120, 2560, "bf16", True, False),
+        # A serving batch of 77 tokens into an odd output width, with a bias: the middle of the range.
+        linear("linear_batch_odd", 77, 1000, 4099, "f16", False, True),
+    ]
+
+
+def recurrence(name, batch, length, channels, dtype, train, carried=False, reset=False):
+    return {"name": name, "op": "recurrence", "batch": batch, "length": length, "channels": channels, "dtype": dtype,
+            "train": train, "carried": carried, "reset": reset}
+
+
+def update(name, batch, channels, dtype):
+    return {"name": name, "op": "update", "batch": batch, "channels": channels, "dtype": dtype}
+
+
+def norm(name, rows, features, dtype, stream):
+    return {"name": name, "op": "norm", "rows": rows, "features": features, "dtype": dtype, "stream": stream}
+
+
+def project(name, rows, inner, outer, dtype):
+    return {"name": name, "op": "project", "rows": rows, "inner": inner, "outer": outer, "dtype": dtype}
+
+
+def linear(name, rows, inner, outer, dtype, quantise, bias):
+    return {"name": name, "op": "linear", "rows": rows, "inner": inner, "outer": outer, "dtype": dtype,
+            "quantise": quantise, "bias": bias}
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """A further case: widths of real layers and odd ones, tokens and lengths over their logarithms."""
+    op = rng.choice(["recurrence"] * 4 + ["update"] * 2 + ["norm"] * 2 + ["project"] * 2 + ["linear"] * 3)
+    dtype = rng.choice(["bf16", "bf16", "bf16", "f16", "f32"])
+    while True:
+        if op == "recurrence":
+            train = rng.random() < 0.6
+            channels = rng.choice([768, 1536, 2048, 2560, 4096, 5120, 1001])
+            case = recurrence("", rng.choice([1, 1, 2, 3, 4, 8]), _log_int(rng, 1, 32768), channels, dtype, train,
+                              rng.random() < 0.4, rng.random() < 0.3)
+            size = case["batch"] * case["length"] * channels * (2 if dtype == "f32" else 1) * (2 if train else 1)
+            most = 2 * 4 * 4096 * 2560
+        elif op == "update":
+            case = update("", _log_int(rng, 1, 256), rng.choice([768, 1536, 2560, 5120, 1001]), dtype)
+            size, most = case["batch"] * case["channels"], 256 * 5120
+        elif op == "norm":
+            case = norm("", _log_int(rng, 1, 8192), rng.choice([768, 1536, 2560, 4096, 5120, 1001]), dtype,
+                        rng.choice([dtype, dtype, "f32"]))
+            size, most = case["rows"] * case["features"] * (2 if dtype == "f32" else 1), 8192 * 2560
+        else:
+            inner = rng.choice([768, 1536, 2048, 2560, 4096, 5120, 1000, 777])
+            outer = rng.choice([768, 1536, 2560, 4096, 5120, 8192, 10240, 4099])
+            rows = _log_int(rng, 1, 8192)
+            if op == "project":  # with 16-bit activations, as layers that quantise theirs have them
+                case = project("", rows, inner, outer, dtype if dtype != "f32" else "bf16")
+            else:
+                case = linear("", rows, inner, outer, dtype, rng.random() < 0.5, rng.random() < 0.3)
+            size, most = rows * inner * outer, 8192 * 2560 * 5120
+        if size <= most:
+            del case["name"]
+            return case
+
+
+# ------------------------------------------------------------------------------------- inputs
+
+
+def _entry_points():
+    path = os.path.join(os.getcwd(), "metal-kernelops_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from metal_kernelops import cv
+    return cv
+
+
+class _Normal:
+    """Normal and uniform numbers on the GPU from one seed."""
+
+    def __init__(self, seed):
+        self.g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(self, *shape, dtype=torch.float32, std=1.0, mean=0.0):
+        return (torch.randn(shape, generator=self.g, device="cuda") * std + mean).to(dtype)
+
+    def uniform(self, lo, hi, *shape):
+        return torch.rand(shape, generator=self.g, device="cuda") * (hi - lo) + lo
+
+
+def _quantised(v):
+    """Rows of ``v`` in 8 bits and their scales: weights as they are laid out once when a model loads."""
+    amax = v.abs().amax(-1)
+    return torch.round(v * (127.0 / amax)[:, None]).to(torch.int8), amax / 127.0
+
+
+def prepare(case, seed):
+    rng, dt, op = _Normal(seed), DTYPES[case["dtype"]], case["op"]
+    s = {"case": case}
+    if op in ("recurrence", "update"):
+        D = case["channels"]
+        shape = (case["batch"], case["length"], D) if op == "recurrence" else (case["batch"], D)
+        s["x"], s["ig"], s["rg"] = (rng.normal(*shape, dtype=dt) for _ in range(3))
+        # at a full gate a channel keeps 0.9 to 0.999 of its state a step
+        rate = -torch.log(rng.uniform(0.9, 0.999, D)) / SCALE
+        s["decay"] = torch.log(torch.expm1(rate))
+        if op == "update":
+            s["state"] = rng.normal(case["batch"], D)
+            return s
+        s["h0"] = rng.normal(case["batch"], D) if case["carried"] else None
+        s["reset"] = rng.uniform(0.0, 1.0, *shape[:2]) < 1 / 256 if case["reset"] else None
+        if case["train"]:
+            s["dy"] = rng.normal(*shape, dtype=dt)
+            s["leaves"] = [t.requires_grad_(True) for t in (s["x"], s["ig"], s["rg"], s["decay"], s["h0"])
+                           if t is not None]
+        return s
+    if op == "norm":
+        R, F = case["rows"], case["features"]
+        st = DTYPES[case["stream"]]
+        s["x"], s["residual"] = rng.normal(R, F, dtype=dt), rng.normal(R, F, dtype=st, std=2.0)
+        s["weight"] = rng.normal(F, std=0.1, mean=1.0)
+        s["dout"], s["dstream"] = rng.normal(R, F, dtype=dt), rng.normal(R, F, dtype=st)
+        s["leaves"] = [t.requires_grad_(True) for t in (s["x"], s["residual"], s["weight"])]
+        return s
+    M, K, N = case["rows"], case["inner"], case["outer"]
+    s["wq"], s["ws"] = _quantised(rng.normal(N, K, std=K ** -0.5))
+    if op == "project":
+        s["x"], s["residual"] = rng.normal(M, K, dtype=dt), rng.normal(M, K, dtype=dt, std=2.0)
+        s["weight"] = rng.normal(K, std=0.1, mean=1.0)
+        return s
+    x = rng.normal(M, K, dtype=dt) * rng.uniform(0.25, 4.0, M, 1).to(dt)
+    s["bias"] = rng.normal(N) if case["bias"] else None
+    if case["quantise"]:
+        s["x"] = x
+    else:
+        s["q"], s["qs"] = _quantised(x.float())
+    return s
+
+
+# ------------------------------------------------------------------------------------- one pass
+
+
+def run(state):
+    return (_run_own if own else _run_plain)(state)
+
+
+def _run_own(s):
+    cv, case = _entry_points(), s["case"]
+    op = case["op"]
+    if op == "update":
+        y, new = cv.gated_recurrence_update(s["state"], s["x"], s["ig"], s["rg"], s["decay"], scale=SCALE)
+        return {"y": y, "state": new}
+    if op == "recurrence":
+        y, final = cv.gated_recurrence(s["x"], s["ig"], s["rg"], s["decay"], initial_state=s["h0"], reset=s["reset"],
+                                       scale=SCALE, return_final_state=True)
+        if not case["train"]:
+            return {"y": y, "final": final}
+        grads = torch.autograd.grad([y], s["leaves"], [s["dy"]])
+        return {"y": y.detach(), "final": final.detach(), "grads": list(grads)}
+    if op == "norm":
+        out, stream = cv.rmsnorm_residual(s["x"], s["weight"], s["residual"], eps=EPS)
+        grads = torch.autograd.grad([out, stream], s["leaves"], [s["dout"], s["dstream"]])
+        return {"out": out.detach(), "stream": stream.detach(), "grads": list(grads)}
+    dt = DTYPES[case["dtype"]]
+    if op == "project":
+        q, qs, stream = cv.rmsnorm_residual_int8(s["x"], s["weight"], s["residual"], eps=EPS)
+        return {"stream": stream, "out": cv.int8_linear(q, qs, s["wq"], s["ws"], out_dtype=dt)}
+    q, qs = cv.quantize_int8(s["x"]) if case["quantise"] else (s["q"], s["qs"])
+    return {"out": cv.int8_linear(q, qs, s["wq"], s["ws"], bias=s["bias"], out_dtype=dt)}
+
+
+@torch.no_grad()
+def _run_plain(s):
+    case = s["case"]
+    op, dt = case["op"], DTYPES[case["dtype"]]
+    if op == "update":
+        a, b = _gates(s["x"], s["ig"], s["rg"], s["decay"], None)[:2]
+        h = a * s["state"] + b
+        return {"y": h.to(dt), "state": h}
+    if op == "recurrence":
+        return _plain_recurrence(s, case["train"], dt)
+    if op == "norm":
+        x, res, w, dout = s["x"].float(), s["residual"].float(), s["weight"], s["dout"].float()
+        stream = (x + res).to(s["residual"].dtype)  # what the layer hands on is what it normalises
+        r = torch.rsqrt(stream.float().square().mean(-1, keepdim=True) + EPS)
+        xh = stream.float() * r
+        gw = dout * w
+        ds = r * (gw - xh * (gw * xh).mean(-1, keepdim=True)) + s["dstream"].float()
+        return {"out": (xh * w).to(dt), "stream": stream,
+                "grads": [ds.to(dt), ds.to(stream.dtype), (dout * xh).sum(0)]}
+    if op == "project":
+        stream = (s["x"].float() + s["residual"].float()).to(dt)
+        v = stream.float()
+        v = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + EPS) * s["weight"]
+        return {"stream": stream, "out": _plain_product(*_plain_quantise(v), s["wq"], s["ws"], None, dt)}
+    q, qs = _plain_quantise(s["x"].float()) if case["quantise"] else (s["q"].float(), s["qs"])
+    return {"out": _plain_product(q, qs, s["wq"], s["ws"], s["bias"], dt)}
+
+
+def _plain_quantise(v):
+    amax = v.abs().amax(-1)
+    return torch.round(v * (127.0 / amax)[:, None]), amax / 127.0
+
+
+def _plain_product(q, qs, wq, ws, bias, dt):
+    out = (q @ wq.float().t()) * qs[:, None] * ws
+    return (out if bias is None else out + bias).to(dt)
+
+
+def _gates(x, ig, rg, decay, reset):
+    """The recurrence's a and b of h = a h + b, and what its gradients read."""
+    sr, si = torch.sigmoid(rg.float()), torch.sigmoid(ig.float())
+    rate = SCALE * torch.where(decay > 20, decay, torch.log1p(torch.exp(decay)))
+    v = rate * sr
+    a, m = torch.exp(-v), torch.sqrt(-torch.expm1(-2 * v))
+    if reset is not None:
+        keep = ~reset[..., None]
+        a, m = a * keep, torch.where(keep, m, torch.ones_like(m))
+    return a, m * si * x.float(), m, si, sr, rate
+
+
+def _scan(a, b):
+    """h[t] = a[t] h[t-1] + b[t] along the second axis, the distance doubled at each step."""
+    step, length = 1, a.shape[1]
+    while step < length:
+        b = torch.cat([b[:, :step], b[:, step:] + a[:, step:] * b[:, :-step]], 1)
+        a = torch.cat([a[:, :step], a[:, step:] * a[:, :-step]], 1)
+        step *= 2
+    return b
+
+
+def _plain_recurrence(s, train, dt):
+    a, b, m, si, sr, rate = _gates(s["x"], s["ig"], s["rg"], s["decay"], s["reset"])
+    h0 = s["h0"] if s["h0"] is not None else torch.zeros_like(b[:, 0])
+    b[:, 0] += a[:, 0] * h0
+    h = _scan(a, b)
+    out = {"y": h.to(dt), "final": h[:, -1].clone()}
+    if not train:
+        return out
+    # g[t] = dy[t] + a[t+1] g[t+1]
+    later = torch.cat([a[:, 1:], torch.zeros_like(a[:, :1])], 1)
+    g = _scan(later.flip(1), s["dy"].float().flip(1)).flip(1)
+    before = torch.cat([h0[:, None], h[:, :-1]], 1)
+    x = s["x"].float()
+    # d/dv of a = exp(-v) and m = sqrt(1 - exp(-2 v)); a reset step has neither
+    dv = g * (si * x * a * a / m - a * before)
+    grads = [(g * m * si).to(dt), (g * m * x * si * (1 - si)).to(dt), (dv * rate * sr * (1 - sr)).to(dt),
+             (dv * sr).sum((0, 1)) * SCALE * torch.sigmoid(s["decay"])]
+    if s["h0"] is not None:
+        grads.append(a[:, 0] * g[:, 0])
+    out["grads"] = grads
+    return out
+
+
+# ------------------------------------------------------------------------------------- 64 bits
+
+
+@torch.no_grad()
+def exact(case, seed):
+    s = {k: v.double() if isinstance(v, torch.Tensor) and v.is_floating_point() else v
+         for k, v in prepare(case, seed).items()}
+    op = case["op"]
+    if op in ("recurrence", "update"):
+        return _exact_recurrence(s, case)
+    if op == "norm":
+        dt = DTYPES[case["stream"]]
+        stream = (s["x"] + s["residual"]).to(dt).double()
+        r = (stream.pow(2).mean(-1, keepdim=True) + EPS).pow(-0.5)
+        gw = s["dout"] * s["weight"]
+        ds = s["dstream"] + r * gw - r ** 3 * stream * (gw * stream).mean(-1, keepdim=True)
+        return {"out": stream * r * s["weight"], "stream": s["x"] + s["residual"],
+                "grads": [ds, ds, (s["dout"] * stream * r).sum(0)]}
+    out = {}
+    if op == "project":
+        out["stream"] = s["x"] + s["residual"]
+        x = out["stream"].to(DTYPES[case["dtype"]]).double()
+        x = s["weight"] * x / (x.pow(2).mean(-1, keepdim=True) + EPS).sqrt()
+    if op == "project" or case["quantise"]:
+        x = x if op == "project" else s["x"]
+        qs = x.abs().max(-1).values / 127
+        q = torch.round(x / qs[:, None])
+    else:
+        q, qs = s["q"].double(), s["qs"]
+    y = torch.mm(q * qs[:, None], (s["wq"].double() * s["ws"][:, None]).t())
+    out["out"] = y if s.get("bias") is None else y + s["bias"]
+    return out
+
+
+def _exact_recurrence(s, case):
+    x, i, r, decay = s["x"], s["ig"].sigmoid(), s["rg"].sigmoid(), s["decay"]
+    v = SCALE * torch.nn.functional.softplus(decay, threshold=50.0) * r
+    a, m = (-v).exp(), (-torch.expm1(-2 * v)).sqrt()
+    if case["op"] == "update":
+        h = a * s["state"] + m * i * x
+        return {"y": h, "state": h}
+    alive = torch.ones_like(x[..., :1]) if s["reset"] is None else (~s["reset"]).double()[..., None]
+    a, m = a * alive, m * alive + (1 - alive)
+    L = x.shape[1]
+    h0 = s["h0"] if s["h0"] is not None else torch.zeros_like(x[:, 0])
+    b, h, last = m * i * x, torch.empty_like(x), h0
+    for t in range(L):
+        last = torch.addcmul(b[:, t], a[:, t], last)
+        h[:, t] = last
+    out = {"y": h, "final": last}
+    if not case["train"]:
+        return out
+    g, last = torch.empty_like(x), torch.zeros_like(h0)
+    for t in reversed(range(L)):
+        last = s["dy"][:, t] + last
+        g[:, t] = last
+        last = last * a[:, t]
+    dv = g * (i * x * a * a / m)
+    dv[:, 0] -= g[:, 0] * a[:, 0] * h0
+    dv[:, 1:] -= g[:, 1:] * a[:, 1:] * h[:, :-1]
+    out["grads"] = [g * m * i, g * m * x * i * (1 - i), dv * v * (1 - r),
+                    (dv * r).sum((0, 1)) * SCALE * decay.sigmoid()] + ([last] if s["h0"] is not None else [])
+    return out
+
+
+# ------------------------------------------------------------------------------------- the work
+
+
+def work(case):
+    op = case["op"]
+    size = {"bf16": 2, "f16": 2, "f32": 4}
+    e = size[case["dtype"]]
+    if op == "update":  # x and two gates in, y out; the float32 state in and out
+        n = case["batch"] * case["channels"]
+        return {"bytes": n * (4 * e + 8) + 4 * case["channels"], "flops": 14 * n}
+    if op == "recurrence":  # x and two gates in, y out; in training dy in and three gradients out
+        n = case["batch"] * case["length"] * case["channels"]
+        ends = 4 * case["batch"] * case["channels"] * (1 + case["carried"] * (2 if case["train"] else 1))
+        more = case["batch"] * case["length"] if case["reset"] else 0
+        more += 4 * case["channels"] * (2 if case["train"] else 1)
+        return {"bytes": n * e * (8 if case["train"] else 4) + ends + more, "flops": n * (44 if case["train"] else 14)}
+    if op == "norm":  # x, the stream and both their gradients in; out, the stream and two gradients out
+        n, st = case["rows"] * case["features"], size[case["stream"]]
+        return {"bytes": n * (4 * e + 4 * st) + 8 * case["features"], "flops": 16 * n}
+    M, K, N = case["rows"], case["inner"], case["outer"]
+    product = {"bytes": N * K + 4 * N + M * N * e, "flops": 2 * M * N * K}
+    if op == "project":  # x and the stream in, the stream out
+        product["bytes"] += 3 * M * K * e + 4 * K
+        product["flops"] += 8 * M * K
+    else:
+        product["bytes"] += M * K * e if case["quantise"] else M * K + 4 * M
+        product["bytes"] += 4 * N if case["bias"] else 0
+    return product
