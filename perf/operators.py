@@ -137,8 +137,8 @@ class _Normal:
 
 def _quantised(v):
     """Rows of ``v`` in 8 bits and their scales: weights as they are laid out once when a model loads."""
-    amax = v.abs().amax(-1)
-    return torch.round(v * (127.0 / amax)[:, None]).to(torch.int8), amax / 127.0
+    q, scale = _plain_quantise(v)
+    return q.to(torch.int8), scale
 
 
 def prepare(case, seed):
@@ -246,7 +246,8 @@ def _run_plain(s):
 
 def _plain_quantise(v):
     amax = v.abs().amax(-1)
-    return torch.round(v * (127.0 / amax)[:, None]), amax / 127.0
+    most = torch.full_like(amax, 127.0)  # a quotient of two tensors is one division, rounded once
+    return torch.round(v * (most / amax)[:, None]), amax / most
 
 
 def _plain_product(q, qs, wq, ws, bias, dt):
