@@ -427,6 +427,147 @@ int mko_gated_norm_fwd(const mko_gated_norm_params* p, void* stream);
 size_t mko_gated_norm_bwd_workspace_size(const mko_gated_norm_params* p);
 int mko_gated_norm_bwd(const mko_gated_norm_params* p, void* stream);
 
+/* ======================================================================== */
+/* Gated linear recurrence                                                   */
+/* ======================================================================== */
+
+/* Per channel d, with rate = scale * softplus(decay[d]) and the logistic function s():
+ *   v[t] = rate * s(decay_gate[t]),  a[t] = exp(-v[t]),  m[t] = sqrt(1 - exp(-2 v[t]))
+ *   h[t] = a[t] h[t-1] + m[t] s(input_gate[t]) x[t],  h[-1] = initial or 0,  y = h
+ * At a step whose reset byte is non-zero the state before it is dropped: a = 0, m = 1.
+ * x, both gates, y, dy and the three gradients are (batch, length, channels) of `dtype`;
+ * x and the gates have unit channel stride and the given batch and step strides (in
+ * elements), the others are contiguous.  Everything else is float32. */
+typedef struct mko_recur_params {
+  const void* x;
+  const void* input_gate;
+  const void* decay_gate;
+  const float* decay;      /* (channels,) */
+  const float* initial;    /* (batch, channels) or NULL */
+  const uint8_t* reset;    /* (batch, length) bytes or NULL */
+  void* y;                 /* forward */
+  float* final_state;      /* forward: (batch, channels) or NULL */
+  float* states;           /* mko_recur_states_size() bytes: the state after every
+                              MKO_RECUR_CHUNK steps, which the backward reads; the forward
+                              always writes it */
+  const void* dy;          /* backward */
+  const float* dfinal;     /* backward: (batch, channels) or NULL */
+  void* dx;                /* backward */
+  void* dinput_gate;       /* backward */
+  void* ddecay_gate;       /* backward */
+  float* ddecay;           /* backward: (channels,), summed over batch and time, or NULL */
+  float* dinitial;         /* backward: (batch, channels) or NULL */
+  void* workspace;         /* mko_recur_{fwd,bwd}_workspace_size() bytes */
+  size_t workspace_bytes;
+  int64_t batch, length, channels;
+  int64_t x_stride_b, x_stride_t, ig_stride_b, ig_stride_t, rg_stride_b, rg_stride_t;
+  float scale;
+  int32_t dtype;
+} mko_recur_params;
+
+#define MKO_RECUR_CHUNK 128 /* steps between the saved states */
+
+size_t mko_sizeof_recur_params(void);
+size_t mko_recur_states_size(const mko_recur_params* p);
+size_t mko_recur_fwd_workspace_size(const mko_recur_params* p);
+int mko_recur_fwd(const mko_recur_params* p, void* stream);
+size_t mko_recur_bwd_workspace_size(const mko_recur_params* p);
+int mko_recur_bwd(const mko_recur_params* p, void* stream);
+
+/* One step of the same for (batch, channels) rows: new_state = h, y = h in `dtype`.  x and
+ * the gates have the given row strides; state and new_state (which may be the same array)
+ * are contiguous, of `state_dtype`; y is contiguous. */
+typedef struct mko_recur_update_params {
+  const void* x;
+  const void* input_gate;
+  const void* decay_gate;
+  const float* decay;
+  const void* state;
+  void* new_state;
+  void* y;
+  int64_t batch, channels, x_stride, ig_stride, rg_stride;
+  float scale;
+  int32_t dtype, state_dtype;
+} mko_recur_update_params;
+
+size_t mko_sizeof_recur_update_params(void);
+int mko_recur_update(const mko_recur_update_params* p, void* stream);
+
+/* ======================================================================== */
+/* RMS norm of the residual stream                                           */
+/* ======================================================================== */
+
+/* Per row:  stream = x + residual, rounded to stream_dtype (x itself without a residual)
+ *           r = 1 / sqrt(mean(stream^2) + eps),  v = stream * r * weight
+ *           out = v;  or, when q is given,  q = rint(v * 127 / amax), q_scale = amax / 127
+ * with amax the row's largest |v|.  The stored stream is what is normalised, so the
+ * backward, which reads it, sees the forward's own values.  A row of zeros has q_scale 0;
+ * one that holds an infinity or a NaN has an infinite or NaN q_scale.
+ * x and residual have unit feature stride and the given row strides; weight is contiguous. */
+typedef struct mko_resnorm_params {
+  const void* x;           /* (rows, features) of dtype; forward */
+  const void* residual;    /* (rows, features) of stream_dtype, or NULL; forward */
+  const void* weight;      /* (features,) of wdtype */
+  void* out;               /* forward: (rows, features) of dtype, or NULL with q */
+  int8_t* q;               /* forward: (rows, q_stride), columns features .. q_stride zeroed */
+  float* q_scale;          /* forward, with q: (rows,) */
+  void* stream;            /* the forward writes it when residual is given; the backward
+                              reads it (contiguous, of stream_dtype) */
+  float* rstd;             /* (rows,): the forward writes it when non-NULL, the backward reads it */
+  const void* dout;        /* backward: (rows, features) of dtype, contiguous */
+  const void* dstream;     /* backward: gradient that reaches stream, of stream_dtype, or NULL */
+  void* dx;                /* backward: (rows, features) of dtype */
+  void* dresidual;         /* backward: the same gradient in stream_dtype, or NULL */
+  float* dweight;          /* backward: (features,), summed over rows in a fixed order, or NULL */
+  void* workspace;         /* backward: mko_resnorm_bwd_workspace_size() bytes */
+  size_t workspace_bytes;
+  int64_t rows, features, x_stride, residual_stride, q_stride;
+  float eps;
+  int32_t dtype, stream_dtype, wdtype;
+} mko_resnorm_params;
+
+size_t mko_sizeof_resnorm_params(void);
+int mko_resnorm_fwd(const mko_resnorm_params* p, void* stream);
+size_t mko_resnorm_bwd_workspace_size(const mko_resnorm_params* p);
+int mko_resnorm_bwd(const mko_resnorm_params* p, void* stream);
+
+/* ======================================================================== */
+/* 8-bit integers: quantisation of rows and the matrix product               */
+/* ======================================================================== */
+
+/* Per row of x: amax = max |x|, q = rint(x * (127 / amax)), scale = amax / 127; the
+ * quotients and the product are rounded once each to float32.  Rows of zeros, infinities
+ * and NaN as in the norm above. */
+typedef struct mko_quantize_params {
+  const void* x;           /* (rows, features) of dtype, row stride x_stride */
+  int8_t* q;               /* (rows, q_stride), columns features .. q_stride zeroed */
+  float* scale;            /* (rows,) */
+  int64_t rows, features, x_stride, q_stride;
+  int32_t dtype;
+} mko_quantize_params;
+
+size_t mko_sizeof_quantize_params(void);
+int mko_quantize_int8(const mko_quantize_params* p, void* stream);
+
+/* out[m][n] = q_scale[m] * w_scale[n] * sum_k q[m][k] w[n][k] + bias[n], the sum exact in
+ * int32 (inner < 131072).  q and w have unit inner stride and any row strides. */
+typedef struct mko_int8_linear_params {
+  const int8_t* q;         /* (rows, inner) */
+  const float* q_scale;    /* (rows,) */
+  const int8_t* w;         /* (outer, inner) */
+  const float* w_scale;    /* (outer,) */
+  const float* bias;       /* (outer,) or NULL */
+  void* out;               /* (rows, outer) of dtype, contiguous */
+  void* workspace;         /* mko_int8_linear_workspace_size() bytes */
+  size_t workspace_bytes;
+  int64_t rows, inner, outer, q_stride, w_stride;
+  int32_t dtype;
+} mko_int8_linear_params;
+
+size_t mko_sizeof_int8_linear_params(void);
+size_t mko_int8_linear_workspace_size(const mko_int8_linear_params* p);
+int mko_int8_linear(const mko_int8_linear_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,45 @@
+// Symmetric 8-bit quantisation of a row: q = rint(v * (127 / amax)), scale = amax / 127.
+#pragma once
+
+#include "common.hpp"
+
+namespace mko {
+
+// |v| as the integer that orders like it.  Its maximum keeps what fmaxf drops: a NaN sorts above
+// an infinity and an infinity above every number.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Maximum over the wave, wave-uniform.  The four DPP steps of row16_sum.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xb1, 0xf, 0xf, false)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4e, 0xf, 0xf, false)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x141, 0xf, 0xf, false)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x140, 0xf, 0xf, false)));
+  const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+  const uint32_t c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+  return max(max(a, b), max(c, d));
+}
+
+struct RowScale {
+  float scale, inv;
+};
+
+// From the row's largest |v| (as abs_bits).  Both quotients are IEEE divisions.  A row below
+// 2^-100 has the scale 0 (its 127 / amax leaves the range); one that holds an infinity or a NaN
+// keeps that in its scale, so that every output of the row is not finite.
+__device__ __forceinline__ RowScale row_scale(uint32_t amax) {
+  const float a = __uint_as_float(amax);
+  RowScale r;
+  const bool tiny = a < 0x1p-100f;
+  r.scale = tiny ? 0.0f : a / 127.0f;
+  r.inv = tiny || amax >= 0x7f800000u ? 0.0f : 127.0f / a;
+  return r;
+}
+
+// rint(v * inv), to nearest even, as an integer in [-127, 127]; NaN gives 0.
+__device__ __forceinline__ int quantise(float v, float inv) {
+  const float q = rintf(fp32_value(v * inv));
+  return static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
+}
+
+}  // namespace mko

@@ -9,6 +9,7 @@ is passed as the launch stream.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -122,6 +123,65 @@ class GatedNormParams(ctypes.Structure):
     ]
 
 
+class RecurParams(ctypes.Structure):
+    """Mirror of ``mko_recur_params``."""
+
+    _fields_ = [
+        ("x", _vp), ("input_gate", _vp), ("decay_gate", _vp), ("decay", _vp), ("initial", _vp), ("reset", _vp),
+        ("y", _vp), ("final_state", _vp), ("states", _vp), ("dy", _vp), ("dfinal", _vp), ("dx", _vp),
+        ("dinput_gate", _vp), ("ddecay_gate", _vp), ("ddecay", _vp), ("dinitial", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("batch", ctypes.c_int64), ("length", ctypes.c_int64), ("channels", ctypes.c_int64),
+        ("x_stride_b", ctypes.c_int64), ("x_stride_t", ctypes.c_int64), ("ig_stride_b", ctypes.c_int64),
+        ("ig_stride_t", ctypes.c_int64), ("rg_stride_b", ctypes.c_int64), ("rg_stride_t", ctypes.c_int64),
+        ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
+    ]
+
+
+class RecurUpdateParams(ctypes.Structure):
+    """Mirror of ``mko_recur_update_params``."""
+
+    _fields_ = [
+        ("x", _vp), ("input_gate", _vp), ("decay_gate", _vp), ("decay", _vp), ("state", _vp), ("new_state", _vp),
+        ("y", _vp), ("batch", ctypes.c_int64), ("channels", ctypes.c_int64), ("x_stride", ctypes.c_int64),
+        ("ig_stride", ctypes.c_int64), ("rg_stride", ctypes.c_int64), ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32), ("state_dtype", ctypes.c_int32),
+    ]
+
+
+class ResnormParams(ctypes.Structure):
+    """Mirror of ``mko_resnorm_params``."""
+
+    _fields_ = [
+        ("x", _vp), ("residual", _vp), ("weight", _vp), ("out", _vp), ("q", _vp), ("q_scale", _vp), ("stream", _vp),
+        ("rstd", _vp), ("dout", _vp), ("dstream", _vp), ("dx", _vp), ("dresidual", _vp), ("dweight", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("rows", ctypes.c_int64), ("features", ctypes.c_int64), ("x_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64), ("q_stride", ctypes.c_int64), ("eps", ctypes.c_float),
+        ("dtype", ctypes.c_int32), ("stream_dtype", ctypes.c_int32), ("wdtype", ctypes.c_int32),
+    ]
+
+
+class QuantizeParams(ctypes.Structure):
+    """Mirror of ``mko_quantize_params``."""
+
+    _fields_ = [
+        ("x", _vp), ("q", _vp), ("scale", _vp), ("rows", ctypes.c_int64), ("features", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64), ("q_stride", ctypes.c_int64), ("dtype", ctypes.c_int32),
+    ]
+
+
+class Int8LinearParams(ctypes.Structure):
+    """Mirror of ``mko_int8_linear_params``."""
+
+    _fields_ = [
+        ("q", _vp), ("q_scale", _vp), ("w", _vp), ("w_scale", _vp), ("bias", _vp), ("out", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("rows", ctypes.c_int64), ("inner", ctypes.c_int64), ("outer", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64), ("dtype", ctypes.c_int32),
+    ]
+
+
 _SIGNATURES = {
     "mko_abi_version": ([], ctypes.c_int),
     "mko_last_error": ([], ctypes.c_char_p),
@@ -164,6 +224,23 @@ _SIGNATURES = {
                            ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
     "mko_state_update_bwd_workspace_size": ([ctypes.POINTER(StateUpdateParams)], ctypes.c_size_t),
     "mko_state_update_bwd": ([ctypes.POINTER(StateUpdateParams), _vp], ctypes.c_int),
+    "mko_sizeof_recur_params": ([], ctypes.c_size_t),
+    "mko_sizeof_recur_update_params": ([], ctypes.c_size_t),
+    "mko_sizeof_resnorm_params": ([], ctypes.c_size_t),
+    "mko_sizeof_quantize_params": ([], ctypes.c_size_t),
+    "mko_sizeof_int8_linear_params": ([], ctypes.c_size_t),
+    "mko_recur_states_size": ([ctypes.POINTER(RecurParams)], ctypes.c_size_t),
+    "mko_recur_fwd_workspace_size": ([ctypes.POINTER(RecurParams)], ctypes.c_size_t),
+    "mko_recur_fwd": ([ctypes.POINTER(RecurParams), _vp], ctypes.c_int),
+    "mko_recur_bwd_workspace_size": ([ctypes.POINTER(RecurParams)], ctypes.c_size_t),
+    "mko_recur_bwd": ([ctypes.POINTER(RecurParams), _vp], ctypes.c_int),
+    "mko_recur_update": ([ctypes.POINTER(RecurUpdateParams), _vp], ctypes.c_int),
+    "mko_resnorm_fwd": ([ctypes.POINTER(ResnormParams), _vp], ctypes.c_int),
+    "mko_resnorm_bwd_workspace_size": ([ctypes.POINTER(ResnormParams)], ctypes.c_size_t),
+    "mko_resnorm_bwd": ([ctypes.POINTER(ResnormParams), _vp], ctypes.c_int),
+    "mko_quantize_int8": ([ctypes.POINTER(QuantizeParams), _vp], ctypes.c_int),
+    "mko_int8_linear_workspace_size": ([ctypes.POINTER(Int8LinearParams)], ctypes.c_size_t),
+    "mko_int8_linear": ([ctypes.POINTER(Int8LinearParams), _vp], ctypes.c_int),
     "mko_state_update_bwd_static": ([ctypes.POINTER(StateUpdateParams), _vp], ctypes.c_int),
 }
 
@@ -201,7 +278,12 @@ def lib():
                            (PathParams, handle.mko_sizeof_path_params),
                            (Conv1dParams, handle.mko_sizeof_conv1d_params),
                            (Conv1dUpdateParams, handle.mko_sizeof_conv1d_update_params),
-                           (GatedNormParams, handle.mko_sizeof_gated_norm_params)):
+                           (GatedNormParams, handle.mko_sizeof_gated_norm_params),
+                           (RecurParams, handle.mko_sizeof_recur_params),
+                           (RecurUpdateParams, handle.mko_sizeof_recur_update_params),
+                           (ResnormParams, handle.mko_sizeof_resnorm_params),
+                           (QuantizeParams, handle.mko_sizeof_quantize_params),
+                           (Int8LinearParams, handle.mko_sizeof_int8_linear_params)):
             if ctypes.sizeof(struct) != fn():
                 raise RuntimeError(f"{struct.__name__} layout does not match libmko.so")
         _lib = handle
@@ -296,6 +378,31 @@ def plain_call(*tensors):
 
 def stream_of(device):
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device):
+    """A context in which ``device`` is the current one, which is where a kernel is launched
+    whatever stream it is given; free of cost where it is current already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def values(t):
+    """``t`` with its values in memory: a negated view or a tensor without memory (a ZeroTensor)
+    hands a kernel other numbers than it holds."""
+    if t.is_neg():
+        t = t.resolve_neg()
+    return torch.zeros(t.shape, dtype=t.dtype, device=t.device) if t._is_zerotensor() else t
+
+
+def rows(t):
+    """``t`` as a kernel reads it in rows: the last axis of unit stride, the others as they are."""
+    t = values(t)
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def workspace(nbytes, device):

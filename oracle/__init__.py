@@ -25,3 +25,4 @@ from .ssm import (  # noqa: F401
 )
 from .conv1d import causal_conv1d, causal_conv1d_update  # noqa: F401,E402
 from .norm import rmsnorm_gated, rmsnorm_gated_bwd  # noqa: F401,E402
+from . import recurrent_layer  # noqa: F401,E402
