@@ -85,6 +85,32 @@ __device__ __forceinline__ void put4(const mko_int8_linear_params& p, int64_t m,
   }
 }
 
+// `cols` of eight consecutive outputs from element `at` on.
+__device__ __forceinline__ void put8(const mko_int8_linear_params& p, int64_t at, int cols, const float (&v)[8]) {
+  struct __attribute__((packed)) Words4 {
+    mko_u32x4 w;
+  };
+  if (cols == 8) {
+    uint32_t w[8];
+    if (p.dtype == MKO_F32) {
+      pack_words<float, 8>(v, w);
+      Words4* o = reinterpret_cast<Words4*>(static_cast<float*>(p.out) + at);
+      o[0].w = mko_u32x4{w[0], w[1], w[2], w[3]};
+      o[1].w = mko_u32x4{w[4], w[5], w[6], w[7]};
+    } else {
+      if (p.dtype == MKO_BF16)
+        pack_words<bf16, 8>(v, w);
+      else
+        pack_words<_Float16, 8>(v, w);
+      reinterpret_cast<Words4*>(static_cast<uint16_t*>(p.out) + at)->w = mko_u32x4{w[0], w[1], w[2], w[3]};
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < cols) store_one(p.out, p.dtype, at + e, v[e]);
+  }
+}
+
 // ---------------------------------------------------------------- few tokens
 
 // A workgroup of W waves computes 16 channels of MT * 16 tokens; the waves take the inner axis in
@@ -148,8 +174,6 @@ __global__ void __launch_bounds__(W * 64) few(mko_int8_linear_params p) {
 
 // ---------------------------------------------------------------- tiles
 
-constexpr int kBk = 128;  // bytes of the inner axis in a stage
-
 __device__ v4i zero_chunk;  // what a lane past the inner axis' end loads instead
 
 template <int VM>
@@ -158,16 +182,22 @@ __device__ __forceinline__ void wait_and_meet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(VM) : "memory");
 }
 
-// A tile of BN channels by BM tokens, by WN x WM waves.  Each stage holds BK bytes of the tile's
-// rows in LDS, 16-byte chunk c of row r at position c ^ (r / 2 mod 8) of its row, which spreads
-// the operand reads of neighbouring rows over the banks.
-template <int BN, int BM, int WN, int WM, int STAGES, bool DIRECT>
+// A tile of BN channels by BM tokens, by WN x WM waves.  A stage holds BK bytes of each of the
+// tile's rows in LDS.  Rows start 256 / BK to a sweep of the banks, and 16-byte chunk c of row r
+// lies at position c ^ (r / (256 / BK)) of its row, which gives the 16 rows that a quarter wave
+// reads at one c 16 different groups of banks.
+template <int BN, int BM, int WN, int WM, int BK, int STAGES, bool DIRECT>
 __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, int tiles_n, int tiles_m) {
   constexpr int kWaves = WN * WM;
   constexpr int kTn = BN / WN / 32, kTm = BM / WM / 32;
-  constexpr int kLn = BN / 8 / kWaves, kLm = BM / 8 / kWaves;  // loads of 8 rows a wave makes for a stage
-  constexpr int kStage = (BN + BM) * kBk;
-  __shared__ __attribute__((aligned(128))) char lds[STAGES * kStage];
+  constexpr int kChunks = BK / 16, kRows = 64 / kChunks, kSweep = 256 / BK;
+  constexpr int kLn = BN / kRows / kWaves, kLm = BM / kRows / kWaves;  // loads of kRows rows a wave makes for a stage
+  constexpr int kLoads = kLn + kLm;
+  constexpr int kSteps = BK / 32;
+  constexpr int kStage = (BN + BM) * BK;
+  static_assert(kLn * kRows * kWaves == BN && kLm * kRows * kWaves == BM, "whole loads");
+  constexpr int kSums = kWaves * 32 * kTn * 32 * 4;  // the output's way through LDS
+  __shared__ __attribute__((aligned(256))) char lds[STAGES * kStage > kSums ? STAGES * kStage : kSums];
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wn = wave / WM, wm = wave % WM;
   const int inner = static_cast<int>(p.inner);
@@ -181,58 +211,59 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
 
   const int8_t* wbase = p.w + n0 * p.w_stride;
   const int8_t* qbase = p.q + m0 * p.q_stride;
-  uint32_t off[kLn + kLm];
-  int chunk_k[kLn + kLm];
-#pragma unroll
-  for (int j = 0; j < kLn + kLm; ++j) {
-    const bool wside = j < kLn;
-    const int row = ((wside ? j : j - kLn) * kWaves + wave) * 8 + (lane >> 3);
-    const int last = static_cast<int>(min(static_cast<int64_t>((wside ? BN : BM) - 1),
-                                          (wside ? p.outer - n0 : p.rows - m0) - 1));
-    chunk_k[j] = ((lane & 7) ^ ((row >> 1) & 7)) * 16;
-    off[j] = static_cast<uint32_t>(min(row, last)) * static_cast<uint32_t>(wside ? p.w_stride : p.q_stride) +
-             static_cast<uint32_t>(chunk_k[j]);
-  }
-  const int nk = (inner + kBk - 1) / kBk;
-
-  auto slot = [&](int st, int j) {  // where a wave's load j lands: 8 rows of a stage
-    return lds + st * kStage + (j < kLn ? 0 : BN * kBk) + ((j < kLn ? j : j - kLn) * kWaves + wave) * 8 * kBk;
+  // load j covers kRows rows of the weights (j < kLn) or the tokens; rows past the end repeat the last
+  auto tile_row = [&](int j) { return ((j < kLn ? j : j - kLn) * kWaves + wave) * kRows + lane / kChunks; };
+  auto source_row = [&](int j) {
+    const int64_t rows = j < kLn ? p.outer - n0 : p.rows - m0;
+    return static_cast<int>(min(static_cast<int64_t>(tile_row(j)), min(static_cast<int64_t>(j < kLn ? BN : BM), rows) - 1));
   };
+  auto source_k = [&](int j) { return ((lane % kChunks) ^ ((tile_row(j) / kSweep) % kChunks)) * 16; };
+  uint32_t off[DIRECT ? kLoads : 1];
+  if constexpr (DIRECT) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+      off[j] = static_cast<uint32_t>(source_row(j)) * static_cast<uint32_t>(j < kLn ? p.w_stride : p.q_stride) +
+               static_cast<uint32_t>(source_k(j));
+  }
+  const int nk = (inner + BK - 1) / BK;
+
+  auto slot = [&](int st, int j) {  // where a wave's load j lands in a stage
+    return lds + st * kStage + (j < kLn ? 0 : BN * BK) + ((j < kLn ? j : j - kLn) * kWaves + wave) * kRows * BK;
+  };
+  const int8_t* zeros = reinterpret_cast<const int8_t*>(&zero_chunk);
+  asm("" : "+s"(zeros));  // its address is formed here, not in the loop
+  auto load_to = [&](int st, int j, const int8_t* src) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
+                                     (__attribute__((address_space(3))) uint32_t*)slot(st, j), 16, 0, 0);
+  };
+  // The loads of stage kt; past the end those of a stage that is there, so that every step makes as
+  // many and the waits' counts hold.
   auto issue = [&](int st, int kt) {
-    const int k0 = kt * kBk;
-    const int8_t* wb = wbase + k0;
-    const int8_t* qb = qbase + k0;
-    if (k0 + kBk <= inner) {
+    if ((kt + 1) * BK <= inner || (kt >= nk && inner >= BK)) {
+      const int k0 = kt < nk ? kt * BK : 0;
+      const int8_t* wb = wbase + k0;
+      const int8_t* qb = qbase + k0;
 #pragma unroll
-      for (int j = 0; j < kLn + kLm; ++j)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) uint32_t*)((j < kLn ? wb : qb) + off[j]),
-            (__attribute__((address_space(3))) uint32_t*)slot(st, j), 16, 0, 0);
+      for (int j = 0; j < kLoads; ++j) load_to(st, j, (j < kLn ? wb : qb) + off[DIRECT ? j : 0]);
     } else {
+      const int k0 = (nk - 1) * BK;
 #pragma unroll
-      for (int j = 0; j < kLn + kLm; ++j) {
-        const int8_t* src = k0 + chunk_k[j] < inner ? (j < kLn ? wb : qb) + off[j]
-                                                    : reinterpret_cast<const int8_t*>(&zero_chunk);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
-                                         (__attribute__((address_space(3))) uint32_t*)slot(st, j), 16, 0, 0);
-      }
+      for (int j = 0; j < kLoads; ++j)
+        load_to(st, j, k0 + source_k(j) < inner ? (j < kLn ? wbase : qbase) + k0 + off[DIRECT ? j : 0] : zeros);
     }
   };
-  v4i held[DIRECT ? 1 : kLn + kLm];
+  v4i held[DIRECT ? 1 : kLoads];
   auto fetch = [&](int kt) {
 #pragma unroll
-    for (int j = 0; j < kLn + kLm; ++j) {
-      const bool wside = j < kLn;
-      const int row = ((wside ? j : j - kLn) * kWaves + wave) * 8 + (lane >> 3);
-      const int64_t last = min(static_cast<int64_t>((wside ? BN : BM) - 1), (wside ? p.outer - n0 : p.rows - m0) - 1);
-      const int64_t r = min(static_cast<int64_t>(row), last);
+    for (int j = 0; j < kLoads; ++j) {
+      const int64_t r = source_row(j);
       held[DIRECT ? 0 : j] =
-          load_chunk(wside ? wbase + r * p.w_stride : qbase + r * p.q_stride, kt * kBk + chunk_k[j], inner);
+          load_chunk(j < kLn ? wbase + r * p.w_stride : qbase + r * p.q_stride, kt * BK + source_k(j), inner);
     }
   };
   auto put_held = [&](int st) {
 #pragma unroll
-    for (int j = 0; j < kLn + kLm; ++j) *reinterpret_cast<v4i*>(slot(st, j) + lane * 16) = held[DIRECT ? 0 : j];
+    for (int j = 0; j < kLoads; ++j) *reinterpret_cast<v4i*>(slot(st, j) + lane * 16) = held[DIRECT ? 0 : j];
   };
 
   v16i acc[kTn][kTm];
@@ -243,37 +274,55 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
+  // operands of one step of 32 bytes: row lane % 32 of each 32-row block, chunk 2 s + lane / 32
   const int lr = lane & 31;
-  uint32_t at[4];
+  uint32_t at[kSteps];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) at[s] = lr * kBk + (((s * 2 + (lane >> 5)) ^ ((lr >> 1) & 7)) << 4);
-
-  auto compute = [&](int st) {
-    const char* wl = lds + st * kStage + wn * kTn * 32 * kBk;
-    const char* ql = lds + st * kStage + BN * kBk + wm * kTm * 32 * kBk;
+  for (int s = 0; s < kSteps; ++s) at[s] = lr * BK + (((s * 2 + (lane >> 5)) ^ ((lr / kSweep) % kChunks)) << 4);
+  v4i a[2][kTn], b[2][kTm];
+  auto read = [&](int st, int s, int to) {
+    const char* wl = lds + st * kStage + wn * kTn * 32 * BK + at[s];
+    const char* ql = lds + st * kStage + BN * BK + wm * kTm * 32 * BK + at[s];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      v4i a[kTn], b[kTm];
+    for (int i = 0; i < kTn; ++i) a[to][i] = *reinterpret_cast<const v4i*>(wl + i * 32 * BK);
 #pragma unroll
-      for (int i = 0; i < kTn; ++i) a[i] = *reinterpret_cast<const v4i*>(wl + i * 32 * kBk + at[s]);
-#pragma unroll
-      for (int j = 0; j < kTm; ++j) b[j] = *reinterpret_cast<const v4i*>(ql + j * 32 * kBk + at[s]);
-#pragma unroll
-      for (int i = 0; i < kTn; ++i)
-#pragma unroll
-        for (int j = 0; j < kTm; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
-    }
+    for (int j = 0; j < kTm; ++j) b[to][j] = *reinterpret_cast<const v4i*>(ql + j * 32 * BK);
   };
-
-  if constexpr (DIRECT) {
-    // STAGES - 1 stages are on their way while one is multiplied.  Every step issues the same
-    // number of loads, past the end into the stage that is free by then, so the wait's count holds.
+  auto multiply = [&](int from) {
 #pragma unroll
-    for (int st = 0; st < STAGES - 1; ++st) issue(st, min(st, nk - 1));  // nk > 0: direct_loads()
-    for (int kt = 0; kt < nk; ++kt) {
-      wait_and_meet<(STAGES - 2) * (kLn + kLm)>();
-      issue((kt + STAGES - 1) % STAGES, min(kt + STAGES - 1, nk - 1));
-      compute(kt % STAGES);
+    for (int i = 0; i < kTn; ++i)
+#pragma unroll
+      for (int j = 0; j < kTm; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[from][i], b[from][j], acc[i][j], 0, 0, 0);
+  };
+  static_assert(kSteps % 2 == 0, "the operand registers alternate");
+
+  // Operands are read one step ahead of their products, across the stages too: the last step's
+  // are in registers when the waves meet, after which the stage just read is free and takes the
+  // loads of the stage STAGES further on.
+  if constexpr (DIRECT) {
+#pragma unroll
+    for (int st = 0; st < STAGES; ++st) issue(st, st);
+    wait_and_meet<(STAGES - 1) * kLoads>();
+    read(0, 0, 0);
+    for (int kt = 0; kt < nk; kt += STAGES) {
+#pragma unroll
+      for (int st = 0; st < STAGES; ++st) {
+        if (st > 0 && kt + st >= nk) break;
+#pragma unroll
+        for (int s = 0; s + 1 < kSteps; ++s) {
+          read(st, s + 1, (s + 1) & 1);
+          __builtin_amdgcn_sched_barrier(0);
+          multiply(s & 1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        wait_and_meet<(STAGES - 2) * kLoads>();
+        issue(st, kt + st + STAGES);
+        read((st + 1) % STAGES, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply((kSteps - 1) & 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     // what was issued past the end must land before this workgroup's LDS is another's
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -283,24 +332,59 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
     for (int kt = 0; kt < nk; ++kt) {
       __syncthreads();
       if (kt + 1 < nk) fetch(kt + 1);
-      compute(kt & 1);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        read(kt & 1, s, 0);
+        multiply(0);
+      }
       if (kt + 1 < nk) put_held((kt + 1) & 1);
     }
   }
 
+  // The sums go through LDS, 32 tokens of the wave's channels at a time, so that a lane has 8
+  // consecutive channels of a token and the stores of a row are contiguous; the channels' scales
+  // are then the same for all of a lane's tokens.  Chunk c of 4 sums lies at c ^ (token / kPer).
+  constexpr int kWide = kTn * 32, kRowChunks = kTn * 8, kPer = kRowChunks >= 16 ? 1 : 16 / kRowChunks;
+  constexpr int kSpread = kRowChunks < 16 ? kRowChunks : 16;
+  wait_and_meet<0>();
+  char* mine = lds + wave * 32 * kWide * 4;
+  constexpr int kPerRow = kWide / 8;  // lanes to a token
+  const int nl = (lane % kPerRow) * 8;
+  const int64_t n = n0 + wn * kWide + nl;
+  const int cols = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(8), p.outer - n)));
+  float ws[8], bias[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    ws[e] = e < cols ? p.w_scale[n + e] : 0.0f;
+    bias[e] = p.bias && e < cols ? p.bias[n + e] : 0.0f;
+  }
 #pragma unroll
   for (int j = 0; j < kTm; ++j) {
-    const int64_t m = m0 + (wm * kTm + j) * 32 + lr;
-    if (m >= p.rows) continue;
-    const float qs = p.q_scale[m];
+    const int shift = (lr / kPer) % kSpread;
 #pragma unroll
     for (int i = 0; i < kTn; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int64_t n = n0 + (wn * kTn + i) * 32 + 8 * g + 4 * (lane >> 5);
-        const int s[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        if (n < p.outer) put4(p, m, n, s, qs);
+        const int c = i * 8 + 2 * g + (lane >> 5);
+        *reinterpret_cast<v4i*>(mine + lr * kWide * 4 + ((c ^ shift) << 4)) =
+            v4i{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
       }
+    wave_lds_sync();
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 64 / kPerRow) {
+      const int row = r0 + lane / kPerRow;
+      const int turn = (row / kPer) % kSpread;
+      const int64_t m = m0 + (wm * kTm + j) * 32 + row;
+      const v4i lo = *reinterpret_cast<const v4i*>(mine + row * kWide * 4 + (((nl / 4) ^ turn) << 4));
+      const v4i hi = *reinterpret_cast<const v4i*>(mine + row * kWide * 4 + (((nl / 4 + 1) ^ turn) << 4));
+      if (m >= p.rows || cols == 0) continue;
+      const float qs = p.q_scale[m];
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(e < 4 ? lo[e] : hi[e - 4]) * qs * ws[e] + bias[e];
+      put8(p, m * p.outer + n, cols, v);
+    }
+    wave_lds_sync();
   }
 }
 
@@ -316,18 +400,18 @@ void launch_few(const mko_int8_linear_params& p, hipStream_t s) {
     MKO_TIMED("int8_linear_few", s, few<MT, 8><<<grid, 8 * 64, 0, s>>>(p));
 }
 
-template <int BN, int BM, int WN, int WM, int STAGES>
+template <int BN, int BM, int WN, int WM, int BK, int STAGES>
 void launch_tile(const mko_int8_linear_params& p, bool direct, hipStream_t s) {
   const int64_t tn = cdiv(p.outer, BN), tm = cdiv(p.rows, BM);
   const unsigned grid = static_cast<unsigned>(tn * tm);
   if (direct)
     MKO_TIMED("int8_linear_tile", s,
-              tile<BN, BM, WN, WM, STAGES, true><<<grid, WN * WM * 64, 0, s>>>(
-                  p, static_cast<int>(tn), static_cast<int>(tm)));
+              tile<BN, BM, WN, WM, BK, STAGES, true><<<grid, WN * WM * 64, 0, s>>>(p, static_cast<int>(tn),
+                                                                                   static_cast<int>(tm)));
   else
     MKO_TIMED("int8_linear_tile", s,
-              tile<BN, BM, WN, WM, 2, false><<<grid, WN * WM * 64, 0, s>>>(p, static_cast<int>(tn),
-                                                                              static_cast<int>(tm)));
+              tile<BN, BM, WN, WM, BK, 2, false><<<grid, WN * WM * 64, 0, s>>>(p, static_cast<int>(tn),
+                                                                               static_cast<int>(tm)));
 }
 
 // Loads straight into LDS take aligned 16-byte chunks and 32-bit offsets within a tile.
@@ -343,9 +427,9 @@ void launch(const mko_int8_linear_params& p, hipStream_t s) {
   if (p.rows <= 32) return launch_few<2>(p, s);
   if (p.rows <= 64) return launch_few<4>(p, s);
   const bool direct = direct_loads(p);
-  if (cdiv(p.rows, 256) * cdiv(p.outer, 256) >= 200) return launch_tile<256, 256, 2, 4, 2>(p, direct, s);
-  if (cdiv(p.rows, 128) * cdiv(p.outer, 128) >= 200) return launch_tile<128, 128, 2, 2, 2>(p, direct, s);
-  launch_tile<64, 64, 2, 2, 3>(p, direct, s);
+  if (cdiv(p.rows, 256) * cdiv(p.outer, 256) >= 200) return launch_tile<256, 256, 2, 4, 128, 2>(p, direct, s);
+  if (cdiv(p.rows, 128) * cdiv(p.outer, 128) >= 200) return launch_tile<128, 128, 2, 2, 128, 2>(p, direct, s);
+  launch_tile<64, 64, 2, 2, 128, 3>(p, direct, s);
 }
 
 bool half_or_float(int32_t dtype) { return dtype == MKO_F32 || dtype == MKO_F16 || dtype == MKO_BF16; }
