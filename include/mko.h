@@ -465,7 +465,7 @@ typedef struct mko_recur_params {
   int32_t dtype;
 } mko_recur_params;
 
-#define MKO_RECUR_CHUNK 128 /* steps between the saved states */
+#define MKO_RECUR_CHUNK 64 /* steps between the saved states */
 
 size_t mko_sizeof_recur_params(void);
 size_t mko_recur_states_size(const mko_recur_params* p);

@@ -45,68 +45,485 @@ __device__ __forceinline__ Step gates(float ig, float rg, float rate, bool reset
   return s;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) forward(mko_recur_params p, int64_t chunks) {
-  const int64_t d = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t b = blockIdx.y;
-  if (d >= p.channels) return;
-  const float rate = p.scale * softplus(p.decay[d]);
-  float h = p.initial ? p.initial[b * p.channels + d] : 0.0f;
-  for (int64_t t = 0; t < p.length; ++t) {
-    const float x = to_f32(static_cast<const T*>(p.x)[b * p.x_stride_b + t * p.x_stride_t + d]);
-    const float ig = to_f32(static_cast<const T*>(p.input_gate)[b * p.ig_stride_b + t * p.ig_stride_t + d]);
-    const float rg = to_f32(static_cast<const T*>(p.decay_gate)[b * p.rg_stride_b + t * p.rg_stride_t + d]);
-    const bool reset = p.reset && p.reset[b * p.length + t];
-    const Step s = gates(ig, rg, rate, reset);
-    h = (reset ? 0.0f : s.a * h) + s.m * s.si * x;  // a dropped state is not read, be it NaN
-    static_cast<T*>(p.y)[(b * p.length + t) * p.channels + d] = from_f32<T>(h);
-    if ((t + 1) % kChunk == 0 || t + 1 == p.length) p.states[(b * chunks + t / kChunk) * p.channels + d] = h;
-  }
-  if (p.final_state) p.final_state[b * p.channels + d] = h;
+// ---------------------------------------------------------------- a channel strip's chunk
+//
+// A workgroup takes kChunk steps of a strip of 64 V channels: lane l the channels l V .. l V + V - 1,
+// wave w the steps w T .. w T + T - 1.  A run of steps maps the state before it to the state after
+// it by h -> P h + H, and runs compose; with resets, a run that drops the state has P = -0, which
+// no product of decays gives and which stays -0 when decays multiply it.
+
+constexpr uint32_t kDropped = 0x80000000u;
+
+template <bool RESET>
+__device__ __forceinline__ bool drops(float P) {
+  return RESET && __float_as_uint(P) == kDropped;
 }
 
-// hs: (batch, length, channels), the state before each step; part: (batch, channels).
-template <typename T>
-__global__ void __launch_bounds__(kThreads) backward(mko_recur_params p, float* hs, float* part) {
-  const int64_t d = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t b = blockIdx.y;
-  if (d >= p.channels) return;
-  const float rate = p.scale * softplus(p.decay[d]);
-  auto load = [&](int64_t t, float& x) {
-    x = to_f32(static_cast<const T*>(p.x)[b * p.x_stride_b + t * p.x_stride_t + d]);
-    const float ig = to_f32(static_cast<const T*>(p.input_gate)[b * p.ig_stride_b + t * p.ig_stride_t + d]);
-    const float rg = to_f32(static_cast<const T*>(p.decay_gate)[b * p.rg_stride_b + t * p.rg_stride_t + d]);
-    return gates(ig, rg, rate, p.reset && p.reset[b * p.length + t]);
+// P h + H; a dropped h is not read, be it NaN.
+template <bool RESET>
+__device__ __forceinline__ float apply(float P, float H, float h) {
+  const float r = P * h + H;
+  return drops<RESET>(P) ? H : r;
+}
+
+// The decays' product over a run and the run beside it.
+template <bool RESET>
+__device__ __forceinline__ float both(float P, float Q) {
+  const float r = P * Q;
+  return drops<RESET>(P) || drops<RESET>(Q) ? __uint_as_float(kDropped) : r;
+}
+
+template <typename T, int V>
+struct Raw {
+  uint32_t w[sizeof(T) == 4 ? V : 1];
+};
+
+// Where a lane's channels are: `d` the first, `full` if the whole strip is inside the tensor.
+struct Place {
+  int64_t d, channels;
+  bool full;
+  __device__ __forceinline__ int64_t at(int e) const { return min(d + e, channels - 1); }  // a channel to read
+  __device__ __forceinline__ bool has(int e) const { return d + e < channels; }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load(const T* row, const Place& c) {
+  struct __attribute__((packed)) Any {
+    Raw<T, V> r;
   };
-  float h = p.initial ? p.initial[b * p.channels + d] : 0.0f, x;
-  for (int64_t t = 0; t < p.length; ++t) {
-    hs[(b * p.length + t) * p.channels + d] = h;
-    const Step s = load(t, x);
-    h = (p.reset && p.reset[b * p.length + t] ? 0.0f : s.a * h) + s.m * s.si * x;
+  Raw<T, V> r;
+  if constexpr (sizeof(T) == 2 && V == 1) {
+    r.w[0] = __builtin_bit_cast(uint16_t, row[c.at(0)]);
+  } else {
+    if (c.full) {
+      r = reinterpret_cast<const Any*>(row + c.d)->r;
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) r.w[e] = __builtin_bit_cast(uint32_t, row[c.at(e)]);
+    } else {
+      r.w[0] = __builtin_bit_cast(uint16_t, row[c.at(0)]) |
+               static_cast<uint32_t>(__builtin_bit_cast(uint16_t, row[c.at(1)])) << 16;
+    }
   }
-  float g = p.dfinal ? p.dfinal[b * p.channels + d] : 0.0f, sum = 0.0f;
-  for (int64_t t = p.length - 1; t >= 0; --t) {
-    const int64_t i = (b * p.length + t) * p.channels + d;
-    const Step s = load(t, x);
-    g += to_f32(static_cast<const T*>(p.dy)[i]);
-    const bool reset = p.reset && p.reset[b * p.length + t];
-    const float dv = reset ? 0.0f : g * (s.si * x * s.a * s.a * s.rm - s.a * hs[i]);
-    static_cast<T*>(p.dx)[i] = from_f32<T>(g * s.m * s.si);
-    static_cast<T*>(p.dinput_gate)[i] = from_f32<T>(g * s.m * x * s.si * (1.0f - s.si));
-    static_cast<T*>(p.ddecay_gate)[i] = from_f32<T>(dv * s.v * (1.0f - s.sr));
-    sum += dv * s.sr;
-    g = reset ? 0.0f : g * s.a;
-  }
-  if (p.dinitial) p.dinitial[b * p.channels + d] = g;
-  part[b * p.channels + d] = sum;
+  return r;
 }
 
-__global__ void __launch_bounds__(kThreads) finish(mko_recur_params p, const float* part) {
-  const int64_t d = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (d >= p.channels) return;
-  float sum = 0.0f;
-  for (int64_t b = 0; b < p.batch; ++b) sum += part[b * p.channels + d];
-  p.ddecay[d] = sum * p.scale * softplus_grad(p.decay[d]);
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Raw<T, V>& r, float (&f)[V]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = __uint_as_float(r.w[e]);
+  } else if constexpr (V == 1) {
+    float hi;
+    unpack2<T>(r.w[0], f[0], hi);
+  } else {
+    unpack2<T>(r.w[0], f[0], f[1]);
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store(T* row, const Place& c, const float (&f)[V]) {
+  if (V == 2 && c.full) {
+    struct __attribute__((packed)) Any {
+      Raw<T, V> r;
+    } o;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) o.r.w[e] = __float_as_uint(f[e]);
+    } else {
+      o.r.w[0] = pack2<T>(f[0], f[V - 1]);
+    }
+    *reinterpret_cast<Any*>(row + c.d) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (c.has(e)) row[c.d + e] = from_f32<T>(f[e]);
+  }
+}
+
+// Bit t set if step t of the wave's run is a reset.
+template <bool RESET, int T>
+__device__ __forceinline__ uint32_t reset_bits(const mko_recur_params& p, int64_t b, int64_t t0, int lane) {
+  if (!RESET) return 0;
+  const int64_t t = t0 + lane;
+  const bool set = lane < T && t < p.length && p.reset[b * p.length + t];
+  return static_cast<uint32_t>(__ballot(set));
+}
+
+// ---------------------------------------------------------------- the chunks' order
+//
+// The chunks of a strip are joined in one pass over the data.  A workgroup publishes its chunk's map
+// as soon as it has it, looks for the nearest chunk before it whose end state is published, carries
+// that state through the maps between, and publishes its own end state.  Whichever end it finds, the
+// same products and sums are formed in the same order, so the bits do not depend on the timing.
+// Each published word says by itself whether it is there (cells start as all ones, which no value
+// is stored as), so relaxed atomics of the whole device are enough.  A workgroup takes its chunk from
+// a counter, chunk by chunk of all chains: whatever it waits for belongs to a workgroup that runs
+// already and that waits in turn only for earlier ones, so every wait ends.
+
+constexpr uint32_t kAbsent = 0xffffffffu;
+constexpr int kWindow = 8;            // chunks looked at in one round trip
+constexpr int kMostRounds = 1 << 22;  // seconds; a wait cut short shows as NaN
+
+// v with a NaN in the one form that is not kAbsent.
+__device__ __forceinline__ uint32_t publishable(float v) {
+  return v == v ? __float_as_uint(v) : 0x7fc00000u;
+}
+
+struct Chain {
+  uint64_t* maps;   // (batch, chunks, channels): P in the high word, H in the low
+  uint32_t* ends;   // (batch, chunks, channels): the value that leaves the chunk
+  uint32_t* ticket;
+};
+
+__device__ __forceinline__ void publish_map(uint64_t* cell, float P, float H) {
+  __hip_atomic_store(cell, static_cast<uint64_t>(publishable(P)) << 32 | __float_as_uint(H), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void publish_end(uint32_t* cell, float h) {
+  __hip_atomic_store(cell, publishable(h), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The value that enters a chunk at channel d, for a whole wave: `before` chunks of the chain lie
+// before it, the nearest in row `cell` of the cells, the others `step` rows apart; `start` enters
+// the first of them.
+template <bool RESET>
+__device__ __forceinline__ float enter(const Chain& ch, int64_t channels, int64_t d, int64_t cell, int64_t step,
+                                       int64_t before, float start) {
+  if (before == 0) return start;
+  for (int round = 0; round < kMostRounds; ++round) {
+    uint32_t end[kWindow];
+    uint64_t map[kWindow];
+#pragma unroll
+    for (int k = 0; k < kWindow; ++k) {
+      const int64_t at = (cell + (k < before ? k : 0) * step) * channels + d;
+      end[k] = __hip_atomic_load(ch.ends + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      map[k] = __hip_atomic_load(ch.maps + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    // the nearest end that is there, with every map nearer than it
+    int found = -1;
+    bool maps = true;
+    float h = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWindow; ++k) {
+      if (found < 0 && maps && k < before) {
+        if (__all(end[k] != kAbsent)) {
+          found = k;
+          h = __uint_as_float(end[k]);
+        }
+        maps = __all(static_cast<uint32_t>(map[k] >> 32) != kAbsent);
+      }
+    }
+    if (found >= 0) {
+#pragma unroll
+      for (int k = kWindow - 2; k >= 0; --k)
+        if (k < found)
+          h = apply<RESET>(__uint_as_float(static_cast<uint32_t>(map[k] >> 32)),
+                           __uint_as_float(static_cast<uint32_t>(map[k])), h);
+      return h;
+    }
+    __builtin_amdgcn_s_sleep(1);
+  }
+  return __uint_as_float(0x7fc00000u);
+}
+
+// A chunk's part in the chain, for a wave whose lanes have one channel each (channel d of the tensor,
+// i of the strip): joins its waves' maps, in the order of the chain, finds what enters the chunk and
+// leaves it in `entered`.  Returns what leaves the chunk.
+template <int NW, int V, bool RESET, bool BACK>
+__device__ __forceinline__ float join(const Chain& ch, const float (&P)[NW][64 * V], const float (&R)[NW][64 * V],
+                                      float* entered, int64_t channels, int64_t d, int i, int64_t cell, int64_t before,
+                                      int64_t after, float start) {
+  constexpr int kFirst = BACK ? NW - 1 : 0, kStep = BACK ? -1 : 1;
+  const int64_t at = min(d, channels - 1);
+  float Pc = P[kFirst][i], Rc = R[kFirst][i];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) {
+    const float Pw = P[kFirst + w * kStep][i];
+    Rc = apply<RESET>(Pw, R[kFirst + w * kStep][i], Rc);
+    Pc = both<RESET>(Pc, Pw);
+  }
+  if (before > 0 && after > 0 && d < channels) publish_map(ch.maps + cell * channels + d, Pc, Rc);
+  const float in = enter<RESET>(ch, channels, at, cell - kStep, -kStep, before, start);
+  entered[i] = in;
+  return apply<RESET>(Pc, Rc, in);
+}
+
+// Marks two runs of cells absent and starts the counter.
+__global__ void __launch_bounds__(kThreads) clear(uint4* a, int64_t na, uint4* b, int64_t nb, uint32_t* ticket) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const uint4 none = make_uint4(kAbsent, kAbsent, kAbsent, kAbsent);
+  if (i < na) a[i] = none;
+  if (i < nb) b[i] = none;
+  if (i == 0) *ticket = 0;
+}
+
+struct Geo {
+  int64_t chunks, strips, chains;  // chains = batch * strips
+};
+
+// This workgroup's place in the order: the chunk of a chain, counted from the end that is first.
+__device__ __forceinline__ int64_t take(const Geo& g, uint32_t* ticket, uint32_t* slot) {
+  if (g.chunks == 1) return blockIdx.x;
+  if (threadIdx.x == 0) *slot = atomicAdd(ticket, 1u);
+  __syncthreads();
+  return *slot;
+}
+
+// ---------------------------------------------------------------- forward
+
+template <typename T, int NW, int NT, int V, bool RESET>
+__global__ void __launch_bounds__(NW * 64) forward(mko_recur_params p, Geo g, Chain ch) {
+  static_assert(NW * NT == kChunk, "a workgroup takes a chunk");
+  __shared__ float runs[2][NW][64 * V], entered[64 * V];
+  __shared__ uint32_t slot;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t turn = take(g, ch.ticket, &slot);
+  const int64_t chunk = turn / g.chains, chain = turn - chunk * g.chains;
+  const int64_t b = chain / g.strips, strip = chain - b * g.strips;
+  const Place c{strip * 64 * V + lane * V, p.channels, (strip + 1) * 64 * V <= p.channels};
+  const int64_t t0 = chunk * kChunk + wave * NT;
+  const int steps = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(NT), p.length - t0)));
+
+  Raw<T, V> xr[NT], ir[NT], rr[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t at = min(t0 + t, p.length - 1);
+    xr[t] = load<T, V>(static_cast<const T*>(p.x) + b * p.x_stride_b + at * p.x_stride_t, c);
+    ir[t] = load<T, V>(static_cast<const T*>(p.input_gate) + b * p.ig_stride_b + at * p.ig_stride_t, c);
+    rr[t] = load<T, V>(static_cast<const T*>(p.decay_gate) + b * p.rg_stride_b + at * p.rg_stride_t, c);
+  }
+  const uint32_t cuts = reset_bits<RESET, NT>(p, b, t0, lane);
+  float rate[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) rate[e] = p.scale * softplus(p.decay[c.at(e)]);
+
+  // the run from a zero state: h = H[t], and P[t] of the state before it
+  float H[NT][V], P[NT][V];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float x[V], ig[V], rg[V];
+    unpack<T, V>(xr[t], x);
+    unpack<T, V>(ir[t], ig);
+    unpack<T, V>(rr[t], rg);
+    const bool cut = RESET && (cuts >> t & 1);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const Step s = gates(ig[e], rg[e], rate[e], cut);
+      const float u = s.m * s.si * x[e];
+      const float before = t ? P[t - 1][e] : 1.0f;
+      H[t][e] = (t == 0 || cut ? 0.0f : s.a * H[t - 1][e]) + u;
+      P[t][e] = cut ? __uint_as_float(kDropped) : s.a * before;
+      if (t >= steps) {  // past the end the state stays
+        H[t][e] = t ? H[t - 1][e] : 0.0f;
+        P[t][e] = before;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    runs[0][wave][lane * V + e] = P[NT - 1][e];
+    runs[1][wave][lane * V + e] = H[NT - 1][e];
+  }
+  __syncthreads();
+
+  if (wave < V) {
+    const int i = wave * 64 + lane;
+    const int64_t d = strip * 64 * V + i, cell = b * g.chunks + chunk;
+    const float start = p.initial ? p.initial[b * p.channels + min(d, p.channels - 1)] : 0.0f;
+    const float h = join<NW, V, RESET, false>(ch, runs[0], runs[1], entered, p.channels, d, i, cell, chunk,
+                                              g.chunks - 1 - chunk, start);
+    if (d < p.channels) {
+      publish_end(ch.ends + cell * p.channels + d, h);
+      if (p.final_state && chunk + 1 == g.chunks) p.final_state[b * p.channels + d] = h;
+    }
+  }
+  __syncthreads();
+
+  float in[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    in[e] = entered[lane * V + e];
+    for (int w = 0; w < wave; ++w) in[e] = apply<RESET>(runs[0][w][lane * V + e], runs[1][w][lane * V + e], in[e]);
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (t >= steps) break;
+    float y[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) y[e] = apply<RESET>(P[t][e], H[t][e], in[e]);
+    store<T, V>(static_cast<T*>(p.y) + (b * p.length + t0 + t) * p.channels, c, y);
+  }
+}
+
+// ---------------------------------------------------------------- backward
+//
+// The states are formed again from the one that enters the chunk, which the forward saved.  What
+// flows from a step to the one before it, a[t] g[t], has the forward's maps in the other direction,
+// and its chunks are joined from the last to the first.
+
+template <typename T, int NW, int NT, int V, bool RESET>
+__global__ void __launch_bounds__(NW * 64) backward(mko_recur_params p, Geo g, Chain ch, float* part) {
+  static_assert(NW * NT == kChunk, "a workgroup takes a chunk");
+  __shared__ float runs[3][NW][64 * V], entered[64 * V];
+  __shared__ uint32_t slot;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t turn = take(g, ch.ticket, &slot);
+  const int64_t behind = turn / g.chains, chain = turn - behind * g.chains;
+  const int64_t chunk = g.chunks - 1 - behind;
+  const int64_t b = chain / g.strips, strip = chain - b * g.strips;
+  const Place c{strip * 64 * V + lane * V, p.channels, (strip + 1) * 64 * V <= p.channels};
+  const int64_t t0 = chunk * kChunk + wave * NT;
+  const int steps = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(NT), p.length - t0)));
+
+  Raw<T, V> xr[NT], ir[NT], rr[NT], gr[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t at = min(t0 + t, p.length - 1);
+    xr[t] = load<T, V>(static_cast<const T*>(p.x) + b * p.x_stride_b + at * p.x_stride_t, c);
+    ir[t] = load<T, V>(static_cast<const T*>(p.input_gate) + b * p.ig_stride_b + at * p.ig_stride_t, c);
+    rr[t] = load<T, V>(static_cast<const T*>(p.decay_gate) + b * p.rg_stride_b + at * p.rg_stride_t, c);
+    gr[t] = load<T, V>(static_cast<const T*>(p.dy) + (b * p.length + at) * p.channels, c);
+  }
+  const uint32_t cuts = reset_bits<RESET, NT>(p, b, t0, lane);
+  float rate[V], first[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    rate[e] = p.scale * softplus(p.decay[c.at(e)]);
+    first[e] = chunk ? p.states[(b * g.chunks + chunk - 1) * p.channels + c.at(e)]
+                     : (p.initial ? p.initial[b * p.channels + c.at(e)] : 0.0f);
+  }
+
+  float si[NT][V], sr[NT][V], a[NT][V], m[NT][V];
+  float P[V], H[V], G[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    P[e] = 1.0f;
+    H[e] = G[e] = 0.0f;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float x[V], ig[V], rg[V];
+    unpack<T, V>(xr[t], x);
+    unpack<T, V>(ir[t], ig);
+    unpack<T, V>(rr[t], rg);
+    const bool cut = RESET && (cuts >> t & 1);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const Step s = gates(ig[e], rg[e], rate[e], cut);
+      si[t][e] = s.si;
+      sr[t][e] = s.sr;
+      a[t][e] = cut ? __uint_as_float(kDropped) : s.a;
+      m[t][e] = s.m;
+      if (t < steps) {
+        H[e] = (cut ? 0.0f : s.a * H[e]) + s.m * s.si * x[e];
+        P[e] = cut ? __uint_as_float(kDropped) : s.a * P[e];
+      }
+    }
+  }
+#pragma unroll
+  for (int t = NT - 1; t >= 0; --t) {
+    if (t >= steps) continue;
+    float dy[V];
+    unpack<T, V>(gr[t], dy);
+#pragma unroll
+    for (int e = 0; e < V; ++e) G[e] = apply<RESET>(a[t][e], 0.0f, G[e] + dy[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    runs[0][wave][lane * V + e] = P[e];
+    runs[1][wave][lane * V + e] = H[e];
+    runs[2][wave][lane * V + e] = G[e];
+  }
+  __syncthreads();
+
+  if (wave < V) {
+    const int i = wave * 64 + lane;
+    const int64_t d = strip * 64 * V + i, cell = b * g.chunks + chunk;
+    const float start = p.dfinal ? p.dfinal[b * p.channels + min(d, p.channels - 1)] : 0.0f;
+    const float out = join<NW, V, RESET, true>(ch, runs[0], runs[2], entered, p.channels, d, i, cell, behind, chunk, start);
+    if (d < p.channels) {
+      if (chunk > 0)
+        publish_end(ch.ends + cell * p.channels + d, out);
+      else if (p.dinitial)
+        p.dinitial[b * p.channels + d] = out;
+    }
+  }
+  __syncthreads();
+
+  float h[NT][V], flow[V], sum[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    float f = first[e];
+    for (int w = 0; w < wave; ++w) f = apply<RESET>(runs[0][w][lane * V + e], runs[1][w][lane * V + e], f);
+    h[0][e] = f;
+    flow[e] = entered[lane * V + e];
+    for (int w = NW - 1; w > wave; --w)
+      flow[e] = apply<RESET>(runs[0][w][lane * V + e], runs[2][w][lane * V + e], flow[e]);
+    sum[e] = 0.0f;
+  }
+#pragma unroll
+  for (int t = 0; t + 1 < NT; ++t) {
+    float x[V];
+    unpack<T, V>(xr[t], x);
+#pragma unroll
+    for (int e = 0; e < V; ++e) h[t + 1][e] = apply<RESET>(a[t][e], m[t][e] * si[t][e] * x[e], h[t][e]);
+  }
+#pragma unroll
+  for (int t = NT - 1; t >= 0; --t) {
+    if (t >= steps) continue;
+    float x[V], dy[V], dx[V], dig[V], drg[V];
+    unpack<T, V>(xr[t], x);
+    unpack<T, V>(gr[t], dy);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float gt = dy[e] + flow[e];
+      const float gm = gt * m[t][e];
+      const float u = si[t][e] * x[e];
+      const float rm = fast_rcp(fmaxf(m[t][e], 1e-19f));  // finite where v is 0
+      float dv = gt * a[t][e] * (u * a[t][e] * rm - h[t][e]);
+      if (drops<RESET>(a[t][e])) dv = 0.0f;
+      dx[e] = gm * si[t][e];
+      dig[e] = gm * u * (1.0f - si[t][e]);
+      drg[e] = dv * (rate[e] * sr[t][e]) * (1.0f - sr[t][e]);
+      sum[e] += dv * sr[t][e];
+      flow[e] = drops<RESET>(a[t][e]) ? 0.0f : a[t][e] * gt;
+    }
+    const int64_t row = (b * p.length + t0 + t) * p.channels;
+    store<T, V>(static_cast<T*>(p.dx) + row, c, dx);
+    store<T, V>(static_cast<T*>(p.dinput_gate) + row, c, dig);
+    store<T, V>(static_cast<T*>(p.ddecay_gate) + row, c, drg);
+  }
+  if (!p.ddecay) return;
+  __syncthreads();  // runs is read no more
+#pragma unroll
+  for (int e = 0; e < V; ++e) runs[0][wave][lane * V + e] = sum[e];
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float s = 0.0f;
+      for (int w = 0; w < NW; ++w) s += runs[0][w][lane * V + e];
+      if (c.has(e)) part[(b * g.chunks + chunk) * p.channels + c.d + e] = s;
+    }
+  }
+}
+
+// ddecay from the chunks' sums (rows of `part`), sixteen rows at a time.
+constexpr int kFinishWaves = 16;
+__global__ void __launch_bounds__(kFinishWaves * 64) finish(mko_recur_params p, const float* part, int64_t rows) {
+  __shared__ float sums[kFinishWaves][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t d = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  float s = 0.0f;
+  if (d < p.channels)
+    for (int64_t r = wave; r < rows; r += kFinishWaves) s += part[r * p.channels + d];
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave || d >= p.channels) return;
+  s = 0.0f;
+  for (int w = 0; w < kFinishWaves; ++w) s += sums[w][lane];
+  p.ddecay[d] = s * p.scale * softplus_grad(p.decay[d]);
 }
 
 template <typename T, typename S>
@@ -139,8 +556,9 @@ int check(const mko_recur_params* p, const char* what) {
     mko_set_error("%s: dtype must be float32, float16 or bfloat16", what);
     return MKO_EINVAL;
   }
-  if (p->batch > 65535) {
-    mko_set_error("%s: batch is at most 65535", what);
+  // a workgroup a chunk and strip, at most 512 threads each
+  if (p->batch > 65535 || cdiv(p->length, kChunk) * cdiv(p->channels, 64) >= (1 << 23) / (p->batch ? p->batch : 1)) {
+    mko_set_error("%s: batch is at most 65535, and batch * length * channels below 2^35", what);
     return MKO_EUNSUPPORTED;
   }
   return MKO_OK;
@@ -148,8 +566,49 @@ int check(const mko_recur_params* p, const char* what) {
 
 bool empty(const mko_recur_params* p) { return p->batch == 0 || p->length == 0 || p->channels == 0; }
 
-size_t hs_bytes(const mko_recur_params* p) {
-  return static_cast<size_t>(p->batch * p->length * p->channels) * sizeof(float);
+constexpr int kV = 2;  // channels a lane takes
+
+Geo geo(const mko_recur_params* p) {
+  Geo g;
+  g.chunks = cdiv(p->length, kChunk);
+  g.strips = cdiv(p->channels, 64 * kV);
+  g.chains = p->batch * g.strips;
+  return g;
+}
+
+int64_t cells(const mko_recur_params* p) { return p->batch * cdiv(p->length, kChunk) * p->channels; }
+int64_t aligned(int64_t n) { return cdiv(n, 16) * 16; }
+
+// maps, then the counter in 16 bytes of its own; the backward's ends and partial sums after them
+int64_t maps_bytes(const mko_recur_params* p) { return aligned(cells(p) * 8); }
+int64_t ends_bytes(const mko_recur_params* p) { return aligned(cells(p) * 4); }
+
+// Clears what the chunks publish.  A chain of one chunk publishes nothing.
+void clear_cells(const mko_recur_params* p, const Chain& ch, hipStream_t s) {
+  const int64_t maps = maps_bytes(p) / 16, ends = ends_bytes(p) / 16;
+  MKO_TIMED("recur_clear", s,
+            clear<<<static_cast<unsigned>(cdiv(maps, kThreads)), kThreads, 0, s>>>(
+                reinterpret_cast<uint4*>(ch.maps), maps, reinterpret_cast<uint4*>(ch.ends), ends, ch.ticket));
+}
+
+template <typename T>
+void launch_fwd(const mko_recur_params& p, const Geo& g, const Chain& ch, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(g.chunks * g.chains);
+  constexpr int kNw = kChunk / 16;
+  if (p.reset)
+    MKO_TIMED("recur_fwd", s, forward<T, kNw, 16, kV, true><<<grid, kNw * 64, 0, s>>>(p, g, ch));
+  else
+    MKO_TIMED("recur_fwd", s, forward<T, kNw, 16, kV, false><<<grid, kNw * 64, 0, s>>>(p, g, ch));
+}
+
+template <typename T>
+void launch_bwd(const mko_recur_params& p, const Geo& g, const Chain& ch, float* part, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(g.chunks * g.chains);
+  constexpr int kNw = kChunk / 8;
+  if (p.reset)
+    MKO_TIMED("recur_bwd", s, backward<T, kNw, 8, kV, true><<<grid, kNw * 64, 0, s>>>(p, g, ch, part));
+  else
+    MKO_TIMED("recur_bwd", s, backward<T, kNw, 8, kV, false><<<grid, kNw * 64, 0, s>>>(p, g, ch, part));
 }
 
 }  // namespace
@@ -163,12 +622,12 @@ extern "C" size_t mko_sizeof_recur_update_params(void) { return sizeof(mko_recur
 
 extern "C" size_t mko_recur_states_size(const mko_recur_params* p) {
   if (recur::check(p, "recur_states_size") != MKO_OK || recur::empty(p)) return 0;
-  return static_cast<size_t>(p->batch * recur::cdiv(p->length, recur::kChunk) * p->channels) * sizeof(float);
+  return static_cast<size_t>(recur::ends_bytes(p));
 }
 
 extern "C" size_t mko_recur_fwd_workspace_size(const mko_recur_params* p) {
-  (void)p;
-  return 0;
+  if (recur::check(p, "recur_fwd") != MKO_OK || recur::empty(p) || p->length <= recur::kChunk) return 0;
+  return static_cast<size_t>(recur::maps_bytes(p) + 16);
 }
 
 extern "C" int mko_recur_fwd(const mko_recur_params* p, void* stream) {
@@ -179,21 +638,34 @@ extern "C" int mko_recur_fwd(const mko_recur_params* p, void* stream) {
     mko_set_error("recur_fwd: x, both gates, decay, y and states are required");
     return MKO_EINVAL;
   }
+  const size_t need = mko_recur_fwd_workspace_size(p);
+  if (need && (!p->workspace || p->workspace_bytes < need)) {
+    mko_set_error("recur_fwd: workspace of %zu bytes needed, %zu given", need, p->workspace_bytes);
+    return MKO_EWORKSPACE;
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t chunks = recur::cdiv(p->length, recur::kChunk);
-  const dim3 grid(static_cast<unsigned>(recur::cdiv(p->channels, recur::kThreads)), static_cast<unsigned>(p->batch));
+  const recur::Geo g = recur::geo(p);
+  recur::Chain ch{};
+  ch.ends = reinterpret_cast<uint32_t*>(p->states);
+  if (g.chunks > 1) {
+    ch.maps = static_cast<uint64_t*>(p->workspace);
+    ch.ticket = reinterpret_cast<uint32_t*>(static_cast<char*>(p->workspace) + recur::maps_bytes(p));
+    recur::clear_cells(p, ch, s);
+  }
   if (p->dtype == MKO_F32)
-    MKO_TIMED("recur_fwd", s, recur::forward<float><<<grid, recur::kThreads, 0, s>>>(*p, chunks));
+    recur::launch_fwd<float>(*p, g, ch, s);
   else if (p->dtype == MKO_BF16)
-    MKO_TIMED("recur_fwd", s, recur::forward<bf16><<<grid, recur::kThreads, 0, s>>>(*p, chunks));
+    recur::launch_fwd<bf16>(*p, g, ch, s);
   else
-    MKO_TIMED("recur_fwd", s, recur::forward<_Float16><<<grid, recur::kThreads, 0, s>>>(*p, chunks));
+    recur::launch_fwd<_Float16>(*p, g, ch, s);
   return mko_check_launch("recur_fwd");
 }
 
 extern "C" size_t mko_recur_bwd_workspace_size(const mko_recur_params* p) {
   if (recur::check(p, "recur_bwd") != MKO_OK || recur::empty(p)) return 0;
-  return recur::hs_bytes(p) + static_cast<size_t>(p->batch * p->channels) * sizeof(float);
+  const int64_t part = p->ddecay ? recur::ends_bytes(p) : 0;
+  const int64_t chain = p->length > recur::kChunk ? recur::maps_bytes(p) + recur::ends_bytes(p) + 16 : 0;
+  return static_cast<size_t>(part + chain);
 }
 
 extern "C" int mko_recur_bwd(const mko_recur_params* p, void* stream) {
@@ -206,22 +678,32 @@ extern "C" int mko_recur_bwd(const mko_recur_params* p, void* stream) {
     return MKO_EINVAL;
   }
   const size_t need = mko_recur_bwd_workspace_size(p);
-  if (!p->workspace || p->workspace_bytes < need) {
+  if (need && (!p->workspace || p->workspace_bytes < need)) {
     mko_set_error("recur_bwd: workspace of %zu bytes needed, %zu given", need, p->workspace_bytes);
     return MKO_EWORKSPACE;
   }
-  float* hs = static_cast<float*>(p->workspace);
-  float* part = hs + p->batch * p->length * p->channels;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(recur::cdiv(p->channels, recur::kThreads)), static_cast<unsigned>(p->batch));
+  const recur::Geo g = recur::geo(p);
+  char* ws = static_cast<char*>(p->workspace);
+  float* part = reinterpret_cast<float*>(ws);
+  if (p->ddecay) ws += recur::ends_bytes(p);
+  recur::Chain ch{};
+  if (g.chunks > 1) {
+    ch.maps = reinterpret_cast<uint64_t*>(ws);
+    ch.ends = reinterpret_cast<uint32_t*>(ws + recur::maps_bytes(p));
+    ch.ticket = reinterpret_cast<uint32_t*>(ws + recur::maps_bytes(p) + recur::ends_bytes(p));
+    recur::clear_cells(p, ch, s);
+  }
   if (p->dtype == MKO_F32)
-    MKO_TIMED("recur_bwd", s, recur::backward<float><<<grid, recur::kThreads, 0, s>>>(*p, hs, part));
+    recur::launch_bwd<float>(*p, g, ch, part, s);
   else if (p->dtype == MKO_BF16)
-    MKO_TIMED("recur_bwd", s, recur::backward<bf16><<<grid, recur::kThreads, 0, s>>>(*p, hs, part));
+    recur::launch_bwd<bf16>(*p, g, ch, part, s);
   else
-    MKO_TIMED("recur_bwd", s, recur::backward<_Float16><<<grid, recur::kThreads, 0, s>>>(*p, hs, part));
+    recur::launch_bwd<_Float16>(*p, g, ch, part, s);
   if (p->ddecay)
-    MKO_TIMED("recur_bwd_finish", s, recur::finish<<<grid.x, recur::kThreads, 0, s>>>(*p, part));
+    MKO_TIMED("recur_bwd_finish", s,
+              recur::finish<<<static_cast<unsigned>(recur::cdiv(p->channels, 64)), recur::kFinishWaves * 64, 0, s>>>(
+                  *p, part, p->batch * g.chunks));
   return mko_check_launch("recur_bwd");
 }
 
