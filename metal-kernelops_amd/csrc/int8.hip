@@ -4,6 +4,7 @@
 #include "common.hpp"
 #include "io.hpp"
 #include "quantize.hpp"
+#include "rows.hpp"
 
 namespace mko {
 namespace int8 {
@@ -15,21 +16,90 @@ constexpr int64_t kMaxSide = 1 << 26;
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// A team of waves holds a row in registers between its largest value and its bytes, NV vectors of 16
+// bytes of x a thread.
+template <typename T, int NV>
+__global__ void __launch_bounds__(1024) quantize_rows(mko_quantize_params p, int team_threads) {
+  constexpr int VEC = kVecOf<T>;
+  __shared__ uint32_t tops[16];
+  const int team = uniform(static_cast<int>(threadIdx.x) / team_threads);
+  const int lt = threadIdx.x - team * team_threads;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / team_threads) + team;
+  const bool live = row < p.rows;
+  const int64_t n = live ? p.features : 0;
+  const T* x = static_cast<const T*>(p.x) + (live ? row * p.x_stride : 0);
+  Words<T, VEC> raw[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) raw[k] = load_part<T, VEC>(x, static_cast<int64_t>(lt + k * team_threads) * VEC, n);
+  uint32_t am = 0;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    float v[VEC];
+    unpack_words<T, VEC>(raw[k].w, v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) am = max(am, abs_bits(v[e]));
+  }
+  am = wave_max(am);
+  if (team_threads > kWave) {
+    const int wave = threadIdx.x >> 6, waves = team_threads >> 6;
+    if ((threadIdx.x & (kWave - 1)) == 0) tops[wave] = am;
+    __syncthreads();
+    for (int i = 0; i < waves; ++i) am = max(am, tops[team * waves + i]);
+  }
+  if (!live) return;
+  const RowScale q = row_scale(am);
+  if (lt == 0) p.scale[row] = q.scale;
+  int8_t* out = p.q + row * p.q_stride;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    float v[VEC];
+    int b[VEC];
+    unpack_words<T, VEC>(raw[k].w, v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) b[e] = quantise(v[e], q.inv);
+    store_bytes<VEC>(out, static_cast<int64_t>(lt + k * team_threads) * VEC, n, p.q_stride, b);
+  }
+  for (int64_t i = cdiv_dev(n, VEC) * VEC + lt; i < p.q_stride; i += team_threads) out[i] = 0;
+}
+
+// Rows wider than a team's registers are read twice.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) quantize_rows(mko_quantize_params p) {
-  __shared__ uint32_t top[kThreads / kWave];
+__global__ void __launch_bounds__(1024) quantize_wide(mko_quantize_params p) {
+  __shared__ uint32_t tops[16];
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
   uint32_t am = 0;
-  for (int64_t i = threadIdx.x; i < p.features; i += kThreads) am = max(am, abs_bits(to_f32(x[i])));
+  for (int64_t i = threadIdx.x; i < p.features; i += 1024) am = max(am, abs_bits(to_f32(x[i])));
   am = wave_max(am);
-  if ((threadIdx.x & (kWave - 1)) == 0) top[threadIdx.x / kWave] = am;
+  if ((threadIdx.x & (kWave - 1)) == 0) tops[threadIdx.x / kWave] = am;
   __syncthreads();
-  for (int w = 0; w < kThreads / kWave; ++w) am = max(am, top[w]);
+  for (int w = 0; w < 16; ++w) am = max(am, tops[w]);
   const RowScale q = row_scale(am);
   if (threadIdx.x == 0) p.scale[row] = q.scale;
-  for (int64_t i = threadIdx.x; i < p.q_stride; i += kThreads)
+  for (int64_t i = threadIdx.x; i < p.q_stride; i += 1024)
     p.q[row * p.q_stride + i] = i < p.features ? static_cast<int8_t>(quantise(to_f32(x[i]), q.inv)) : 0;
+}
+
+template <typename T, int NV>
+void launch_quantize_n(const mko_quantize_params& p, int team, hipStream_t s) {
+  const int threads = team > 4 ? team * kWave : 4 / team * team * kWave;
+  const unsigned grid = static_cast<unsigned>(cdiv(p.rows, threads / (team * kWave)));
+  MKO_TIMED("quantize_int8", s, quantize_rows<T, NV><<<grid, threads, 0, s>>>(p, team * kWave));
+}
+
+// Teams as for the norm (residual_norm.hip): a vector a thread for few rows, a wave a row for many.
+template <typename T>
+void launch_quantize(const mko_quantize_params& p, hipStream_t s) {
+  const int64_t waves = cdiv(p.features, kVecOf<T> * kWave);
+  int team = 1;
+  while (team < 16 && team < waves && (cdiv(waves, team) > 8 || p.rows * team < 2048)) ++team;
+  const int64_t nv = cdiv(waves, team);
+  if (nv <= 1) return launch_quantize_n<T, 1>(p, team, s);
+  if (nv <= 2) return launch_quantize_n<T, 2>(p, team, s);
+  if (nv <= 3) return launch_quantize_n<T, 3>(p, team, s);
+  if (nv <= 5) return launch_quantize_n<T, 5>(p, team, s);
+  if (nv <= 8) return launch_quantize_n<T, 8>(p, team, s);
+  MKO_TIMED("quantize_int8_wide", s, quantize_wide<T><<<static_cast<unsigned>(p.rows), 1024, 0, s>>>(p));
 }
 
 typedef int v4i __attribute__((ext_vector_type(4)));
@@ -471,23 +541,22 @@ extern "C" int mko_quantize_int8(const mko_quantize_params* p, void* stream) {
     mko_set_error("quantize_int8: dtype must be float32, float16 or bfloat16");
     return MKO_EINVAL;
   }
-  if (p->rows > 0x7fffff) {
-    mko_set_error("quantize_int8: rows is at most 2^23 - 1");
+  if (p->rows >= 1 << 22) {
+    mko_set_error("quantize_int8: rows is below 2^22");
     return MKO_EUNSUPPORTED;
   }
-  if (p->rows == 0) return MKO_OK;
+  if (p->rows == 0 || p->q_stride == 0) return MKO_OK;
   if (!p->scale || (p->features && (!p->x || !p->q))) {
     mko_set_error("quantize_int8: x, q and scale are required");
     return MKO_EINVAL;
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned grid = static_cast<unsigned>(p->rows);
   if (p->dtype == MKO_F32)
-    MKO_TIMED("quantize_int8", s, int8::quantize_rows<float><<<grid, int8::kThreads, 0, s>>>(*p));
+    int8::launch_quantize<float>(*p, s);
   else if (p->dtype == MKO_BF16)
-    MKO_TIMED("quantize_int8", s, int8::quantize_rows<bf16><<<grid, int8::kThreads, 0, s>>>(*p));
+    int8::launch_quantize<bf16>(*p, s);
   else
-    MKO_TIMED("quantize_int8", s, int8::quantize_rows<_Float16><<<grid, int8::kThreads, 0, s>>>(*p));
+    int8::launch_quantize<_Float16>(*p, s);
   return mko_check_launch("quantize_int8");
 }
 

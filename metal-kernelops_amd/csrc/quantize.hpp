@@ -42,4 +42,33 @@ __device__ __forceinline__ int quantise(float v, float inv) {
   return static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
 }
 
+__device__ __forceinline__ int64_t cdiv_dev(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// NE bytes from column i of a row of n columns padded to `pitch`, the padding zero.  Rows start at
+// any byte.
+template <int NE>
+__device__ __forceinline__ void store_bytes(int8_t* row, int64_t i, int64_t n, int64_t pitch, const int (&b)[NE]) {
+  if (i >= n) return;
+  uint32_t w[NE / 4];
+#pragma unroll
+  for (int k = 0; k < NE / 4; ++k) {
+    w[k] = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[k] |= (i + 4 * k + e < n ? static_cast<uint32_t>(b[4 * k + e]) & 0xffu : 0u) << (8 * e);
+  }
+  struct __attribute__((packed)) Any {
+    uint32_t w[NE / 4];
+  };
+  if (i + NE <= pitch) {
+    Any o;
+#pragma unroll
+    for (int k = 0; k < NE / 4; ++k) o.w[k] = w[k];
+    *reinterpret_cast<Any*>(row + i) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+      if (i + e < pitch) row[i + e] = static_cast<int8_t>(w[e / 4] >> (8 * (e % 4)));
+  }
+}
+
 }  // namespace mko

@@ -6,6 +6,7 @@
 //   dx = g m s(ig),  dig = g m x s(ig) (1 - s(ig)),  drg = dv v (1 - s(rg)),
 //   dv = g (s(ig) x a^2 / m - a h[t-1]),  ddecay = scale s(decay) sum(dv s(rg))
 #include "common.hpp"
+#include "rows.hpp"
 
 namespace mko {
 namespace recur {
@@ -509,21 +510,11 @@ __global__ void __launch_bounds__(NW * 64) backward(mko_recur_params p, Geo g, C
   }
 }
 
-// ddecay from the chunks' sums (rows of `part`), sixteen rows at a time.
-constexpr int kFinishWaves = 16;
-__global__ void __launch_bounds__(kFinishWaves * 64) finish(mko_recur_params p, const float* part, int64_t rows) {
-  __shared__ float sums[kFinishWaves][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t d = static_cast<int64_t>(blockIdx.x) * 64 + lane;
-  float s = 0.0f;
-  if (d < p.channels)
-    for (int64_t r = wave; r < rows; r += kFinishWaves) s += part[r * p.channels + d];
-  sums[wave][lane] = s;
-  __syncthreads();
-  if (wave || d >= p.channels) return;
-  s = 0.0f;
-  for (int w = 0; w < kFinishWaves; ++w) s += sums[w][lane];
-  p.ddecay[d] = s * p.scale * softplus_grad(p.decay[d]);
+// ddecay from the chunks' sums (rows of `part`).
+__global__ void __launch_bounds__(kColumnThreads) finish(mko_recur_params p, const float* part, int64_t rows) {
+  const int64_t d = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
+  const float s = column_sum(part, rows, p.channels, d);
+  if (threadIdx.x < 32 && d < p.channels) p.ddecay[d] = s * p.scale * softplus_grad(p.decay[d]);
 }
 
 template <typename T, typename S>
@@ -702,7 +693,7 @@ extern "C" int mko_recur_bwd(const mko_recur_params* p, void* stream) {
     recur::launch_bwd<_Float16>(*p, g, ch, part, s);
   if (p->ddecay)
     MKO_TIMED("recur_bwd_finish", s,
-              recur::finish<<<static_cast<unsigned>(recur::cdiv(p->channels, 64)), recur::kFinishWaves * 64, 0, s>>>(
+              recur::finish<<<static_cast<unsigned>(recur::cdiv(p->channels, 32)), kColumnThreads, 0, s>>>(
                   *p, part, p->batch * g.chunks));
   return mko_check_launch("recur_bwd");
 }

@@ -51,7 +51,7 @@ def quantize_int8(x):
     features, lead = x.shape[-1], x.shape[:-1]
     x2 = nat.rows(x.reshape(-1, features)) if features else x.reshape(lead.numel(), 0)
     rows = x2.shape[0]
-    rules.require(rows < 1 << 23, f"at most 2^23 - 1 rows (got {rows})")
+    rules.require(rows < 1 << 22, f"at most 2^22 - 1 rows (got {rows})")
     pitch = -(-features // ALIGN) * ALIGN
     q = torch.empty((rows, pitch), dtype=torch.int8, device=x.device)
     if not features:

@@ -127,7 +127,7 @@ def _checked(op, x, weight, residual):
     if residual is not None:
         rules.dtype_in((x.dtype, torch.float32), residual=residual)
     rows = x.shape[:-1].numel()
-    rules.require(rows < 1 << 23, f"at most 2^23 - 1 rows (got {rows})")
+    rules.require(rows < 1 << 22, f"at most 2^22 - 1 rows (got {rows})")
     return nat.values(weight).contiguous()
 
 
