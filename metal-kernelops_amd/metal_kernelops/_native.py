@@ -9,7 +9,6 @@ is passed as the launch stream.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -380,15 +379,20 @@ def stream_of(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def on_device(device):
-    """A context in which ``device`` is the current one, which is where a kernel is launched
-    whatever stream it is given; free of cost where it is current already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
-
-
-_HERE = contextlib.nullcontext()
+def launch(name, params, device):
+    """Calls the entry point ``name`` on the current stream of ``device`` and raises on its status.
+    A kernel is launched on the current device whatever stream it is given, so another one is made
+    current for the call.  The stream is asked for as a raw handle: the Stream object that
+    ``torch.cuda.current_stream`` builds takes 2 us of host time, as much as a small launch."""
+    index = device.index
+    fn = getattr(lib(), name)
+    if index == torch._C._cuda_getDevice():
+        status = fn(ctypes.byref(params), torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(ctypes.byref(params), torch._C._cuda_getCurrentRawStream(index))
+    if status != 0:
+        check(status, name)
 
 
 def values(t):
@@ -401,8 +405,21 @@ def values(t):
 
 def rows(t):
     """``t`` as a kernel reads it in rows: the last axis of unit stride, the others as they are."""
-    t = values(t)
+    if t.is_neg() or t._is_zerotensor():
+        t = values(t)
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def dense(t):
+    """``t`` as a kernel reads it whole: contiguous, its values in memory."""
+    if t.is_neg() or t._is_zerotensor():
+        t = values(t)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def dense_f32(t):
+    """The same in float32; None stays None."""
+    return None if t is None else dense(t if t.dtype == torch.float32 else t.float())
 
 
 def workspace(nbytes, device):

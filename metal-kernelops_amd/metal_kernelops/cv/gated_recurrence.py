@@ -21,6 +21,7 @@ dbydd/metal-kernelops.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -35,41 +36,41 @@ __all__ = ["gated_recurrence", "gated_recurrence_reference", "gated_recurrence_u
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _params(x, input_gate, decay_gate, decay, initial, reset, scale):
-    p = nat.RecurParams()
-    p.x, p.input_gate, p.decay_gate = x.data_ptr(), input_gate.data_ptr(), decay_gate.data_ptr()
-    p.decay, p.initial, p.reset = decay.data_ptr(), nat.ptr(initial), nat.ptr(reset)
-    p.batch, p.length, p.channels = x.shape
-    p.x_stride_b, p.x_stride_t = x.stride(0), x.stride(1)
-    p.ig_stride_b, p.ig_stride_t = input_gate.stride(0), input_gate.stride(1)
-    p.rg_stride_b, p.rg_stride_t = decay_gate.stride(0), decay_gate.stride(1)
-    p.scale, p.dtype = scale, nat.code(x.dtype)
-    return p
+@functools.lru_cache(maxsize=256)
+def _sizes(batch, length, channels):
+    """Bytes of the saved states and of the forward's and the backward's workspaces."""
+    p = nat.RecurParams(batch=batch, length=length, channels=channels, ddecay=1)
+    lib, at = nat.lib(), ctypes.byref(p)
+    return lib.mko_recur_states_size(at), lib.mko_recur_fwd_workspace_size(at), lib.mko_recur_bwd_workspace_size(at)
+
+
+def _params(x, input_gate, decay_gate, decay, initial, reset, scale, y, final, states, dy, dfinal, dx, dig, drg, ddecay,
+            dinitial, space):
+    batch, length, channels = x.shape
+    return nat.RecurParams(
+        x.data_ptr(), input_gate.data_ptr(), decay_gate.data_ptr(), decay.data_ptr(), nat.ptr(initial), nat.ptr(reset),
+        nat.ptr(y), nat.ptr(final), states.data_ptr(), nat.ptr(dy), nat.ptr(dfinal), nat.ptr(dx), nat.ptr(dig),
+        nat.ptr(drg), nat.ptr(ddecay), nat.ptr(dinitial), nat.ptr(space), 0 if space is None else space.numel(),
+        batch, length, channels, x.stride(0), x.stride(1), input_gate.stride(0), input_gate.stride(1),
+        decay_gate.stride(0), decay_gate.stride(1), scale, nat.code(x.dtype))
 
 
 def _forward(x, input_gate, decay_gate, decay, initial, reset, scale, want_final):
     """``(y, final, states)``; ``states`` is what the backward reads, ``final`` None if unwanted."""
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    batch, length, channels = x.shape
+    y = torch.empty((batch, length, channels), dtype=x.dtype, device=x.device)
     final = None
-    if x.shape[1] == 0:
-        if want_final:
-            final = initial.clone() if initial is not None else x.new_zeros((x.shape[0], x.shape[2]),
-                                                                            dtype=torch.float32)
-        return y, final, None
     if want_final:
-        final = torch.empty((x.shape[0], x.shape[2]), dtype=torch.float32, device=x.device)
+        final = torch.empty((batch, channels), dtype=torch.float32, device=x.device)
+        if length == 0:
+            final.zero_() if initial is None else final.copy_(initial)
     if y.numel() == 0:
         return y, final, None
-    lib = nat.lib()
-    p = _params(x, input_gate, decay_gate, decay, initial, reset, scale)
-    at = ctypes.byref(p)
-    states = nat.workspace(lib.mko_recur_states_size(at), x.device)
-    size = lib.mko_recur_fwd_workspace_size(at)
-    ws = nat.workspace(size, x.device) if size else None
-    p.y, p.final_state, p.states = y.data_ptr(), nat.ptr(final), states.data_ptr()
-    p.workspace, p.workspace_bytes = nat.ptr(ws), size
-    with nat.on_device(x.device):
-        nat.check(lib.mko_recur_fwd(at, nat.stream_of(x.device)), "mko_recur_fwd")
+    saved, size, _ = _sizes(batch, length, channels)
+    states = torch.empty(saved, dtype=torch.uint8, device=x.device)
+    space = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    nat.launch("mko_recur_fwd", _params(x, input_gate, decay_gate, decay, initial, reset, scale, y, final, states, None,
+                                        None, None, None, None, None, None, space), x.device)
     return y, final, states
 
 
@@ -77,8 +78,8 @@ class _Recurrence(torch.autograd.Function):
     """Forward and analytic first-order backward through the C ABI."""
 
     @staticmethod
-    def forward(ctx, x, input_gate, decay_gate, decay, initial, reset, scale):
-        y, final, states = _forward(x, input_gate, decay_gate, decay, initial, reset, scale, True)
+    def forward(ctx, x, input_gate, decay_gate, decay, initial, reset, scale, want_final):
+        y, final, states = _forward(x, input_gate, decay_gate, decay, initial, reset, scale, want_final)
         ctx.save_for_backward(x, input_gate, decay_gate, decay, initial, reset, states)
         ctx.scale = scale
         ctx.set_materialize_grads(False)  # an unused output reaches backward as None
@@ -89,46 +90,51 @@ class _Recurrence(torch.autograd.Function):
     def backward(ctx, dy, dfinal):
         x, input_gate, decay_gate, decay, initial, reset, states = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dfinal = None if dfinal is None else nat.values(dfinal).contiguous()
-        dx, dig, drg = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(3))
-        ddecay = torch.zeros_like(decay) if need[3] else None
+        if dfinal is not None:
+            dfinal = nat.dense(dfinal)
+        shape, dtype, device = x.shape, x.dtype, x.device
+        dx, dig, drg = (torch.empty(shape, dtype=dtype, device=device) for _ in range(3))
+        ddecay = torch.empty(decay.shape, dtype=torch.float32, device=device) if need[3] else None
         dinitial = None
         if initial is not None and need[4]:
-            dinitial = torch.zeros_like(initial) if dfinal is None else dfinal.clone()
+            dinitial = torch.empty(initial.shape, dtype=torch.float32, device=device)
         if x.numel():
-            dy = torch.zeros_like(dx) if dy is None else nat.values(dy).contiguous()
-            lib = nat.lib()
-            p = _params(x, input_gate, decay_gate, decay, initial, reset, ctx.scale)
-            at = ctypes.byref(p)
-            p.states, p.dy, p.dfinal = states.data_ptr(), dy.data_ptr(), nat.ptr(dfinal)
-            p.dx, p.dinput_gate, p.ddecay_gate = dx.data_ptr(), dig.data_ptr(), drg.data_ptr()
-            p.ddecay, p.dinitial = nat.ptr(ddecay), nat.ptr(dinitial)
-            size = lib.mko_recur_bwd_workspace_size(at)
-            ws = nat.workspace(size, x.device) if size else None
-            p.workspace, p.workspace_bytes = nat.ptr(ws), size
-            with nat.on_device(x.device):
-                nat.check(lib.mko_recur_bwd(at, nat.stream_of(x.device)), "mko_recur_bwd")
-        return dx, dig, drg, ddecay, dinitial, None, None
+            dy = torch.zeros_like(dx) if dy is None else nat.dense(dy)
+            space = torch.empty(_sizes(*shape)[2], dtype=torch.uint8, device=device)
+            nat.launch("mko_recur_bwd", _params(x, input_gate, decay_gate, decay, initial, reset, ctx.scale, None, None,
+                                                states, dy, dfinal, dx, dig, drg, ddecay, dinitial, space), device)
+        else:
+            if ddecay is not None:
+                ddecay.zero_()
+            if dinitial is not None:
+                dinitial.zero_() if dfinal is None else dinitial.copy_(dfinal)
+        return dx, dig, drg, ddecay, dinitial, None, None, None
 
 
 def _check(op, x, input_gate, decay_gate, decay, scale, layout):
-    """The argument rules that the scan and the update share, in their order."""
+    """The argument rules that the scan and the update share, in their order.  Messages are formed
+    only for an argument that breaks a rule: a decode step's checks are host time."""
     rules = Rules(op)
-    rules.dims("x", x, len(layout), f"({', '.join(layout)})")
-    rules.shape("input_gate", input_gate, tuple(x.shape))
-    rules.shape("decay_gate", decay_gate, tuple(x.shape))
-    rules.shape("decay", decay, (x.shape[-1],))
+    rules.dims("x", x, layout.count(",") + 1, layout)
+    shape = x.shape
+    if input_gate.shape != shape or decay_gate.shape != shape or decay.shape != shape[-1:]:
+        rules.shape("input_gate", input_gate, shape)
+        rules.shape("decay_gate", decay_gate, shape)
+        rules.shape("decay", decay, shape[-1:])
     _require_gpu(x)
-    rules.same_device(x.device, input_gate=input_gate, decay_gate=decay_gate, decay=decay)
-    rules.dtype_in(_FLOATS, x=x)
-    rules.dtype_in((x.dtype,), input_gate=input_gate, decay_gate=decay_gate)
-    rules.require(decay.is_floating_point(), f"decay should be a floating tensor; it is {decay.dtype}")
-    rules.require(scale > 0, f"scale should be positive; it is {scale}")
+    device, dtype = x.device, x.dtype
+    if input_gate.device != device or decay_gate.device != device or decay.device != device:
+        rules.same_device(device, input_gate=input_gate, decay_gate=decay_gate, decay=decay)
+    if dtype not in _FLOATS or input_gate.dtype != dtype or decay_gate.dtype != dtype:
+        rules.dtype_in(_FLOATS, x=x)
+        rules.dtype_in((dtype,), input_gate=input_gate, decay_gate=decay_gate)
+    if not decay.is_floating_point():
+        rules.fail(f"decay should be a floating tensor; it is {decay.dtype}")
+    if not scale > 0:
+        rules.fail(f"scale should be positive; it is {scale}")
+    if shape[0] > 65535:
+        rules.fail(f"batch is at most 65535 (got {shape[0]})")
     return rules
-
-
-def _f32(t):
-    return None if t is None else nat.values(t if t.dtype == torch.float32 else t.float()).contiguous()
 
 
 def gated_recurrence(x, input_gate, decay_gate, decay, initial_state=None, reset=None, scale=8.0,
@@ -149,23 +155,24 @@ def gated_recurrence(x, input_gate, decay_gate, decay, initial_state=None, reset
     Returns:
         ``y`` in ``x.dtype``, or ``(y, final_state)``.
     """
-    rules = _check("gated_recurrence", x, input_gate, decay_gate, decay, scale, ("batch", "length", "channels"))
+    rules = _check("gated_recurrence", x, input_gate, decay_gate, decay, scale, "(batch, length, channels)")
     batch, length, channels = x.shape
-    rules.require(batch <= 65535, f"batch is at most 65535 (got {batch})")
-    rules.shape("initial_state", initial_state, (batch, channels))
-    rules.shape("reset", reset, (batch, length))
-    rules.same_device(x.device, initial_state=initial_state, reset=reset)
     if initial_state is not None:
-        rules.require(initial_state.is_floating_point(),
-                      f"initial_state should be a floating tensor; it is {initial_state.dtype}")
+        rules.shape("initial_state", initial_state, (batch, channels))
+        rules.same_device(x.device, initial_state=initial_state)
+        if not initial_state.is_floating_point():
+            rules.fail(f"initial_state should be a floating tensor; it is {initial_state.dtype}")
     if reset is not None:
+        rules.shape("reset", reset, (batch, length))
+        rules.same_device(x.device, reset=reset)
         rules.dtype_in((torch.bool,), reset=reset)
         reset = reset.contiguous()
-    decay, initial = _f32(decay), _f32(initial_state)
+    decay, initial = nat.dense_f32(decay), nat.dense_f32(initial_state)
     x, input_gate, decay_gate = nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate)
     if torch.is_grad_enabled() and (x.requires_grad or input_gate.requires_grad or decay_gate.requires_grad
                                     or decay.requires_grad or (initial is not None and initial.requires_grad)):
-        y, final = _Recurrence.apply(x, input_gate, decay_gate, decay, initial, reset, float(scale))
+        y, final = _Recurrence.apply(x, input_gate, decay_gate, decay, initial, reset, float(scale),
+                                     bool(return_final_state))
     else:
         y, final, _ = _forward(x, input_gate, decay_gate, decay, initial, reset, float(scale), return_final_state)
     return (y, final) if return_final_state else y
@@ -183,17 +190,20 @@ def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, 
 
     Where a gradient is wanted the step is a :func:`gated_recurrence` of length one.
     """
-    rules = _check("gated_recurrence_update", x, input_gate, decay_gate, decay, scale, ("batch", "channels"))
-    rules.shape("state", state, tuple(x.shape))
-    rules.same_device(x.device, state=state, out_state=out_state)
-    rules.dtype_in(_FLOATS, state=state)
-    rules.require(x.shape[0] <= 65535, f"batch is at most 65535 (got {x.shape[0]})")
+    rules = _check("gated_recurrence_update", x, input_gate, decay_gate, decay, scale, "(batch, channels)")
+    if state.shape != x.shape or state.device != x.device or state.dtype not in _FLOATS:
+        rules.shape("state", state, x.shape)
+        rules.same_device(x.device, state=state)
+        rules.dtype_in(_FLOATS, state=state)
     if out_state is not None:
-        rules.require(out_state.shape == state.shape and out_state.dtype == state.dtype,
-                      "out_state should have the shape and dtype of state")
-        rules.require(out_state.is_contiguous(), "out_state should be contiguous")
-        rules.require(not out_state.requires_grad, "out_state is overwritten in place, so it may not require grad")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (state, x, input_gate, decay_gate, decay)):
+        if out_state.shape != state.shape or out_state.dtype != state.dtype or out_state.device != state.device:
+            rules.fail("out_state should have the shape, dtype and device of state")
+        if not out_state.is_contiguous():
+            rules.fail("out_state should be contiguous")
+        if out_state.requires_grad:
+            rules.fail("out_state is overwritten in place, so it may not require grad")
+    if torch.is_grad_enabled() and (state.requires_grad or x.requires_grad or input_gate.requires_grad
+                                    or decay_gate.requires_grad or decay.requires_grad):
         y, final = gated_recurrence(x[:, None], input_gate[:, None], decay_gate[:, None], decay, initial_state=state,
                                     scale=scale, return_final_state=True)
         final = final.to(state.dtype)
@@ -203,16 +213,17 @@ def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, 
             out_state.copy_(final)
         return y[:, 0], out_state
     x, input_gate, decay_gate = nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate)
-    state, decay = nat.values(state).contiguous(), _f32(decay)
-    new_state = out_state if out_state is not None else torch.empty_like(state)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if y.numel():
-        p = nat.RecurUpdateParams(x.data_ptr(), input_gate.data_ptr(), decay_gate.data_ptr(), decay.data_ptr(),
-                                  state.data_ptr(), new_state.data_ptr(), y.data_ptr(), x.shape[0], x.shape[1],
-                                  x.stride(0), input_gate.stride(0), decay_gate.stride(0), scale,
-                                  nat.code(x.dtype), nat.code(state.dtype))
-        with nat.on_device(x.device):
-            nat.check(nat.lib().mko_recur_update(ctypes.byref(p), nat.stream_of(x.device)), "mko_recur_update")
+    state, decay = nat.dense(state), nat.dense_f32(decay)
+    batch, channels = shape = x.shape
+    new_state = out_state
+    if new_state is None:
+        new_state = torch.empty(shape, dtype=state.dtype, device=x.device)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    if batch and channels:
+        nat.launch("mko_recur_update", nat.RecurUpdateParams(
+            x.data_ptr(), input_gate.data_ptr(), decay_gate.data_ptr(), decay.data_ptr(), state.data_ptr(),
+            new_state.data_ptr(), y.data_ptr(), batch, channels, x.stride(0), input_gate.stride(0), decay_gate.stride(0),
+            scale, nat.code(x.dtype), nat.code(state.dtype)), x.device)
     return y, new_state
 
 

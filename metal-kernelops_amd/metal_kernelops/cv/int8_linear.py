@@ -14,8 +14,6 @@ counterpart in dbydd/metal-kernelops.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from .. import _native as nat
@@ -43,26 +41,30 @@ def quantize_int8(x):
     is refused while grad mode is on.
     """
     rules = Rules("quantize_int8")
-    rules.require(x.dim() >= 1, "x needs a feature axis")
+    if x.dim() < 1:
+        rules.fail("x needs a feature axis")
     _require_gpu(x)
-    rules.dtype_in(_FLOATS, x=x)
-    rules.require(not (torch.is_grad_enabled() and x.requires_grad),
-                  "8-bit outputs have no gradient; call it under torch.no_grad()")
+    if x.dtype not in _FLOATS:
+        rules.dtype_in(_FLOATS, x=x)
+    if x.requires_grad and torch.is_grad_enabled():
+        rules.fail("8-bit outputs have no gradient; call it under torch.no_grad()")
     features, lead = x.shape[-1], x.shape[:-1]
-    x2 = nat.rows(x.reshape(-1, features)) if features else x.reshape(lead.numel(), 0)
-    rows = x2.shape[0]
-    rules.require(rows < 1 << 22, f"at most 2^22 - 1 rows (got {rows})")
     pitch = -(-features // ALIGN) * ALIGN
-    q = torch.empty((rows, pitch), dtype=torch.int8, device=x.device)
-    if not features:
-        return q.view(*lead, 0), x.new_zeros(lead, dtype=torch.float32)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    if rows:
-        p = nat.QuantizeParams(x2.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, features, x2.stride(0), pitch,
-                               nat.code(x.dtype))
-        with nat.on_device(x.device):
-            nat.check(nat.lib().mko_quantize_int8(ctypes.byref(p), nat.stream_of(x.device)), "mko_quantize_int8")
-    return q.view(*lead, pitch)[..., :features], scale.view(lead)
+    q = torch.empty((*lead, pitch), dtype=torch.int8, device=x.device)
+    scale = torch.empty(lead, dtype=torch.float32, device=x.device)
+    if q.numel():
+        rows = q.numel() // pitch
+        if rows >= 1 << 22:
+            rules.fail(f"at most 2^22 - 1 rows (got {rows})")
+        if x.dim() != 2 and not x.is_contiguous():
+            x = x.reshape(-1, features)
+        x = nat.rows(x)
+        nat.launch("mko_quantize_int8", nat.QuantizeParams(
+            x.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, features, x.stride(0) if x.dim() == 2 else features, pitch,
+            nat.code(x.dtype)), x.device)
+    elif not features:
+        scale.zero_()
+    return q if pitch == features else q[..., :features], scale
 
 
 def int8_linear(q, q_scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16):
@@ -80,44 +82,44 @@ def int8_linear(q, q_scale, weight, weight_scale, bias=None, out_dtype=torch.bfl
     bias that requires grad is refused while grad mode is on.
     """
     rules = Rules("int8_linear")
-    rules.require(q.dim() >= 1, "q needs an inner axis")
-    rules.dims("weight", weight, 2, "(outer, inner)")
+    if q.dim() < 1:
+        rules.fail("q needs an inner axis")
+    if weight.dim() != 2:
+        rules.dims("weight", weight, 2, "(outer, inner)")
     outer, inner = weight.shape
     lead = q.shape[:-1]
-    rules.require(q.shape[-1] == inner, f"q has {q.shape[-1]} inner features, weight has {inner}")
-    rules.shape("q_scale", q_scale, tuple(lead))
-    rules.shape("weight_scale", weight_scale, (outer,))
-    rules.shape("bias", bias, (outer,))
+    if q.shape[-1] != inner:
+        rules.fail(f"q has {q.shape[-1]} inner features, weight has {inner}")
+    if q_scale.shape != lead or weight_scale.shape != (outer,) or (bias is not None and bias.shape != (outer,)):
+        rules.shape("q_scale", q_scale, lead)
+        rules.shape("weight_scale", weight_scale, (outer,))
+        rules.shape("bias", bias, (outer,))
     _require_gpu(q)
     rules.same_device(q.device, q_scale=q_scale, weight=weight, weight_scale=weight_scale, bias=bias)
-    rules.dtype_in((torch.int8,), q=q, weight=weight)
+    if q.dtype != torch.int8 or weight.dtype != torch.int8:
+        rules.dtype_in((torch.int8,), q=q, weight=weight)
     for name, t in (("q_scale", q_scale), ("weight_scale", weight_scale), ("bias", bias)):
         if t is not None:
-            rules.require(t.is_floating_point(), f"{name} should be a floating tensor; it is {t.dtype}")
-            rules.require(not (torch.is_grad_enabled() and t.requires_grad),
-                          f"{name} requires grad, and this product has no gradient; call it under torch.no_grad()")
-    rules.require(out_dtype in _FLOATS, f"out_dtype should be float32, float16 or bfloat16; it is {out_dtype}")
-    rules.require(inner <= MAX_INNER, f"inner is at most {MAX_INNER} here (got {inner})")
-    q2 = nat.rows(q.reshape(-1, inner)) if inner else q.reshape(lead.numel(), 0)
-    rows = q2.shape[0]
-    out = torch.empty((rows, outer), dtype=out_dtype, device=q.device)
-    if rows and outer:
-        weight, qs, ws, b = nat.rows(weight) if inner else weight, _f32(q_scale), _f32(weight_scale), _f32(bias)
-        lib = nat.lib()
-        p = nat.Int8LinearParams(q2.data_ptr(), qs.data_ptr(), weight.data_ptr(), ws.data_ptr(), nat.ptr(b),
-                                 out.data_ptr(), None, 0, rows, inner, outer, q2.stride(0), weight.stride(0),
-                                 nat.code(out_dtype))
-        size = lib.mko_int8_linear_workspace_size(ctypes.byref(p))
-        if size:
-            space = nat.workspace(size, q.device)
-            p.workspace, p.workspace_bytes = space.data_ptr(), size
-        with nat.on_device(q.device):
-            nat.check(lib.mko_int8_linear(ctypes.byref(p), nat.stream_of(q.device)), "mko_int8_linear")
-    return out.view(*lead, outer)
-
-
-def _f32(t):
-    return None if t is None else nat.values(t if t.dtype == torch.float32 else t.float()).contiguous()
+            if not t.is_floating_point():
+                rules.fail(f"{name} should be a floating tensor; it is {t.dtype}")
+            if t.requires_grad and torch.is_grad_enabled():
+                rules.fail(f"{name} requires grad, and this product has no gradient; call it under torch.no_grad()")
+    if out_dtype not in _FLOATS:
+        rules.fail(f"out_dtype should be float32, float16 or bfloat16; it is {out_dtype}")
+    if inner > MAX_INNER:
+        rules.fail(f"inner is at most {MAX_INNER} here (got {inner})")
+    out = torch.empty((*lead, outer), dtype=out_dtype, device=q.device)
+    if out.numel():
+        rows = out.numel() // outer
+        if inner:
+            if q.dim() != 2 and not q.is_contiguous():
+                q = q.reshape(-1, inner)
+            q, weight = nat.rows(q), nat.rows(weight)
+        qs, ws, b = nat.dense_f32(q_scale), nat.dense_f32(weight_scale), nat.dense_f32(bias)
+        nat.launch("mko_int8_linear", nat.Int8LinearParams(
+            q.data_ptr(), qs.data_ptr(), weight.data_ptr(), ws.data_ptr(), nat.ptr(b), out.data_ptr(), None, 0, rows,
+            inner, outer, q.stride(0) if q.dim() == 2 else inner, weight.stride(0), nat.code(out_dtype)), q.device)
+    return out
 
 
 def quantize_int8_reference(x):

@@ -19,6 +19,7 @@ RMSNorm, :func:`~metal_kernelops.cv.rmsnorm_gated`, has no residual).
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -34,58 +35,60 @@ __all__ = ["rmsnorm_residual", "rmsnorm_residual_int8", "rmsnorm_residual_int8_r
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _params(x, weight, residual, eps):
-    p = nat.ResnormParams()
-    p.x, p.weight, p.residual = x.data_ptr(), weight.data_ptr(), nat.ptr(residual)
-    p.rows, p.features = x.shape
-    p.x_stride, p.residual_stride = x.stride(0), 0 if residual is None else residual.stride(0)
-    p.eps, p.dtype, p.wdtype = eps, nat.code(x.dtype), nat.code(weight.dtype)
-    p.stream_dtype = nat.code(x.dtype if residual is None else residual.dtype)
-    return p
-
-
-def _launch_fwd(p, x):
-    with nat.on_device(x.device):
-        nat.check(nat.lib().mko_resnorm_fwd(ctypes.byref(p), nat.stream_of(x.device)), "mko_resnorm_fwd")
-
-
 def _rows(t):
-    return nat.rows(t.reshape(-1, t.shape[-1]))
+    """The rows of ``t`` at one stride: ``t`` itself where it has them, as a 2-d view or a copy."""
+    if t.dim() == 2 or t.is_contiguous():
+        t = nat.rows(t)
+        return t, t.stride(-2) if t.dim() == 2 else t.shape[-1]
+    t = nat.rows(t.reshape(-1, t.shape[-1]))
+    return t, t.stride(0)
+
+
+def _launch_fwd(x, weight, residual, out, q, scale, stream, rstd, pitch, eps):
+    (x, xs), (r, rs) = _rows(x), (None, 0) if residual is None else _rows(residual)
+    features = x.shape[-1]
+    nat.launch("mko_resnorm_fwd", nat.ResnormParams(
+        x.data_ptr(), nat.ptr(r), weight.data_ptr(), nat.ptr(out), nat.ptr(q), nat.ptr(scale), nat.ptr(stream),
+        nat.ptr(rstd), None, None, None, None, None, None, 0, x.numel() // features, features, xs, rs, pitch, eps,
+        nat.code(x.dtype), nat.code(x.dtype if r is None else r.dtype), nat.code(weight.dtype)), x.device)
 
 
 def _forward(x, weight, residual, eps, want_rstd):
     """``(out, stream, rstd)``; stream is None without a residual."""
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     stream = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    rstd = torch.empty(x.shape[:-1].numel(), dtype=torch.float32, device=x.device) if want_rstd else None
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if want_rstd else None
     if x.numel():
-        x2 = _rows(x)
-        p = _params(x2, weight, None if residual is None else _rows(residual), eps)
-        p.out, p.stream, p.rstd = out.data_ptr(), nat.ptr(stream), nat.ptr(rstd)
-        _launch_fwd(p, x)
+        _launch_fwd(x, weight, residual, out, None, None, stream, rstd, 0, eps)
     return out, stream, rstd
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(rows, features, dtype, stream_dtype):
+    """Bytes of the backward's partial sums of dweight."""
+    p = nat.ResnormParams(rows=rows, features=features, dtype=dtype, stream_dtype=stream_dtype, dweight=1)
+    return nat.lib().mko_resnorm_bwd_workspace_size(ctypes.byref(p))
 
 
 def _backward(dout, dstream, stream, weight, rstd, dtype, need_weight):
     """``(dx, dresidual, dweight)`` of dense operands; one tensor for both where the types agree."""
-    dx = torch.empty(stream.shape, dtype=dtype, device=stream.device)
-    dres = dx if stream.dtype == dtype else torch.empty(stream.shape, dtype=stream.dtype, device=stream.device)
-    dweight = torch.zeros(weight.shape, dtype=torch.float32, device=stream.device) if need_weight else None
+    shape, device = stream.shape, stream.device
+    dx = torch.empty(shape, dtype=dtype, device=device)
+    dres = dx if stream.dtype == dtype else torch.empty(shape, dtype=stream.dtype, device=device)
+    dweight = torch.empty(weight.shape, dtype=torch.float32, device=device) if need_weight else None
     if stream.numel():
-        lib = nat.lib()
-        p = nat.ResnormParams()
-        at = ctypes.byref(p)
-        p.stream, p.weight, p.rstd = stream.data_ptr(), weight.data_ptr(), rstd.data_ptr()
-        p.dout, p.dstream, p.dx = dout.data_ptr(), nat.ptr(dstream), dx.data_ptr()
-        p.dresidual, p.dweight = None if dres is dx else dres.data_ptr(), nat.ptr(dweight)
-        p.features = stream.shape[-1]
-        p.rows = stream.numel() // p.features
-        p.dtype, p.stream_dtype, p.wdtype = nat.code(dtype), nat.code(stream.dtype), nat.code(weight.dtype)
-        size = lib.mko_resnorm_bwd_workspace_size(at)
-        ws = nat.workspace(size, stream.device) if size else None
-        p.workspace, p.workspace_bytes = nat.ptr(ws), size
-        with nat.on_device(stream.device):
-            nat.check(lib.mko_resnorm_bwd(at, nat.stream_of(stream.device)), "mko_resnorm_bwd")
+        features = shape[-1]
+        rows, code, scode = stream.numel() // features, nat.code(dtype), nat.code(stream.dtype)
+        space = None
+        if need_weight:
+            space = torch.empty(_workspace(rows, features, code, scode), dtype=torch.uint8, device=device)
+        nat.launch("mko_resnorm_bwd", nat.ResnormParams(
+            None, None, weight.data_ptr(), None, None, None, stream.data_ptr(), rstd.data_ptr(), dout.data_ptr(),
+            nat.ptr(dstream), dx.data_ptr(), None if dres is dx else dres.data_ptr(), nat.ptr(dweight), nat.ptr(space),
+            0 if space is None else space.numel(), rows, features, 0, 0, 0, 0.0, code, scode, nat.code(weight.dtype)),
+            device)
+    elif need_weight:
+        dweight.zero_()
     return dx, dres, dweight
 
 
@@ -107,32 +110,40 @@ class _ResidualNorm(torch.autograd.Function):
     def backward(ctx, dout, dstream):
         stream, weight, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dstream = None if dstream is None else nat.values(dstream).contiguous()
+        dstream = None if dstream is None else nat.dense(dstream)
         if dout is None:  # only the stream was used
             return (None if dstream is None else dstream.to(ctx.dtype), None, dstream if need[2] else None, None)
-        dx, dres, dweight = _backward(nat.values(dout).contiguous(), dstream, nat.values(stream).contiguous(), weight,
-                                      rstd, ctx.dtype, need[1])
-        return dx, None if dweight is None else dweight.to(weight.dtype), dres if need[2] else None, None
+        dx, dres, dweight = _backward(nat.dense(dout), dstream, nat.dense(stream), weight, rstd, ctx.dtype, need[1])
+        if dweight is not None and weight.dtype != torch.float32:
+            dweight = dweight.to(weight.dtype)
+        return dx, dweight, dres if need[2] else None, None
 
 
 def _checked(op, x, weight, residual):
-    """The argument rules, in their order; returns the weight as the kernels read it."""
+    """The argument rules, in their order; returns the weight as the kernels read it.  Messages are
+    formed only for an argument that breaks a rule: the checks are host time."""
     rules = Rules(op)
-    rules.require(x.dim() >= 1, "x needs a feature axis")
-    rules.shape("weight", weight, (x.shape[-1],))
-    rules.shape("residual", residual, tuple(x.shape))
+    if x.dim() < 1:
+        rules.fail("x needs a feature axis")
+    shape, device = x.shape, x.device
+    if weight.shape != shape[-1:] or (residual is not None and residual.shape != shape):
+        rules.shape("weight", weight, shape[-1:])
+        rules.shape("residual", residual, shape)
     _require_gpu(x)
-    rules.same_device(x.device, weight=weight, residual=residual)
-    rules.dtype_in(_FLOATS, x=x, weight=weight)
-    if residual is not None:
+    if weight.device != device or (residual is not None and residual.device != device):
+        rules.same_device(device, weight=weight, residual=residual)
+    if x.dtype not in _FLOATS or weight.dtype not in _FLOATS:
+        rules.dtype_in(_FLOATS, x=x, weight=weight)
+    if residual is not None and residual.dtype != x.dtype:
         rules.dtype_in((x.dtype, torch.float32), residual=residual)
-    rows = x.shape[:-1].numel()
-    rules.require(rows < 1 << 22, f"at most 2^22 - 1 rows (got {rows})")
-    return nat.values(weight).contiguous()
+    if shape[:-1].numel() >= 1 << 22:
+        rules.fail(f"at most 2^22 - 1 rows (got {shape[:-1].numel()})")
+    return nat.dense(weight)
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _wants_grad(x, weight, residual):
+    return torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                        or (residual is not None and residual.requires_grad))
 
 
 def rmsnorm_residual(x, weight, residual=None, eps=1e-5):
@@ -166,21 +177,18 @@ def rmsnorm_residual_int8(x, weight, residual=None, eps=1e-5):
     For inference: arguments that require grad are refused while grad mode is on.
     """
     w = _checked("rmsnorm_residual_int8", x, weight, residual)
-    Rules("rmsnorm_residual_int8").require(not _wants_grad(x, weight, residual),
-                                           "8-bit outputs have no gradient; call it under torch.no_grad()")
+    if _wants_grad(x, weight, residual):
+        Rules("rmsnorm_residual_int8").fail("8-bit outputs have no gradient; call it under torch.no_grad()")
     lead, features = x.shape[:-1], x.shape[-1]
     pitch = -(-features // ALIGN) * ALIGN
     q = torch.empty((*lead, pitch), dtype=torch.int8, device=x.device)
     scale = torch.empty(lead, dtype=torch.float32, device=x.device)
     stream = x if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
     if x.numel():
-        p = _params(_rows(x), w, None if residual is None else _rows(residual), float(eps))
-        p.q, p.q_scale, p.q_stride = q.data_ptr(), scale.data_ptr(), pitch
-        p.stream = None if residual is None else stream.data_ptr()
-        _launch_fwd(p, x)
+        _launch_fwd(x, w, residual, None, q, scale, None if residual is None else stream, None, pitch, float(eps))
     elif not features:
         scale.zero_()
-    return q[..., :features], scale, stream
+    return q if pitch == features else q[..., :features], scale, stream
 
 
 def rmsnorm_residual_reference(x, weight, residual=None, eps=1e-5):
