@@ -5,6 +5,8 @@
 // Backward, with g[t] = dy[t] + a[t+1] g[t+1]:
 //   dx = g m s(ig),  dig = g m x s(ig) (1 - s(ig)),  drg = dv v (1 - s(rg)),
 //   dv = g (s(ig) x a^2 / m - a h[t-1]),  ddecay = scale s(decay) sum(dv s(rg))
+#include <type_traits>
+
 #include "common.hpp"
 #include "rows.hpp"
 
@@ -14,33 +16,37 @@ namespace {
 
 constexpr int kChunk = MKO_RECUR_CHUNK;
 constexpr int kThreads = 256;
+constexpr int kV = 2;  // channels a lane of the scans takes
+constexpr int64_t kMostBatch = 65535, kMostSide = int64_t{1} << 31;
+constexpr int64_t kMostWorkgroups = int64_t{1} << 22;  // of 512 threads: 2^31 threads in a launch
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// 1 - e^-2v from v and a = e^-v: below v = 1/8 a six-term series (truncation (2v)^6 / 5040, 5e-8
-// relative), where 1 - a^2 would cancel.
-__device__ __forceinline__ float one_minus_square(float v, float a) {
-  const float w = 2.0f * v;
-  const float s = w * (1.0f - w * (1.0f / 2) *
-                  (1.0f - w * (1.0f / 3) * (1.0f - w * (1.0f / 4) * (1.0f - w * (1.0f / 5) * (1.0f - w * (1.0f / 6))))));
-  return v < 0.125f ? s : 1.0f - a * a;
+// A channel's rate in units of the binary exponential: v log2(e) = rate s(rg).
+__device__ __forceinline__ float binary_rate(float scale, float decay) { return scale * kLog2e * softplus(decay); }
+
+// 1 - 2^-2u from u and a = 2^-u.  Below u = 1/4 / ln 2, where 1 - a^2 would cancel, u times a fourth
+// degree polynomial fitted to (1 - 2^-2u) / u there at Chebyshev points (8.4e-8 relative).
+__device__ __forceinline__ float one_minus_square(float u, float a) {
+  const float s =
+      u * (1.3862942457f + u * (-0.9608914256f + u * (0.4437149763f + u * (-0.1514232010f + u * 0.0346555375f))));
+  return u < 0.25f / kLn2 ? s : 1.0f - a * a;
 }
 
 struct Step {
-  float si, sr, v, a, m, rm;  // rm = 1 / m, kept finite where v is 0
+  float si, sr, a, m;
 };
 
+// `rate` from binary_rate().
 __device__ __forceinline__ Step gates(float ig, float rg, float rate, bool reset) {
   Step s;
   s.si = sigmoid(ig);
   s.sr = sigmoid(rg);
-  s.v = rate * s.sr;
-  s.a = fast_exp(-s.v);
-  const float om = one_minus_square(s.v, s.a);
-  s.rm = __builtin_amdgcn_rsqf(fmaxf(om, 1e-37f));
-  s.m = om * s.rm;
+  const float u = rate * s.sr;
+  s.a = fast_exp2(-u);
+  s.m = __builtin_amdgcn_sqrtf(one_minus_square(u, s.a));
   if (reset) {  // nothing of the decay gate is used, a NaN in it included
-    s.a = s.v = s.sr = 0.0f;
+    s.a = s.sr = 0.0f;
     s.m = 1.0f;
   }
   return s;
@@ -79,31 +85,52 @@ struct Raw {
   uint32_t w[sizeof(T) == 4 ? V : 1];
 };
 
-// Where a lane's channels are: `d` the first, `full` if the whole strip is inside the tensor.
+// Where a lane's channels are.  What is the same for a wave (the strip's first channel, a row's
+// address) stays apart from the lane's 32-bit offset, so that an access needs one register for its
+// address instead of two.
+template <bool FULL>
 struct Place {
-  int64_t d, channels;
-  bool full;
-  __device__ __forceinline__ int64_t at(int e) const { return min(d + e, channels - 1); }  // a channel to read
-  __device__ __forceinline__ bool has(int e) const { return d + e < channels; }
+  int64_t first;   // of the strip
+  uint32_t off;    // of the lane's first channel in the strip
+  uint32_t count;  // channels of the strip; FULL: 64 V in every one
+  __device__ __forceinline__ uint32_t at(int e) const { return FULL ? off + e : min(off + e, count - 1); }  // to read
+  __device__ __forceinline__ bool has(int e) const { return FULL || off + e < count; }
 };
 
-template <typename T, int V>
-__device__ __forceinline__ Raw<T, V> load(const T* row, const Place& c) {
+template <int V, bool FULL>
+__device__ __forceinline__ Place<FULL> place(int64_t strip, int64_t channels, int lane) {
+  const int64_t first = strip * 64 * V;
+  const uint32_t count = static_cast<uint32_t>(min(static_cast<int64_t>(64 * V), channels - first));
+  return Place<FULL>{first, static_cast<uint32_t>(lane * V), count};
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t bits_at(const T* row, uint32_t i) {
+  const T v = *at_bytes(row, i * static_cast<uint32_t>(sizeof(T)));
+  if constexpr (sizeof(T) == 4)
+    return __builtin_bit_cast(uint32_t, v);
+  else
+    return __builtin_bit_cast(uint16_t, v);
+}
+
+// A row's values of a lane; `row` is the same for the wave.
+template <typename T, int V, bool FULL>
+__device__ __forceinline__ Raw<T, V> load(const T* row, const Place<FULL>& c) {
   struct __attribute__((packed)) Any {
     Raw<T, V> r;
   };
+  const T* p = row + c.first;
   Raw<T, V> r;
   if constexpr (sizeof(T) == 2 && V == 1) {
-    r.w[0] = __builtin_bit_cast(uint16_t, row[c.at(0)]);
+    r.w[0] = bits_at(p, c.at(0));
   } else {
-    if (c.full) {
-      r = reinterpret_cast<const Any*>(row + c.d)->r;
+    if constexpr (FULL) {
+      r = reinterpret_cast<const Any*>(at_bytes(p, c.off * static_cast<uint32_t>(sizeof(T))))->r;
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) r.w[e] = __builtin_bit_cast(uint32_t, row[c.at(e)]);
+      for (int e = 0; e < V; ++e) r.w[e] = bits_at(p, c.at(e));
     } else {
-      r.w[0] = __builtin_bit_cast(uint16_t, row[c.at(0)]) |
-               static_cast<uint32_t>(__builtin_bit_cast(uint16_t, row[c.at(1)])) << 16;
+      r.w[0] = bits_at(p, c.at(0)) | bits_at(p, c.at(1)) << 16;
     }
   }
   return r;
@@ -122,9 +149,9 @@ __device__ __forceinline__ void unpack(const Raw<T, V>& r, float (&f)[V]) {
   }
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void store(T* row, const Place& c, const float (&f)[V]) {
-  if (V == 2 && c.full) {
+template <typename T, int V, bool FULL>
+__device__ __forceinline__ void store(T* row, const Place<FULL>& c, const float (&f)[V]) {
+  if constexpr (V == 2 && FULL) {
     struct __attribute__((packed)) Any {
       Raw<T, V> r;
     } o;
@@ -134,11 +161,23 @@ __device__ __forceinline__ void store(T* row, const Place& c, const float (&f)[V
     } else {
       o.r.w[0] = pack2<T>(f[0], f[V - 1]);
     }
-    *reinterpret_cast<Any*>(row + c.d) = o;
+    *reinterpret_cast<Any*>(at_bytes(row + c.first, c.off * static_cast<uint32_t>(sizeof(T)))) = o;
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      if (c.has(e)) row[c.d + e] = from_f32<T>(f[e]);
+      if (c.has(e)) *at_bytes(row + c.first, (c.off + e) * static_cast<uint32_t>(sizeof(T))) = from_f32<T>(f[e]);
+  }
+}
+
+// The NT rows of a wave's run, from row t0 of a sequence on; past its end (unless WHOLE) the last again.
+template <typename T, int NT, int V, bool WHOLE, bool FULL>
+__device__ __forceinline__ void load_run(const void* p, int64_t sequence, int64_t stride, int64_t t0, int64_t length,
+                                         const Place<FULL>& c, Raw<T, V> (&r)[NT]) {
+  const T* row = static_cast<const T*>(p) + sequence + (WHOLE ? t0 : min(t0, length - 1)) * stride;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    r[t] = load<T, V>(row, c);
+    if (WHOLE || t0 + t + 1 < length) row += stride;
   }
 }
 
@@ -163,7 +202,7 @@ __device__ __forceinline__ uint32_t reset_bits(const mko_recur_params& p, int64_
 // already and that waits in turn only for earlier ones, so every wait ends.
 
 constexpr uint32_t kAbsent = 0xffffffffu;
-constexpr int kWindow = 8;            // chunks looked at in one round trip
+constexpr int kWindow = 4;            // chunks looked at in one round trip
 constexpr int kMostRounds = 1 << 22;  // seconds; a wait cut short shows as NaN
 
 // v with a NaN in the one form that is not kAbsent.
@@ -174,8 +213,9 @@ __device__ __forceinline__ uint32_t publishable(float v) {
 struct Chain {
   uint64_t* maps;   // (batch, chunks, channels): P in the high word, H in the low
   uint32_t* ends;   // (batch, chunks, channels): the value that leaves the chunk
-  uint32_t* ticket;
+  uint32_t* tickets;  // up to kCounters counters, kCounterGap words apart
 };
+constexpr int kCounters = kXcds, kCounterGap = 32;
 
 __device__ __forceinline__ void publish_map(uint64_t* cell, float P, float H) {
   __hip_atomic_store(cell, static_cast<uint64_t>(publishable(P)) << 32 | __float_as_uint(H), __ATOMIC_RELAXED,
@@ -185,21 +225,21 @@ __device__ __forceinline__ void publish_end(uint32_t* cell, float h) {
   __hip_atomic_store(cell, publishable(h), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The value that enters a chunk at channel d, for a whole wave: `before` chunks of the chain lie
-// before it, the nearest in row `cell` of the cells, the others `step` rows apart; `start` enters
-// the first of them.
+// The value that enters a chunk, for a whole wave; the lane's channel is `off` channels into the
+// strip, whose first is `first`.  `before` chunks of the chain lie before it, the nearest in row
+// `cell` of the cells, the others `step` rows apart; `start` enters the first of them.
 template <bool RESET>
-__device__ __forceinline__ float enter(const Chain& ch, int64_t channels, int64_t d, int64_t cell, int64_t step,
-                                       int64_t before, float start) {
+__device__ __forceinline__ float enter(const Chain& ch, int64_t channels, int64_t first, uint32_t off, int64_t cell,
+                                       int step, int before, float start) {
   if (before == 0) return start;
   for (int round = 0; round < kMostRounds; ++round) {
     uint32_t end[kWindow];
     uint64_t map[kWindow];
 #pragma unroll
     for (int k = 0; k < kWindow; ++k) {
-      const int64_t at = (cell + (k < before ? k : 0) * step) * channels + d;
-      end[k] = __hip_atomic_load(ch.ends + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      map[k] = __hip_atomic_load(ch.maps + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int64_t row = (cell + (k < before ? k : 0) * step) * channels + first;
+      end[k] = __hip_atomic_load(at_bytes(ch.ends + row, off * 4), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      map[k] = __hip_atomic_load(at_bytes(ch.maps + row, off * 8), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     // the nearest end that is there, with every map nearer than it
     int found = -1;
@@ -228,15 +268,14 @@ __device__ __forceinline__ float enter(const Chain& ch, int64_t channels, int64_
   return __uint_as_float(0x7fc00000u);
 }
 
-// A chunk's part in the chain, for a wave whose lanes have one channel each (channel d of the tensor,
-// i of the strip): joins its waves' maps, in the order of the chain, finds what enters the chunk and
-// leaves it in `entered`.  Returns what leaves the chunk.
+// A chunk's part in the chain, for a wave whose lanes have channel i of the strip each: joins its
+// waves' maps, in the order of the chain, finds what enters the chunk and leaves it in `entered`.
+// Returns what leaves the chunk.
 template <int NW, int V, bool RESET, bool BACK>
 __device__ __forceinline__ float join(const Chain& ch, const float (&P)[NW][64 * V], const float (&R)[NW][64 * V],
-                                      float* entered, int64_t channels, int64_t d, int i, int64_t cell, int64_t before,
-                                      int64_t after, float start) {
+                                      float* entered, int64_t channels, int64_t first, uint32_t count, int i,
+                                      int64_t cell, int before, int after, float start) {
   constexpr int kFirst = BACK ? NW - 1 : 0, kStep = BACK ? -1 : 1;
-  const int64_t at = min(d, channels - 1);
   float Pc = P[kFirst][i], Rc = R[kFirst][i];
 #pragma unroll
   for (int w = 1; w < NW; ++w) {
@@ -244,83 +283,99 @@ __device__ __forceinline__ float join(const Chain& ch, const float (&P)[NW][64 *
     Rc = apply<RESET>(Pw, R[kFirst + w * kStep][i], Rc);
     Pc = both<RESET>(Pc, Pw);
   }
-  if (before > 0 && after > 0 && d < channels) publish_map(ch.maps + cell * channels + d, Pc, Rc);
-  const float in = enter<RESET>(ch, channels, at, cell - kStep, -kStep, before, start);
+  const uint32_t off = static_cast<uint32_t>(i);
+  if (before > 0 && after > 0 && off < count)
+    publish_map(at_bytes(ch.maps + cell * channels + first, off * 8), Pc, Rc);
+  const float in = enter<RESET>(ch, channels, first, min(off, count - 1), cell - kStep, -kStep, before, start);
   entered[i] = in;
   return apply<RESET>(Pc, Rc, in);
 }
 
-// Marks two runs of cells absent and starts the counter.
-__global__ void __launch_bounds__(kThreads) clear(uint4* a, int64_t na, uint4* b, int64_t nb, uint32_t* ticket) {
+// Marks two runs of cells absent and starts the counters.
+__global__ void __launch_bounds__(kThreads) clear(uint4* a, int64_t na, uint4* b, int64_t nb, uint32_t* tickets) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const uint4 none = make_uint4(kAbsent, kAbsent, kAbsent, kAbsent);
   if (i < na) a[i] = none;
   if (i < nb) b[i] = none;
-  if (i == 0) *ticket = 0;
+  if (i < kCounters) tickets[i * kCounterGap] = 0;
 }
 
 struct Geo {
-  int64_t chunks, strips, chains;  // chains = batch * strips
+  int chunks, strips, chains;  // chains = batch * strips
+  int counters;
 };
 
-// This workgroup's place in the order: the chunk of a chain, counted from the end that is first.
-__device__ __forceinline__ int64_t take(const Geo& g, uint32_t* ticket, uint32_t* slot) {
-  if (g.chunks == 1) return blockIdx.x;
-  if (threadIdx.x == 0) *slot = atomicAdd(ticket, 1u);
-  __syncthreads();
-  return *slot;
+// This workgroup's chunk, counted from the end that is first, and its chain, the same for the wave;
+// false if there is none for it.  With several counters the chains are dealt to them: workgroup w
+// draws from counter w mod `counters`, one for each XCD, so that a chain stays with an XCD.
+__device__ __forceinline__ bool take(const Geo& g, uint32_t* tickets, uint32_t* slot, int& chunk, int& chain) {
+  const int counter = static_cast<int>(blockIdx.x) % g.counters;
+  const int mine = (g.chains + g.counters - 1 - counter) / g.counters;  // chains of this counter
+  int turn = static_cast<int>(blockIdx.x) / g.counters;
+  if (turn >= mine * g.chunks) return false;
+  if (g.chunks > 1) {
+    if (threadIdx.x == 0) *slot = atomicAdd(tickets + counter * kCounterGap, 1u);
+    __syncthreads();
+    turn = uniform(static_cast<int>(*slot));
+  }
+  chunk = turn / mine;
+  chain = (turn - chunk * mine) * g.counters + counter;
+  return true;
 }
 
 // ---------------------------------------------------------------- forward
 
-template <typename T, int NW, int NT, int V, bool RESET>
+template <typename T, int NW, int NT, int V, bool RESET, bool FULL>
 __global__ void __launch_bounds__(NW * 64) forward(mko_recur_params p, Geo g, Chain ch) {
   static_assert(NW * NT == kChunk, "a workgroup takes a chunk");
   __shared__ float runs[2][NW][64 * V], entered[64 * V];
   __shared__ uint32_t slot;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t turn = take(g, ch.ticket, &slot);
-  const int64_t chunk = turn / g.chains, chain = turn - chunk * g.chains;
-  const int64_t b = chain / g.strips, strip = chain - b * g.strips;
-  const Place c{strip * 64 * V + lane * V, p.channels, (strip + 1) * 64 * V <= p.channels};
-  const int64_t t0 = chunk * kChunk + wave * NT;
+  int chunk, chain;
+  if (!take(g, ch.tickets, &slot, chunk, chain)) return;
+  const int64_t b = chain / g.strips, strip = chain % g.strips;
+  const Place<FULL> c = place<V, FULL>(strip, p.channels, lane);
+  const int64_t t0 = static_cast<int64_t>(chunk) * kChunk + wave * NT;
   const int steps = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(NT), p.length - t0)));
-
-  Raw<T, V> xr[NT], ir[NT], rr[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t at = min(t0 + t, p.length - 1);
-    xr[t] = load<T, V>(static_cast<const T*>(p.x) + b * p.x_stride_b + at * p.x_stride_t, c);
-    ir[t] = load<T, V>(static_cast<const T*>(p.input_gate) + b * p.ig_stride_b + at * p.ig_stride_t, c);
-    rr[t] = load<T, V>(static_cast<const T*>(p.decay_gate) + b * p.rg_stride_b + at * p.rg_stride_t, c);
-  }
-  const uint32_t cuts = reset_bits<RESET, NT>(p, b, t0, lane);
-  float rate[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) rate[e] = p.scale * softplus(p.decay[c.at(e)]);
 
   // the run from a zero state: h = H[t], and P[t] of the state before it
   float H[NT][V], P[NT][V];
+  auto form = [&](auto whole) {  // whole: no step of the run is past the end
+    constexpr bool WHOLE = decltype(whole)::value;
+    Raw<T, V> xr[NT], ir[NT], rr[NT];
+    load_run<T, NT, V, WHOLE>(p.x, b * p.x_stride_b, p.x_stride_t, t0, p.length, c, xr);
+    load_run<T, NT, V, WHOLE>(p.input_gate, b * p.ig_stride_b, p.ig_stride_t, t0, p.length, c, ir);
+    load_run<T, NT, V, WHOLE>(p.decay_gate, b * p.rg_stride_b, p.rg_stride_t, t0, p.length, c, rr);
+    const uint32_t cuts = reset_bits<RESET, NT>(p, b, t0, lane);
+    float rate[V];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float x[V], ig[V], rg[V];
-    unpack<T, V>(xr[t], x);
-    unpack<T, V>(ir[t], ig);
-    unpack<T, V>(rr[t], rg);
-    const bool cut = RESET && (cuts >> t & 1);
+    for (int e = 0; e < V; ++e) rate[e] = binary_rate(p.scale, p.decay[c.first + c.at(e)]);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const Step s = gates(ig[e], rg[e], rate[e], cut);
-      const float u = s.m * s.si * x[e];
-      const float before = t ? P[t - 1][e] : 1.0f;
-      H[t][e] = (t == 0 || cut ? 0.0f : s.a * H[t - 1][e]) + u;
-      P[t][e] = cut ? __uint_as_float(kDropped) : s.a * before;
-      if (t >= steps) {  // past the end the state stays
-        H[t][e] = t ? H[t - 1][e] : 0.0f;
-        P[t][e] = before;
+    for (int t = 0; t < NT; ++t) {
+      float x[V], ig[V], rg[V];
+      unpack<T, V>(xr[t], x);
+      unpack<T, V>(ir[t], ig);
+      unpack<T, V>(rr[t], rg);
+      const bool cut = RESET && (cuts >> t & 1);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const Step s = gates(ig[e], rg[e], rate[e], cut);
+        const float u = s.m * s.si * x[e];
+        const float before = t ? P[t ? t - 1 : 0][e] : 1.0f;
+        const float h = t ? H[t ? t - 1 : 0][e] : 0.0f;
+        H[t][e] = (t == 0 || cut ? 0.0f : s.a * h) + u;
+        P[t][e] = cut ? __uint_as_float(kDropped) : s.a * before;
+        if (!WHOLE && t >= steps) {  // past the end the state stays
+          H[t][e] = h;
+          P[t][e] = before;
+        }
       }
     }
-  }
+  };
+  if (steps == NT)
+    form(std::true_type{});
+  else
+    form(std::false_type{});
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     runs[0][wave][lane * V + e] = P[NT - 1][e];
@@ -330,13 +385,14 @@ __global__ void __launch_bounds__(NW * 64) forward(mko_recur_params p, Geo g, Ch
 
   if (wave < V) {
     const int i = wave * 64 + lane;
-    const int64_t d = strip * 64 * V + i, cell = b * g.chunks + chunk;
-    const float start = p.initial ? p.initial[b * p.channels + min(d, p.channels - 1)] : 0.0f;
-    const float h = join<NW, V, RESET, false>(ch, runs[0], runs[1], entered, p.channels, d, i, cell, chunk,
+    const int64_t cell = b * g.chunks + chunk;
+    const uint32_t off = static_cast<uint32_t>(i);
+    const float start = p.initial ? p.initial[b * p.channels + c.first + min(off, c.count - 1)] : 0.0f;
+    const float h = join<NW, V, RESET, false>(ch, runs[0], runs[1], entered, p.channels, c.first, c.count, i, cell, chunk,
                                               g.chunks - 1 - chunk, start);
-    if (d < p.channels) {
-      publish_end(ch.ends + cell * p.channels + d, h);
-      if (p.final_state && chunk + 1 == g.chunks) p.final_state[b * p.channels + d] = h;
+    if (off < c.count) {
+      publish_end(at_bytes(ch.ends + cell * p.channels + c.first, off * 4), h);
+      if (p.final_state && chunk + 1 == g.chunks) p.final_state[b * p.channels + c.first + i] = h;
     }
   }
   __syncthreads();
@@ -363,73 +419,73 @@ __global__ void __launch_bounds__(NW * 64) forward(mko_recur_params p, Geo g, Ch
 // flows from a step to the one before it, a[t] g[t], has the forward's maps in the other direction,
 // and its chunks are joined from the last to the first.
 
-template <typename T, int NW, int NT, int V, bool RESET>
-__global__ void __launch_bounds__(NW * 64) backward(mko_recur_params p, Geo g, Chain ch, float* part) {
+template <typename T, int NW, int NT, int V, bool RESET, bool FULL>
+__global__ void __launch_bounds__(NW * 64, 4) backward(mko_recur_params p, Geo g, Chain ch, float* part) {
   static_assert(NW * NT == kChunk, "a workgroup takes a chunk");
   __shared__ float runs[3][NW][64 * V], entered[64 * V];
   __shared__ uint32_t slot;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t turn = take(g, ch.ticket, &slot);
-  const int64_t behind = turn / g.chains, chain = turn - behind * g.chains;
-  const int64_t chunk = g.chunks - 1 - behind;
-  const int64_t b = chain / g.strips, strip = chain - b * g.strips;
-  const Place c{strip * 64 * V + lane * V, p.channels, (strip + 1) * 64 * V <= p.channels};
-  const int64_t t0 = chunk * kChunk + wave * NT;
+  int behind, chain;
+  if (!take(g, ch.tickets, &slot, behind, chain)) return;
+  const int chunk = g.chunks - 1 - behind;
+  const int64_t b = chain / g.strips, strip = chain % g.strips;
+  const Place<FULL> c = place<V, FULL>(strip, p.channels, lane);
+  const int64_t t0 = static_cast<int64_t>(chunk) * kChunk + wave * NT;
   const int steps = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(NT), p.length - t0)));
 
-  Raw<T, V> xr[NT], ir[NT], rr[NT], gr[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t at = min(t0 + t, p.length - 1);
-    xr[t] = load<T, V>(static_cast<const T*>(p.x) + b * p.x_stride_b + at * p.x_stride_t, c);
-    ir[t] = load<T, V>(static_cast<const T*>(p.input_gate) + b * p.ig_stride_b + at * p.ig_stride_t, c);
-    rr[t] = load<T, V>(static_cast<const T*>(p.decay_gate) + b * p.rg_stride_b + at * p.rg_stride_t, c);
-    gr[t] = load<T, V>(static_cast<const T*>(p.dy) + (b * p.length + at) * p.channels, c);
-  }
-  const uint32_t cuts = reset_bits<RESET, NT>(p, b, t0, lane);
+  Raw<T, V> xr[NT], gr[NT];
   float rate[V], first[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    rate[e] = p.scale * softplus(p.decay[c.at(e)]);
-    first[e] = chunk ? p.states[(b * g.chunks + chunk - 1) * p.channels + c.at(e)]
-                     : (p.initial ? p.initial[b * p.channels + c.at(e)] : 0.0f);
-  }
-
   float si[NT][V], sr[NT][V], a[NT][V], m[NT][V];
   float P[V], H[V], G[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    P[e] = 1.0f;
-    H[e] = G[e] = 0.0f;
-  }
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float x[V], ig[V], rg[V];
-    unpack<T, V>(xr[t], x);
-    unpack<T, V>(ir[t], ig);
-    unpack<T, V>(rr[t], rg);
-    const bool cut = RESET && (cuts >> t & 1);
+  auto form = [&](auto whole) {  // whole: no step of the run is past the end
+    constexpr bool WHOLE = decltype(whole)::value;
+    Raw<T, V> ir[NT], rr[NT];
+    load_run<T, NT, V, WHOLE>(p.decay_gate, b * p.rg_stride_b, p.rg_stride_t, t0, p.length, c, rr);
+    load_run<T, NT, V, WHOLE>(p.input_gate, b * p.ig_stride_b, p.ig_stride_t, t0, p.length, c, ir);
+    load_run<T, NT, V, WHOLE>(p.x, b * p.x_stride_b, p.x_stride_t, t0, p.length, c, xr);
+    load_run<T, NT, V, WHOLE>(p.dy, b * p.length * p.channels, p.channels, t0, p.length, c, gr);
+    const uint32_t cuts = reset_bits<RESET, NT>(p, b, t0, lane);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const Step s = gates(ig[e], rg[e], rate[e], cut);
-      si[t][e] = s.si;
-      sr[t][e] = s.sr;
-      a[t][e] = cut ? __uint_as_float(kDropped) : s.a;
-      m[t][e] = s.m;
-      if (t < steps) {
-        H[e] = (cut ? 0.0f : s.a * H[e]) + s.m * s.si * x[e];
-        P[e] = cut ? __uint_as_float(kDropped) : s.a * P[e];
+      rate[e] = binary_rate(p.scale, p.decay[c.first + c.at(e)]);
+      first[e] = chunk ? p.states[(b * g.chunks + chunk - 1) * p.channels + c.first + c.at(e)]
+                       : (p.initial ? p.initial[b * p.channels + c.first + c.at(e)] : 0.0f);
+      P[e] = 1.0f;
+      H[e] = G[e] = 0.0f;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float x[V], ig[V], rg[V];
+      unpack<T, V>(xr[t], x);
+      unpack<T, V>(ir[t], ig);
+      unpack<T, V>(rr[t], rg);
+      const bool cut = RESET && (cuts >> t & 1);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const Step s = gates(ig[e], rg[e], rate[e], cut);
+        si[t][e] = s.si;
+        sr[t][e] = s.sr;
+        a[t][e] = cut ? __uint_as_float(kDropped) : s.a;
+        m[t][e] = s.m;
+        if (WHOLE || t < steps) {
+          H[e] = (cut ? 0.0f : s.a * H[e]) + s.m * s.si * x[e];
+          P[e] = cut ? __uint_as_float(kDropped) : s.a * P[e];
+        }
       }
     }
-  }
 #pragma unroll
-  for (int t = NT - 1; t >= 0; --t) {
-    if (t >= steps) continue;
-    float dy[V];
-    unpack<T, V>(gr[t], dy);
+    for (int t = NT - 1; t >= 0; --t) {
+      if (!WHOLE && t >= steps) continue;
+      float dy[V];
+      unpack<T, V>(gr[t], dy);
 #pragma unroll
-    for (int e = 0; e < V; ++e) G[e] = apply<RESET>(a[t][e], 0.0f, G[e] + dy[e]);
-  }
+      for (int e = 0; e < V; ++e) G[e] = apply<RESET>(a[t][e], 0.0f, G[e] + dy[e]);
+    }
+  };
+  if (steps == NT)
+    form(std::true_type{});
+  else
+    form(std::false_type{});
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     runs[0][wave][lane * V + e] = P[e];
@@ -440,18 +496,35 @@ __global__ void __launch_bounds__(NW * 64) backward(mko_recur_params p, Geo g, C
 
   if (wave < V) {
     const int i = wave * 64 + lane;
-    const int64_t d = strip * 64 * V + i, cell = b * g.chunks + chunk;
-    const float start = p.dfinal ? p.dfinal[b * p.channels + min(d, p.channels - 1)] : 0.0f;
-    const float out = join<NW, V, RESET, true>(ch, runs[0], runs[2], entered, p.channels, d, i, cell, behind, chunk, start);
-    if (d < p.channels) {
+    const int64_t cell = b * g.chunks + chunk;
+    const uint32_t off = static_cast<uint32_t>(i);
+    const float start = p.dfinal ? p.dfinal[b * p.channels + c.first + min(off, c.count - 1)] : 0.0f;
+    const float out = join<NW, V, RESET, true>(ch, runs[0], runs[2], entered, p.channels, c.first, c.count, i, cell,
+                                               behind, chunk, start);
+    if (off < c.count) {
       if (chunk > 0)
-        publish_end(ch.ends + cell * p.channels + d, out);
+        publish_end(at_bytes(ch.ends + cell * p.channels + c.first, off * 4), out);
       else if (p.dinitial)
-        p.dinitial[b * p.channels + d] = out;
+        p.dinitial[b * p.channels + c.first + i] = out;
     }
   }
   __syncthreads();
 
+  // From here on these are new to the compiler: carried along, the terms it formed of them above
+  // would take more registers than it takes to form them again.
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (uint32_t& w : xr[t].w) w = opaque(w);
+#pragma unroll
+    for (uint32_t& w : gr[t].w) w = opaque(w);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      m[t][e] = fp32_value(m[t][e]);
+      si[t][e] = fp32_value(si[t][e]);
+      sr[t][e] = fp32_value(sr[t][e]);
+    }
+  }
   float h[NT][V], flow[V], sum[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -465,6 +538,7 @@ __global__ void __launch_bounds__(NW * 64) backward(mko_recur_params p, Geo g, C
   }
 #pragma unroll
   for (int t = 0; t + 1 < NT; ++t) {
+    __builtin_amdgcn_sched_barrier(0);
     float x[V];
     unpack<T, V>(xr[t], x);
 #pragma unroll
@@ -472,6 +546,7 @@ __global__ void __launch_bounds__(NW * 64) backward(mko_recur_params p, Geo g, C
   }
 #pragma unroll
   for (int t = NT - 1; t >= 0; --t) {
+    __builtin_amdgcn_sched_barrier(0);  // a step at a time: formed ahead, the steps' terms would not fit the registers
     if (t >= steps) continue;
     float x[V], dy[V], dx[V], dig[V], drg[V];
     unpack<T, V>(xr[t], x);
@@ -486,7 +561,7 @@ __global__ void __launch_bounds__(NW * 64) backward(mko_recur_params p, Geo g, C
       if (drops<RESET>(a[t][e])) dv = 0.0f;
       dx[e] = gm * si[t][e];
       dig[e] = gm * u * (1.0f - si[t][e]);
-      drg[e] = dv * (rate[e] * sr[t][e]) * (1.0f - sr[t][e]);
+      drg[e] = dv * (rate[e] * kLn2 * sr[t][e]) * (1.0f - sr[t][e]);
       sum[e] += dv * sr[t][e];
       flow[e] = drops<RESET>(a[t][e]) ? 0.0f : a[t][e] * gt;
     }
@@ -505,7 +580,7 @@ __global__ void __launch_bounds__(NW * 64) backward(mko_recur_params p, Geo g, C
     for (int e = 0; e < V; ++e) {
       float s = 0.0f;
       for (int w = 0; w < NW; ++w) s += runs[0][w][lane * V + e];
-      if (c.has(e)) part[(b * g.chunks + chunk) * p.channels + c.d + e] = s;
+      if (c.has(e)) part[(b * g.chunks + chunk) * p.channels + c.first + c.off + e] = s;
     }
   }
 }
@@ -522,7 +597,7 @@ __global__ void __launch_bounds__(kThreads) update(mko_recur_update_params p) {
   const int64_t d = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t b = blockIdx.y;
   if (d >= p.channels) return;
-  const float rate = p.scale * softplus(p.decay[d]);
+  const float rate = binary_rate(p.scale, p.decay[d]);
   const float x = to_f32(static_cast<const T*>(p.x)[b * p.x_stride + d]);
   const float ig = to_f32(static_cast<const T*>(p.input_gate)[b * p.ig_stride + d]);
   const float rg = to_f32(static_cast<const T*>(p.decay_gate)[b * p.rg_stride + d]);
@@ -547,9 +622,10 @@ int check(const mko_recur_params* p, const char* what) {
     mko_set_error("%s: dtype must be float32, float16 or bfloat16", what);
     return MKO_EINVAL;
   }
-  // a workgroup a chunk and strip, at most 512 threads each
-  if (p->batch > 65535 || cdiv(p->length, kChunk) * cdiv(p->channels, 64) >= (1 << 23) / (p->batch ? p->batch : 1)) {
-    mko_set_error("%s: batch is at most 65535, and batch * length * channels below 2^35", what);
+  if (p->batch > kMostBatch || p->channels > kMostSide || p->length > kMostSide ||
+      cdiv(p->batch * cdiv(p->channels, 64 * kV), kCounters) * kCounters * cdiv(p->length, kChunk) > kMostWorkgroups) {
+    mko_set_error("%s: batch is at most 65535, and batch * channels / 128, up to the next multiple of 8, times "
+                  "length / 64 at most 2^22", what);
     return MKO_EUNSUPPORTED;
   }
   return MKO_OK;
@@ -557,20 +633,22 @@ int check(const mko_recur_params* p, const char* what) {
 
 bool empty(const mko_recur_params* p) { return p->batch == 0 || p->length == 0 || p->channels == 0; }
 
-constexpr int kV = 2;  // channels a lane takes
-
 Geo geo(const mko_recur_params* p) {
-  Geo g;
-  g.chunks = cdiv(p->length, kChunk);
-  g.strips = cdiv(p->channels, 64 * kV);
-  g.chains = p->batch * g.strips;
+  Geo g;  // check() keeps the products below 2^23
+  g.chunks = static_cast<int>(cdiv(p->length, kChunk));
+  g.strips = static_cast<int>(cdiv(p->channels, 64 * kV));
+  g.chains = static_cast<int>(p->batch) * g.strips;
+  // Eight counters where they share the chains within an eighth: 36 chains of 16 chunks 26 -> 21 us.
+  // 20 chains of 512 chunks, three on some XCDs and two on others, 173 us with one counter and 206
+  // with eight.
+  g.counters = cdiv(g.chains, kCounters) * kCounters * 8 <= 9 * g.chains ? kCounters : 1;
   return g;
 }
 
 int64_t cells(const mko_recur_params* p) { return p->batch * cdiv(p->length, kChunk) * p->channels; }
+constexpr int64_t kTicketBytes = kCounters * kCounterGap * 4;
 int64_t aligned(int64_t n) { return cdiv(n, 16) * 16; }
 
-// maps, then the counter in 16 bytes of its own; the backward's ends and partial sums after them
 int64_t maps_bytes(const mko_recur_params* p) { return aligned(cells(p) * 8); }
 int64_t ends_bytes(const mko_recur_params* p) { return aligned(cells(p) * 4); }
 
@@ -579,27 +657,44 @@ void clear_cells(const mko_recur_params* p, const Chain& ch, hipStream_t s) {
   const int64_t maps = maps_bytes(p) / 16, ends = ends_bytes(p) / 16;
   MKO_TIMED("recur_clear", s,
             clear<<<static_cast<unsigned>(cdiv(maps, kThreads)), kThreads, 0, s>>>(
-                reinterpret_cast<uint4*>(ch.maps), maps, reinterpret_cast<uint4*>(ch.ends), ends, ch.ticket));
+                reinterpret_cast<uint4*>(ch.maps), maps, reinterpret_cast<uint4*>(ch.ends), ends, ch.tickets));
 }
 
-template <typename T>
+unsigned workgroups(const Geo& g) {
+  return static_cast<unsigned>(cdiv(g.chains, g.counters) * g.counters * g.chunks);
+}
+
+constexpr int kFwdSteps = 8, kBwdSteps = 8;  // steps of a wave
+
+template <typename T, bool RESET, bool FULL>
 void launch_fwd(const mko_recur_params& p, const Geo& g, const Chain& ch, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(g.chunks * g.chains);
-  constexpr int kNw = kChunk / 16;
-  if (p.reset)
-    MKO_TIMED("recur_fwd", s, forward<T, kNw, 16, kV, true><<<grid, kNw * 64, 0, s>>>(p, g, ch));
-  else
-    MKO_TIMED("recur_fwd", s, forward<T, kNw, 16, kV, false><<<grid, kNw * 64, 0, s>>>(p, g, ch));
+  const unsigned grid = workgroups(g);
+  constexpr int kNw = kChunk / kFwdSteps;
+  MKO_TIMED("recur_fwd", s, forward<T, kNw, kFwdSteps, kV, RESET, FULL><<<grid, kNw * 64, 0, s>>>(p, g, ch));
 }
 
-template <typename T>
+template <typename T, bool RESET, bool FULL>
 void launch_bwd(const mko_recur_params& p, const Geo& g, const Chain& ch, float* part, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(g.chunks * g.chains);
-  constexpr int kNw = kChunk / 8;
-  if (p.reset)
-    MKO_TIMED("recur_bwd", s, backward<T, kNw, 8, kV, true><<<grid, kNw * 64, 0, s>>>(p, g, ch, part));
-  else
-    MKO_TIMED("recur_bwd", s, backward<T, kNw, 8, kV, false><<<grid, kNw * 64, 0, s>>>(p, g, ch, part));
+  const unsigned grid = workgroups(g);
+  constexpr int kNw = kChunk / kBwdSteps;
+  MKO_TIMED("recur_bwd", s, backward<T, kNw, kBwdSteps, kV, RESET, FULL><<<grid, kNw * 64, 0, s>>>(p, g, ch, part));
+}
+
+// The kernels of a dtype, with or without resets, for whole strips or ragged ones.
+template <typename T>
+void launch(const mko_recur_params& p, const Geo& g, const Chain& ch, float* part, bool back, hipStream_t s) {
+  const bool full = p.channels % (64 * kV) == 0;
+  if (back) {
+    if (p.reset)
+      full ? launch_bwd<T, true, true>(p, g, ch, part, s) : launch_bwd<T, true, false>(p, g, ch, part, s);
+    else
+      full ? launch_bwd<T, false, true>(p, g, ch, part, s) : launch_bwd<T, false, false>(p, g, ch, part, s);
+  } else {
+    if (p.reset)
+      full ? launch_fwd<T, true, true>(p, g, ch, s) : launch_fwd<T, true, false>(p, g, ch, s);
+    else
+      full ? launch_fwd<T, false, true>(p, g, ch, s) : launch_fwd<T, false, false>(p, g, ch, s);
+  }
 }
 
 }  // namespace
@@ -618,7 +713,7 @@ extern "C" size_t mko_recur_states_size(const mko_recur_params* p) {
 
 extern "C" size_t mko_recur_fwd_workspace_size(const mko_recur_params* p) {
   if (recur::check(p, "recur_fwd") != MKO_OK || recur::empty(p) || p->length <= recur::kChunk) return 0;
-  return static_cast<size_t>(recur::maps_bytes(p) + 16);
+  return static_cast<size_t>(recur::maps_bytes(p) + recur::kTicketBytes);
 }
 
 extern "C" int mko_recur_fwd(const mko_recur_params* p, void* stream) {
@@ -640,22 +735,22 @@ extern "C" int mko_recur_fwd(const mko_recur_params* p, void* stream) {
   ch.ends = reinterpret_cast<uint32_t*>(p->states);
   if (g.chunks > 1) {
     ch.maps = static_cast<uint64_t*>(p->workspace);
-    ch.ticket = reinterpret_cast<uint32_t*>(static_cast<char*>(p->workspace) + recur::maps_bytes(p));
+    ch.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(p->workspace) + recur::maps_bytes(p));
     recur::clear_cells(p, ch, s);
   }
   if (p->dtype == MKO_F32)
-    recur::launch_fwd<float>(*p, g, ch, s);
+    recur::launch<float>(*p, g, ch, nullptr, false, s);
   else if (p->dtype == MKO_BF16)
-    recur::launch_fwd<bf16>(*p, g, ch, s);
+    recur::launch<bf16>(*p, g, ch, nullptr, false, s);
   else
-    recur::launch_fwd<_Float16>(*p, g, ch, s);
+    recur::launch<_Float16>(*p, g, ch, nullptr, false, s);
   return mko_check_launch("recur_fwd");
 }
 
 extern "C" size_t mko_recur_bwd_workspace_size(const mko_recur_params* p) {
   if (recur::check(p, "recur_bwd") != MKO_OK || recur::empty(p)) return 0;
   const int64_t part = p->ddecay ? recur::ends_bytes(p) : 0;
-  const int64_t chain = p->length > recur::kChunk ? recur::maps_bytes(p) + recur::ends_bytes(p) + 16 : 0;
+  const int64_t chain = p->length > recur::kChunk ? recur::maps_bytes(p) + recur::ends_bytes(p) + recur::kTicketBytes : 0;
   return static_cast<size_t>(part + chain);
 }
 
@@ -682,15 +777,15 @@ extern "C" int mko_recur_bwd(const mko_recur_params* p, void* stream) {
   if (g.chunks > 1) {
     ch.maps = reinterpret_cast<uint64_t*>(ws);
     ch.ends = reinterpret_cast<uint32_t*>(ws + recur::maps_bytes(p));
-    ch.ticket = reinterpret_cast<uint32_t*>(ws + recur::maps_bytes(p) + recur::ends_bytes(p));
+    ch.tickets = reinterpret_cast<uint32_t*>(ws + recur::maps_bytes(p) + recur::ends_bytes(p));
     recur::clear_cells(p, ch, s);
   }
   if (p->dtype == MKO_F32)
-    recur::launch_bwd<float>(*p, g, ch, part, s);
+    recur::launch<float>(*p, g, ch, part, true, s);
   else if (p->dtype == MKO_BF16)
-    recur::launch_bwd<bf16>(*p, g, ch, part, s);
+    recur::launch<bf16>(*p, g, ch, part, true, s);
   else
-    recur::launch_bwd<_Float16>(*p, g, ch, part, s);
+    recur::launch<_Float16>(*p, g, ch, part, true, s);
   if (p->ddecay)
     MKO_TIMED("recur_bwd_finish", s,
               recur::finish<<<static_cast<unsigned>(recur::cdiv(p->channels, 32)), kColumnThreads, 0, s>>>(
