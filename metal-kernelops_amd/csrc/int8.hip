@@ -1,6 +1,8 @@
 // 8-bit integers for gfx950: quantisation of rows, and the matrix product
 //   out[m][n] = q_scale[m] w_scale[n] sum_k q[m][k] w[n][k] + bias[n]
 // with the sum in int32, exact for fewer than 2^17 terms of at most 2^14.
+#include <type_traits>
+
 #include "common.hpp"
 #include "io.hpp"
 #include "quantize.hpp"
@@ -256,7 +258,7 @@ __device__ __forceinline__ void wait_and_meet() {
 // tile's rows in LDS.  Rows start 256 / BK to a sweep of the banks, and 16-byte chunk c of row r
 // lies at position c ^ (r / (256 / BK)) of its row, which gives the 16 rows that a quarter wave
 // reads at one c 16 different groups of banks.
-template <int BN, int BM, int WN, int WM, int BK, int STAGES, bool DIRECT>
+template <int BN, int BM, int WN, int WM, int BK, int STAGES, bool SPLIT, bool DIRECT>
 __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, int tiles_n, int tiles_m) {
   constexpr int kWaves = WN * WM;
   constexpr int kTn = BN / WN / 32, kTm = BM / WM / 32;
@@ -306,22 +308,26 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
                                      (__attribute__((address_space(3))) uint32_t*)slot(st, j), 16, 0, 0);
   };
-  // The loads of stage kt; past the end those of a stage that is there, so that every step makes as
-  // many and the waits' counts hold.
-  auto issue = [&](int st, int kt) {
+  // Part `part` of the loads of stage kt; past the end those of a stage that is there, so that every
+  // step makes as many and the waits' counts hold.
+  auto issue = [&](int st, int kt, auto part) {
+    constexpr int kFrom = decltype(part)::value * kLoads / 3, kTo = (decltype(part)::value + 1) * kLoads / 3;
     if ((kt + 1) * BK <= inner || (kt >= nk && inner >= BK)) {
       const int k0 = kt < nk ? kt * BK : 0;
       const int8_t* wb = wbase + k0;
       const int8_t* qb = qbase + k0;
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) load_to(st, j, (j < kLn ? wb : qb) + off[DIRECT ? j : 0]);
+      for (int j = kFrom; j < kTo; ++j) load_to(st, j, (j < kLn ? wb : qb) + off[DIRECT ? j : 0]);
     } else {
       const int k0 = (nk - 1) * BK;
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j)
+      for (int j = kFrom; j < kTo; ++j)
         load_to(st, j, k0 + source_k(j) < inner ? (j < kLn ? wbase : qbase) + k0 + off[DIRECT ? j : 0] : zeros);
     }
   };
+  constexpr std::integral_constant<int, 0> part0;
+  constexpr std::integral_constant<int, 1> part1;
+  constexpr std::integral_constant<int, 2> part2;
   v4i held[DIRECT ? 1 : kLoads];
   auto fetch = [&](int kt) {
 #pragma unroll
@@ -369,11 +375,19 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
 
   // Operands are read one step ahead of their products, across the stages too: the last step's
   // are in registers when the waves meet, after which the stage just read is free and takes the
-  // loads of the stage STAGES further on.
+  // loads of the stage STAGES further on.  With SPLIT those are issued in three parts, a part to a
+  // step: a wave that issues all at once waits for the address unit, 27 cycles a load, and multiplies
+  // nothing.  Where several workgroups share a CU another one multiplies then, and the earlier
+  // loads are worth more: 128 x 128 tiles of 8192 x 8192 x 4096 take 347 us, split 389.
   if constexpr (DIRECT) {
 #pragma unroll
-    for (int st = 0; st < STAGES; ++st) issue(st, st);
-    wait_and_meet<(STAGES - 1) * kLoads>();
+    for (int st = 0; st < STAGES; ++st) {
+      issue(st, st, part0);
+      if (SPLIT && st + 1 == STAGES) break;
+      issue(st, st, part1);
+      issue(st, st, part2);
+    }
+    wait_and_meet<(STAGES - 2) * kLoads + (SPLIT ? kLoads / 3 : kLoads)>();
     read(0, 0, 0);
     for (int kt = 0; kt < nk; kt += STAGES) {
 #pragma unroll
@@ -381,17 +395,19 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
         if (st > 0 && kt + st >= nk) break;
 #pragma unroll
         for (int s = 0; s + 1 < kSteps; ++s) {
+          if (SPLIT && s == 0) issue((st + STAGES - 1) % STAGES, kt + st + STAGES - 1, part1);
+          if (SPLIT && s == (kSteps > 2 ? 1 : 0)) issue((st + STAGES - 1) % STAGES, kt + st + STAGES - 1, part2);
           read(st, s + 1, (s + 1) & 1);
-          __builtin_amdgcn_sched_barrier(0);
           multiply(s & 1);
-          __builtin_amdgcn_sched_barrier(0);
         }
         wait_and_meet<(STAGES - 2) * kLoads>();
-        issue(st, kt + st + STAGES);
+        issue(st, kt + st + STAGES, part0);
+        if (!SPLIT) {
+          issue(st, kt + st + STAGES, part1);
+          issue(st, kt + st + STAGES, part2);
+        }
         read((st + 1) % STAGES, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
         multiply((kSteps - 1) & 1);
-        __builtin_amdgcn_sched_barrier(0);
       }
     }
     // what was issued past the end must land before this workgroup's LDS is another's
@@ -470,18 +486,15 @@ void launch_few(const mko_int8_linear_params& p, hipStream_t s) {
     MKO_TIMED("int8_linear_few", s, few<MT, 8><<<grid, 8 * 64, 0, s>>>(p));
 }
 
-template <int BN, int BM, int WN, int WM, int BK, int STAGES>
+template <int BN, int BM, int WN, int WM, int BK, int STAGES, bool SPLIT>
 void launch_tile(const mko_int8_linear_params& p, bool direct, hipStream_t s) {
-  const int64_t tn = cdiv(p.outer, BN), tm = cdiv(p.rows, BM);
-  const unsigned grid = static_cast<unsigned>(tn * tm);
+  const int tn = static_cast<int>(cdiv(p.outer, BN)), tm = static_cast<int>(cdiv(p.rows, BM));
+  const unsigned grid = static_cast<unsigned>(tn) * static_cast<unsigned>(tm);
   if (direct)
     MKO_TIMED("int8_linear_tile", s,
-              tile<BN, BM, WN, WM, BK, STAGES, true><<<grid, WN * WM * 64, 0, s>>>(p, static_cast<int>(tn),
-                                                                                   static_cast<int>(tm)));
+              tile<BN, BM, WN, WM, BK, STAGES, SPLIT, true><<<grid, WN * WM * 64, 0, s>>>(p, tn, tm));
   else
-    MKO_TIMED("int8_linear_tile", s,
-              tile<BN, BM, WN, WM, BK, 2, false><<<grid, WN * WM * 64, 0, s>>>(p, static_cast<int>(tn),
-                                                                               static_cast<int>(tm)));
+    MKO_TIMED("int8_linear_tile", s, tile<BN, BM, WN, WM, BK, 2, false, false><<<grid, WN * WM * 64, 0, s>>>(p, tn, tm));
 }
 
 // Loads straight into LDS take aligned 16-byte chunks and 32-bit offsets within a tile.
@@ -492,14 +505,29 @@ bool direct_loads(const mko_int8_linear_params& p) {
   return p.inner > 0 && bits % 16 == 0 && p.q_stride >= 0 && p.w_stride >= 0 && p.q_stride < (1 << 23) && p.w_stride < (1 << 23);
 }
 
+// The tile whose rate times the share of the last round of CUs that it fills is the largest.  The
+// rates are POP/s of full rounds at inner lengths of 2560 to 5120; a lone 128 x 128 workgroup has a
+// CU's four SIMDs one wave each and half the rate of two.  us, of 256 x 256, 256 x 128, 128 x 128 and
+// 64 x 64 tiles:
+//   8192 x 8192 x 4096: 260, 306, 331, -;   8192 x 2560 x 5120: 144, 126, 136, -;
+//   1999 x 10240 x 2560: 76, 68, 69, -;     1000 x 2560 x 2560: -, 25, 20, 16.
 void launch(const mko_int8_linear_params& p, hipStream_t s) {
   if (p.rows <= 16) return launch_few<1>(p, s);
   if (p.rows <= 32) return launch_few<2>(p, s);
   if (p.rows <= 64) return launch_few<4>(p, s);
   const bool direct = direct_loads(p);
-  if (cdiv(p.rows, 256) * cdiv(p.outer, 256) >= 200) return launch_tile<256, 256, 2, 4, 128, 2>(p, direct, s);
-  if (cdiv(p.rows, 128) * cdiv(p.outer, 128) >= 200) return launch_tile<128, 128, 2, 2, 128, 2>(p, direct, s);
-  launch_tile<64, 64, 2, 2, 128, 3>(p, direct, s);
+  constexpr int64_t kCus = 256;
+  auto score = [&](int64_t bn, int64_t bm, double rate) {
+    const int64_t tiles = cdiv(p.outer, bn) * cdiv(p.rows, bm);
+    return rate * static_cast<double>(tiles) / static_cast<double>(cdiv(tiles, kCus) * kCus);
+  };
+  const bool pairs = cdiv(p.outer, 128) * cdiv(p.rows, 128) > kCus;
+  const double large = score(256, 256, 2.1), wide = score(256, 128, 1.95), middle = score(128, 128, pairs ? 1.58 : 0.85);
+  const double small = score(64, 64, 1.0);
+  if (large >= wide && large >= middle && large >= small) return launch_tile<256, 256, 4, 2, 128, 2, true>(p, direct, s);
+  if (wide >= middle && wide >= small) return launch_tile<256, 128, 4, 2, 128, 3, true>(p, direct, s);
+  if (middle >= small) return launch_tile<128, 128, 2, 2, 128, 2, false>(p, direct, s);
+  launch_tile<64, 64, 2, 2, 128, 3, true>(p, direct, s);
 }
 
 bool half_or_float(int32_t dtype) { return dtype == MKO_F32 || dtype == MKO_F16 || dtype == MKO_BF16; }
