@@ -58,7 +58,7 @@ def _params(x, input_gate, decay_gate, decay, initial, reset, scale, y, final, s
 def _forward(x, input_gate, decay_gate, decay, initial, reset, scale, want_final):
     """``(y, final, states)``; ``states`` is what the backward reads, ``final`` None if unwanted."""
     batch, length, channels = x.shape
-    y = torch.empty((batch, length, channels), dtype=x.dtype, device=x.device)
+    y = nat.empty_as(x)
     final = None
     if want_final:
         final = torch.empty((batch, channels), dtype=torch.float32, device=x.device)
@@ -92,15 +92,13 @@ class _Recurrence(torch.autograd.Function):
         need = ctx.needs_input_grad
         if dfinal is not None:
             dfinal = nat.dense(dfinal)
-        shape, dtype, device = x.shape, x.dtype, x.device
-        dx, dig, drg = (torch.empty(shape, dtype=dtype, device=device) for _ in range(3))
-        ddecay = torch.empty(decay.shape, dtype=torch.float32, device=device) if need[3] else None
-        dinitial = None
-        if initial is not None and need[4]:
-            dinitial = torch.empty(initial.shape, dtype=torch.float32, device=device)
+        device = x.device
+        dx, dig, drg = nat.empty_as(x), nat.empty_as(x), nat.empty_as(x)
+        ddecay = nat.empty_as(decay) if need[3] else None
+        dinitial = nat.empty_as(initial) if initial is not None and need[4] else None
         if x.numel():
             dy = torch.zeros_like(dx) if dy is None else nat.dense(dy)
-            space = torch.empty(_sizes(*shape)[2], dtype=torch.uint8, device=device)
+            space = torch.empty(_sizes(*x.shape)[2], dtype=torch.uint8, device=device)
             nat.launch("mko_recur_bwd", _params(x, input_gate, decay_gate, decay, initial, reset, ctx.scale, None, None,
                                                 states, dy, dfinal, dx, dig, drg, ddecay, dinitial, space), device)
         else:
@@ -214,11 +212,9 @@ def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, 
         return y[:, 0], out_state
     x, input_gate, decay_gate = nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate)
     state, decay = nat.dense(state), nat.dense_f32(decay)
-    batch, channels = shape = x.shape
-    new_state = out_state
-    if new_state is None:
-        new_state = torch.empty(shape, dtype=state.dtype, device=x.device)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    batch, channels = x.shape
+    new_state = nat.empty_as(state) if out_state is None else out_state
+    y = nat.empty_as(x)
     if batch and channels:
         nat.launch("mko_recur_update", nat.RecurUpdateParams(
             x.data_ptr(), input_gate.data_ptr(), decay_gate.data_ptr(), decay.data_ptr(), state.data_ptr(),

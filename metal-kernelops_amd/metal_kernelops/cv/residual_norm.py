@@ -55,8 +55,8 @@ def _launch_fwd(x, weight, residual, out, q, scale, stream, rstd, pitch, eps):
 
 def _forward(x, weight, residual, eps, want_rstd):
     """``(out, stream, rstd)``; stream is None without a residual."""
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stream = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    out = nat.empty_as(x)
+    stream = None if residual is None else nat.empty_as(residual)
     rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if want_rstd else None
     if x.numel():
         _launch_fwd(x, weight, residual, out, None, None, stream, rstd, 0, eps)
@@ -72,12 +72,11 @@ def _workspace(rows, features, dtype, stream_dtype):
 
 def _backward(dout, dstream, stream, weight, rstd, dtype, need_weight):
     """``(dx, dresidual, dweight)`` of dense operands; one tensor for both where the types agree."""
-    shape, device = stream.shape, stream.device
-    dx = torch.empty(shape, dtype=dtype, device=device)
-    dres = dx if stream.dtype == dtype else torch.empty(shape, dtype=stream.dtype, device=device)
+    device, dres = stream.device, nat.empty_as(stream)
+    dx = dres if stream.dtype == dtype else torch.empty(stream.shape, dtype=dtype, device=device)
     dweight = torch.empty(weight.shape, dtype=torch.float32, device=device) if need_weight else None
     if stream.numel():
-        features = shape[-1]
+        features = stream.shape[-1]
         rows, code, scode = stream.numel() // features, nat.code(dtype), nat.code(stream.dtype)
         space = None
         if need_weight:
@@ -183,7 +182,7 @@ def rmsnorm_residual_int8(x, weight, residual=None, eps=1e-5):
     pitch = -(-features // ALIGN) * ALIGN
     q = torch.empty((*lead, pitch), dtype=torch.int8, device=x.device)
     scale = torch.empty(lead, dtype=torch.float32, device=x.device)
-    stream = x if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    stream = x if residual is None else nat.empty_as(residual)
     if x.numel():
         _launch_fwd(x, w, residual, None, q, scale, None if residual is None else stream, None, pitch, float(eps))
     elif not features:
