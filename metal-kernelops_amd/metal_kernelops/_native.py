@@ -422,6 +422,19 @@ def dense_f32(t):
     return None if t is None else dense(t if t.dtype == torch.float32 else t.float())
 
 
+def wants_grad(*tensors):
+    """Whether a call on ``tensors`` (None among them allowed) has to go through autograd: one of
+    them requires grad in grad mode, or forward-mode derivatives are being taken, which an autograd
+    Function refuses and a launch without it would drop."""
+    if torch.autograd.forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def empty_as(t):
     """A contiguous tensor of ``t``'s shape, dtype and device: ``empty_like`` takes 1.3 us of host
     time where ``torch.empty`` with three arguments takes 2.1."""

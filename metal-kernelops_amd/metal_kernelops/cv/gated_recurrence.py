@@ -167,8 +167,7 @@ def gated_recurrence(x, input_gate, decay_gate, decay, initial_state=None, reset
         reset = reset.contiguous()
     decay, initial = nat.dense_f32(decay), nat.dense_f32(initial_state)
     x, input_gate, decay_gate = nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate)
-    if torch.is_grad_enabled() and (x.requires_grad or input_gate.requires_grad or decay_gate.requires_grad
-                                    or decay.requires_grad or (initial is not None and initial.requires_grad)):
+    if nat.wants_grad(x, input_gate, decay_gate, decay, initial):
         y, final = _Recurrence.apply(x, input_gate, decay_gate, decay, initial, reset, float(scale),
                                      bool(return_final_state))
     else:
@@ -196,12 +195,11 @@ def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, 
     if out_state is not None:
         if out_state.shape != state.shape or out_state.dtype != state.dtype or out_state.device != state.device:
             rules.fail("out_state should have the shape, dtype and device of state")
-        if not out_state.is_contiguous():
+        if not out_state.is_contiguous() or out_state.is_neg():
             rules.fail("out_state should be contiguous")
         if out_state.requires_grad:
             rules.fail("out_state is overwritten in place, so it may not require grad")
-    if torch.is_grad_enabled() and (state.requires_grad or x.requires_grad or input_gate.requires_grad
-                                    or decay_gate.requires_grad or decay.requires_grad):
+    if nat.wants_grad(state, x, input_gate, decay_gate, decay):
         y, final = gated_recurrence(x[:, None], input_gate[:, None], decay_gate[:, None], decay, initial_state=state,
                                     scale=scale, return_final_state=True)
         final = final.to(state.dtype)

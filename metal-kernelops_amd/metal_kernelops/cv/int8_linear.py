@@ -46,7 +46,7 @@ def quantize_int8(x):
     _require_gpu(x)
     if x.dtype not in _FLOATS:
         rules.dtype_in(_FLOATS, x=x)
-    if x.requires_grad and torch.is_grad_enabled():
+    if nat.wants_grad(x):
         rules.fail("8-bit outputs have no gradient; call it under torch.no_grad()")
     features, lead = x.shape[-1], x.shape[:-1]
     pitch = -(-features // ALIGN) * ALIGN
@@ -102,7 +102,7 @@ def int8_linear(q, q_scale, weight, weight_scale, bias=None, out_dtype=torch.bfl
         if t is not None:
             if not t.is_floating_point():
                 rules.fail(f"{name} should be a floating tensor; it is {t.dtype}")
-            if t.requires_grad and torch.is_grad_enabled():
+            if nat.wants_grad(t):
                 rules.fail(f"{name} requires grad, and this product has no gradient; call it under torch.no_grad()")
     if out_dtype not in _FLOATS:
         rules.fail(f"out_dtype should be float32, float16 or bfloat16; it is {out_dtype}")

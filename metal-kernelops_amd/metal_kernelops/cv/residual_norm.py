@@ -140,11 +140,6 @@ def _checked(op, x, weight, residual):
     return nat.dense(weight)
 
 
-def _wants_grad(x, weight, residual):
-    return torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                        or (residual is not None and residual.requires_grad))
-
-
 def rmsnorm_residual(x, weight, residual=None, eps=1e-5):
     """Add ``x`` to the residual stream and normalise it; returns ``(out, stream)``.
 
@@ -159,7 +154,7 @@ def rmsnorm_residual(x, weight, residual=None, eps=1e-5):
         ``out`` in ``x.dtype`` and ``stream`` in the residual's.
     """
     w = _checked("rmsnorm_residual", x, weight, residual)
-    if _wants_grad(x, weight, residual):
+    if nat.wants_grad(x, weight, residual):
         out, stream = _ResidualNorm.apply(x, w, residual, float(eps))
     else:
         out, stream, _ = _forward(x, w, residual, float(eps), False)
@@ -176,7 +171,7 @@ def rmsnorm_residual_int8(x, weight, residual=None, eps=1e-5):
     For inference: arguments that require grad are refused while grad mode is on.
     """
     w = _checked("rmsnorm_residual_int8", x, weight, residual)
-    if _wants_grad(x, weight, residual):
+    if nat.wants_grad(x, weight, residual):
         Rules("rmsnorm_residual_int8").fail("8-bit outputs have no gradient; call it under torch.no_grad()")
     lead, features = x.shape[:-1], x.shape[-1]
     pitch = -(-features // ALIGN) * ALIGN

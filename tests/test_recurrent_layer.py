@@ -160,3 +160,29 @@ def test_results_do_not_depend_on_old_memory(name):
     for k, (a, b) in enumerate(zip(run(False), run(True))):
         assert torch.isfinite(b.float()).all(), k
         assert torch.equal(a, b), k
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused_not_dropped():
+    import torch.autograd.forward_ad as fwd
+    from metal_kernelops.cv import (gated_recurrence, gated_recurrence_update, int8_linear, quantize_int8,
+                                    rmsnorm_residual, rmsnorm_residual_int8)
+    x, d = torch.randn(2, 5, 8, device=DEV), torch.randn(8, device=DEV)
+    q, s = quantize_int8(x[0])
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        calls = [lambda: gated_recurrence(dual, x, x, d),
+                 lambda: gated_recurrence_update(x[:, 0], dual[:, 0], x[:, 0], x[:, 0], d),
+                 lambda: rmsnorm_residual(dual, d, x), lambda: rmsnorm_residual_int8(dual, d, x),
+                 lambda: quantize_int8(dual), lambda: int8_linear(q, s, q, s)]
+        for call in calls:
+            with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
+                call()
+
+
+@pytest.mark.gpu
+def test_a_negated_destination_is_refused():
+    from metal_kernelops.cv import gated_recurrence_update
+    x, d = torch.randn(2, 8, device=DEV), torch.randn(8, device=DEV)
+    with pytest.raises(ValueError, match="contiguous"):
+        gated_recurrence_update(x, x, x, x, d, out_state=torch._neg_view(torch.zeros(2, 8, device=DEV)))
