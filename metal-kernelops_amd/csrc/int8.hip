@@ -157,7 +157,9 @@ __device__ __forceinline__ void put4(const mko_int8_linear_params& p, int64_t m,
   }
 }
 
-// `cols` of eight consecutive outputs from element `at` on.
+// `cols` of eight consecutive outputs from element `at` on.  ALIGNED: 16-byte stores, with the
+// nontemporal hint, which leaves the operands in the L2s (8192 x 2560 x 5120: 128 -> 121 us).
+template <bool ALIGNED>
 __device__ __forceinline__ void put8(const mko_int8_linear_params& p, int64_t at, int cols, const float (&v)[8]) {
   struct __attribute__((packed)) Words4 {
     mko_u32x4 w;
@@ -166,15 +168,23 @@ __device__ __forceinline__ void put8(const mko_int8_linear_params& p, int64_t at
     uint32_t w[8];
     if (p.dtype == MKO_F32) {
       pack_words<float, 8>(v, w);
-      Words4* o = reinterpret_cast<Words4*>(static_cast<float*>(p.out) + at);
-      o[0].w = mko_u32x4{w[0], w[1], w[2], w[3]};
-      o[1].w = mko_u32x4{w[4], w[5], w[6], w[7]};
+      if (ALIGNED) {
+        store_words_nt(static_cast<float*>(p.out) + at, w);
+      } else {
+        Words4* o = reinterpret_cast<Words4*>(static_cast<float*>(p.out) + at);
+        o[0].w = mko_u32x4{w[0], w[1], w[2], w[3]};
+        o[1].w = mko_u32x4{w[4], w[5], w[6], w[7]};
+      }
     } else {
       if (p.dtype == MKO_BF16)
         pack_words<bf16, 8>(v, w);
       else
         pack_words<_Float16, 8>(v, w);
-      reinterpret_cast<Words4*>(static_cast<uint16_t*>(p.out) + at)->w = mko_u32x4{w[0], w[1], w[2], w[3]};
+      const uint32_t half[4] = {w[0], w[1], w[2], w[3]};
+      if (ALIGNED)
+        store_words_nt(static_cast<uint16_t*>(p.out) + at, half);
+      else
+        reinterpret_cast<Words4*>(static_cast<uint16_t*>(p.out) + at)->w = mko_u32x4{w[0], w[1], w[2], w[3]};
     }
   } else {
 #pragma unroll
@@ -435,6 +445,7 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
   wait_and_meet<0>();
   char* mine = lds + wave * 32 * kWide * 4;
   constexpr int kPerRow = kWide / 8;  // lanes to a token
+  const bool aligned = (static_cast<uint64_t>(p.outer) % 8 | reinterpret_cast<uintptr_t>(p.out) % 16) == 0;
   const int nl = (lane % kPerRow) * 8;
   const int64_t n = n0 + wn * kWide + nl;
   const int cols = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(8), p.outer - n)));
@@ -468,7 +479,10 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(e < 4 ? lo[e] : hi[e - 4]) * qs * ws[e] + bias[e];
-      put8(p, m * p.outer + n, cols, v);
+      if (aligned)
+        put8<true>(p, m * p.outer + n, cols, v);
+      else
+        put8<false>(p, m * p.outer + n, cols, v);
     }
     wave_lds_sync();
   }
@@ -509,8 +523,8 @@ bool direct_loads(const mko_int8_linear_params& p) {
 // rates are POP/s of full rounds at inner lengths of 2560 to 5120; a lone 128 x 128 workgroup has a
 // CU's four SIMDs one wave each and half the rate of two.  us, of 256 x 256, 256 x 128, 128 x 128 and
 // 64 x 64 tiles:
-//   8192 x 8192 x 4096: 260, 306, 331, -;   8192 x 2560 x 5120: 144, 126, 136, -;
-//   1999 x 10240 x 2560: 76, 68, 69, -;     1000 x 2560 x 2560: -, 25, 20, 16.
+//   8192 x 8192 x 4096: 265, 292, 331, -;   8192 x 2560 x 5120: 140, 121, 125, -;
+//   1999 x 10240 x 2560: 77, 67, 68, -;     1000 x 2560 x 2560: -, 25, 20, 16.
 void launch(const mko_int8_linear_params& p, hipStream_t s) {
   if (p.rows <= 16) return launch_few<1>(p, s);
   if (p.rows <= 32) return launch_few<2>(p, s);
