@@ -10,6 +10,7 @@ is passed as the launch stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -433,6 +434,18 @@ def wants_grad(*tensors):
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def first_order(backward):
+    """A Function's ``backward`` that has no derivative of its own: ``once_differentiable``, which is
+    what says so, only where the graph of the backward is recorded (it takes 5 us of host time)."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return call
 
 
 def empty_as(t):

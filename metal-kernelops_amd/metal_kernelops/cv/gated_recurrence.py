@@ -24,7 +24,6 @@ import ctypes
 import functools
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
 from .._contract import Rules
@@ -86,7 +85,7 @@ class _Recurrence(torch.autograd.Function):
         return y, final
 
     @staticmethod
-    @once_differentiable
+    @nat.first_order
     def backward(ctx, dy, dfinal):
         x, input_gate, decay_gate, decay, initial, reset, states = ctx.saved_tensors
         need = ctx.needs_input_grad

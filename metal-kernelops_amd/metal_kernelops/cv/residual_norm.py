@@ -22,7 +22,6 @@ import ctypes
 import functools
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
 from .._contract import Rules
@@ -105,7 +104,7 @@ class _ResidualNorm(torch.autograd.Function):
         return out, stream
 
     @staticmethod
-    @once_differentiable
+    @nat.first_order
     def backward(ctx, dout, dstream):
         stream, weight, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
