@@ -12,13 +12,14 @@
  * behind mko_state_update_bwd_static, comes with the code object).  Inputs are
  * never written.
  * All tensors are dense row-major (contiguous) in the layouts documented per
- * field.  dtype fields take MKO_F32 / MKO_F16 / MKO_BF16 (and MKO_F64 for the SSD); every
+ * field, where no strides are given.  dtype fields take MKO_F32 / MKO_F16 / MKO_BF16 (and MKO_F64 for the SSD); every
  * kernel computes in float32 (float64 for float64 SSD inputs) and rounds once when it stores a
  * 16-bit output.
  *
  * The reference (dbydd/metal-kernelops) has no native ABI: its Python launches
  * Metal kernels through torch.mps.compile_shader.  Each entry point below names
- * the reference function it replaces (paths relative to src/metal_kernelops/).
+ * the reference function it replaces (paths relative to src/metal_kernelops/); the
+ * gated linear recurrence, the residual norm and the 8-bit products have none.
  */
 #ifndef MKO_H
 #define MKO_H
@@ -558,14 +559,11 @@ typedef struct mko_int8_linear_params {
   const float* w_scale;    /* (outer,) */
   const float* bias;       /* (outer,) or NULL */
   void* out;               /* (rows, outer) of dtype, contiguous */
-  void* workspace;         /* mko_int8_linear_workspace_size() bytes */
-  size_t workspace_bytes;
   int64_t rows, inner, outer, q_stride, w_stride;
   int32_t dtype;
 } mko_int8_linear_params;
 
 size_t mko_sizeof_int8_linear_params(void);
-size_t mko_int8_linear_workspace_size(const mko_int8_linear_params* p);
 int mko_int8_linear(const mko_int8_linear_params* p, void* stream);
 
 #ifdef __cplusplus

@@ -176,7 +176,6 @@ class Int8LinearParams(ctypes.Structure):
 
     _fields_ = [
         ("q", _vp), ("q_scale", _vp), ("w", _vp), ("w_scale", _vp), ("bias", _vp), ("out", _vp),
-        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
         ("rows", ctypes.c_int64), ("inner", ctypes.c_int64), ("outer", ctypes.c_int64),
         ("q_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64), ("dtype", ctypes.c_int32),
     ]
@@ -239,7 +238,6 @@ _SIGNATURES = {
     "mko_resnorm_bwd_workspace_size": ([ctypes.POINTER(ResnormParams)], ctypes.c_size_t),
     "mko_resnorm_bwd": ([ctypes.POINTER(ResnormParams), _vp], ctypes.c_int),
     "mko_quantize_int8": ([ctypes.POINTER(QuantizeParams), _vp], ctypes.c_int),
-    "mko_int8_linear_workspace_size": ([ctypes.POINTER(Int8LinearParams)], ctypes.c_size_t),
     "mko_int8_linear": ([ctypes.POINTER(Int8LinearParams), _vp], ctypes.c_int),
     "mko_state_update_bwd_static": ([ctypes.POINTER(StateUpdateParams), _vp], ctypes.c_int),
 }

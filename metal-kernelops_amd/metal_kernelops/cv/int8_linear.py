@@ -117,8 +117,8 @@ def int8_linear(q, q_scale, weight, weight_scale, bias=None, out_dtype=torch.bfl
             q, weight = nat.rows(q), nat.rows(weight)
         qs, ws, b = nat.dense_f32(q_scale), nat.dense_f32(weight_scale), nat.dense_f32(bias)
         nat.launch("mko_int8_linear", nat.Int8LinearParams(
-            q.data_ptr(), qs.data_ptr(), weight.data_ptr(), ws.data_ptr(), nat.ptr(b), out.data_ptr(), None, 0, rows,
-            inner, outer, q.stride(0) if q.dim() == 2 else inner, weight.stride(0), nat.code(out_dtype)), q.device)
+            q.data_ptr(), qs.data_ptr(), weight.data_ptr(), ws.data_ptr(), nat.ptr(b), out.data_ptr(), rows, inner,
+            outer, q.stride(0) if q.dim() == 2 else inner, weight.stride(0), nat.code(out_dtype)), q.device)
     return out
 
 
