@@ -198,7 +198,7 @@ __device__ __forceinline__ void put8(const mko_int8_linear_params& p, int64_t at
 
 // ---------------------------------------------------------------- few tokens
 
-// A workgroup of W waves computes 16 channels of MT * 16 tokens; the waves take the inner axis in
+// A workgroup of W waves computes 16 channels of MT * 16 tokens (grid: channels, tokens); the waves take the inner axis in
 // turns of 256 bytes, load both operands straight into the matrix cores' registers, and their
 // sums are added in LDS.  The weights are read once, which is what bounds it: one token into
 // 10240 x 2560 takes 8.0 us (3.3 TB/s), 64 tokens into 2560 x 2560 take 8.1, where 64 x 64 tiles take 11.
@@ -207,13 +207,13 @@ __global__ void __launch_bounds__(W * 64) few(mko_int8_linear_params p) {
   __shared__ __attribute__((aligned(16))) int sums[W][MT][256];
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int inner = static_cast<int>(p.inner);
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16, m0 = static_cast<int64_t>(blockIdx.y) * (MT * 16);
   const int64_t nrow = min(n0 + (lane & 15), p.outer - 1);
   const int8_t* wrow = p.w + nrow * p.w_stride;
   const int8_t* qrow[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
-    qrow[t] = p.q + min(static_cast<int64_t>(t * 16 + (lane & 15)), p.rows - 1) * p.q_stride;
+    qrow[t] = p.q + min(m0 + t * 16 + (lane & 15), p.rows - 1) * p.q_stride;
   v4i acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = v4i{0, 0, 0, 0};
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(W * 64) few(mko_int8_linear_params p) {
   __syncthreads();
   for (int i = threadIdx.x; i < MT * 64; i += W * 64) {
     const int t = i >> 6, e = (i & 63) * 4;
-    const int64_t m = t * 16 + (e >> 4), n = n0 + (e & 15);
+    const int64_t m = m0 + t * 16 + (e >> 4), n = n0 + (e & 15);
     if (m >= p.rows || n >= p.outer) continue;
     int s[4] = {0, 0, 0, 0};
     for (int w = 0; w < W; ++w)
@@ -496,9 +496,9 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
 
 template <int MT>
 void launch_few(const mko_int8_linear_params& p, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(cdiv(p.outer, 16));
+  const dim3 grid(static_cast<unsigned>(cdiv(p.outer, 16)), static_cast<unsigned>(cdiv(p.rows, MT * 16)));
   const int64_t turns = cdiv(p.inner, 256);
-  if (turns <= 4 || grid >= 2048)
+  if (turns <= 4 || grid.x >= 2048)
     MKO_TIMED("int8_linear_few", s, few<MT, 4><<<grid, 4 * 64, 0, s>>>(p));
   else
     MKO_TIMED("int8_linear_few", s, few<MT, 8><<<grid, 8 * 64, 0, s>>>(p));
@@ -530,10 +530,16 @@ bool direct_loads(const mko_int8_linear_params& p) {
 //   8192 x 8192 x 4096: 265, 292, 331, -;   8192 x 2560 x 5120: 140, 121, 125, -;
 //   1999 x 10240 x 2560: 77, 67, 68, -;     1000 x 2560 x 2560: -, 25, 20, 16.
 void launch(const mko_int8_linear_params& p, hipStream_t s) {
-  if (p.rows <= 16) return launch_few<1>(p, s);
-  if (p.rows <= 32) return launch_few<2>(p, s);
-  if (p.rows <= 64) return launch_few<4>(p, s);
+  // `few` reads the tokens again for every 16 channels, so it is for small outputs, and without direct
+  // loads for somewhat larger ones.  us, few against 64 x 64 tiles: 17 x 2560 x 2560 5.5 and 8.6, 32 x 2560 x
+  // 2560 6.1 and 8.5, 48 x 2560 x 2560 7.6 and 8.6; 17 x 10240 x 2560 10.4 and 9.4, 48 x 5120 x 2560 12.3 and
+  // 9.0; unaligned, 77 x 4099 x 1000 9.4 and 11.0, 256 x 2560 x 2568 26.7 and 19.0.
   const bool direct = direct_loads(p);
+  const int64_t outputs = p.rows * p.outer;
+  if (p.rows <= 16) return launch_few<1>(p, s);
+  if (p.rows <= 32 && outputs <= 1 << 17) return launch_few<2>(p, s);
+  if (p.rows <= 64 && outputs <= 1 << 17) return launch_few<4>(p, s);
+  if (p.inner > 0 && !direct && outputs <= 3 << 17) return launch_few<2>(p, s);
   constexpr int64_t kCus = 256;
   auto score = [&](int64_t bn, int64_t bm, double rate) {
     const int64_t tiles = cdiv(p.outer, bn) * cdiv(p.rows, bm);

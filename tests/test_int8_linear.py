@@ -116,6 +116,17 @@ def test_product(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("inner", [96, 100, 257])
+@pytest.mark.parametrize("rows,outer", [(700, 600), (2048, 4352), (4100, 4099), (4090, 4096)])
+def test_every_tile(rows, outer, inner):
+    """Sizes that each tile is chosen for, 64 x 64 to 256 x 256, with direct loads and without."""
+    q, qs = quantised(rows, inner, rows)
+    w, ws = quantised(outer, inner, outer)
+    bias = torch.randn(outer, generator=torch.Generator().manual_seed(1))
+    check(q, qs, w, ws, bias, torch.bfloat16 if inner == 96 else torch.float32)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 40, 150, 700])
 def test_largest_values_stay_exact(rows):
     """-128 and 127 throughout, at the longest sum that int32 holds."""
