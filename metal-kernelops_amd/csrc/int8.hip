@@ -286,7 +286,8 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
   __shared__ __attribute__((aligned(256))) char lds[STAGES * kStage > kSums ? STAGES * kStage : kSums];
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wn = wave / WM, wm = wave % WM;
-  const int inner = static_cast<int>(p.inner);
+  const int whole = static_cast<int>(p.inner);
+  const int inner = DIRECT ? whole & ~15 : whole;  // direct loads take whole chunks; the rest comes first
 
   // bands of 8 token tiles, token tile fastest: an XCD's workgroups share both operands in its L2
   const WgId id = wg_id(tiles_n * tiles_m, 1);
@@ -394,6 +395,19 @@ __global__ void __launch_bounds__(WN * WM * 64) tile(mko_int8_linear_params p, i
   // nothing.  Where several workgroups share a CU another one multiplies then, and the earlier
   // loads are worth more: 128 x 128 tiles of 8192 x 8192 x 4096 take 347 us, split 389.
   if constexpr (DIRECT) {
+    if (inner < whole) {  // first the step of the bytes that fill no chunk, in the lanes of its first half
+#pragma unroll
+      for (int i = 0; i < kTn; ++i) {
+        const int64_t n = min(n0 + (wn * kTn + i) * 32 + lr, p.outer - 1);
+        a[0][i] = load_chunk(p.w + n * p.w_stride, lane < 32 ? inner : whole, whole);
+      }
+#pragma unroll
+      for (int j = 0; j < kTm; ++j) {
+        const int64_t m = min(m0 + (wm * kTm + j) * 32 + lr, p.rows - 1);
+        b[0][j] = load_chunk(p.q + m * p.q_stride, lane < 32 ? inner : whole, whole);
+      }
+      multiply(0);
+    }
 #pragma unroll
     for (int st = 0; st < STAGES; ++st) {
       issue(st, st, part0);
@@ -515,12 +529,12 @@ void launch_tile(const mko_int8_linear_params& p, bool direct, hipStream_t s) {
     MKO_TIMED("int8_linear_tile", s, tile<BN, BM, WN, WM, BK, 2, false, false><<<grid, WN * WM * 64, 0, s>>>(p, tn, tm));
 }
 
-// Loads straight into LDS take aligned 16-byte chunks and 32-bit offsets within a tile.
+// Loads straight into LDS take aligned 16-byte chunks and 32-bit offsets within a tile.  Rows that
+// rmsnorm_residual_int8 and quantize_int8 wrote start at such addresses whatever their length.
 bool direct_loads(const mko_int8_linear_params& p) {
   const uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.w) |
-                         static_cast<uintptr_t>(p.q_stride) | static_cast<uintptr_t>(p.w_stride) |
-                         static_cast<uintptr_t>(p.inner);
-  return p.inner > 0 && bits % 16 == 0 && p.q_stride >= 0 && p.w_stride >= 0 && p.q_stride < (1 << 23) && p.w_stride < (1 << 23);
+                         static_cast<uintptr_t>(p.q_stride) | static_cast<uintptr_t>(p.w_stride);
+  return p.inner >= 16 && bits % 16 == 0 && p.q_stride >= 0 && p.w_stride >= 0 && p.q_stride < (1 << 23) && p.w_stride < (1 << 23);
 }
 
 // The tile whose rate times the share of the last round of CUs that it fills is the largest.  The

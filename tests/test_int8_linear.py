@@ -159,6 +159,22 @@ def test_strides_offsets_and_poison(rows, inner):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("inner", [1, 15, 17, 100, 127, 1000, 1001])
+@pytest.mark.parametrize("rows,outer", [(30, 70), (100, 1500), (700, 600), (2048, 4352), (4090, 4096)])
+def test_aligned_rows_of_odd_lengths(rows, outer, inner):
+    """Rows at multiples of 16 bytes, as the quantisations write them, with other values after their end."""
+    pitch = -(-inner // 16) * 16
+    q, qs = quantised(rows, inner, 7)
+    w, ws = quantised(outer, inner, 8)
+    wide_q = torch.full((rows, pitch), 77, dtype=torch.int8, device=DEV)
+    wide_w = torch.full((outer, pitch), -99, dtype=torch.int8, device=DEV)
+    vq, vw = wide_q[:, :inner], wide_w[:, :inner]
+    vq.copy_(q)
+    vw.copy_(w)
+    check(q, qs, w, ws, None, torch.float32, (vq, vw))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 30, 128, 520])
 def test_the_end_of_an_allocation(rows):
     """Operands whose last byte is the last of their memory."""
