@@ -186,3 +186,39 @@ def test_a_negated_destination_is_refused():
     x, d = torch.randn(2, 8, device=DEV), torch.randn(8, device=DEV)
     with pytest.raises(ValueError, match="contiguous"):
         gated_recurrence_update(x, x, x, x, d, out_state=torch._neg_view(torch.zeros(2, 8, device=DEV)))
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^32 bytes: their last rows against the same rows alone.  The scan's
+    channels forget (0.8 a step), so that 2048 steps before them are all that its last rows hold."""
+    from metal_kernelops.cv import gated_recurrence, int8_linear, quantize_int8, rmsnorm_residual
+    g = torch.Generator(device=DEV).manual_seed(0)
+    length, channels = 900_000, 2560
+    x = torch.empty(1, length, channels, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    gate = torch.zeros(1, 1, channels, dtype=torch.bfloat16, device=DEV).expand(1, length, channels)
+    decay = torch.full((channels,), 0.0, device=DEV)  # a = exp(-scale log(2) / 2) = 0.8
+    scale = 2 * 0.2231 / 0.6931
+    y = gated_recurrence(x, gate, gate, decay, scale=scale)
+    tail = slice(length - 2048, length)
+    want = gated_recurrence(x[:, tail], gate[:, tail], gate[:, tail], decay, scale=scale)
+    assert rel(y[:, -500:], want[:, -500:]) <= 2.0 ** -8
+    leaf = x.requires_grad_(True)
+    (dx,) = torch.autograd.grad(gated_recurrence(leaf, gate, gate, decay, scale=scale), leaf, y)
+    part = x[:, :2048].detach().requires_grad_(True)
+    (dpart,) = torch.autograd.grad(gated_recurrence(part, gate[:, :2048], gate[:, :2048], decay, scale=scale), part,
+                                   y[:, :2048])
+    assert rel(dx[:, :500], dpart[:, :500]) <= 2.0 ** -8
+    del y, dx, want
+    rows = x.detach()[0]
+    weight = torch.ones(channels, device=DEV)
+    out, stream = rmsnorm_residual(rows, weight, rows)
+    last, last_stream = rmsnorm_residual(rows[-3:], weight, rows[-3:])
+    assert torch.equal(out[-3:], last) and torch.equal(stream[-3:], last_stream)
+    del out, stream
+    q, s = quantize_int8(rows[:, :2048])
+    q2 = torch.cat([q, q, q])  # 2.7 million rows of 2048 bytes
+    wq, ws = quantize_int8(torch.randn(20, 2048, generator=g, device=DEV))
+    whole = int8_linear(q2, torch.cat([s, s, s]), wq, ws, out_dtype=torch.float32)
+    assert torch.equal(whole[-5:], int8_linear(q[-5:], s[-5:], wq, ws, out_dtype=torch.float32))
+    assert torch.equal(whole[:70], int8_linear(q[:70], s[:70], wq, ws, out_dtype=torch.float32))
