@@ -1,9 +1,9 @@
 // 8-bit integers for gfx950: quantisation of rows, and the matrix product
 //   out[m][n] = q_scale[m] w_scale[n] sum_k q[m][k] w[n][k] + bias[n]
-// with the sum in int32, exact for fewer than 2^17 terms of at most 2^14.  Up to 64 tokens it is bound
-// by the weights' bytes (`few`), beyond by the matrix cores' feed and the power limit (`tile`):
-// 8192 x 2560 x 5120 in 121 us (1.78 POP/s), 8192 x 8192 x 4096 in 265 (2.1), of 2.9 to 3.4 POP/s that
-// products of random bytes reach from registers alone.  quantize_rows moves 8192 x 5120 bf16 in 24 us,
+// with the sum in int32, exact for fewer than 2^17 terms of at most 2^14.  Small outputs are
+// bound by the weights' bytes (`few`), larger ones by the matrix cores' feed and the power limit
+// (`tile`): 8192 x 2560 x 5120 in 121 us (1.78 POP/s), 8192 x 8192 x 4096 in 255 to 265 (2.1), of 2.9 to
+// 3.4 POP/s that products of random bytes reach from registers alone.  quantize_rows moves 8192 x 5120 bf16 in 24 us,
 // 5.2 TB/s.
 #include <type_traits>
 
@@ -198,10 +198,10 @@ __device__ __forceinline__ void put8(const mko_int8_linear_params& p, int64_t at
 
 // ---------------------------------------------------------------- few tokens
 
-// A workgroup of W waves computes 16 channels of MT * 16 tokens (grid: channels, tokens); the waves take the inner axis in
-// turns of 256 bytes, load both operands straight into the matrix cores' registers, and their
-// sums are added in LDS.  The weights are read once, which is what bounds it: one token into
-// 10240 x 2560 takes 8.0 us (3.3 TB/s), 64 tokens into 2560 x 2560 take 8.1, where 64 x 64 tiles take 11.
+// A workgroup of W waves computes 16 channels of MT * 16 tokens (grid: channels, tokens); the waves
+// take the inner axis in turns of 256 bytes, load both operands straight into the matrix cores'
+// registers, and their sums are added in LDS.  Each block of tokens reads the weights once, which is
+// what bounds it: one token into 10240 x 2560 takes 8.0 us (3.3 TB/s), 48 tokens into 2560 x 2560 7.6.
 template <int MT, int W>
 __global__ void __launch_bounds__(W * 64) few(mko_int8_linear_params p) {
   __shared__ __attribute__((aligned(16))) int sums[W][MT][256];
