@@ -10,7 +10,6 @@ is passed as the launch stream.
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 import threading
 
@@ -353,25 +352,48 @@ def dense_op(name, impl):
                                    schema=torch.library.infer_schema(impl, mutates_args=()))
 
 
+# looked up once: every call of an operator asks them all
+_is_compiling, _is_tracing = torch.compiler.is_compiling, torch._C._is_tracing
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_transform, _profiling = torch._C._functorch.peek_interpreter_stack, torch._C._autograd._profiler_enabled
+_forward_ad, _is_grad_enabled = torch.autograd.forward_ad, torch.is_grad_enabled
+
+
+def watched(*tensors):
+    """Whether something besides the operator has to see a call on ``tensors`` (None among them
+    allowed), so that it goes through the custom op: compiling or tracing, a profiler that is
+    recording (it names the op), tensor subclasses, dispatch or function modes, functorch transforms
+    and forward-mode levels, and tensors whose values are not what their memory holds (negated views,
+    and those without memory: ZeroTensors, functional wrappers, empty tensors), which the dispatcher
+    materialises.  A launch through ctypes is invisible to all of them: a trace would record the
+    allocation of the outputs and nothing that fills them."""
+    if _is_compiling() or _is_tracing() or _dispatch_modes() or _function_modes() or _transform() is not None \
+            or _forward_ad._current_level >= 0 or _profiling():
+        return True
+    for t in tensors:
+        if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter)
+                              or t.is_neg() or t.data_ptr() == 0):
+            return True
+    return False
+
+
 def plain_call(*tensors):
     """Whether a call on ``tensors`` (None among them allowed) is an ordinary eager one that no
     gradient, tracer or mode has to see, so that the implementation behind a custom op may be
     called without the dispatcher: its round trip costs 10-25 us of host time, as much as the
-    kernels of a short prompt.  Not plain: grad mode with an input that requires grad, compiling
-    or tracing, a profiler that is recording (it names the op), tensor subclasses, dispatch or
-    function modes, functorch transforms and forward-mode levels, and tensors whose values are not
-    what their memory holds (negated views, and those without memory: ZeroTensors, functional
-    wrappers, empty tensors); those go through the op, which does with them what it always did."""
-    if torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() \
-            or torch._C._len_torch_function_stack() or torch._C._functorch.peek_interpreter_stack() is not None \
-            or torch.autograd.forward_ad._current_level >= 0 or torch._C._autograd._profiler_enabled():
-        return False
-    grad = torch.is_grad_enabled()
-    for t in tensors:
-        if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter)
-                              or (grad and t.requires_grad) or t.is_neg() or t.data_ptr() == 0):
-            return False
-    return True
+    kernels of a short prompt.  Not plain: grad mode with an input that requires grad, and what
+    :func:`watched` names; those go through the op, which does with them what it always did."""
+    return not watched(*tensors) and not wants_grad(*tensors)
+
+
+def through(op, *args):
+    """The custom op ``op`` on ``args``; forward-mode derivatives, which the dispatcher would drop
+    for an op that has none, are refused."""
+    if _forward_ad._current_level >= 0:
+        for t in args:
+            if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{op} has no forward-mode derivative")
+    return op(*args)
 
 
 def stream_of(device):
@@ -394,56 +416,40 @@ def launch(name, params, device):
         check(status, name)
 
 
-def values(t):
-    """``t`` with its values in memory: a negated view or a tensor without memory (a ZeroTensor)
-    hands a kernel other numbers than it holds."""
-    if t.is_neg():
-        t = t.resolve_neg()
-    return torch.zeros(t.shape, dtype=t.dtype, device=t.device) if t._is_zerotensor() else t
-
-
 def rows(t):
     """``t`` as a kernel reads it in rows: the last axis of unit stride, the others as they are."""
-    if t.is_neg() or t._is_zerotensor():
-        t = values(t)
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def dense(t):
-    """``t`` as a kernel reads it whole: contiguous, its values in memory."""
-    if t.is_neg() or t._is_zerotensor():
-        t = values(t)
-    return t if t.is_contiguous() else t.contiguous()
+    """``t`` as a kernel reads it whole; None stays None."""
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def dense_f32(t):
-    """The same in float32; None stays None."""
-    return None if t is None else dense(t if t.dtype == torch.float32 else t.float())
+    """The same in float32."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32:
+        t = t.float()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def absent(t, like, dtype=None):
+    """What a custom op returns in the place of an output that is None: an empty tensor."""
+    return like.new_empty(0, dtype=dtype) if t is None else t
 
 
 def wants_grad(*tensors):
-    """Whether a call on ``tensors`` (None among them allowed) has to go through autograd: one of
-    them requires grad in grad mode, or forward-mode derivatives are being taken, which an autograd
-    Function refuses and a launch without it would drop."""
-    if torch.autograd.forward_ad._current_level >= 0:
+    """Whether derivatives of a call on ``tensors`` (None among them allowed) may be wanted: one of
+    them requires grad in grad mode, or forward-mode derivatives are being taken."""
+    if _forward_ad._current_level >= 0:
         return True
-    if torch.is_grad_enabled():
+    if _is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
     return False
-
-
-def first_order(backward):
-    """A Function's ``backward`` that has no derivative of its own: ``once_differentiable``, which is
-    what says so, only where the graph of the backward is recorded (it takes 5 us of host time)."""
-    recorded = torch.autograd.function.once_differentiable(backward)
-
-    @functools.wraps(backward)
-    def call(ctx, *grads):
-        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
-
-    return call
 
 
 def empty_as(t):

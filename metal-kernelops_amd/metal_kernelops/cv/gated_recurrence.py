@@ -22,8 +22,10 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from typing import Optional, Tuple
 
 import torch
+from torch import Tensor
 
 from .. import _native as nat
 from .._contract import Rules
@@ -33,6 +35,9 @@ __all__ = ["gated_recurrence", "gated_recurrence_reference", "gated_recurrence_u
            "gated_recurrence_update_reference"]
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+CHUNK = 64
+"""MKO_RECUR_CHUNK: steps between the saved states."""
 
 
 @functools.lru_cache(maxsize=256)
@@ -73,6 +78,38 @@ def _forward(x, input_gate, decay_gate, decay, initial, reset, scale, want_final
     return y, final, states
 
 
+def _backward(dy, dfinal, x, input_gate, decay_gate, decay, initial, reset, states, scale, need_decay, need_initial):
+    """``(dx, dinput_gate, ddecay_gate, ddecay, dinitial)``, the last two None if unwanted."""
+    dfinal = nat.dense(dfinal)
+    dx, dig, drg = nat.empty_as(x), nat.empty_as(x), nat.empty_as(x)
+    ddecay = nat.empty_as(decay) if need_decay else None
+    dinitial = nat.empty_as(initial) if need_initial else None
+    if x.numel():
+        dy = torch.zeros_like(dx) if dy is None else nat.dense(dy)
+        space = torch.empty(_sizes(*x.shape)[2], dtype=torch.uint8, device=x.device)
+        nat.launch("mko_recur_bwd", _params(x, input_gate, decay_gate, decay, initial, reset, scale, None, None,
+                                            states, dy, dfinal, dx, dig, drg, ddecay, dinitial, space), x.device)
+    else:
+        if ddecay is not None:
+            ddecay.zero_()
+        if dinitial is not None:
+            dinitial.zero_() if dfinal is None else dinitial.copy_(dfinal)
+    return dx, dig, drg, ddecay, dinitial
+
+
+def _grads(ctx, dy, dfinal, _states=None):
+    """The gradients of the inputs of :class:`_Recurrence` and of the custom op."""
+    x, input_gate, decay_gate, decay, initial, reset, states = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    need_decay, need_initial = need[3], initial is not None and need[4]
+    args = (dy, dfinal if ctx.want_final else None, x, input_gate, decay_gate, decay, initial, reset, states)
+    # a backward that is itself recorded goes through the op, which refuses to be differentiated
+    plain = not torch.is_grad_enabled() and nat.plain_call(*args)
+    backward = _backward if plain else torch.ops.mko.recur_bwd
+    dx, dig, drg, ddecay, dinitial = backward(*args, ctx.scale, need_decay, need_initial)
+    return dx, dig, drg, ddecay if need_decay else None, dinitial if need_initial else None, None, None, None
+
+
 class _Recurrence(torch.autograd.Function):
     """Forward and analytic first-order backward through the C ABI."""
 
@@ -80,32 +117,81 @@ class _Recurrence(torch.autograd.Function):
     def forward(ctx, x, input_gate, decay_gate, decay, initial, reset, scale, want_final):
         y, final, states = _forward(x, input_gate, decay_gate, decay, initial, reset, scale, want_final)
         ctx.save_for_backward(x, input_gate, decay_gate, decay, initial, reset, states)
-        ctx.scale = scale
+        ctx.scale, ctx.want_final = scale, want_final
         ctx.set_materialize_grads(False)  # an unused output reaches backward as None
         return y, final
 
-    @staticmethod
-    @nat.first_order
-    def backward(ctx, dy, dfinal):
-        x, input_gate, decay_gate, decay, initial, reset, states = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        if dfinal is not None:
-            dfinal = nat.dense(dfinal)
-        device = x.device
-        dx, dig, drg = nat.empty_as(x), nat.empty_as(x), nat.empty_as(x)
-        ddecay = nat.empty_as(decay) if need[3] else None
-        dinitial = nat.empty_as(initial) if initial is not None and need[4] else None
-        if x.numel():
-            dy = torch.zeros_like(dx) if dy is None else nat.dense(dy)
-            space = torch.empty(_sizes(*x.shape)[2], dtype=torch.uint8, device=device)
-            nat.launch("mko_recur_bwd", _params(x, input_gate, decay_gate, decay, initial, reset, ctx.scale, None, None,
-                                                states, dy, dfinal, dx, dig, drg, ddecay, dinitial, space), device)
-        else:
-            if ddecay is not None:
-                ddecay.zero_()
-            if dinitial is not None:
-                dinitial.zero_() if dfinal is None else dinitial.copy_(dfinal)
-        return dx, dig, drg, ddecay, dinitial, None, None, None
+    backward = staticmethod(_grads)
+
+
+def _recur_fwd_op(x: Tensor, input_gate: Tensor, decay_gate: Tensor, decay: Tensor, initial: Optional[Tensor],
+                  reset: Optional[Tensor], scale: float, want_final: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    y, final, states = _forward(nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate), nat.dense(decay),
+                                nat.dense(initial), nat.dense(reset), scale, want_final)
+    return y, nat.absent(final, decay), nat.absent(states, decay, torch.uint8)
+
+
+_recur_fwd = torch.library.custom_op("mko::recur_fwd", _recur_fwd_op, mutates_args=(), device_types="cuda")
+
+
+@_recur_fwd.register_fake
+def _(x, input_gate, decay_gate, decay, initial, reset, scale, want_final):
+    batch, length, channels = x.shape
+    saved = -(-(batch * -(-length // CHUNK) * channels * 4) // 16) * 16
+    return (x.new_empty(x.shape), x.new_empty((batch, channels) if want_final else 0, dtype=torch.float32),
+            x.new_empty(saved, dtype=torch.uint8))
+
+
+def _recur_bwd_op(dy: Optional[Tensor], dfinal: Optional[Tensor], x: Tensor, input_gate: Tensor, decay_gate: Tensor,
+                  decay: Tensor, initial: Optional[Tensor], reset: Optional[Tensor], states: Optional[Tensor],
+                  scale: float, need_decay: bool, need_initial: bool
+                  ) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    dx, dig, drg, ddecay, dinitial = _backward(
+        dy, dfinal, nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate), nat.dense(decay), nat.dense(initial),
+        nat.dense(reset), states, scale, need_decay, need_initial)
+    return dx, dig, drg, nat.absent(ddecay, decay), nat.absent(dinitial, decay)
+
+
+_recur_bwd = torch.library.custom_op("mko::recur_bwd", _recur_bwd_op, mutates_args=(), device_types="cuda")
+
+
+@_recur_bwd.register_fake
+def _(dy, dfinal, x, input_gate, decay_gate, decay, initial, reset, states, scale, need_decay, need_initial):
+    return (*(x.new_empty(x.shape) for _ in range(3)), decay.new_empty(decay.shape if need_decay else 0),
+            decay.new_empty(initial.shape if need_initial else 0))
+
+
+def _setup(ctx, inputs, output):
+    x, input_gate, decay_gate, decay, initial, reset, ctx.scale, ctx.want_final = inputs
+    ctx.save_for_backward(x, input_gate, decay_gate, decay, initial, reset, output[2])
+    ctx.set_materialize_grads(False)
+
+
+torch.library.register_autograd("mko::recur_fwd", _grads, setup_context=_setup)
+
+
+def _update(state, x, input_gate, decay_gate, decay, scale, new_state, y):
+    batch, channels = x.shape
+    if batch and channels:
+        nat.launch("mko_recur_update", nat.RecurUpdateParams(
+            x.data_ptr(), input_gate.data_ptr(), decay_gate.data_ptr(), decay.data_ptr(), state.data_ptr(),
+            new_state.data_ptr(), y.data_ptr(), batch, channels, x.stride(0), input_gate.stride(0), decay_gate.stride(0),
+            scale, nat.code(x.dtype), nat.code(state.dtype)), x.device)
+    return y, new_state
+
+
+def _recur_update_op(state: Tensor, x: Tensor, input_gate: Tensor, decay_gate: Tensor, decay: Tensor, scale: float
+                     ) -> Tuple[Tensor, Tensor]:
+    return _update(nat.dense(state), nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate), nat.dense(decay), scale,
+                   nat.empty_as(state), nat.empty_as(x))
+
+
+_recur_update = torch.library.custom_op("mko::recur_update", _recur_update_op, mutates_args=(), device_types="cuda")
+
+
+@_recur_update.register_fake
+def _(state, x, input_gate, decay_gate, decay, scale):
+    return x.new_empty(x.shape), state.new_empty(state.shape)
 
 
 def _check(op, x, input_gate, decay_gate, decay, scale, layout):
@@ -165,13 +251,17 @@ def gated_recurrence(x, input_gate, decay_gate, decay, initial_state=None, reset
         rules.dtype_in((torch.bool,), reset=reset)
         reset = reset.contiguous()
     decay, initial = nat.dense_f32(decay), nat.dense_f32(initial_state)
+    scale, want_final = float(scale), bool(return_final_state)
+    if nat.watched(x, input_gate, decay_gate, decay, initial, reset):
+        y, final, _ = nat.through(torch.ops.mko.recur_fwd, x, input_gate, decay_gate, decay, initial, reset, scale,
+                                  want_final)
+        return (y, final) if want_final else y
     x, input_gate, decay_gate = nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate)
     if nat.wants_grad(x, input_gate, decay_gate, decay, initial):
-        y, final = _Recurrence.apply(x, input_gate, decay_gate, decay, initial, reset, float(scale),
-                                     bool(return_final_state))
+        y, final = _Recurrence.apply(x, input_gate, decay_gate, decay, initial, reset, scale, want_final)
     else:
-        y, final, _ = _forward(x, input_gate, decay_gate, decay, initial, reset, float(scale), return_final_state)
-    return (y, final) if return_final_state else y
+        y, final, _ = _forward(x, input_gate, decay_gate, decay, initial, reset, scale, want_final)
+    return (y, final) if want_final else y
 
 
 def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, out_state=None):
@@ -207,17 +297,12 @@ def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, 
         with torch.no_grad():
             out_state.copy_(final)
         return y[:, 0], out_state
-    x, input_gate, decay_gate = nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate)
-    state, decay = nat.dense(state), nat.dense_f32(decay)
-    batch, channels = x.shape
-    new_state = nat.empty_as(state) if out_state is None else out_state
-    y = nat.empty_as(x)
-    if batch and channels:
-        nat.launch("mko_recur_update", nat.RecurUpdateParams(
-            x.data_ptr(), input_gate.data_ptr(), decay_gate.data_ptr(), decay.data_ptr(), state.data_ptr(),
-            new_state.data_ptr(), y.data_ptr(), batch, channels, x.stride(0), input_gate.stride(0), decay_gate.stride(0),
-            scale, nat.code(x.dtype), nat.code(state.dtype)), x.device)
-    return y, new_state
+    decay = nat.dense_f32(decay)
+    if nat.watched(state, x, input_gate, decay_gate, decay, out_state):
+        y, new_state = nat.through(torch.ops.mko.recur_update, state, x, input_gate, decay_gate, decay, float(scale))
+        return y, new_state if out_state is None else out_state.copy_(new_state)
+    return _update(nat.dense(state), nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate), decay, scale,
+                   nat.empty_as(state) if out_state is None else out_state, nat.empty_as(x))
 
 
 def _step(x, input_gate, decay_gate, decay, scale):

@@ -14,7 +14,10 @@ counterpart in dbydd/metal-kernelops.
 
 from __future__ import annotations
 
+from typing import Optional, Tuple
+
 import torch
+from torch import Tensor
 
 from .. import _native as nat
 from .._contract import Rules
@@ -29,6 +32,58 @@ MAX_INNER = 131071
 """Longest sum of products of two bytes that stays inside int32."""
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _quantize(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """``(q, scale)``, q with its rows' padding."""
+    features, lead = x.shape[-1], x.shape[:-1]
+    pitch = -(-features // ALIGN) * ALIGN
+    q = torch.empty((*lead, pitch), dtype=torch.int8, device=x.device)
+    scale = torch.empty(lead, dtype=torch.float32, device=x.device)
+    if q.numel():
+        if x.dim() != 2 and not x.is_contiguous():
+            x = x.reshape(-1, features)
+        x = nat.rows(x)
+        nat.launch("mko_quantize_int8", nat.QuantizeParams(
+            x.data_ptr(), q.data_ptr(), scale.data_ptr(), q.numel() // pitch, features,
+            x.stride(0) if x.dim() == 2 else features, pitch, nat.code(x.dtype)), x.device)
+    elif not features:
+        scale.zero_()
+    return q, scale
+
+
+_quantize_op = torch.library.custom_op("mko::quantize_int8", _quantize, mutates_args=(), device_types="cuda")
+
+
+@_quantize_op.register_fake
+def _(x):
+    pitch = -(-x.shape[-1] // ALIGN) * ALIGN
+    return x.new_empty((*x.shape[:-1], pitch), dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+def _linear(q: Tensor, q_scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor],
+            out_dtype: torch.dtype) -> Tensor:
+    outer, inner = weight.shape
+    out = torch.empty((*q.shape[:-1], outer), dtype=out_dtype, device=q.device)
+    if out.numel():
+        if inner:
+            if q.dim() != 2 and not q.is_contiguous():
+                q = q.reshape(-1, inner)
+            q, weight = nat.rows(q), nat.rows(weight)
+        qs, ws, b = nat.dense_f32(q_scale), nat.dense_f32(weight_scale), nat.dense_f32(bias)
+        nat.launch("mko_int8_linear", nat.Int8LinearParams(
+            q.data_ptr(), qs.data_ptr(), weight.data_ptr(), ws.data_ptr(), nat.ptr(b), out.data_ptr(),
+            out.numel() // outer, inner, outer, q.stride(0) if q.dim() == 2 else inner, weight.stride(0),
+            nat.code(out_dtype)), q.device)
+    return out
+
+
+_linear_op = torch.library.custom_op("mko::int8_linear", _linear, mutates_args=(), device_types="cuda")
+
+
+@_linear_op.register_fake
+def _(q, q_scale, weight, weight_scale, bias, out_dtype):
+    return q.new_empty((*q.shape[:-1], weight.shape[0]), dtype=out_dtype)
 
 
 def quantize_int8(x):
@@ -48,23 +103,14 @@ def quantize_int8(x):
         rules.dtype_in(_FLOATS, x=x)
     if nat.wants_grad(x):
         rules.fail("8-bit outputs have no gradient; call it under torch.no_grad()")
-    features, lead = x.shape[-1], x.shape[:-1]
-    pitch = -(-features // ALIGN) * ALIGN
-    q = torch.empty((*lead, pitch), dtype=torch.int8, device=x.device)
-    scale = torch.empty(lead, dtype=torch.float32, device=x.device)
-    if q.numel():
-        rows = q.numel() // pitch
-        if rows >= 1 << 22:
-            rules.fail(f"at most 2^22 - 1 rows (got {rows})")
-        if x.dim() != 2 and not x.is_contiguous():
-            x = x.reshape(-1, features)
-        x = nat.rows(x)
-        nat.launch("mko_quantize_int8", nat.QuantizeParams(
-            x.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, features, x.stride(0) if x.dim() == 2 else features, pitch,
-            nat.code(x.dtype)), x.device)
-    elif not features:
-        scale.zero_()
-    return q if pitch == features else q[..., :features], scale
+    features = x.shape[-1]
+    if features and x.numel() >= features << 22:
+        rules.fail(f"at most 2^22 - 1 rows (got {x.numel() // features})")
+    if nat.watched(x):
+        q, scale = nat.through(torch.ops.mko.quantize_int8, x)
+    else:
+        q, scale = _quantize(x)
+    return q if q.shape[-1] == features else q[..., :features], scale
 
 
 def int8_linear(q, q_scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16):
@@ -108,18 +154,9 @@ def int8_linear(q, q_scale, weight, weight_scale, bias=None, out_dtype=torch.bfl
         rules.fail(f"out_dtype should be float32, float16 or bfloat16; it is {out_dtype}")
     if inner > MAX_INNER:
         rules.fail(f"inner is at most {MAX_INNER} here (got {inner})")
-    out = torch.empty((*lead, outer), dtype=out_dtype, device=q.device)
-    if out.numel():
-        rows = out.numel() // outer
-        if inner:
-            if q.dim() != 2 and not q.is_contiguous():
-                q = q.reshape(-1, inner)
-            q, weight = nat.rows(q), nat.rows(weight)
-        qs, ws, b = nat.dense_f32(q_scale), nat.dense_f32(weight_scale), nat.dense_f32(bias)
-        nat.launch("mko_int8_linear", nat.Int8LinearParams(
-            q.data_ptr(), qs.data_ptr(), weight.data_ptr(), ws.data_ptr(), nat.ptr(b), out.data_ptr(), rows, inner,
-            outer, q.stride(0) if q.dim() == 2 else inner, weight.stride(0), nat.code(out_dtype)), q.device)
-    return out
+    if nat.watched(q, q_scale, weight, weight_scale, bias):
+        return nat.through(torch.ops.mko.int8_linear, q, q_scale, weight, weight_scale, bias, out_dtype)
+    return _linear(q, q_scale, weight, weight_scale, bias, out_dtype)
 
 
 def quantize_int8_reference(x):

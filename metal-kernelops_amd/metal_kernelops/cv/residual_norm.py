@@ -20,8 +20,10 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from typing import Optional, Tuple
 
 import torch
+from torch import Tensor
 
 from .. import _native as nat
 from .._contract import Rules
@@ -70,7 +72,8 @@ def _workspace(rows, features, dtype, stream_dtype):
 
 
 def _backward(dout, dstream, stream, weight, rstd, dtype, need_weight):
-    """``(dx, dresidual, dweight)`` of dense operands; one tensor for both where the types agree."""
+    """``(dx, dresidual, dweight)``; one tensor for both where the types agree."""
+    dout, dstream, stream = nat.dense(dout), nat.dense(dstream), nat.dense(stream)
     device, dres = stream.device, nat.empty_as(stream)
     dx = dres if stream.dtype == dtype else torch.empty(stream.shape, dtype=dtype, device=device)
     dweight = torch.empty(weight.shape, dtype=torch.float32, device=device) if need_weight else None
@@ -90,6 +93,21 @@ def _backward(dout, dstream, stream, weight, rstd, dtype, need_weight):
     return dx, dres, dweight
 
 
+def _grads(ctx, dout, dstream, _drstd=None):
+    """The gradients of the inputs of :class:`_ResidualNorm` and of the custom op."""
+    stream, weight, rstd = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    if dout is None:  # only the stream was used
+        return (None if dstream is None else dstream.to(ctx.dtype), None, dstream if need[2] else None, None)
+    # a backward that is itself recorded goes through the op, which refuses to be differentiated
+    plain = not torch.is_grad_enabled() and nat.plain_call(dout, dstream, stream, weight, rstd)
+    backward = _backward if plain else torch.ops.mko.resnorm_bwd
+    dx, dres, dweight = backward(dout, dstream, stream, weight, rstd, ctx.dtype, need[1])
+    if stream.dtype == ctx.dtype:
+        dres = dx
+    return dx, dweight.to(weight.dtype) if need[1] else None, dres if need[2] else None, None
+
+
 class _ResidualNorm(torch.autograd.Function):
     """Forward and analytic first-order backward through the C ABI.  It takes and returns whole
     shapes: x and the residual get one gradient tensor where their types agree, and autograd
@@ -103,18 +121,79 @@ class _ResidualNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)  # an unused output reaches backward as None
         return out, stream
 
-    @staticmethod
-    @nat.first_order
-    def backward(ctx, dout, dstream):
-        stream, weight, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dstream = None if dstream is None else nat.dense(dstream)
-        if dout is None:  # only the stream was used
-            return (None if dstream is None else dstream.to(ctx.dtype), None, dstream if need[2] else None, None)
-        dx, dres, dweight = _backward(nat.dense(dout), dstream, nat.dense(stream), weight, rstd, ctx.dtype, need[1])
-        if dweight is not None and weight.dtype != torch.float32:
-            dweight = dweight.to(weight.dtype)
-        return dx, dweight, dres if need[2] else None, None
+    backward = staticmethod(_grads)
+
+
+def _resnorm_fwd_op(x: Tensor, weight: Tensor, residual: Optional[Tensor], eps: float
+                    ) -> Tuple[Tensor, Tensor, Tensor]:
+    out, stream, rstd = _forward(x, nat.dense(weight), residual, eps, True)
+    return out, nat.absent(stream, x), rstd
+
+
+_resnorm_fwd = torch.library.custom_op("mko::resnorm_fwd", _resnorm_fwd_op, mutates_args=(), device_types="cuda")
+
+
+@_resnorm_fwd.register_fake
+def _(x, weight, residual, eps):
+    return (x.new_empty(x.shape), x.new_empty(0) if residual is None else residual.new_empty(residual.shape),
+            x.new_empty(x.shape[:-1], dtype=torch.float32))
+
+
+def _resnorm_bwd_op(dout: Tensor, dstream: Optional[Tensor], stream: Tensor, weight: Tensor, rstd: Tensor,
+                    dtype: torch.dtype, need_weight: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    dx, dres, dweight = _backward(dout, dstream, stream, nat.dense(weight), rstd, dtype, need_weight)
+    return dx, nat.absent(None if dres is dx else dres, dx), nat.absent(dweight, rstd)
+
+
+_resnorm_bwd = torch.library.custom_op("mko::resnorm_bwd", _resnorm_bwd_op, mutates_args=(), device_types="cuda")
+
+
+@_resnorm_bwd.register_fake
+def _(dout, dstream, stream, weight, rstd, dtype, need_weight):
+    return (stream.new_empty(stream.shape, dtype=dtype),
+            stream.new_empty(0 if stream.dtype == dtype else stream.shape),
+            rstd.new_empty(weight.shape if need_weight else 0))
+
+
+def _setup(ctx, inputs, output):
+    x, weight, residual, _ = inputs
+    ctx.save_for_backward(x if residual is None else output[1], weight, output[2])
+    ctx.dtype = x.dtype
+    ctx.set_materialize_grads(False)
+
+
+torch.library.register_autograd("mko::resnorm_fwd", _grads, setup_context=_setup)
+
+
+def _int8(x, weight, residual, eps):
+    """``(q, scale, stream)``, q with its rows' padding; stream is None without a residual."""
+    lead, features = x.shape[:-1], x.shape[-1]
+    pitch = -(-features // ALIGN) * ALIGN
+    q = torch.empty((*lead, pitch), dtype=torch.int8, device=x.device)
+    scale = torch.empty(lead, dtype=torch.float32, device=x.device)
+    stream = None if residual is None else nat.empty_as(residual)
+    if x.numel():
+        _launch_fwd(x, weight, residual, None, q, scale, stream, None, pitch, eps)
+    elif not features:
+        scale.zero_()
+    return q, scale, stream
+
+
+def _resnorm_int8_op(x: Tensor, weight: Tensor, residual: Optional[Tensor], eps: float
+                     ) -> Tuple[Tensor, Tensor, Tensor]:
+    q, scale, stream = _int8(x, nat.dense(weight), residual, eps)
+    return q, scale, nat.absent(stream, x)
+
+
+_resnorm_int8 = torch.library.custom_op("mko::resnorm_int8", _resnorm_int8_op, mutates_args=(), device_types="cuda")
+
+
+@_resnorm_int8.register_fake
+def _(x, weight, residual, eps):
+    lead, features = x.shape[:-1], x.shape[-1]
+    return (x.new_empty((*lead, -(-features // ALIGN) * ALIGN), dtype=torch.int8),
+            x.new_empty(lead, dtype=torch.float32),
+            x.new_empty(0) if residual is None else residual.new_empty(residual.shape))
 
 
 def _checked(op, x, weight, residual):
@@ -153,10 +232,13 @@ def rmsnorm_residual(x, weight, residual=None, eps=1e-5):
         ``out`` in ``x.dtype`` and ``stream`` in the residual's.
     """
     w = _checked("rmsnorm_residual", x, weight, residual)
-    if nat.wants_grad(x, weight, residual):
-        out, stream = _ResidualNorm.apply(x, w, residual, float(eps))
+    eps = float(eps)
+    if nat.watched(x, w, residual):
+        out, stream, _ = nat.through(torch.ops.mko.resnorm_fwd, x, w, residual, eps)
+    elif nat.wants_grad(x, w, residual):
+        out, stream = _ResidualNorm.apply(x, w, residual, eps)
     else:
-        out, stream, _ = _forward(x, w, residual, float(eps), False)
+        out, stream, _ = _forward(x, w, residual, eps, False)
     return out, x if residual is None else stream
 
 
@@ -172,16 +254,12 @@ def rmsnorm_residual_int8(x, weight, residual=None, eps=1e-5):
     w = _checked("rmsnorm_residual_int8", x, weight, residual)
     if nat.wants_grad(x, weight, residual):
         Rules("rmsnorm_residual_int8").fail("8-bit outputs have no gradient; call it under torch.no_grad()")
-    lead, features = x.shape[:-1], x.shape[-1]
-    pitch = -(-features // ALIGN) * ALIGN
-    q = torch.empty((*lead, pitch), dtype=torch.int8, device=x.device)
-    scale = torch.empty(lead, dtype=torch.float32, device=x.device)
-    stream = x if residual is None else nat.empty_as(residual)
-    if x.numel():
-        _launch_fwd(x, w, residual, None, q, scale, None if residual is None else stream, None, pitch, float(eps))
-    elif not features:
-        scale.zero_()
-    return q if pitch == features else q[..., :features], scale, stream
+    if nat.watched(x, w, residual):
+        q, scale, stream = nat.through(torch.ops.mko.resnorm_int8, x, w, residual, float(eps))
+    else:
+        q, scale, stream = _int8(x, w, residual, float(eps))
+    features = x.shape[-1]
+    return q if q.shape[-1] == features else q[..., :features], scale, x if residual is None else stream
 
 
 def rmsnorm_residual_reference(x, weight, residual=None, eps=1e-5):
