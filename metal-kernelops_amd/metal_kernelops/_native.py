@@ -396,6 +396,12 @@ def through(op, *args):
     return op(*args)
 
 
+def written(t):
+    """Tells autograd that a kernel has written ``t``, so that a graph that saved it before refuses its
+    backward, as after a torch operation in place."""
+    torch._C._increment_version((t,))
+
+
 def stream_of(device):
     return torch.cuda.current_stream(device).cuda_stream
 

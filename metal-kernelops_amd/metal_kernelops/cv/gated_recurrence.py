@@ -301,8 +301,11 @@ def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, 
     if nat.watched(state, x, input_gate, decay_gate, decay, out_state):
         y, new_state = nat.through(torch.ops.mko.recur_update, state, x, input_gate, decay_gate, decay, float(scale))
         return y, new_state if out_state is None else out_state.copy_(new_state)
-    return _update(nat.dense(state), nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate), decay, scale,
-                   nat.empty_as(state) if out_state is None else out_state, nat.empty_as(x))
+    y, new_state = _update(nat.dense(state), nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate), decay, scale,
+                           nat.empty_as(state) if out_state is None else out_state, nat.empty_as(x))
+    if out_state is not None:
+        nat.written(out_state)
+    return y, new_state
 
 
 def _step(x, input_gate, decay_gate, decay, scale):
