@@ -289,6 +289,8 @@ def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, 
         if out_state.requires_grad:
             rules.fail("out_state is overwritten in place, so it may not require grad")
     if nat.wants_grad(state, x, input_gate, decay_gate, decay):
+        if out_state is not None and out_state.untyped_storage()._cdata == state.untyped_storage()._cdata:
+            state = state.clone()  # the backward reads the entering state, which its destination overwrites
         y, final = gated_recurrence(x[:, None], input_gate[:, None], decay_gate[:, None], decay, initial_state=state,
                                     scale=scale, return_final_state=True)
         final = final.to(state.dtype)

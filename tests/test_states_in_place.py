@@ -19,7 +19,7 @@ def _recurrence_step(state, batch=2, channels=24):
 def test_an_update_in_place_moves_the_version(monkeypatch):
     from metal_kernelops import _native as nat
     from metal_kernelops.cv import gated_recurrence
-    monkeypatch.setattr(gated_recurrence.__globals__["nat"], "launch", lambda *a: None)
+    monkeypatch.setattr(nat, "launch", lambda *a: None)
     monkeypatch.setitem(gated_recurrence.__globals__, "_require_gpu", lambda t: None)
     state = torch.randn(2, 24)
     leaf = torch.ones(2, 24, requires_grad=True)
@@ -33,6 +33,27 @@ def test_an_update_in_place_moves_the_version(monkeypatch):
     with torch.inference_mode():  # such tensors have no version
         _recurrence_step(torch.zeros(2, 24))
     assert nat.written(state) is None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("alias", ["itself", "data", "detached"])
+def test_a_recorded_update_keeps_the_entering_state(monkeypatch, alias, dtype):
+    from metal_kernelops import _native as nat
+    from metal_kernelops.cv import gated_recurrence, gated_recurrence_update
+    kept = []
+    monkeypatch.setattr(nat, "launch", lambda name, p, device: kept.append((name, p.initial)))
+    monkeypatch.setitem(gated_recurrence.__globals__, "_require_gpu", lambda t: None)
+    state = torch.randn(2, 24).to(dtype)
+    if alias != "itself":
+        state.requires_grad_(True)
+    out = {"itself": state, "data": state.data, "detached": state.detach()}[alias]
+    x = torch.randn(2, 24, requires_grad=True)
+    y, new = gated_recurrence_update(state, x, x, x, torch.randn(24), out_state=out)
+    assert new is out and not new.requires_grad
+    y.sum().backward()
+    assert [name for name, _ in kept] == ["mko_recur_fwd", "mko_recur_bwd"]
+    assert kept[0][1] == kept[1][1] != out.data_ptr()  # both read the state from memory of its own
+    assert x.grad is not None and (alias == "itself" or state.grad.dtype == dtype)
 
 
 # --------------------------------------------------------------------------- GPU
@@ -52,3 +73,24 @@ def test_a_scan_whose_state_was_overwritten_refuses_its_backward():
     with torch.inference_mode():
         held = torch.zeros(2, 24, device=DEV)
         assert torch.isfinite(_recurrence_step(held)[1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("alias", ["itself", "data"])
+def test_gradients_of_an_update_in_place(alias, dtype):
+    """Those of the same call with a destination of its own, bit for bit."""
+    from metal_kernelops.cv import gated_recurrence_update
+    x, ig, rg = (torch.randn(3, 40, device=DEV) for _ in range(3))
+    start, decay, dy = torch.randn(3, 40, device=DEV).to(dtype), torch.randn(40, device=DEV), torch.randn(3, 40, device=DEV)
+
+    def run(in_place):
+        state = start.clone().requires_grad_(alias == "data")
+        leaves = [t.clone().requires_grad_(True) for t in (x, ig, rg, decay)]
+        out = (state.data if alias == "data" else state) if in_place else None
+        y, new = gated_recurrence_update(state, *leaves, out_state=out)
+        grads = torch.autograd.grad(y, leaves + ([state] if alias == "data" else []), dy)
+        assert out is None or new is out
+        return [y.detach(), new.detach(), *grads]
+
+    assert all(torch.equal(a, b) for a, b in zip(run(True), run(False)))
