@@ -56,6 +56,22 @@ def test_a_recorded_update_keeps_the_entering_state(monkeypatch, alias, dtype):
     assert x.grad is not None and (alias == "itself" or state.grad.dtype == dtype)
 
 
+@pytest.mark.parametrize("shift", [0, 1, -1, 3])
+def test_a_shifted_destination_is_not_read(monkeypatch, shift):
+    """Rows of one buffer moved by ``shift`` rows: the kernel reads a copy unless they are the same."""
+    from metal_kernelops import _native as nat
+    from metal_kernelops.cv import gated_recurrence, gated_recurrence_update
+    seen = []
+    monkeypatch.setattr(nat, "launch", lambda name, p, device: seen.append((p.state, p.new_state)))
+    monkeypatch.setitem(gated_recurrence.__globals__, "_require_gpu", lambda t: None)
+    buffer, x = torch.zeros(9, 24), torch.zeros(3, 24)
+    state, out = buffer[3:6], buffer[3 + shift:6 + shift]
+    gated_recurrence_update(state, x, x, x, x[0], out_state=out)
+    read, wrote = seen[0]
+    assert wrote == out.data_ptr()
+    assert (read == state.data_ptr()) == (shift in (0, 3))  # three rows on is another place altogether
+
+
 # --------------------------------------------------------------------------- GPU
 
 
@@ -94,3 +110,13 @@ def test_gradients_of_an_update_in_place(alias, dtype):
         return [y.detach(), new.detach(), *grads]
 
     assert all(torch.equal(a, b) for a, b in zip(run(True), run(False)))
+
+
+@pytest.mark.gpu
+def test_a_destination_shifted_against_the_state():
+    from metal_kernelops.cv import gated_recurrence_update
+    buffer, x = torch.randn(600, 520, device=DEV), torch.randn(599, 520, device=DEV)
+    decay = torch.randn(520, device=DEV)
+    want = gated_recurrence_update(buffer[:-1].clone(), x, x, x, decay)
+    got = gated_recurrence_update(buffer[:-1], x, x, x, decay, out_state=buffer[1:])
+    assert torch.equal(got[0], want[0]) and torch.equal(buffer[1:], want[1])
