@@ -247,6 +247,8 @@ def mamba2_state_update(state, x, dt, A, B, C, D=None, z=None, dt_bias=None,
         new_state = out_state if out_state is not None else torch.empty_like(kstate)
         y = torch.empty(state.shape[:3], dtype=dtype, device=state.device)
         _launch(kstate, kx, kdt, kA, kB, kC, kD, kz, kbias, bool(dt_softplus), new_state, y)
+        if out_state is not None:
+            nat.written(out_state)
         return y, new_state
 
     if (out_state is not None and state.requires_grad

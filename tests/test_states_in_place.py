@@ -13,6 +13,13 @@ def _recurrence_step(state, batch=2, channels=24):
     return gated_recurrence_update(state, x, x, x, x[0].clone(), out_state=state)
 
 
+def _ssm_step(state, **kw):
+    from metal_kernelops.cv import mamba2_state_update
+    (b, h, d, n), dev = state.shape, state.device
+    x, B = torch.randn(b, h, d, device=dev), torch.randn(b, 1, n, device=dev)
+    return mamba2_state_update(state, x, torch.rand(b, h, device=dev), -torch.rand(h, device=dev), B, B, **kw)
+
+
 # --------------------------------------------------------------------------- CPU: the launch replaced
 
 
@@ -120,3 +127,19 @@ def test_a_destination_shifted_against_the_state():
     want = gated_recurrence_update(buffer[:-1].clone(), x, x, x, decay)
     got = gated_recurrence_update(buffer[:-1], x, x, x, decay, out_state=buffer[1:])
     assert torch.equal(got[0], want[0]) and torch.equal(buffer[1:], want[1])
+
+
+@pytest.mark.gpu
+def test_an_ssm_state_in_place_moves_the_version():
+    state = torch.randn(2, 4, 8, 16, device=DEV)
+    dt = torch.rand(2, 4, device=DEV, requires_grad=True)
+    from metal_kernelops.cv import mamba2_state_update
+    x, B = torch.randn(2, 4, 8, device=DEV), torch.randn(2, 1, 16, device=DEV)
+    y, _ = mamba2_state_update(state, x, dt, -torch.rand(4, device=DEV), B, B)
+    with torch.no_grad():
+        assert _ssm_step(state, out_state=state)[1] is state
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    with torch.inference_mode():
+        held = torch.zeros(2, 4, 8, 16, device=DEV)
+        assert torch.isfinite(_ssm_step(held, out_state=held)[1]).all()
