@@ -251,7 +251,7 @@ def mamba2_state_update(state, x, dt, A, B, C, D=None, z=None, dt_bias=None,
             nat.written(out_state)
         return y, new_state
 
-    if (out_state is not None and state.requires_grad
+    if (out_state is not None
             and out_state.untyped_storage().data_ptr() == state.untyped_storage().data_ptr()):
         # The backward needs the entering state, which an aliasing destination overwrites.
         state = state.clone()

@@ -143,3 +143,22 @@ def test_an_ssm_state_in_place_moves_the_version():
     with torch.inference_mode():
         held = torch.zeros(2, 4, 8, 16, device=DEV)
         assert torch.isfinite(_ssm_step(held, out_state=held)[1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("alias", ["itself", "data"])
+def test_gradients_of_an_ssm_update_in_place(alias):
+    from metal_kernelops.cv import mamba2_state_update
+    start, x, dt = (torch.randn(s, device=DEV) for s in ((2, 4, 8, 16), (2, 4, 8), (2, 4)))
+    A, B, dy = -torch.rand(4, device=DEV), torch.randn(2, 1, 16, device=DEV), torch.randn(2, 4, 8, device=DEV)
+
+    def run(in_place):
+        state = start.clone().requires_grad_(alias == "data")
+        leaves = [t.clone().requires_grad_(True) for t in (x, dt, A, B)]
+        out = (state.data if alias == "data" else state) if in_place else None
+        y, new = mamba2_state_update(state, *leaves, leaves[-1], out_state=out)
+        grads = torch.autograd.grad(y, leaves + ([state] if alias == "data" else []), dy)
+        assert out is None or new is out
+        return [y.detach(), new.detach(), *grads]
+
+    assert all(torch.equal(a, b) for a, b in zip(run(True), run(False)))
