@@ -14,7 +14,7 @@ Layouts: ``state (batch, nheads, dim, dstate)``, ``x/z (batch, nheads, dim)``,
 ``B/C (batch, ngroups, dstate)``, ``D (nheads,)`` or ``(nheads, dim)``.
 
 Kernels (``libmko.so``): the forward is one fused read-modify-write of the state
-per step; with no input requiring grad the entry point launches it directly, the
+per step; an ordinary eager call with no input requiring grad launches it directly, the
 path a decode loop takes.  The backward is two launches with one writer per
 gradient element, so repeated runs are bit-identical.  Inputs are read in the
 dtype the reference would hand its kernel: x/dt/B/C/z are rounded to
@@ -118,14 +118,16 @@ def _launch(state, x, dt, A, B, C, D, z, dt_bias, softplus, new_state, y):
               "mko_state_update_fwd")
 
 
-@torch.library.custom_op("mko::state_update_fwd", mutates_args=(), device_types="cuda")
-def _su_fwd(state: Tensor, x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor,
-            D: Optional[Tensor], z: Optional[Tensor], dt_bias: Optional[Tensor], softplus: bool
-            ) -> Tuple[Tensor, Tensor]:
+def _su_fwd_impl(state: Tensor, x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor,
+                 D: Optional[Tensor], z: Optional[Tensor], dt_bias: Optional[Tensor], softplus: bool
+                 ) -> Tuple[Tensor, Tensor]:
     new_state = torch.empty_like(state)
     y = torch.empty(state.shape[:3], dtype=state.dtype, device=state.device)
     _launch(state, x, dt, A, B, C, D, z, dt_bias, softplus, new_state, y)
     return y, new_state
+
+
+_su_fwd = nat.dense_op("mko::state_update_fwd", _su_fwd_impl)
 
 
 @_su_fwd.register_fake
@@ -242,6 +244,10 @@ def mamba2_state_update(state, x, dt, A, B, C, D=None, z=None, dt_bias=None,
 
     needs_grad = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (state, x, dt, A, B, C, D, z, dt_bias))
+    if not needs_grad and nat.watched(state, kx, kdt, kA, kB, kC, kD, kz, kbias, out_state):
+        y, new_state = nat.through(torch.ops.mko.state_update_fwd, state, kx, kdt, kA, kB, kC, kD, kz, kbias,
+                                   bool(dt_softplus))
+        return y, new_state if out_state is None else out_state.copy_(new_state)
     if not needs_grad:
         kstate = state if state.is_contiguous() else state.contiguous()
         new_state = out_state if out_state is not None else torch.empty_like(kstate)

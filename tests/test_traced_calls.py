@@ -1,4 +1,4 @@
-"""The recurrent layer's operators under what watches a call: a trace holds the operators themselves, not
+"""Operators under what watches a call: a trace holds the operators themselves, not
 only the allocation of their outputs, and its replay on other inputs gives the eager results; modes and
 a recording profiler see them by name.  The CPU tests trace fake GPU tensors and launch nothing."""
 
@@ -61,6 +61,11 @@ def _linear(q, qs, w, ws, bias):
     return (int8_linear(q, qs, w, ws, bias, out_dtype=torch.float32),)
 
 
+def _ssm_update(state, x, dt, A, B):
+    from metal_kernelops.cv import mamba2_state_update
+    return mamba2_state_update(state, x, dt, A, B, B, dt_softplus=True)
+
+
 def _normal(*shape, dtype=torch.float32):
     return lambda g: torch.randn(shape, generator=g).to(dtype)
 
@@ -80,6 +85,8 @@ CALLS = {
     "norm first": (_norm_first, [_normal(5, 50), _normal(50)], "resnorm_fwd", True),
     "norm int8": (_norm_int8, [_normal(5, 50, dtype=BF16), _normal(50), _normal(5, 50)], "resnorm_int8", False),
     "quantise": (_quantise, [_normal(2, 3, 50)], "quantize_int8", False),
+    "ssm update": (_ssm_update, [_normal(2, 4, 8, 16), _normal(2, 4, 8), _normal(2, 4), _normal(4), _normal(2, 1, 16)],
+                   "state_update_fwd", True),
     "linear": (_linear, [_bytes(20, 64), _normal(20), _bytes(30, 64), _normal(30), _normal(30)], "int8_linear", False),
 }
 
