@@ -33,8 +33,10 @@ reference's composed arithmetic for that case.
 from __future__ import annotations
 
 import ctypes
+from typing import Optional, Tuple
 
 import torch
+from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
@@ -92,14 +94,44 @@ def _backward(dout, x, weight, bias, z, rstd, group, gate, need_weight, need_bia
     return dx, dz, dweight, dbias
 
 
+def _fwd_op(x: Tensor, weight: Tensor, bias: Optional[Tensor], z: Optional[Tensor], eps: float, group: int, gate: int
+            ) -> Tuple[Tensor, Tensor]:
+    return _forward(x, weight, bias, z, eps, group, gate)
+
+
+_gated_norm_fwd = nat.dense_op("mko::gated_norm_fwd", _fwd_op)
+
+
+@_gated_norm_fwd.register_fake
+def _(x, weight, bias, z, eps, group, gate):
+    return x.new_empty(x.shape), x.new_empty(x.shape[0] * (x.shape[1] // group), dtype=torch.float32)
+
+
+def _bwd_op(dout: Tensor, x: Tensor, weight: Tensor, bias: Optional[Tensor], z: Optional[Tensor], rstd: Tensor,
+            group: int, gate: int, need_weight: bool, need_bias: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    grads = _backward(dout, x, weight, bias, z, rstd, group, gate, need_weight, need_bias)
+    return tuple(nat.absent(g, rstd) for g in grads)
+
+
+_gated_norm_bwd = nat.dense_op("mko::gated_norm_bwd", _bwd_op)
+
+
+@_gated_norm_bwd.register_fake
+def _(dout, x, weight, bias, z, rstd, group, gate, need_weight, need_bias):
+    return (x.new_empty(x.shape), rstd.new_empty(0) if z is None else z.new_empty(z.shape),
+            rstd.new_empty(weight.shape if need_weight else 0), rstd.new_empty(bias.shape if need_bias else 0))
+
+
 class _GatedRMSNorm(torch.autograd.Function):
     """Fused forward, analytic first-order backward (as the reference's ``_GatedRMSNorm``,
     ``cv/gated_norm.py:563-645``).  A plain autograd Function calling the C ABI: the
-    host cost per call is a few microseconds, which is what a layer this short needs."""
+    host cost per call is a few microseconds, which is what a layer this short needs.  A
+    trace or a mode gets the custom ops."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, z, eps, group, gate):
-        out, rstd = _forward(x, weight, bias, z, eps, group, gate)
+        forward = torch.ops.mko.gated_norm_fwd if nat.watched(x, weight, bias, z) else _forward
+        out, rstd = forward(x, weight, bias, z, eps, group, gate)
         ctx.save_for_backward(x, weight, bias, z, rstd)
         ctx.group, ctx.gate = group, gate
         return out
@@ -110,8 +142,9 @@ class _GatedRMSNorm(torch.autograd.Function):
         x, weight, bias, z, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
         need_bias = bool(need[2] and bias is not None)
-        dx, dz, dweight, dbias = _backward(dout.contiguous(), x, weight, bias, z, rstd, ctx.group, ctx.gate,
-                                           bool(need[1]), need_bias)
+        backward = torch.ops.mko.gated_norm_bwd if nat.watched(dout, x, weight, bias, z, rstd) else _backward
+        dx, dz, dweight, dbias = backward(dout.contiguous(), x, weight, bias, z, rstd, ctx.group, ctx.gate,
+                                          bool(need[1]), need_bias)
         return (dx, dweight.to(weight.dtype) if need[1] else None, dbias.to(bias.dtype) if need_bias else None,
                 dz if z is not None and need[3] else None, None, None, None)
 

@@ -66,6 +66,11 @@ def _ssm_update(state, x, dt, A, B):
     return mamba2_state_update(state, x, dt, A, B, B, dt_softplus=True)
 
 
+def _gated_norm(x, weight, bias, z):
+    from metal_kernelops.cv import rmsnorm_gated
+    return (rmsnorm_gated(x, weight, bias, z),)
+
+
 def _normal(*shape, dtype=torch.float32):
     return lambda g: torch.randn(shape, generator=g).to(dtype)
 
@@ -87,6 +92,7 @@ CALLS = {
     "quantise": (_quantise, [_normal(2, 3, 50)], "quantize_int8", False),
     "ssm update": (_ssm_update, [_normal(2, 4, 8, 16), _normal(2, 4, 8), _normal(2, 4), _normal(4), _normal(2, 1, 16)],
                    "state_update_fwd", True),
+    "gated norm": (_gated_norm, [_normal(2, 5, 48), _normal(48), _normal(48), _normal(2, 5, 48)], "gated_norm_fwd", True),
     "linear": (_linear, [_bytes(20, 64), _normal(20), _bytes(30, 64), _normal(30), _normal(30)], "int8_linear", False),
 }
 
