@@ -130,11 +130,11 @@ def _merge_impl(x: Tensor, height: int, width: int, scale: float) -> Tensor:
     return _merge_all([x], height, width, scale)[0]
 
 
-# The layout launches as torch ops; the 2D scan's own autograd function calls the
-# implementations directly (a dispatcher round trip per launch costs more host time than
+# The layout launches as torch ops; in an ordinary eager call the 2D scan's own autograd function
+# calls the implementations directly (a dispatcher round trip per launch costs more host time than
 # the launch itself on these small maps).
-_path_stack = torch.library.custom_op("mko::path_stack", _stack_impl, mutates_args=(), device_types="cuda")
-_path_merge = torch.library.custom_op("mko::path_merge", _merge_impl, mutates_args=(), device_types="cuda")
+_path_stack = nat.dense_op("mko::path_stack", _stack_impl)
+_path_merge = nat.dense_op("mko::path_merge", _merge_impl)
 
 
 @_path_stack.register_fake
@@ -147,12 +147,39 @@ def _(x, height, width, scale):
     return x.new_empty(x.shape[0], x.shape[1] // 4, x.shape[2])
 
 
-def _stacked(u, dt, A, B, C):
+class _Ops:
+    """The launches of the 2D scan as custom ops, for a call that a trace or a mode has to see."""
+
+    @staticmethod
+    def stack_all(xs, height, width, scale):
+        return [torch.ops.mko.path_stack(x, height, width, scale) for x in xs]
+
+    @staticmethod
+    def merge_all(xs, height, width, scale):
+        return [torch.ops.mko.path_merge(x, height, width, scale) for x in xs]
+
+    @staticmethod
+    def scan(*args):
+        return torch.ops.mko.selscan_fwd(*args)
+
+    @staticmethod
+    def scan_backward(*args):
+        return torch.ops.mko.selscan_bwd(*args)
+
+
+class _Direct:
+    """The same launched directly."""
+
+    stack_all, merge_all = staticmethod(_stack_all), staticmethod(_merge_all)
+    scan, scan_backward = staticmethod(selscan_fwd_impl), staticmethod(selscan_bwd_impl)
+
+
+def _stacked(run, u, dt, A, B, C):
     """The four-path problem as one Mamba-1 problem: (b, 4C, L), (4C, N), (b, 4G, N, L)."""
     batch, channels, height, width = u.shape
     groups, states = B.shape[1], A.shape[1]
     length = height * width
-    su, sdt, sb, sc = _stack_all(
+    su, sdt, sb, sc = run.stack_all(
         [u.reshape(batch, channels, length), dt.reshape(batch, channels, length),
          B.reshape(batch, groups * states, length), C.reshape(batch, groups * states, length)], height, width, 1.0)
     shape = (batch, 4 * groups, states, length)
@@ -163,9 +190,10 @@ class _PathScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, dt, A, B, C, scale):
         batch, channels, height, width = u.shape
-        su, sdt, sa, sb, sc = _stacked(u, dt, A, B, C)
-        ys, ck = selscan_fwd_impl(su, sdt, sa, sb, sc, None, None, None, False)
-        out = _merge_impl(ys, height, width, scale)
+        run = _Ops if nat.watched(u, dt, A, B, C) else _Direct
+        su, sdt, sa, sb, sc = _stacked(run, u, dt, A, B, C)
+        ys, ck = run.scan(su, sdt, sa, sb, sc, None, None, None, False)
+        (out,) = run.merge_all([ys], height, width, scale)
         ctx.scale = scale
         ctx.dims = (batch, channels, height, width, B.shape[1], A.shape[1])
         ctx.u_dtype = u.dtype
@@ -180,10 +208,12 @@ class _PathScan(torch.autograd.Function):
         su, sdt, sa, sb, sc, ck = ctx.saved_tensors
         batch, channels, height, width, groups, states = ctx.dims
         length = height * width
-        sdy = _stack_impl(dy.to(ctx.u_dtype).contiguous().reshape(batch, channels, length), height, width, ctx.scale)
-        dus, ddts, das, dbs, dcs, _, _, _ = selscan_bwd_impl(sdy, su, sdt, sa, sb, sc, None, None, None, False, ck)
+        run = _Ops if nat.watched(dy, su, sdt, sa, sb, sc, ck) else _Direct
+        (sdy,) = run.stack_all([dy.to(ctx.u_dtype).contiguous().reshape(batch, channels, length)], height, width,
+                               ctx.scale)
+        dus, ddts, das, dbs, dcs, _, _, _ = run.scan_backward(sdy, su, sdt, sa, sb, sc, None, None, None, False, ck)
         rows = (batch, 4 * groups * states, length)
-        du, ddt, dB, dC = _merge_all([dus, ddts, dbs.reshape(rows), dcs.reshape(rows)], height, width, 1.0)
+        du, ddt, dB, dC = run.merge_all([dus, ddts, dbs.reshape(rows), dcs.reshape(rows)], height, width, 1.0)
         du, ddt = (t.view(batch, channels, height, width) for t in (du, ddt))
         dB, dC = (t.view(batch, groups, states, height, width) for t in (dB, dC))
         dA = das.view(4, channels, states).sum(0)

@@ -71,6 +71,11 @@ def _gated_norm(x, weight, bias, z):
     return (rmsnorm_gated(x, weight, bias, z),)
 
 
+def _ss2d(u, dt, A, B, C):
+    from metal_kernelops.cv import ss2d_scan
+    return (ss2d_scan(u, dt.abs(), -A.abs(), B, C, merge="mean"),)
+
+
 def _normal(*shape, dtype=torch.float32):
     return lambda g: torch.randn(shape, generator=g).to(dtype)
 
@@ -93,6 +98,8 @@ CALLS = {
     "ssm update": (_ssm_update, [_normal(2, 4, 8, 16), _normal(2, 4, 8), _normal(2, 4), _normal(4), _normal(2, 1, 16)],
                    "state_update_fwd", True),
     "gated norm": (_gated_norm, [_normal(2, 5, 48), _normal(48), _normal(48), _normal(2, 5, 48)], "gated_norm_fwd", True),
+    "ss2d": (_ss2d, [_normal(1, 4, 5, 6), _normal(1, 4, 5, 6), _normal(4, 8), _normal(1, 2, 8, 5, 6), _normal(1, 2, 8, 5, 6)],
+             "selscan_fwd", True),
     "linear": (_linear, [_bytes(20, 64), _normal(20), _bytes(30, 64), _normal(30), _normal(30)], "int8_linear", False),
 }
 
