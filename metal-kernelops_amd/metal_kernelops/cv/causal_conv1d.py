@@ -181,6 +181,7 @@ torch.library.register_autograd("mko::conv1d_fwd", _backward, setup_context=_set
 
 @torch.library.custom_op("mko::conv1d_update", mutates_args=("state",), device_types="cuda")
 def _conv1d_update(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Tensor], silu: bool) -> Tensor:
+    x, weight, bias = x.contiguous(), weight.contiguous(), nat.dense(bias)  # a ZeroTensor comes as one element
     out = torch.empty_like(x)
     if x.numel() == 0:
         return out

@@ -148,7 +148,7 @@ def _recur_bwd_op(dy: Optional[Tensor], dfinal: Optional[Tensor], x: Tensor, inp
                   ) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     dx, dig, drg, ddecay, dinitial = _backward(
         dy, dfinal, nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate), nat.dense(decay), nat.dense(initial),
-        nat.dense(reset), states, scale, need_decay, need_initial)
+        nat.dense(reset), nat.dense(states), scale, need_decay, need_initial)
     return dx, dig, drg, nat.absent(ddecay, decay), nat.absent(dinitial, decay)
 
 

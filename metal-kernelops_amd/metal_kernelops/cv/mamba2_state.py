@@ -135,11 +135,10 @@ def _(state, x, dt, A, B, C, D, z, dt_bias, softplus):
     return state.new_empty(state.shape[:3]), torch.empty_like(state)
 
 
-@torch.library.custom_op("mko::state_update_bwd", mutates_args=(), device_types="cuda")
-def _su_bwd(state: Tensor, x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor,
-            D: Optional[Tensor], z: Optional[Tensor], dt_bias: Optional[Tensor], softplus: bool,
-            dy: Optional[Tensor], dnew: Optional[Tensor]
-            ) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+def _su_bwd_impl(state: Tensor, x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor,
+                 D: Optional[Tensor], z: Optional[Tensor], dt_bias: Optional[Tensor], softplus: bool,
+                 dy: Optional[Tensor], dnew: Optional[Tensor]
+                 ) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
     f32 = dict(dtype=torch.float32, device=state.device)
     gstate = torch.empty(state.shape, **f32)
     dx = torch.empty(x.shape, **f32)
@@ -165,6 +164,9 @@ def _su_bwd(state: Tensor, x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tenso
     nat.check(lib.mko_state_update_bwd(ctypes.byref(p), nat.stream_of(state.device)),
               "mko_state_update_bwd")
     return gstate, dx, ddt, dA, dB, dC, dD, dz, dbias
+
+
+_su_bwd = nat.dense_op("mko::state_update_bwd", _su_bwd_impl)
 
 
 @_su_bwd.register_fake

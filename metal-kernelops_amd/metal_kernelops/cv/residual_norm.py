@@ -141,7 +141,7 @@ def _(x, weight, residual, eps):
 
 def _resnorm_bwd_op(dout: Tensor, dstream: Optional[Tensor], stream: Tensor, weight: Tensor, rstd: Tensor,
                     dtype: torch.dtype, need_weight: bool) -> Tuple[Tensor, Tensor, Tensor]:
-    dx, dres, dweight = _backward(dout, dstream, stream, nat.dense(weight), rstd, dtype, need_weight)
+    dx, dres, dweight = _backward(dout, dstream, stream, nat.dense(weight), nat.dense(rstd), dtype, need_weight)
     return dx, nat.absent(None if dres is dx else dres, dx), nat.absent(dweight, rstd)
 
 

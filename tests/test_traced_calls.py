@@ -264,3 +264,21 @@ def test_a_traced_update_in_place_replays():
             states = args[0].clone(), args[0].clone()
             got, want = graph(states[0], *args[1:]), call(states[1], *args[1:])
             assert same(got, want) and torch.equal(*states)
+
+
+@pytest.mark.gpu
+def test_conv1d_update_materialises_negated_views_and_zero_tensors():
+    from metal_kernelops.cv import causal_conv1d_update
+    g = torch.Generator().manual_seed(6)
+    x, window, weight, bias = (torch.randn(s, generator=g).to(DEV) for s in ((2, 40), (2, 40, 3), (40, 4), (40,)))
+
+    def call(x, weight, bias):
+        state = window.clone()
+        return causal_conv1d_update(x, state, weight, bias, activation="silu"), state
+
+    def zero(t):
+        return torch._efficientzerotensor(tuple(t.shape), device=DEV)
+
+    assert same(call(torch._neg_view(x), weight, bias), call(-x, weight, bias))
+    assert same(call(zero(x), weight, bias), call(torch.zeros_like(x), weight, bias))
+    assert same(call(x, zero(weight), zero(bias)), call(x, torch.zeros_like(weight), torch.zeros_like(bias)))
