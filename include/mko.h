@@ -538,10 +538,10 @@ int mko_resnorm_bwd(const mko_resnorm_params* p, void* stream);
 
 /* Per row of x: amax = max |x|, q = rint(x * (127 / amax)), scale = amax / 127; the
  * quotients and the product are rounded once each to float32.  Rows of zeros, infinities
- * and NaN as in the norm above. */
+ * and NaN as in the norm above; rows without features have scale 0. */
 typedef struct mko_quantize_params {
-  const void* x;           /* (rows, features) of dtype, row stride x_stride */
-  int8_t* q;               /* (rows, q_stride), columns features .. q_stride zeroed */
+  const void* x;           /* (rows, features) of dtype, row stride x_stride; NULL without features */
+  int8_t* q;               /* (rows, q_stride), columns features .. q_stride zeroed; NULL if q_stride is 0 */
   float* scale;            /* (rows,) */
   int64_t rows, features, x_stride, q_stride;
   int32_t dtype;

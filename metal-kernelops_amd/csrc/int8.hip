@@ -611,9 +611,9 @@ extern "C" int mko_quantize_int8(const mko_quantize_params* p, void* stream) {
     mko_set_error("quantize_int8: rows is below 2^22");
     return MKO_EUNSUPPORTED;
   }
-  if (p->rows == 0 || p->q_stride == 0) return MKO_OK;
-  if (!p->scale || (p->features && (!p->x || !p->q))) {
-    mko_set_error("quantize_int8: x, q and scale are required");
+  if (p->rows == 0) return MKO_OK;
+  if (!p->scale || (p->features && !p->x) || (p->q_stride && !p->q)) {
+    mko_set_error("quantize_int8: x, q (of a padding alone too) and scale are required");
     return MKO_EINVAL;
   }
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -40,15 +40,13 @@ def _quantize(x: Tensor) -> Tuple[Tensor, Tensor]:
     pitch = -(-features // ALIGN) * ALIGN
     q = torch.empty((*lead, pitch), dtype=torch.int8, device=x.device)
     scale = torch.empty(lead, dtype=torch.float32, device=x.device)
-    if q.numel():
+    if scale.numel():
         if x.dim() != 2 and not x.is_contiguous():
-            x = x.reshape(-1, features)
+            x = x.reshape(scale.numel(), features)
         x = nat.rows(x)
         nat.launch("mko_quantize_int8", nat.QuantizeParams(
-            x.data_ptr(), q.data_ptr(), scale.data_ptr(), q.numel() // pitch, features,
+            x.data_ptr(), q.data_ptr(), scale.data_ptr(), scale.numel(), features,
             x.stride(0) if x.dim() == 2 else features, pitch, nat.code(x.dtype)), x.device)
-    elif not features:
-        scale.zero_()
     return q, scale
 
 
@@ -104,8 +102,8 @@ def quantize_int8(x):
     if nat.wants_grad(x):
         rules.fail("8-bit outputs have no gradient; call it under torch.no_grad()")
     features = x.shape[-1]
-    if features and x.numel() >= features << 22:
-        rules.fail(f"at most 2^22 - 1 rows (got {x.numel() // features})")
+    if x.numel() >= features << 22 and x.shape[:-1].numel() >= 1 << 22:
+        rules.fail(f"at most 2^22 - 1 rows (got {x.shape[:-1].numel()})")
     if nat.watched(x):
         q, scale = nat.through(torch.ops.mko.quantize_int8, x)
     else:
