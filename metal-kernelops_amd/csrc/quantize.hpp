@@ -36,7 +36,8 @@ __device__ __forceinline__ RowScale row_scale(uint32_t amax) {
   return r;
 }
 
-// rint(v * inv), to nearest even, as an integer in [-127, 127]; NaN gives 0.
+// rint(v * inv), to nearest even, as an integer in [-127, 127].  A NaN, in whose row the scale is not
+// finite, gives -127: the maximum drops it.
 __device__ __forceinline__ int quantise(float v, float inv) {
   const float q = rintf(fp32_value(v * inv));
   return static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
