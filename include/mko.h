@@ -450,7 +450,7 @@ typedef struct mko_recur_params {
   float* final_state;      /* forward: (batch, channels) or NULL */
   float* states;           /* mko_recur_states_size() bytes: the state after every
                               MKO_RECUR_CHUNK steps, which the backward reads; the forward
-                              always writes it */
+                              always writes it.  At a multiple of 16 bytes */
   const void* dy;          /* backward */
   const float* dfinal;     /* backward: (batch, channels) or NULL */
   void* dx;                /* backward */
@@ -458,7 +458,7 @@ typedef struct mko_recur_params {
   void* ddecay_gate;       /* backward */
   float* ddecay;           /* backward: (channels,), summed over batch and time, or NULL */
   float* dinitial;         /* backward: (batch, channels) or NULL */
-  void* workspace;         /* mko_recur_{fwd,bwd}_workspace_size() bytes */
+  void* workspace;         /* mko_recur_{fwd,bwd}_workspace_size() bytes, at a multiple of 16 */
   size_t workspace_bytes;
   int64_t batch, length, channels;
   int64_t x_stride_b, x_stride_t, ig_stride_b, ig_stride_t, rg_stride_b, rg_stride_t;

@@ -682,6 +682,9 @@ void clear_cells(const mko_recur_params* p, const Chain& ch, hipStream_t s) {
                 reinterpret_cast<uint4*>(ch.maps), maps, reinterpret_cast<uint4*>(ch.ends), ends, ch.tickets));
 }
 
+// The chain's cells are cleared 16 bytes at a time, and a map is one 64-bit atomic word.
+bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+
 unsigned workgroups(const Geo& g) {
   return static_cast<unsigned>(cdiv(g.chains, g.counters) * g.counters * g.chunks);
 }
@@ -755,6 +758,10 @@ extern "C" int mko_recur_fwd(const mko_recur_params* p, void* stream) {
     mko_set_error("recur_fwd: workspace of %zu bytes needed, %zu given", need, p->workspace_bytes);
     return MKO_EWORKSPACE;
   }
+  if (need && (recur::misaligned(p->workspace) || recur::misaligned(p->states))) {
+    mko_set_error("recur_fwd: workspace and states start at multiples of 16 bytes");
+    return MKO_EINVAL;
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   const recur::Geo g = recur::geo(p);
   recur::Chain ch{};
@@ -793,6 +800,10 @@ extern "C" int mko_recur_bwd(const mko_recur_params* p, void* stream) {
   if (need && (!p->workspace || p->workspace_bytes < need)) {
     mko_set_error("recur_bwd: workspace of %zu bytes needed, %zu given", need, p->workspace_bytes);
     return MKO_EWORKSPACE;
+  }
+  if (need && recur::misaligned(p->workspace)) {
+    mko_set_error("recur_bwd: workspace starts at a multiple of 16 bytes");
+    return MKO_EINVAL;
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   const recur::Geo g = recur::geo(p);
