@@ -644,8 +644,10 @@ int check(const mko_recur_params* p, const char* what) {
     mko_set_error("%s: dtype must be float32, float16 or bfloat16", what);
     return MKO_EINVAL;
   }
-  if (p->batch > kMostBatch || p->channels > kMostSide || p->length > kMostSide ||
-      cdiv(p->batch * cdiv(p->channels, 64 * kV), kCounters) * kCounters * cdiv(p->length, kChunk) > kMostWorkgroups) {
+  const bool sides = p->batch <= kMostBatch && p->channels <= kMostSide && p->length <= kMostSide;
+  const int64_t chains = sides ? cdiv(p->batch * cdiv(p->channels, 64 * kV), kCounters) * kCounters : 0;
+  // chains * chunks may pass 64 bits
+  if (!sides || (p->length > 0 && chains > kMostWorkgroups / cdiv(p->length, kChunk))) {
     mko_set_error("%s: batch is at most 65535, and batch * channels / 128, up to the next multiple of 8, times "
                   "length / 64 at most 2^22", what);
     return MKO_EUNSUPPORTED;
