@@ -19,8 +19,6 @@ namespace {
 constexpr int64_t kMaxInner = 131071;
 constexpr int64_t kMaxSide = 1 << 26;
 
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // A team of waves holds a row in registers between its largest value and its bytes, NV vectors of 16
 // bytes of x a thread.
 template <typename T, int NV>
@@ -64,7 +62,7 @@ __global__ void __launch_bounds__(1024) quantize_rows(mko_quantize_params p, int
     for (int e = 0; e < VEC; ++e) b[e] = quantise(v[e], q.inv);
     store_bytes<VEC>(out, static_cast<int64_t>(lt + k * team_threads) * VEC, n, p.q_stride, b);
   }
-  for (int64_t i = cdiv_dev(n, VEC) * VEC + lt; i < p.q_stride; i += team_threads) out[i] = 0;
+  for (int64_t i = cdiv(n, VEC) * VEC + lt; i < p.q_stride; i += team_threads) out[i] = 0;
 }
 
 // Rows wider than a team's registers are read twice.
@@ -568,8 +566,6 @@ void launch(const mko_int8_linear_params& p, hipStream_t s) {
   launch_tile<64, 64, 2, 2, 128, 3, true>(p, direct, s);
 }
 
-bool half_or_float(int32_t dtype) { return dtype == MKO_F32 || dtype == MKO_F16 || dtype == MKO_BF16; }
-
 int check(const mko_int8_linear_params* p) {
   if (!p || p->rows < 0 || p->inner < 0 || p->outer < 0) {
     mko_set_error("int8_linear: params is NULL or a size is negative");
@@ -603,7 +599,7 @@ extern "C" int mko_quantize_int8(const mko_quantize_params* p, void* stream) {
     mko_set_error("quantize_int8: params is NULL, a size is negative or q_stride is smaller than features");
     return MKO_EINVAL;
   }
-  if (!int8::half_or_float(p->dtype)) {
+  if (!half_or_float(p->dtype)) {
     mko_set_error("quantize_int8: dtype must be float32, float16 or bfloat16");
     return MKO_EINVAL;
   }

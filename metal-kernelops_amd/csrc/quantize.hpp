@@ -43,8 +43,6 @@ __device__ __forceinline__ int quantise(float v, float inv) {
   return static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
 }
 
-__device__ __forceinline__ int64_t cdiv_dev(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // NE bytes from column i of a row of n columns padded to `pitch`, the padding zero.  Rows start at
 // any byte.
 template <int NE>

@@ -27,8 +27,6 @@ constexpr int kV = 2;  // channels a lane of the scans takes
 constexpr int64_t kMostBatch = 65535, kMostSide = int64_t{1} << 31;
 constexpr int64_t kMostWorkgroups = int64_t{1} << 22;  // of 512 threads: 2^31 threads in a launch
 
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // A channel's rate in units of the binary exponential: v log2(e) = rate s(rg).
 __device__ __forceinline__ float binary_rate(float scale, float decay) { return scale * kLog2e * softplus(decay); }
 
@@ -89,6 +87,7 @@ __device__ __forceinline__ float both(float P, float Q) {
 
 template <typename T, int V>
 struct Raw {
+  static_assert(V == 2, "a word of 16-bit values");
   uint32_t w[sizeof(T) == 4 ? V : 1];
 };
 
@@ -128,17 +127,13 @@ __device__ __forceinline__ Raw<T, V> load(const T* row, const Place<FULL>& c) {
   };
   const T* p = row + c.first;
   Raw<T, V> r;
-  if constexpr (sizeof(T) == 2 && V == 1) {
-    r.w[0] = bits_at(p, c.at(0));
-  } else {
-    if constexpr (FULL) {
-      r = reinterpret_cast<const Any*>(at_bytes(p, c.off * static_cast<uint32_t>(sizeof(T))))->r;
-    } else if constexpr (sizeof(T) == 4) {
+  if constexpr (FULL) {
+    r = reinterpret_cast<const Any*>(at_bytes(p, c.off * static_cast<uint32_t>(sizeof(T))))->r;
+  } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) r.w[e] = bits_at(p, c.at(e));
-    } else {
-      r.w[0] = bits_at(p, c.at(0)) | bits_at(p, c.at(1)) << 16;
-    }
+    for (int e = 0; e < V; ++e) r.w[e] = bits_at(p, c.at(e));
+  } else {
+    r.w[0] = bits_at(p, c.at(0)) | bits_at(p, c.at(1)) << 16;
   }
   return r;
 }
@@ -148,9 +143,6 @@ __device__ __forceinline__ void unpack(const Raw<T, V>& r, float (&f)[V]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = __uint_as_float(r.w[e]);
-  } else if constexpr (V == 1) {
-    float hi;
-    unpack2<T>(r.w[0], f[0], hi);
   } else {
     unpack2<T>(r.w[0], f[0], f[1]);
   }
@@ -158,7 +150,7 @@ __device__ __forceinline__ void unpack(const Raw<T, V>& r, float (&f)[V]) {
 
 template <typename T, int V, bool FULL>
 __device__ __forceinline__ void store(T* row, const Place<FULL>& c, const float (&f)[V]) {
-  if constexpr (V == 2 && FULL) {
+  if constexpr (FULL) {
     Raw<T, V> r;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -629,8 +621,6 @@ __global__ void __launch_bounds__(kThreads) update(mko_recur_update_params p) {
   static_cast<T*>(p.y)[b * p.channels + d] = from_f32<T>(h);
 }
 
-bool half_or_float(int32_t dtype) { return dtype == MKO_F32 || dtype == MKO_F16 || dtype == MKO_BF16; }
-
 int check(const mko_recur_params* p, const char* what) {
   if (!p) {
     mko_set_error("%s: params is NULL", what);
@@ -827,7 +817,7 @@ extern "C" int mko_recur_bwd(const mko_recur_params* p, void* stream) {
     recur::launch<_Float16>(*p, g, ch, part, true, s);
   if (p->ddecay)
     MKO_TIMED("recur_bwd_finish", s,
-              recur::finish<<<static_cast<unsigned>(recur::cdiv(p->channels, 32)), kColumnThreads, 0, s>>>(
+              recur::finish<<<static_cast<unsigned>(cdiv(p->channels, 32)), kColumnThreads, 0, s>>>(
                   *p, part, p->batch * g.chunks));
   return mko_check_launch("recur_bwd");
 }
@@ -854,7 +844,7 @@ extern "C" int mko_recur_update(const mko_recur_update_params* p, void* stream) 
     mko_set_error("recur_update: params is NULL or a size is negative");
     return MKO_EINVAL;
   }
-  if (!recur::half_or_float(p->dtype) || !recur::half_or_float(p->state_dtype)) {
+  if (!half_or_float(p->dtype) || !half_or_float(p->state_dtype)) {
     mko_set_error("recur_update: dtype and state_dtype must be float32, float16 or bfloat16");
     return MKO_EINVAL;
   }

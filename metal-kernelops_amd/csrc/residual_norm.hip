@@ -26,8 +26,6 @@ constexpr int kBwdThreads = 512;
 constexpr int kBwdMostVectors = 3;  // with five arrays a vector, more would leave one wave a SIMD
 constexpr int kBwdBlocks = 512;     // two workgroups a CU; more only add partial sums
 
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 struct Geo {
   int team;         // threads of a team
   int64_t blocks;   // backward: workgroups
@@ -130,7 +128,7 @@ __global__ void __launch_bounds__(kMostWaves * kWave) forward(mko_resnorm_params
       store_bytes<VEC>(out, i, n, p.q_stride, b);
     }
     // whole vectors past the end, where the rows are padded by more than one
-    for (int64_t i = cdiv_dev(n, VEC) * VEC + lt; i < p.q_stride; i += g.team) out[i] = 0;
+    for (int64_t i = cdiv(n, VEC) * VEC + lt; i < p.q_stride; i += g.team) out[i] = 0;
   } else {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -336,8 +334,6 @@ __global__ void __launch_bounds__(kThreads) weight_wide(mko_resnorm_params p, fl
 }
 
 // ------------------------------------------------------------------ the choice
-
-bool half_or_float(int32_t dtype) { return dtype == MKO_F32 || dtype == MKO_F16 || dtype == MKO_BF16; }
 
 int check(const mko_resnorm_params* p, const char* what) {
   if (!p || p->rows < 0 || p->features < 0) {

@@ -1,9 +1,14 @@
-// Vectors of consecutive elements of a row at any alignment, and column sums in a fixed order.
+// Vectors of consecutive elements of a row at any alignment, column sums in a fixed order, and what
+// the entry points of the row operators share.
 #pragma once
 
 #include "common.hpp"
 
 namespace mko {
+
+__host__ __device__ __forceinline__ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+inline bool half_or_float(int32_t dtype) { return dtype == MKO_F32 || dtype == MKO_F16 || dtype == MKO_BF16; }
 
 // Elements of a 16-byte vector of T.
 template <typename T>
