@@ -16,7 +16,7 @@ DEV = "cuda"
 F32_TOL = 1e-5
 TOL = {torch.float32: F32_TOL, torch.float16: F32_TOL + 2.0 ** -11, torch.bfloat16: F32_TOL + 2.0 ** -8}
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
-# one step, one channel; lengths around the 128 steps of a chunk and its fractions; many chunks;
+# one step, one channel; lengths around two chunks of 64 steps and their fractions; many chunks;
 # channel counts around a wavefront's and odd ones
 SHAPES = [(1, 1, 1), (2, 1, 64), (1, 2, 130), (3, 15, 65), (2, 127, 3), (1, 128, 64), (2, 129, 129), (1, 257, 200),
           (5, 64, 31), (2, 1000, 77), (1, 4500, 40)]
