@@ -503,7 +503,8 @@ int mko_recur_update(const mko_recur_update_params* p, void* stream);
  *           out = v;  or, when q is given,  q = rint(v * 127 / amax), q_scale = amax / 127
  * with amax the row's largest |v|.  The stored stream is what is normalised, so the
  * backward, which reads it, sees the forward's own values.  A row of zeros has q_scale 0;
- * one that holds an infinity or a NaN has an infinite or NaN q_scale.
+ * one that holds an infinity or a NaN has an infinite or NaN q_scale.  Without features (or rows)
+ * nothing is launched or written.
  * x and residual have unit feature stride and the given row strides; weight is contiguous. */
 typedef struct mko_resnorm_params {
   const void* x;           /* (rows, features) of dtype; forward */

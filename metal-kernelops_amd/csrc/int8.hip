@@ -545,7 +545,9 @@ void launch(const mko_int8_linear_params& p, hipStream_t s) {
   // `few` reads the tokens again for every 16 channels, so it is for small outputs, and without direct
   // loads for somewhat larger ones.  us, few against 64 x 64 tiles: 17 x 2560 x 2560 5.5 and 8.6, 32 x 2560 x
   // 2560 6.1 and 8.5, 48 x 2560 x 2560 7.6 and 8.6; 17 x 10240 x 2560 10.4 and 9.4, 48 x 5120 x 2560 12.3 and
-  // 9.0; unaligned, 77 x 4099 x 1000 9.4 and 11.0, 256 x 2560 x 2568 26.7 and 19.0.
+  // 9.0.  Unaligned, of 256 x 1000, 256 x 1536 and 512 x 1000 outputs (1.95, 3 and 3.9 times 2^17):
+  //   inner 1000:  7.5 and 11.2,   8.5 and 10.7,   9.7 and 11.3;   inner 777:   9.4 and 11.0,  11.7 and 10.6,  14.3 and 11.1;
+  //   inner 2568:  9.7 and 16.1,  12.5 and 15.7,  20.4 and 16.2;   inner 5000: 18.6 and 24.1,  20.0 and 23.7,  33.6 and 24.1.
   const bool direct = direct_loads(p);
   const int64_t outputs = p.rows * p.outer;
   if (p.rows <= 16) return launch_few<1>(p, s);
