@@ -130,7 +130,8 @@ class _GatedRMSNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, z, eps, group, gate):
-        forward = torch.ops.mko.gated_norm_fwd if nat.watched(x, weight, bias, z) else _forward
+        ctx.through_op = nat.watched(x, weight, bias, z)
+        forward = torch.ops.mko.gated_norm_fwd if ctx.through_op else _forward
         out, rstd = forward(x, weight, bias, z, eps, group, gate)
         ctx.save_for_backward(x, weight, bias, z, rstd)
         ctx.group, ctx.gate = group, gate
@@ -142,7 +143,7 @@ class _GatedRMSNorm(torch.autograd.Function):
         x, weight, bias, z, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
         need_bias = bool(need[2] and bias is not None)
-        backward = torch.ops.mko.gated_norm_bwd if nat.watched(dout, x, weight, bias, z, rstd) else _backward
+        backward = torch.ops.mko.gated_norm_bwd if ctx.through_op or nat.watched(dout) else _backward
         dx, dz, dweight, dbias = backward(dout.contiguous(), x, weight, bias, z, rstd, ctx.group, ctx.gate,
                                           bool(need[1]), need_bias)
         return (dx, dweight.to(weight.dtype) if need[1] else None, dbias.to(bias.dtype) if need_bias else None,

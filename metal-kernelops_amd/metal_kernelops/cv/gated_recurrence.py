@@ -102,11 +102,13 @@ def _grads(ctx, dy, dfinal, _states=None):
     x, input_gate, decay_gate, decay, initial, reset, states = ctx.saved_tensors
     need = ctx.needs_input_grad
     need_decay, need_initial = need[3], initial is not None and need[4]
-    args = (dy, dfinal if ctx.want_final else None, x, input_gate, decay_gate, decay, initial, reset, states)
+    if not ctx.want_final:
+        dfinal = None
     # a backward that is itself recorded goes through the op, which refuses to be differentiated
-    plain = not torch.is_grad_enabled() and nat.plain_call(*args)
-    backward = _backward if plain else torch.ops.mko.recur_bwd
-    dx, dig, drg, ddecay, dinitial = backward(*args, ctx.scale, need_decay, need_initial)
+    op = ctx.through_op or torch.is_grad_enabled() or nat.watched(dy, dfinal)
+    backward = torch.ops.mko.recur_bwd if op else _backward
+    dx, dig, drg, ddecay, dinitial = backward(dy, dfinal, x, input_gate, decay_gate, decay, initial, reset, states,
+                                              ctx.scale, need_decay, need_initial)
     return dx, dig, drg, ddecay if need_decay else None, dinitial if need_initial else None, None, None, None
 
 
@@ -117,7 +119,7 @@ class _Recurrence(torch.autograd.Function):
     def forward(ctx, x, input_gate, decay_gate, decay, initial, reset, scale, want_final):
         y, final, states = _forward(x, input_gate, decay_gate, decay, initial, reset, scale, want_final)
         ctx.save_for_backward(x, input_gate, decay_gate, decay, initial, reset, states)
-        ctx.scale, ctx.want_final = scale, want_final
+        ctx.scale, ctx.want_final, ctx.through_op = scale, want_final, False
         ctx.set_materialize_grads(False)  # an unused output reaches backward as None
         return y, final
 
@@ -164,6 +166,7 @@ def _(dy, dfinal, x, input_gate, decay_gate, decay, initial, reset, states, scal
 def _setup(ctx, inputs, output):
     x, input_gate, decay_gate, decay, initial, reset, ctx.scale, ctx.want_final = inputs
     ctx.save_for_backward(x, input_gate, decay_gate, decay, initial, reset, output[2])
+    ctx.through_op = True  # whatever the forward's tensors were
     ctx.set_materialize_grads(False)
 
 

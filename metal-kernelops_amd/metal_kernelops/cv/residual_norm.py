@@ -100,8 +100,8 @@ def _grads(ctx, dout, dstream, _drstd=None):
     if dout is None:  # only the stream was used
         return (None if dstream is None else dstream.to(ctx.dtype), None, dstream if need[2] else None, None)
     # a backward that is itself recorded goes through the op, which refuses to be differentiated
-    plain = not torch.is_grad_enabled() and nat.plain_call(dout, dstream, stream, weight, rstd)
-    backward = _backward if plain else torch.ops.mko.resnorm_bwd
+    op = ctx.through_op or torch.is_grad_enabled() or nat.watched(dout, dstream)
+    backward = torch.ops.mko.resnorm_bwd if op else _backward
     dx, dres, dweight = backward(dout, dstream, stream, weight, rstd, ctx.dtype, need[1])
     if stream.dtype == ctx.dtype:
         dres = dx
@@ -117,7 +117,7 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps):
         out, stream, rstd = _forward(x, weight, residual, eps, True)
         ctx.save_for_backward(x if stream is None else stream, weight, rstd)
-        ctx.dtype = x.dtype
+        ctx.dtype, ctx.through_op = x.dtype, False
         ctx.set_materialize_grads(False)  # an unused output reaches backward as None
         return out, stream
 
@@ -158,7 +158,7 @@ def _(dout, dstream, stream, weight, rstd, dtype, need_weight):
 def _setup(ctx, inputs, output):
     x, weight, residual, _ = inputs
     ctx.save_for_backward(x if residual is None else output[1], weight, output[2])
-    ctx.dtype = x.dtype
+    ctx.dtype, ctx.through_op = x.dtype, True
     ctx.set_materialize_grads(False)
 
 
