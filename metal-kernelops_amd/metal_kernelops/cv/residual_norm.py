@@ -38,10 +38,9 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 def _rows(t):
     """The rows of ``t`` at one stride: ``t`` itself where it has them, as a 2-d view or a copy."""
-    if t.dim() == 2 or t.is_contiguous():
-        t = nat.rows(t)
-        return t, t.stride(-2) if t.dim() == 2 else t.shape[-1]
-    t = nat.rows(t.reshape(-1, t.shape[-1]))
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    t = nat.rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
     return t, t.stride(0)
 
 
@@ -105,7 +104,11 @@ def _grads(ctx, dout, dstream, _drstd=None):
     dx, dres, dweight = backward(dout, dstream, stream, weight, rstd, ctx.dtype, need[1])
     if stream.dtype == ctx.dtype:
         dres = dx
-    return dx, dweight.to(weight.dtype) if need[1] else None, dres if need[2] else None, None
+    if not need[1]:
+        dweight = None
+    elif weight.dtype != torch.float32:
+        dweight = dweight.to(weight.dtype)
+    return dx, dweight, dres if need[2] else None, None
 
 
 class _ResidualNorm(torch.autograd.Function):
