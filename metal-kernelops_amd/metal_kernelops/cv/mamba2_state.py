@@ -113,9 +113,7 @@ def _launch(state, x, dt, A, B, C, D, z, dt_bias, softplus, new_state, y):
         return
     p = _params(state, x, dt, A, B, C, D, z, dt_bias, softplus)
     p.new_state, p.y = new_state.data_ptr(), y.data_ptr()
-    lib = nat.lib()
-    nat.check(lib.mko_state_update_fwd(ctypes.byref(p), nat.stream_of(state.device)),
-              "mko_state_update_fwd")
+    nat.launch("mko_state_update_fwd", p, state.device)
 
 
 def _su_fwd_impl(state: Tensor, x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor,
