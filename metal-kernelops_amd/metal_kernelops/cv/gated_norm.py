@@ -72,7 +72,7 @@ def _forward(x, weight, bias, z, eps, group, gate):
     if x.numel():
         p = _params(x, weight, bias, z, eps, group, gate)
         p.out, p.rstd = out.data_ptr(), rstd.data_ptr()
-        nat.check(nat.lib().mko_gated_norm_fwd(ctypes.byref(p), nat.stream_of(x.device)), "mko_gated_norm_fwd")
+        nat.launch("mko_gated_norm_fwd", p, x.device)
     return out, rstd
 
 
@@ -90,7 +90,7 @@ def _backward(dout, x, weight, bias, z, rstd, group, gate, need_weight, need_bia
         size = nat.lib().mko_gated_norm_bwd_workspace_size(ctypes.byref(p))
         ws = nat.workspace(size, x.device) if size else None
         p.workspace, p.workspace_bytes = nat.ptr(ws), size
-        nat.check(nat.lib().mko_gated_norm_bwd(ctypes.byref(p), nat.stream_of(x.device)), "mko_gated_norm_bwd")
+        nat.launch("mko_gated_norm_bwd", p, x.device)
     return dx, dz, dweight, dbias
 
 
