@@ -396,6 +396,12 @@ def through(op, *args):
     return op(*args)
 
 
+def unshifted(t, out):
+    """``t``, or a copy of it where its memory overlaps that of its destination ``out`` (both dense, of
+    one size) without being the same: threads would overwrite what others have yet to read."""
+    return t.clone() if 0 < abs(out.data_ptr() - t.data_ptr()) < t.numel() * t.element_size() else t
+
+
 def written(t):
     """Tells autograd that a kernel has written ``t``, so that a graph that saved it before refuses its
     backward, as after a torch operation in place."""

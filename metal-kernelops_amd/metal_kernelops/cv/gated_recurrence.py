@@ -308,9 +308,7 @@ def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, 
         return y, new_state if out_state is None else out_state.copy_(new_state)
     state = nat.dense(state)
     if out_state is not None and out_state is not state:
-        apart = abs(out_state.data_ptr() - state.data_ptr())
-        if 0 < apart < state.numel() * state.element_size():
-            state = state.clone()  # shifted against its destination: other threads' values would be overwritten
+        state = nat.unshifted(state, out_state)
     y, new_state = _update(state, nat.rows(x), nat.rows(input_gate), nat.rows(decay_gate), decay, scale,
                            nat.empty_as(state) if out_state is None else out_state, nat.empty_as(x))
     if out_state is not None:

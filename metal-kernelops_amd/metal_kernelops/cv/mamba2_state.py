@@ -250,6 +250,8 @@ def mamba2_state_update(state, x, dt, A, B, C, D=None, z=None, dt_bias=None,
         return y, new_state if out_state is None else out_state.copy_(new_state)
     if not needs_grad:
         kstate = state if state.is_contiguous() else state.contiguous()
+        if out_state is not None and out_state is not kstate:
+            kstate = nat.unshifted(kstate, out_state)
         new_state = out_state if out_state is not None else torch.empty_like(kstate)
         y = torch.empty(state.shape[:3], dtype=dtype, device=state.device)
         _launch(kstate, kx, kdt, kA, kB, kC, kD, kz, kbias, bool(dt_softplus), new_state, y)

@@ -129,6 +129,24 @@ def test_a_destination_shifted_against_the_state():
     assert torch.equal(got[0], want[0]) and torch.equal(buffer[1:], want[1])
 
 
+def test_only_shifted_memory_is_copied():
+    from metal_kernelops import _native as nat
+    t = torch.zeros(9, 24)
+    for shift in range(-3, 4):
+        state, out = t[3:6], t[3 + shift:6 + shift]
+        assert (nat.unshifted(state, out) is state) == (shift in (0, 3, -3))
+
+
+@pytest.mark.gpu
+def test_an_ssm_destination_shifted_against_the_state():
+    from metal_kernelops.cv import mamba2_state_update
+    buffer, x = torch.randn(300, 4, 8, 16, device=DEV), torch.randn(299, 4, 8, device=DEV)
+    dt, A, B = torch.rand(299, 4, device=DEV), -torch.rand(4, device=DEV), torch.randn(299, 1, 16, device=DEV)
+    want = mamba2_state_update(buffer[:-1].clone(), x, dt, A, B, B)
+    got = mamba2_state_update(buffer[:-1], x, dt, A, B, B, out_state=buffer[1:])
+    assert torch.equal(got[0], want[0]) and torch.equal(buffer[1:], want[1])
+
+
 @pytest.mark.gpu
 def test_an_ssm_state_in_place_moves_the_version():
     state = torch.randn(2, 4, 8, 16, device=DEV)
