@@ -357,6 +357,10 @@ _is_compiling, _is_tracing = torch.compiler.is_compiling, torch._C._is_tracing
 _dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
 _transform, _profiling = torch._C._functorch.peek_interpreter_stack, torch._C._autograd._profiler_enabled
 _forward_ad, _is_grad_enabled = torch.autograd.forward_ad, torch.is_grad_enabled
+_byref = ctypes.byref
+# a torch without GPUs has neither, and no tensor to launch on
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def watched(*tensors):
@@ -418,12 +422,12 @@ def launch(name, params, device):
     current for the call.  The stream is asked for as a raw handle: the Stream object that
     ``torch.cuda.current_stream`` builds takes 2 us of host time, as much as a small launch."""
     index = device.index
-    fn = getattr(lib(), name)
-    if index == torch._C._cuda_getDevice():
-        status = fn(ctypes.byref(params), torch._C._cuda_getCurrentRawStream(index))
+    fn = getattr(_lib or lib(), name)
+    if index == _current_device():
+        status = fn(_byref(params), _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(ctypes.byref(params), torch._C._cuda_getCurrentRawStream(index))
+            status = fn(_byref(params), _raw_stream(index))
     if status != 0:
         check(status, name)
 

@@ -201,8 +201,9 @@ def _check(op, x, input_gate, decay_gate, decay, scale, layout):
     """The argument rules that the scan and the update share, in their order.  Messages are formed
     only for an argument that breaks a rule: a decode step's checks are host time."""
     rules = Rules(op)
-    rules.dims("x", x, layout.count(",") + 1, layout)
     shape = x.shape
+    if len(shape) != layout.count(",") + 1:
+        rules.dims("x", x, layout.count(",") + 1, layout)
     if input_gate.shape != shape or decay_gate.shape != shape or decay.shape != shape[-1:]:
         rules.shape("input_gate", input_gate, shape)
         rules.shape("decay_gate", decay_gate, shape)
