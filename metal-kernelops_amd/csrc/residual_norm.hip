@@ -8,8 +8,8 @@
 // row's largest |stream weight| beside its sum of squares; both come from one pass.  The backward's
 // teams walk rows and keep dweight of their columns in registers; a workgroup adds its teams' in
 // order and writes one row of partial sums.  Bound by memory: 8192 x 2560 bf16 forward 30 us (5.6 TB/s),
-// backward 49 us (3.5 TB/s: three operands of a row in registers leave eight waves a CU) and 4 us for
-// the 512 partial rows; in 8 bits 1999 x 2560 in 12 us.
+// backward 49 us (3.5 TB/s: a row's loads are issued after the row before it is stored) and 4 us for the
+// 512 partial rows; in 8 bits 1999 x 2560 in 12 us.
 #include "common.hpp"
 #include "io.hpp"
 #include "quantize.hpp"

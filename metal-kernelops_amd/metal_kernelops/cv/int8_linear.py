@@ -7,8 +7,9 @@ magnitude.  The product of tokens ``(..., inner)`` and weights ``(outer, inner)`
     out[m, n] = q_scale[m] * weight_scale[n] * sum_k q[m, k] * weight[n, k] + bias[n]
 
 on the int8 matrix cores.  The sum is exact in int32 (``inner`` below 2^17); the scales and the
-bias are applied in float32 and the result is rounded once.  A row of zeros has scale 0; a row
-with an infinity or a NaN has a scale that is not finite, and so are its outputs.  There is no
+bias are applied in float32 and the result is rounded once.  A row of zeros, or of magnitudes below
+2^-100, has scale 0; a row with an infinity or a NaN has a scale that is not finite, and so are its
+outputs.  There is no
 counterpart in dbydd/metal-kernelops.
 """
 
