@@ -32,6 +32,7 @@ and bfloat16 run the kernels and other dtypes raise ``ValueError``; ``K <= 32``.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -277,7 +278,7 @@ def causal_conv1d_fn(x, weight, bias=None, activation=None, initial_state=None, 
     # slice of cat(initial_state, x) so that its gradient reaches both
     fused_final = return_final_state and not grads
     args = (work, weight.contiguous(), shift, init)
-    forward = _conv1d_fwd_impl if nat.plain_call(*args) else torch.ops.mko.conv1d_fwd
+    forward = _conv1d_fwd_impl if nat.plain_call(*args) else functools.partial(nat.through, torch.ops.mko.conv1d_fwd)
     out, final = forward(*args, activation is not None, bool(fused_final and work.numel()))
     out = out.to(x.dtype)
     if not return_final_state:
@@ -340,8 +341,7 @@ def causal_conv1d_update(x, state, weight, bias=None, activation=None):
     # the kernel reads and writes every tensor in the state's dtype, computing in float32
     dtype = state.dtype
     work = x.to(dtype).contiguous()
-    out = torch.ops.mko.conv1d_update(work, state, weight.to(dtype).contiguous(),
-                                      bias.to(dtype).contiguous() if bias is not None else None,
-                                      activation is not None)
+    out = nat.through(torch.ops.mko.conv1d_update, work, state, weight.to(dtype).contiguous(),
+                      bias.to(dtype).contiguous() if bias is not None else None, activation is not None)
     out = out.to(x.dtype)
     return out.squeeze(-1) if squeezed else out

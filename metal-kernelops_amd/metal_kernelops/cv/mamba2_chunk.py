@@ -32,6 +32,7 @@ composition); it is once-differentiable.  Tensors must live on a ROCm GPU.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -263,7 +264,7 @@ def mamba2_chunk_scan(x, dt, A, B, C, chunk_size=64, D=None, z=None, dt_bias=Non
     save_y = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (x, dt, A, B, C, D, z, dt_bias, initial_states))
     args = (x, dt, A, B, C, D, z, dt_bias, initial_states)
-    forward = _ssd_fwd_impl if nat.plain_call(*args) else torch.ops.mko.ssd_fwd
+    forward = _ssd_fwd_impl if nat.plain_call(*args) else functools.partial(nat.through, torch.ops.mko.ssd_fwd)
     y, final, _ = forward(*args, bool(dt_softplus), bool(save_y))
     return y, final
 

@@ -21,6 +21,7 @@ bit-deterministic.  The backward is once-differentiable, as in the reference
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -221,7 +222,7 @@ def _run(u, dt, A, B, C, D, z, delta_bias, softplus):
     u, dt, B, C = (t.contiguous() for t in (u, dt, B, C))
     z = None if z is None else z.contiguous()
     args = (u, dt, A, B, C, D, z, delta_bias)
-    forward = selscan_fwd_impl if nat.plain_call(*args) else torch.ops.mko.selscan_fwd
+    forward = selscan_fwd_impl if nat.plain_call(*args) else functools.partial(nat.through, torch.ops.mko.selscan_fwd)
     return forward(*args, bool(softplus))[0]
 
 

@@ -282,3 +282,32 @@ def test_conv1d_update_materialises_negated_views_and_zero_tensors():
     assert same(call(torch._neg_view(x), weight, bias), call(-x, weight, bias))
     assert same(call(zero(x), weight, bias), call(torch.zeros_like(x), weight, bias))
     assert same(call(x, zero(weight), zero(bias)), call(x, torch.zeros_like(weight), torch.zeros_like(bias)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["selscan", "ssd", "conv1d", "conv1d update", "state update", "gated norm", "ss2d"])
+def test_forward_mode_derivatives_are_refused(name):
+    """The dispatcher drops the tangent of an op that has no formula for it; the calls refuse it."""
+    import torch.autograd.forward_ad as fwd
+    from metal_kernelops import cv, selective_scan
+    g = torch.Generator().manual_seed(7)
+
+    def r(*shape):
+        return torch.randn(shape, generator=g).to(DEV)
+
+    calls = {
+        "selscan": (lambda u, *a: selective_scan(u, u.abs(), *a), [r(1, 8, 20), -r(8, 4).abs(), r(1, 1, 4, 20), r(1, 1, 4, 20)]),
+        "ssd": (cv.mamba2_chunk_scan, [r(1, 20, 2, 8), r(1, 20, 2).abs(), -r(2).abs(), r(1, 20, 1, 8), r(1, 20, 1, 8)]),
+        "conv1d": (cv.causal_conv1d_fn, [r(1, 8, 20), r(8, 4), r(8)]),
+        "conv1d update": (cv.causal_conv1d_update, [r(2, 8), r(2, 8, 3), r(8, 4)]),
+        "state update": (_ssm_update, on_gpu("ssm update", 7)),
+        "gated norm": (_gated_norm, on_gpu("gated norm", 7)),
+        "ss2d": (_ss2d, on_gpu("ss2d", 7)),
+    }
+    call, args = calls[name]
+    call(*args)
+    with fwd.dual_level():
+        call(*args)  # no tangent, nothing to refuse
+        dual = fwd.make_dual(args[0], torch.ones_like(args[0]))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call(dual, *args[1:])
