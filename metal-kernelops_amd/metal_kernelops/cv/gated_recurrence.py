@@ -288,7 +288,7 @@ def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, 
     if out_state is not None:
         if out_state.shape != state.shape or out_state.dtype != state.dtype or out_state.device != state.device:
             rules.fail("out_state should have the shape, dtype and device of state")
-        if not out_state.is_contiguous() or out_state.is_neg():
+        if not out_state.is_contiguous():
             rules.fail("out_state should be contiguous")
         if out_state.requires_grad:
             rules.fail("out_state is overwritten in place, so it may not require grad")
@@ -305,6 +305,8 @@ def gated_recurrence_update(state, x, input_gate, decay_gate, decay, scale=8.0, 
         return y[:, 0], out_state
     decay = nat.dense_f32(decay)
     if nat.watched(state, x, input_gate, decay_gate, decay, out_state):
+        if out_state is not None and not torch.compiler.is_compiling() and out_state.is_neg():
+            rules.fail("out_state should be contiguous, and not a negated view")
         y, new_state = nat.through(torch.ops.mko.recur_update, state, x, input_gate, decay_gate, decay, float(scale))
         return y, new_state if out_state is None else out_state.copy_(new_state)
     state = nat.dense(state)

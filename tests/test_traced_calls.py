@@ -311,3 +311,24 @@ def test_forward_mode_derivatives_are_refused(name):
         dual = fwd.make_dual(args[0], torch.ones_like(args[0]))
         with pytest.raises((RuntimeError, NotImplementedError)):
             call(dual, *args[1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", [*CALLS, "update in place"])
+def test_compiles_without_a_graph_break(name):
+    torch._dynamo.reset()
+    if name == "update in place":
+        from metal_kernelops.cv import gated_recurrence_update
+
+        def call(state, *rest):
+            return (gated_recurrence_update(state, *rest, out_state=state)[0],)
+
+        args = on_gpu("update", 8)
+    else:
+        call, args = CALLS[name][0], on_gpu(name, 8)
+    compiled = torch.compile(call, backend="aot_eager", fullgraph=True)
+    with torch.no_grad():
+        mine, theirs = [a.clone() for a in args], [a.clone() for a in args]
+        assert same(compiled(*mine), call(*theirs)) and same(mine, theirs)
+    if CALLS.get(name, (None,) * 4)[3]:
+        assert same(with_gradients(compiled)(*args), with_gradients(call)(*args))
