@@ -567,6 +567,118 @@ typedef struct mko_int8_linear_params {
 size_t mko_sizeof_int8_linear_params(void);
 int mko_int8_linear(const mko_int8_linear_params* p, void* stream);
 
+/* ======================================================================== */
+/* Gated delta rule                                                          */
+/* ======================================================================== */
+
+/* Per (batch, value head h), with the key head h / (heads / key_heads) and a state S of
+ * (value, key), S[-1] = initial or 0:
+ *   e[t] = v[t] - exp(log_decay[t]) S[t-1] k[t]
+ *   S[t] = exp(log_decay[t]) S[t-1] + beta[t] e[t] k[t]^T,  y[t] = scale S[t] q[t]
+ * A log decay below -1e4, -infinity among them, counts as -1e4: it clears the state.
+ * q and k are (batch, length, key_heads, key), v (batch, length, heads, value), of `dtype`, with
+ * unit stride in the last axis and the given strides (in elements) in the others; log_decay and
+ * beta (batch, length, heads) of their own dtypes; states (batch, heads, value, key) of
+ * `state_dtype`.  These and all outputs and gradients are contiguous; a gradient has its
+ * input's dtype.  The recurrence runs over chunks of MKO_DELTA_CHUNK tokens in float32, its
+ * operands rounded to `dtype`; a value that is not finite reaches its whole chunk. */
+typedef struct mko_delta_params {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* log_decay;
+  const void* beta;
+  const void* initial;     /* or NULL */
+  void* y;                 /* forward */
+  void* final_state;       /* forward, or NULL */
+  void* saved;             /* mko_delta_saved_size() bytes at a multiple of 16, which the forward
+                              writes and the backward reads; NULL for a forward without one */
+  const void* dy;          /* backward */
+  const void* dfinal;      /* backward, or NULL */
+  void* dq;                /* backward */
+  void* dk;
+  void* dv;
+  void* dlog_decay;
+  void* dbeta;
+  void* dinitial;          /* backward, or NULL */
+  void* workspace;         /* mko_delta_{fwd,bwd}_workspace_size() bytes at a multiple of 16; the
+                              forward's depends on whether saved is given */
+  size_t workspace_bytes;
+  int64_t batch, length, key_heads, heads, key, value;
+  int64_t q_stride_b, q_stride_t, q_stride_h, k_stride_b, k_stride_t, k_stride_h;
+  int64_t v_stride_b, v_stride_t, v_stride_h;
+  float scale;
+  int32_t dtype, decay_dtype, beta_dtype, state_dtype;
+} mko_delta_params;
+
+#define MKO_DELTA_CHUNK 64
+#define MKO_DELTA_MAX_KEY 256
+
+size_t mko_sizeof_delta_params(void);
+size_t mko_delta_saved_size(const mko_delta_params* p);
+size_t mko_delta_fwd_workspace_size(const mko_delta_params* p);
+int mko_delta_fwd(const mko_delta_params* p, void* stream);
+size_t mko_delta_bwd_workspace_size(const mko_delta_params* p);
+int mko_delta_bwd(const mko_delta_params* p, void* stream);
+
+/* One step of the same: q and k (batch, key_heads, key), v (batch, heads, value), log_decay and
+ * beta (batch, heads), contiguous but for the given batch and head strides of q, k and v; state
+ * and new_state (which may be the same array) of `state_dtype`; y contiguous, of `dtype`. */
+typedef struct mko_delta_update_params {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* log_decay;
+  const void* beta;
+  const void* state;
+  void* new_state;
+  void* y;
+  int64_t batch, key_heads, heads, key, value;
+  int64_t q_stride_b, q_stride_h, k_stride_b, k_stride_h, v_stride_b, v_stride_h;
+  float scale;
+  int32_t dtype, decay_dtype, beta_dtype, state_dtype;
+} mko_delta_update_params;
+
+size_t mko_sizeof_delta_update_params(void);
+int mko_delta_update(const mko_delta_update_params* p, void* stream);
+
+/* ======================================================================== */
+/* Layer norm of the residual stream                                         */
+/* ======================================================================== */
+
+/* Per row:  stream = x + residual, rounded to stream_dtype (x itself without a residual)
+ *           mu = mean(stream),  r = 1 / sqrt(mean((stream - mu)^2) + eps)
+ *           out = (stream - mu) * r * weight + bias
+ * The stored stream is what is normalised.  Without features (or rows) nothing is launched or
+ * written.  x and residual have unit feature stride and the given row strides; the rest is
+ * contiguous. */
+typedef struct mko_layernorm_params {
+  const void* x;           /* (rows, features) of dtype; forward */
+  const void* residual;    /* (rows, features) of stream_dtype, or NULL; forward */
+  const void* weight;      /* (features,) of wdtype */
+  const void* bias;        /* (features,) of bdtype, or NULL; forward */
+  void* out;               /* forward: (rows, features) of dtype */
+  void* stream;            /* the forward writes it when residual is given; the backward reads it */
+  float* stats;            /* (rows, 2): mu and r; the forward writes them when non-NULL, the
+                              backward reads them */
+  const void* dout;        /* backward: (rows, features) of dtype */
+  const void* dstream;     /* backward: gradient that reaches stream, of stream_dtype, or NULL */
+  void* dx;                /* backward: (rows, features) of dtype */
+  void* dresidual;         /* backward: the same gradient in stream_dtype, or NULL */
+  float* dweight;          /* backward: (features,), summed over rows in a fixed order, or NULL */
+  float* dbias;            /* backward: the same, or NULL */
+  void* workspace;         /* backward: mko_layernorm_bwd_workspace_size() bytes */
+  size_t workspace_bytes;
+  int64_t rows, features, x_stride, residual_stride;
+  float eps;
+  int32_t dtype, stream_dtype, wdtype, bdtype;
+} mko_layernorm_params;
+
+size_t mko_sizeof_layernorm_params(void);
+int mko_layernorm_fwd(const mko_layernorm_params* p, void* stream);
+size_t mko_layernorm_bwd_workspace_size(const mko_layernorm_params* p);
+int mko_layernorm_bwd(const mko_layernorm_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -32,16 +32,6 @@ struct Geo {
   int64_t rows_of;  // backward: rows a team walks
 };
 
-// 1 / sqrt(ss * inv_n + eps), rounded once.  In 64 bits, because the backward takes the
-// difference of two terms that each hold r twice: a narrow row amplifies every rounding of r.
-// v_rsq_f64 and one Newton step.
-__device__ __forceinline__ float inverse_norm(float ss, double inv_n, float eps) {
-  const double a = static_cast<double>(ss) * inv_n + static_cast<double>(eps);
-  const double y = __builtin_amdgcn_rsq(a);
-  const double e = 0.5 - 0.5 * a * y * y;
-  return static_cast<float>(e == e ? y + y * e : y);  // a is 0 or infinite: y is exact
-}
-
 // The stream's value at (row, i): x + residual rounded to the stream's type.
 template <typename T, typename S>
 __device__ __forceinline__ float stream_at(const mko_resnorm_params& p, int64_t row, int64_t i) {

@@ -54,6 +54,16 @@ __device__ __forceinline__ void store_part(T* row, int64_t i, int64_t n, const f
     if (i + e < n) row[i + e] = from_f32<T>(f[e]);
 }
 
+// 1 / sqrt(ss * inv_n + eps), rounded once.  In 64 bits, because the backward takes the
+// difference of two terms that each hold r twice: a narrow row amplifies every rounding of r.
+// v_rsq_f64 and one Newton step.
+__device__ __forceinline__ float inverse_norm(float ss, double inv_n, float eps) {
+  const double a = static_cast<double>(ss) * inv_n + static_cast<double>(eps);
+  const double y = __builtin_amdgcn_rsq(a);
+  const double e = 0.5 - 0.5 * a * y * y;
+  return static_cast<float>(e == e ? y + y * e : y);  // a is 0 or infinite: y is exact
+}
+
 // NE values of a parameter of a runtime dtype as float32.
 template <int NE>
 __device__ __forceinline__ void load_param_part(const void* p, int dtype, int64_t i, int64_t n, float (&f)[NE]) {

@@ -180,6 +180,48 @@ class Int8LinearParams(ctypes.Structure):
     ]
 
 
+class LayernormParams(ctypes.Structure):
+    """Mirror of ``mko_layernorm_params``."""
+
+    _fields_ = [
+        ("x", _vp), ("residual", _vp), ("weight", _vp), ("bias", _vp), ("out", _vp), ("stream", _vp), ("stats", _vp),
+        ("dout", _vp), ("dstream", _vp), ("dx", _vp), ("dresidual", _vp), ("dweight", _vp), ("dbias", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("rows", ctypes.c_int64), ("features", ctypes.c_int64), ("x_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64), ("eps", ctypes.c_float), ("dtype", ctypes.c_int32),
+        ("stream_dtype", ctypes.c_int32), ("wdtype", ctypes.c_int32), ("bdtype", ctypes.c_int32),
+    ]
+
+
+class DeltaParams(ctypes.Structure):
+    """Mirror of ``mko_delta_params``."""
+
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("log_decay", _vp), ("beta", _vp), ("initial", _vp), ("y", _vp),
+        ("final_state", _vp), ("saved", _vp), ("dy", _vp), ("dfinal", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+        ("dlog_decay", _vp), ("dbeta", _vp), ("dinitial", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("batch", ctypes.c_int64), ("length", ctypes.c_int64), ("key_heads", ctypes.c_int64), ("heads", ctypes.c_int64),
+        ("key", ctypes.c_int64), ("value", ctypes.c_int64), ("q_stride_b", ctypes.c_int64), ("q_stride_t", ctypes.c_int64),
+        ("q_stride_h", ctypes.c_int64), ("k_stride_b", ctypes.c_int64), ("k_stride_t", ctypes.c_int64),
+        ("k_stride_h", ctypes.c_int64), ("v_stride_b", ctypes.c_int64), ("v_stride_t", ctypes.c_int64),
+        ("v_stride_h", ctypes.c_int64), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
+        ("decay_dtype", ctypes.c_int32), ("beta_dtype", ctypes.c_int32), ("state_dtype", ctypes.c_int32),
+    ]
+
+
+class DeltaUpdateParams(ctypes.Structure):
+    """Mirror of ``mko_delta_update_params``."""
+
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("log_decay", _vp), ("beta", _vp), ("state", _vp), ("new_state", _vp),
+        ("y", _vp), ("batch", ctypes.c_int64), ("key_heads", ctypes.c_int64), ("heads", ctypes.c_int64),
+        ("key", ctypes.c_int64), ("value", ctypes.c_int64), ("q_stride_b", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("k_stride_b", ctypes.c_int64), ("k_stride_h", ctypes.c_int64), ("v_stride_b", ctypes.c_int64),
+        ("v_stride_h", ctypes.c_int64), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
+        ("decay_dtype", ctypes.c_int32), ("beta_dtype", ctypes.c_int32), ("state_dtype", ctypes.c_int32),
+    ]
+
+
 _SIGNATURES = {
     "mko_abi_version": ([], ctypes.c_int),
     "mko_last_error": ([], ctypes.c_char_p),
@@ -238,6 +280,18 @@ _SIGNATURES = {
     "mko_resnorm_bwd": ([ctypes.POINTER(ResnormParams), _vp], ctypes.c_int),
     "mko_quantize_int8": ([ctypes.POINTER(QuantizeParams), _vp], ctypes.c_int),
     "mko_int8_linear": ([ctypes.POINTER(Int8LinearParams), _vp], ctypes.c_int),
+    "mko_sizeof_layernorm_params": ([], ctypes.c_size_t),
+    "mko_layernorm_fwd": ([ctypes.POINTER(LayernormParams), _vp], ctypes.c_int),
+    "mko_layernorm_bwd_workspace_size": ([ctypes.POINTER(LayernormParams)], ctypes.c_size_t),
+    "mko_layernorm_bwd": ([ctypes.POINTER(LayernormParams), _vp], ctypes.c_int),
+    "mko_sizeof_delta_params": ([], ctypes.c_size_t),
+    "mko_delta_saved_size": ([ctypes.POINTER(DeltaParams)], ctypes.c_size_t),
+    "mko_delta_fwd_workspace_size": ([ctypes.POINTER(DeltaParams)], ctypes.c_size_t),
+    "mko_delta_fwd": ([ctypes.POINTER(DeltaParams), _vp], ctypes.c_int),
+    "mko_delta_bwd_workspace_size": ([ctypes.POINTER(DeltaParams)], ctypes.c_size_t),
+    "mko_delta_bwd": ([ctypes.POINTER(DeltaParams), _vp], ctypes.c_int),
+    "mko_sizeof_delta_update_params": ([], ctypes.c_size_t),
+    "mko_delta_update": ([ctypes.POINTER(DeltaUpdateParams), _vp], ctypes.c_int),
     "mko_state_update_bwd_static": ([ctypes.POINTER(StateUpdateParams), _vp], ctypes.c_int),
 }
 
@@ -280,7 +334,10 @@ def lib():
                            (RecurUpdateParams, handle.mko_sizeof_recur_update_params),
                            (ResnormParams, handle.mko_sizeof_resnorm_params),
                            (QuantizeParams, handle.mko_sizeof_quantize_params),
-                           (Int8LinearParams, handle.mko_sizeof_int8_linear_params)):
+                           (Int8LinearParams, handle.mko_sizeof_int8_linear_params),
+                           (LayernormParams, handle.mko_sizeof_layernorm_params),
+                           (DeltaParams, handle.mko_sizeof_delta_params),
+                           (DeltaUpdateParams, handle.mko_sizeof_delta_update_params)):
             if ctypes.sizeof(struct) != fn():
                 raise RuntimeError(f"{struct.__name__} layout does not match libmko.so")
         _lib = handle
