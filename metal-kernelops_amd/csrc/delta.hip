@@ -1,9 +1,10 @@
 // Gated delta rule, forward (delta.hpp has the formulas).
 //
-//   prep  per (batch, head, chunk): the decays' sums, T by blocked substitution in float32, and the
-//         operands T and P (and their transposes, for the backward)
-//   scan  per (batch, head, 16 W value columns), sequential over the chunks: S stays in float32
-//         accumulators, and E and Y of the chunk come out of it on the way
+//   prep  per (batch, head, chunk): the decays' sums, T by blocked substitution in float32, the
+//         operands T and P (and their transposes, for the backward), and W
+//   scan  per (batch, head, 16 W value columns), sequential over the chunks.  W waves carry S in float32
+//         accumulators and do only what the next chunk waits for, E = T V - W S^T and S's update; W
+//         others follow a chunk behind with Y and the stores, and four fetch the chunk ahead.
 #include "delta.hpp"
 
 namespace mko {
@@ -107,9 +108,11 @@ __device__ __forceinline__ void store_half(TM* p, int h, const float (&f)[4]) {
 
 // Wave w owns the row tile w of A and P.
 template <typename TM, int KB, bool TRAIN>
-__global__ void __launch_bounds__(256) prep(Geo g, Ptrs p) {
+__global__ void __launch_bounds__(256) prep(Geo g, Ptrs p, bool fast) {
+  typedef Tile<TM, 32 * KB> KTile;
   __shared__ Tokens tok;
   __shared__ __align__(16) float a[kC * kPitch];
+  __shared__ __align__(16) TM kt[KTile::kElements];
   const WgId id = wg_id(static_cast<int>(g.heads), static_cast<int>(g.chunks));
   const int64_t h = id.x, c = id.y, b = id.z;
   const int64_t at = (b * g.heads + h) * g.chunks + c, t0 = c * kC;
@@ -121,6 +124,13 @@ __global__ void __launch_bounds__(256) prep(Geo g, Ptrs p) {
   TM* lp = static_cast<TM*>(p.lower) + (2 * at + 1) * kSquare;              // P; T is ahead of it
   TM* up = TRAIN ? static_cast<TM*>(p.upper) + (2 * at + 1) * kSquare : lp;  // and their transposes
 
+  if (fast)
+    KTile::template issue<4>(kt, k, g.k_t, rows, key, wave, reinterpret_cast<const TM*>(&zero_unit));
+  else
+    KTile::template copy<256>(kt, k, g.k_t, rows, key);
+  Frag<TM> qf[KB];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) qf[kb] = frag_memory(q, g.q_t, 16 * wave, 32 * kb, rows, key);
   if (wave == 0) {
     const int64_t i = (b * g.length + t0 + lane) * g.heads + h;
     float d = lane < rows ? load_one(p.decay, g.decay_dtype, i) : 0.0f;
@@ -134,27 +144,27 @@ __global__ void __launch_bounds__(256) prep(Geo g, Ptrs p) {
     const double last = __shfl(s, kC - 1);
     tok.c[lane] = s;
     tok.in[lane] = fast_exp2(static_cast<float>(s));
-    tok.out[lane] = fast_exp2(static_cast<float>(last - s));
-    tok.beta[lane] = lane < rows ? load_one(p.beta, g.beta_dtype, i) : 0.0f;
+    const float out = fast_exp2(static_cast<float>(last - s));
+    const float beta = lane < rows ? load_one(p.beta, g.beta_dtype, i) : 0.0f;
+    tok.out[lane] = out;
+    tok.beta[lane] = beta;
+    tok.write[lane] = out * beta;
   }
-  __syncthreads();
+  direct_wait();
   {
     uint32_t* to = reinterpret_cast<uint32_t*>(p.tokens + at);
     const uint32_t* from = reinterpret_cast<const uint32_t*>(&tok);
     for (int i = threadIdx.x; i < static_cast<int>(sizeof(Tokens) / 4); i += 256) to[i] = from[i];
   }
-  Frag<TM> kf[KB], qf[KB];
+  Frag<TM> kf[KB];
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb) {
-    kf[kb] = frag_memory(k, g.k_t, 16 * wave, 32 * kb, rows, key);
-    qf[kb] = frag_memory(q, g.q_t, 16 * wave, 32 * kb, rows, key);
-  }
+  for (int kb = 0; kb < KB; ++kb) kf[kb] = KTile::rows(kt, 16 * wave, 32 * kb);
   const int tr = 16 * wave + 4 * lane_quad(), tc = 16 * wave + lane_col();  // this tile's tokens as rows and columns
   for (int j = 0; j <= wave; ++j) {
     f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0}, kq = {0, 0, 0, 0};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const Frag<TM> o = j == wave ? kf[kb] : frag_memory(k, g.k_t, 16 * j, 32 * kb, rows, key);
+      const Frag<TM> o = KTile::rows(kt, 16 * j, 32 * kb);
       mma(kk, kf[kb], o);             // [t][s]
       mma(kq, o, qf[kb]);             // [s][t]
       if (TRAIN) mma(qk, qf[kb], o);  // [t][s]
@@ -179,14 +189,18 @@ __global__ void __launch_bounds__(256) prep(Geo g, Ptrs p) {
   }
   __syncthreads();
   invert(a);
+  float te[4][4];  // -T exp(c), the lane's token's
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (j / 2 <= wave / 2) {  // T's rows of tile `wave`, columns of tile j
-      const float4 v = *reinterpret_cast<const float4*>(a + tc * kPitch + 16 * j + 4 * lane_quad());
-      const bool in = j <= wave;
-      const float f[4] = {in ? v.x : 0.0f, in ? v.y : 0.0f, in ? v.z : 0.0f, in ? v.w : 0.0f};
-      store_half<TM>(lp - kSquare + lower_at(wave, j / 2), j % 2, f);
-    }
+    const bool in = j <= wave;
+    const float4 v = *reinterpret_cast<const float4*>(a + tc * kPitch + 16 * j + 4 * lane_quad());
+    const float f[4] = {in ? v.x : 0.0f, in ? v.y : 0.0f, in ? v.z : 0.0f, in ? v.w : 0.0f};
+    if (j / 2 <= wave / 2) store_half<TM>(lp - kSquare + lower_at(wave, j / 2), j % 2, f);  // T's rows of tile `wave`
+    const float4 d = *reinterpret_cast<const float4*>(tok.in + 16 * j + 4 * lane_quad());
+    te[j][0] = -f[0] * d.x;
+    te[j][1] = -f[1] * d.y;
+    te[j][2] = -f[2] * d.z;
+    te[j][3] = -f[3] * d.w;
     if (TRAIN && j / 2 >= wave / 2) {  // its columns of tile `wave`, rows of tile j
       float f[4];
 #pragma unroll
@@ -194,129 +208,342 @@ __global__ void __launch_bounds__(256) prep(Geo g, Ptrs p) {
       store_half<TM>(up - kSquare + upper_at(wave, j / 2), j % 2, f);
     }
   }
+  // -W of tile `wave`, [key][token], so that a lane stores eight keys of its token
+  Frag<TM> tf[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    tf[j] = frag_of<TM>(f32x4{te[2 * j][0], te[2 * j][1], te[2 * j][2], te[2 * j][3]},
+                        f32x4{te[2 * j + 1][0], te[2 * j + 1][1], te[2 * j + 1][2], te[2 * j + 1][3]});
+  TM* wp = static_cast<TM*>(p.w) + (at * kC + tc) * key;
+#pragma unroll
+  for (int i = 0; i < KB; ++i) {
+    f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      mma(x[n], KTile::keys_over_tokens(kt, 0, 2 * i + n), tf[0]);
+      if (wave >= 2) mma(x[n], KTile::keys_over_tokens(kt, 32, 2 * i + n), tf[1]);
+    }
+    const float f[8] = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+    store_part<TM, 8>(wp, 32 * i + 8 * lane_quad(), key, f);
+  }
 }
 
-// W waves of 16 value columns each.
+// What a workgroup of `scan` holds in LDS.  FAST (rows of whole units at multiples of 16 bytes): two buffers,
+// and the next chunk's loads fly while one is worked on.  Otherwise one buffer, filled between two barriers.
+template <typename TM, int KB, int W, bool FAST>
+struct ScanLds {
+  static constexpr int kBufs = FAST ? 2 : 1;
+  static constexpr bool kT = FAST && KB * sizeof(TM) <= 8;  // T too; wider keys leave no room
+  static constexpr bool kQ = kT && sizeof(TM) == 2;         // and Q and P
+  typedef Tile<TM, 32 * KB> KTile;
+  struct Buf {
+    TM w[KTile::kElements], k[KTile::kElements], v[Tile<TM, 16 * W>::kElements];
+    float in[kC], write[kC];
+    TM t[kT ? 6 * kFrag : 8], p[kQ ? 6 * kFrag : 8], q[kQ ? KTile::kElements : 8];
+  };
+  struct Hand {
+    TM s[KB * kFrag], e[2 * kFrag];
+  };
+  // Two where there is room; one is read and written in one turn, on two sides of a barrier.
+  static constexpr int kHands = FAST && kBufs * sizeof(Buf) + 2 * W * sizeof(Hand) <= 160 * 1024 ? 2 : 1;
+  Buf bufs[kBufs];
+  Hand hand[kHands][W];  // S and E of a chunk as operands, from the wave that carries to the one that follows
+};
+
+// Waves that fetch: a wave issues a direct load in about 75 cycles, so one alone brings 13.6 bytes a cycle to LDS,
+// two 25.7 and four, one on each SIMD, 44; eight no more (64 KB of rows of 256 bytes in L2, 256 workgroups).
+template <bool FAST>
+constexpr int kFetchers = FAST ? 4 : 0;
+
+template <typename TM>
+__device__ __forceinline__ void put_frag(TM* p, const Frag<TM>& f) {
+  store_words(p + 8 * lane_id(), f.w);
+}
+
+// W waves carry 16 value columns each through the chunks, W follow, and four fetch.  Turn n: the first do chunk n,
+// the second finish chunk n - 1 and the last bring chunk n + 1.
 template <typename TM, int KB, int W, bool TRAIN, bool FAST>
-__global__ void __launch_bounds__(64 * W) scan(Geo g, Ptrs p, int parts) {
-  constexpr int KP = 32 * KB, BV = 16 * W;
-  typedef Feed<TM, KP, BV, W, FAST> Feeder;
+__global__ void __launch_bounds__(128 * W + 64 * kFetchers<FAST>) scan(Geo g, Ptrs p, int parts) {
+  constexpr int KP = 32 * KB, BV = 16 * W, kThreads = 128 * W + 64 * kFetchers<FAST>;
+  typedef ScanLds<TM, KB, W, FAST> Lds;
   typedef Tile<TM, KP> KTile;
-  __shared__ __align__(16) typename Feeder::Buf bufs[Feeder::kBufs];
+  typedef Tile<TM, BV> VTile;
+  __shared__ __align__(16) Lds lds;
   const WgId id = wg_id(parts, static_cast<int>(g.heads));
   const int64_t h = id.y, b = id.z, bh = b * g.heads + h;
   const int wave = uniform(threadIdx.x >> 6), col = lane_col(), quad = lane_quad();
-  const int v0 = id.x * BV, vc = v0 + 16 * wave + col;  // the lane's column of S and E
+  const int mine = wave % W;  // of the value tiles
+  const int v0 = id.x * BV, vt = v0 + 16 * mine, vc = vt + col;  // the lane's column of S and E
   const int key = static_cast<int>(g.key), value = static_cast<int>(g.value);
   const TM* zeros = reinterpret_cast<const TM*>(&zero_unit);
-  const Feeder feed{static_cast<const TM*>(p.k) + b * g.k_b + h / g.rep * g.k_h,
-                    static_cast<const TM*>(p.q) + b * g.q_b + h / g.rep * g.q_h,
-                    static_cast<const TM*>(p.v) + b * g.v_b + h * g.v_h + v0, g.k_t, g.q_t, g.v_t, g.length,
-                    p.tokens + bh * g.chunks, static_cast<const TM*>(p.lower) + bh * g.chunks * 2 * kSquare, key, value - v0};
+  const TM* k = static_cast<const TM*>(p.k) + b * g.k_b + h / g.rep * g.k_h;
+  const TM* q = static_cast<const TM*>(p.q) + b * g.q_b + h / g.rep * g.q_h;
+  const TM* v = static_cast<const TM*>(p.v) + b * g.v_b + h * g.v_h + v0;
+  const TM* w = static_cast<const TM*>(p.w) + bh * g.chunks * kC * key;
+  const TM* squares = static_cast<const TM*>(p.lower) + bh * g.chunks * 2 * kSquare;
+  const Tokens* tokens = p.tokens + bh * g.chunks;
+  auto rows_of = [&](int64_t c) { return static_cast<int>(min(static_cast<int64_t>(kC), g.length - c * kC)); };
+  auto copy = [&](int64_t c) {  // by all
+    typename Lds::Buf& bf = lds.bufs[0];
+    KTile::template copy<kThreads>(bf.w, w + c * kC * key, key, kC, key);
+    KTile::template copy<kThreads>(bf.k, k + c * kC * g.k_t, g.k_t, rows_of(c), key);
+    VTile::template copy<kThreads>(bf.v, v + c * kC * g.v_t, g.v_t, rows_of(c), value - v0);
+    for (int i = static_cast<int>(threadIdx.x); i < 2 * kC; i += kThreads) bf.in[i] = tokens[c].in[i];
+  };
 
-  f32x4 s[2 * KB];  // S transposed: [key][value]
-#pragma unroll
-  for (int i = 0; i < 2 * KB; ++i) s[i] = f32x4{0, 0, 0, 0};
-  if (p.initial && vc < value) load_state<FAST>(s, p.initial, g.state_dtype, (bh * value + vc) * key, key);
-  if (FAST && g.chunks > 0) feed.fetch(bufs, 0, wave, zeros);
-  for (int64_t c = 0; c < g.chunks; ++c) {
-    const int64_t at = bh * g.chunks + c, t0 = c * kC;
-    Frag<TM> held[Feeder::kSquares ? 1 : 12];
-    if constexpr (!Feeder::kSquares) {
-#pragma unroll
-      for (int i = 0; i < 12; ++i) held[i] = frag_at(feed.squares + (12 * c + i) * kFrag);
+  if (FAST && key < KP) {  // keys that no load fills
+    for (int i = static_cast<int>(threadIdx.x); i < Lds::kBufs * KTile::kElements / KTile::kUnit; i += kThreads) {
+      const uint32_t none[4] = {0, 0, 0, 0};
+      typename Lds::Buf& bf = lds.bufs[i / (KTile::kElements / KTile::kUnit)];
+      const int at = i % (KTile::kElements / KTile::kUnit) * KTile::kUnit;
+      store_words(bf.w + at, none);
+      store_words(bf.k + at, none);
+      if constexpr (Lds::kQ) store_words(bf.q + at, none);
     }
-    const typename Feeder::Buf& bf = feed.turn(bufs, c, c + 1, c + 1 < g.chunks, wave, zeros);
-    auto square = [&](int which, int i, int j) {  // T, P
-      if constexpr (Feeder::kSquares)
-        return frag_at(bf.squares + which * kSquare + lower_at(i, j));
-      else
-        return held[6 * which + lower_at(i, j) / kFrag];
-    };
-
-    Frag<TM> so[KB];  // S as an operand over the keys
+    __syncthreads();
+  }
+  if constexpr (FAST) {
+    if (wave >= 2 * W) {
+      constexpr int F = kFetchers<FAST>;
+      const int part = wave - 2 * W;
+      const Lines<TM, KP, F> w_lines(key, key, part), k_lines(g.k_t, key, part), q_lines(g.q_t, key, part);
+      const Lines<TM, BV, F> v_lines(g.v_t, value - v0, part);
+      for (int64_t c = 0; c <= g.chunks + 1; ++c) {  // turn c - 1
+        if (c < g.chunks) {
+          typename Lds::Buf& bf = lds.bufs[c & 1];
+          w_lines.issue(bf.w, w + c * kC * key, part);
+          if (Lds::kHands == 1 && c > 0) __syncthreads();  // where the others hand over
+          if (rows_of(c) == kC) {
+            k_lines.issue(bf.k, k + c * kC * g.k_t, part);
+            v_lines.issue(bf.v, v + c * kC * g.v_t, part);
+          } else {
+            KTile::template issue<F>(bf.k, k + c * kC * g.k_t, g.k_t, rows_of(c), key, part, zeros);
+            VTile::template issue<F>(bf.v, v + c * kC * g.v_t, g.v_t, rows_of(c), value - v0, part, zeros);
+          }
+          if (part == 0 && lane_id() < 2 * kC / 4) direct_load(tokens[c].in + 4 * lane_id(), bf.in);
+          if constexpr (Lds::kT) {  // P behind T in memory and in LDS
+            constexpr int kPer = 16 / static_cast<int>(sizeof(TM)) * kWave;  // elements of a load
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) so[kb] = frag_of<TM>(s[2 * kb], s[2 * kb + 1]);
-    if (TRAIN && vc < value)
-      store_operands<TM, FAST>(static_cast<TM*>(p.states) + (at * value + vc) * key, key, so);
-    // V - exp(c) K S0^T
-    f32x4 e[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f32x4 z = {0, 0, 0, 0};
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) mma(z, KTile::rows(bf.k, 16 * i, 32 * kb), so[kb]);
-      const f32x4 vv = Tile<TM, BV>::values(bf.v, 16 * i, 16 * wave);
-      const float4 d = *reinterpret_cast<const float4*>(bf.in + 16 * i + 4 * quad);
-      e[i] = f32x4{vv[0] - d.x * z[0], vv[1] - d.y * z[1], vv[2] - d.z * z[2], vv[3] - d.w * z[3]};
-    }
-    const Frag<TM> zo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      e[i] = f32x4{0, 0, 0, 0};
-      f32x4 et = {0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j <= i / 2; ++j) {
-        const Frag<TM> t = square(0, i, j);
-        mma(e[i], t, zo[j]);
-        if (TRAIN) mma(et, zo[j], t);  // [value][t], whose lanes hold four values of a token
+            for (int i = 0; i < (Lds::kQ ? 2 : 1) * 6 * kFrag / kPer / F; ++i) {
+              const int f = (i * F + part) * kPer;
+              direct_load(squares + c * 2 * kSquare + f, 16u * lane_id(), bf.t + f);
+            }
+          }
+          if constexpr (Lds::kQ) {
+            if (rows_of(c) == kC)
+              q_lines.issue(bf.q, q + c * kC * g.q_t, part);
+            else
+              KTile::template issue<F>(bf.q, q + c * kC * g.q_t, g.q_t, rows_of(c), key, part, zeros);
+          }
+          // every vector memory operation of this wave is done, loads to LDS among them; then everyone's
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else if (Lds::kHands == 1 && c > 0) {
+          __syncthreads();
+        }
+        if (c <= g.chunks) __syncthreads();
       }
-      if (TRAIN)
-        store_four<TM, FAST>(static_cast<TM*>(p.e) + (at * kC + 16 * i + col) * value, v0 + 16 * wave + 4 * quad, value, et);
-    }
-    const Frag<TM> eo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
-    // Y transposed, so that a lane holds four values of a token
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f32x4 y = {0, 0, 0, 0};
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) mma(y, so[kb], KTile::rows(bf.q, 16 * i, 32 * kb));
-      const float d = g.scale * bf.in[16 * i + col];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] *= d;
-#pragma unroll
-      for (int j = 0; j <= i / 2; ++j) mma(y, eo[j], square(1, i, j));
-      const int64_t t = t0 + 16 * i + col;
-      if (t < g.length)
-        store_four<TM, FAST>(static_cast<TM*>(p.y) + ((b * g.length + t) * g.heads + h) * value, v0 + 16 * wave + 4 * quad,
-                             value, y);
-    }
-    // S' = exp(c_63) S0 + E^T (beta exp(c_63 - c) K)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 d = *reinterpret_cast<const float4*>(bf.out + 16 * i + 4 * quad);
-      const float4 bt = *reinterpret_cast<const float4*>(bf.beta + 16 * i + 4 * quad);
-      e[i] = f32x4{e[i][0] * (d.x * bt.x), e[i][1] * (d.y * bt.y), e[i][2] * (d.z * bt.z), e[i][3] * (d.w * bt.w)};
-    }
-    const Frag<TM> wo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
-    const float last = bf.in[kC - 1];
-#pragma unroll
-    for (int i = 0; i < 2 * KB; ++i) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[i][r] *= last;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) mma(s[i], KTile::keys_over_tokens(bf.k, 32 * j, i), wo[j]);
+      return;
     }
   }
-  if (p.final_state && vc < value) store_state<FAST>(p.final_state, g.state_dtype, (bh * value + vc) * key, key, s);
+  if (wave < W) {
+    f32x4 s[2 * KB];  // S transposed: [key][value]
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i) s[i] = f32x4{0, 0, 0, 0};
+    if (p.initial && vc < value) load_state<FAST>(s, p.initial, g.state_dtype, (bh * value + vc) * key, key);
+    Frag<TM> held[Lds::kT ? 1 : 6];
+    auto hold = [&](int64_t c) {
+      if constexpr (!Lds::kT) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) held[i] = frag_at(squares + c * 2 * kSquare + i * kFrag);
+      }
+    };
+    if (g.chunks > 0) hold(0);
+    for (int64_t n = 0; n < g.chunks; ++n) {
+      __syncthreads();
+      if constexpr (!FAST) {
+        copy(n);
+        __syncthreads();
+      }
+      const typename Lds::Buf& bf = lds.bufs[n & (Lds::kBufs - 1)];
+      f32x4 e[4];
+      Frag<TM> so[KB];  // S as an operand over the keys
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) so[kb] = frag_of<TM>(s[2 * kb], s[2 * kb + 1]);
+      const Frag<TM> vo[2] = {VTile::over_tokens(bf.v, 0, 16 * mine), VTile::over_tokens(bf.v, 32, 16 * mine)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j <= i / 2; ++j) {
+          if constexpr (Lds::kT)
+            mma(e[i], frag_at(bf.t + lower_at(i, j)), vo[j]);
+          else
+            mma(e[i], held[lower_at(i, j) / kFrag], vo[j]);
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) mma(e[i], KTile::rows(bf.w, 16 * i, 32 * kb), so[kb]);
+      }
+      const Frag<TM> eo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
+      if (n + 1 < g.chunks) hold(n + 1);
+      if constexpr (FAST && Lds::kHands == 1) __syncthreads();  // what was handed over last has been read
+      typename Lds::Hand& hand = lds.hand[n & (Lds::kHands - 1)][mine];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) put_frag(hand.s + kb * kFrag, so[kb]);
+      put_frag(hand.e, eo[0]);
+      put_frag(hand.e + kFrag, eo[1]);
+      // S' = exp(c_63) S0 + E^T (beta exp(c_63 - c) K)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 d = *reinterpret_cast<const float4*>(bf.write + 16 * i + 4 * quad);
+        e[i] = f32x4{e[i][0] * d.x, e[i][1] * d.y, e[i][2] * d.z, e[i][3] * d.w};
+      }
+      const Frag<TM> wo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
+      const float last = bf.in[kC - 1];
+#pragma unroll
+      for (int i = 0; i < 2 * KB; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[i][r] *= last;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mma(s[i], KTile::keys_over_tokens(bf.k, 32 * j, i), wo[j]);
+      }
+    }
+    __syncthreads();  // the last turn of those that follow
+    if constexpr (FAST && Lds::kHands == 1) __syncthreads();
+    if (p.final_state && vc < value) store_state<FAST>(p.final_state, g.state_dtype, (bh * value + vc) * key, key, s);
+    return;
+  }
+
+  // Q and P of chunk n are loaded in turn n, from LDS where they are there, and used in the next; wider keys
+  // would need more registers than there are, and are loaded where they are used.
+  constexpr bool kAhead = KB * sizeof(TM) <= 8;
+  Frag<TM> qf[4][kAhead ? KB : 1], pf[6], one[2];
+  float in[4];
+  // a half of the unit matrix as an operand, which transposes E exactly
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f32x4 x[2];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[0][r] = i == 0 && 4 * quad + r == col ? 1.0f : 0.0f;
+      x[1][r] = i == 1 && 4 * quad + r == col ? 1.0f : 0.0f;
+    }
+    one[i] = frag_of<TM>(x[0], x[1]);
+  }
+  for (int64_t n = 0; n <= g.chunks; ++n) {
+    __syncthreads();
+    Frag<TM> so[KB], eo[2];
+    if (n > 0) {
+      const typename Lds::Hand& hand = lds.hand[(n - 1) & (Lds::kHands - 1)][mine];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) so[kb] = frag_at(hand.s + kb * kFrag);
+      eo[0] = frag_at(hand.e);
+      eo[1] = frag_at(hand.e + kFrag);
+    }
+    if (!FAST && n < g.chunks) copy(n);
+    if (FAST ? Lds::kHands == 1 : n < g.chunks) __syncthreads();
+    // of tokens and keys that are not there, others' values: those tokens are not stored, and S has zeros at
+    // those keys
+    auto load_q = [&](int64_t c, int i, int kb) {
+      if constexpr (FAST) {
+        const char* from = reinterpret_cast<const char*>(q + c * kC * g.q_t);
+        const uint32_t row = min(16 * i + col, rows_of(c) - 1) * static_cast<uint32_t>(g.q_t);
+        const uint32_t at = (row + (32 * kb + 8 * quad < key ? 32 * kb + 8 * quad : 0)) * static_cast<uint32_t>(sizeof(TM));
+        Frag<TM> f;
+#pragma unroll
+        for (int j = 0; j < kWordsOf<TM, 8> / 4; ++j) {
+          const uint4 x = *reinterpret_cast<const uint4*>(from + at + 16 * j);
+          f.w[4 * j] = x.x;
+          f.w[4 * j + 1] = x.y;
+          f.w[4 * j + 2] = x.z;
+          f.w[4 * j + 3] = x.w;
+        }
+        return f;
+      } else {
+        return frag_memory(q + c * kC * g.q_t, g.q_t, 16 * i, 32 * kb, rows_of(c), key);
+      }
+    };
+    if (n > 0) {
+      const int64_t c = n - 1, at = bh * g.chunks + c;
+      TM* yp = static_cast<TM*>(p.y) + ((b * g.length + c * kC) * g.heads + h) * value;
+      const auto y_row = [&] {  // of FAST, 32 bits
+        if constexpr (FAST) return static_cast<uint32_t>(g.heads * value);
+        else return g.heads * value;
+      }();
+      // Y transposed, so that a lane holds four values of a token
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4 y = {0, 0, 0, 0};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          if constexpr (kAhead)
+            mma(y, so[kb], qf[i][kb]);
+          else
+            mma(y, so[kb], load_q(c, i, kb));
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] *= in[i];
+#pragma unroll
+        for (int j = 0; j <= i / 2; ++j) mma(y, eo[j], pf[lower_at(i, j) / kFrag]);
+        if (16 * i + col < rows_of(c))
+          store_four<TM, FAST>(yp + (16 * i + col) * y_row, vt + 4 * quad, value, y);
+      }
+      if constexpr (TRAIN) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f32x4 et = {0, 0, 0, 0};
+          mma(et, eo[i / 2], one[i % 2]);
+          store_four<TM, FAST>(static_cast<TM*>(p.e) + (at * kC + 16 * i + col) * value, vt + 4 * quad, value, et);
+        }
+        if (vc < value) store_operands<TM, FAST>(static_cast<TM*>(p.states) + (at * value + vc) * key, key, so);
+      }
+    }
+    if (n < g.chunks) {
+      const typename Lds::Buf& bf = lds.bufs[n & (Lds::kBufs - 1)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        in[i] = g.scale * bf.in[16 * i + col];
+        if constexpr (kAhead) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            if constexpr (Lds::kQ)
+              qf[i][kb] = KTile::rows(bf.q, 16 * i, 32 * kb);
+            else
+              qf[i][kb] = load_q(n, i, kb);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 6; ++i) {
+        if constexpr (Lds::kQ)
+          pf[i] = frag_at(bf.p + i * kFrag);
+        else
+          pf[i] = frag_at(squares + (2 * n + 1) * kSquare + i * kFrag);
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------ the choice
 
+// Value tiles of a workgroup: two, and one where the LDS has no room for two.
+template <typename TM, int KB>
+constexpr int kTiles = sizeof(TM) == 4 && KB >= 4 ? 1 : 2;
+
 template <typename TM, int KB, bool TRAIN>
 void launch(const Geo& g, const Ptrs& p, hipStream_t s) {
-  constexpr int W = 2;
+  constexpr int W = kTiles<TM, KB>;
   const unsigned cells = static_cast<unsigned>(g.batch * g.heads * g.chunks);
   const int parts = static_cast<int>(cdiv(g.value, 16 * W));
-  if (cells) MKO_TIMED("delta_prep", s, prep<TM, KB, TRAIN><<<cells, 256, 0, s>>>(g, p));
+  const bool fast = fast_rows(g, p);
+  if (cells) MKO_TIMED("delta_prep", s, prep<TM, KB, TRAIN><<<cells, 256, 0, s>>>(g, p, fast));
   const unsigned grid = static_cast<unsigned>(g.batch * g.heads * parts);
-  if constexpr (sizeof(TM) == 2) {
-    if (fast_rows(g, p)) {
-      MKO_TIMED("delta_scan", s, scan<TM, KB, W, TRAIN, true><<<grid, 64 * W, 0, s>>>(g, p, parts));
+  if constexpr (KB * sizeof(TM) <= 16) {
+    if (fast) {
+      MKO_TIMED("delta_scan", s, scan<TM, KB, W, TRAIN, true><<<grid, 128 * W + 64 * kFetchers<true>, 0, s>>>(g, p, parts));
       return;
     }
   }
-  MKO_TIMED("delta_scan", s, scan<TM, KB, W, TRAIN, false><<<grid, 64 * W, 0, s>>>(g, p, parts));
+  MKO_TIMED("delta_scan", s, scan<TM, KB, W, TRAIN, false><<<grid, 128 * W, 0, s>>>(g, p, parts));
 }
 
 template <typename TM, bool TRAIN>
@@ -392,7 +619,7 @@ Ptrs base_ptrs(const mko_delta_params* prm) {
 bool fast_rows(const Geo& g, const Ptrs& p) {
   bool fast = g.key % 8 == 0 && g.value % 8 == 0;
   for (int64_t n : {g.q_b, g.q_t, g.q_h, g.k_b, g.k_t, g.k_h, g.v_b, g.v_t, g.v_h}) fast = fast && n % 8 == 0;
-  for (int64_t n : {g.q_t, g.k_t, g.v_t, g.heads * g.value}) fast = fast && n >= 0 && n < int64_t(1) << 24;  // 32-bit offsets of 16 rows
+  for (int64_t n : {g.q_t, g.k_t, g.v_t, g.heads * g.value}) fast = fast && n >= 0 && n < int64_t(1) << 23;  // 32-bit offsets of 64 rows
   for (const void* a : {p.q, p.k, p.v, p.dy, static_cast<const void*>(p.dv)}) fast = fast && reinterpret_cast<uintptr_t>(a) % 16 == 0;
   return fast;
 }
@@ -414,6 +641,7 @@ Layout forward_layout(const Geo& g, bool train) {
   const size_t cells = static_cast<size_t>(g.batch * g.heads * g.chunks), el = element_size(g.dtype);
   size_t o = 0;
   l.lower = o; o = align256(o + cells * 2 * kSquare * el);
+  l.w = o; o = align256(o + cells * kC * g.key * el);
   l.tokens = o;
   if (!train) o = align256(o + cells * sizeof(Tokens));
   l.total = o;
@@ -460,6 +688,7 @@ extern "C" int mko_delta_fwd(const mko_delta_params* prm, void* stream) {
   Ptrs p = base_ptrs(prm);
   char* ws = static_cast<char*>(prm->workspace);
   p.lower = ws + w.lower;
+  p.w = ws + w.w;
   if (train) {
     const Layout l = saved_layout(g);
     char* sv = static_cast<char*>(prm->saved);

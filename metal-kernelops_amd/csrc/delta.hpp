@@ -3,8 +3,8 @@
 // Per (batch, value head), with state S (value x key) and c the running sum of the log decay:
 //   e_t = v_t - exp(g_t) S_{t-1} k_t,  S_t = exp(g_t) S_{t-1} + beta_t e_t k_t^T,  y_t = scale S_t q_t
 // In a chunk of 64 tokens with entering state S0 the e of all tokens solve one triangular system:
-//   A[t][s] = exp(c_t - c_s) (k_t . k_s) beta_s for s < t,  T = (I + A)^-1
-//   E = T (V - exp(c) K S0^T),  P[t][s] = scale exp(c_t - c_s) (q_t . k_s) beta_s for s <= t
+//   A[t][s] = exp(c_t - c_s) (k_t . k_s) beta_s for s < t,  T = (I + A)^-1,  W = T exp(c) K
+//   E = T V - W S0^T,  P[t][s] = scale exp(c_t - c_s) (q_t . k_s) beta_s for s <= t
 //   Y = scale exp(c) Q S0^T + P E,  S' = exp(c_63) S0 + E^T (beta exp(c_63 - c) K)
 //
 // Everything runs on 16x16 tiles of the matrix cores, whose accumulator layout (lane l holds column
@@ -40,10 +40,11 @@ struct Geo {
   int dtype, decay_dtype, beta_dtype, state_dtype;
 };
 
-// Per chunk and head, in float32 after 64 doubles: exp(c), exp(c_63 - c) and beta of its tokens.
+// Per chunk and head, in float32 after 64 doubles: exp(c), beta exp(c_63 - c), exp(c_63 - c) and beta of
+// its tokens.
 struct Tokens {
   double c[kC];  // c log2(e)
-  float in[kC], out[kC], beta[kC];
+  float in[kC], write[kC], out[kC], beta[kC];
 };
 
 struct Ptrs {
@@ -51,6 +52,7 @@ struct Ptrs {
   void *y, *final_state, *dq, *dk, *dv, *ddecay, *dbeta, *dinitial;
   Tokens* tokens;        // (batch, heads, chunks)
   void *lower, *upper;   // T and P as operands, and their transposes, (batch, heads, chunks, 2, kSquare)
+  void* w;               // -W, (batch, heads, chunks, kC, key)
   void *states, *grads;  // S0 and the gradient of S' of each chunk, (batch, heads, chunks, value, key)
   void* e;               // E, (batch, heads, chunks, kC, value)
   float *pq, *pk;        // dq and dk of each value head, where key heads are shared
@@ -121,6 +123,21 @@ __device__ __forceinline__ Frag<TM> frag_memory(const TM* base, int64_t stride, 
 __device__ __forceinline__ void direct_load(const void* from, void* to) {
   const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to));  // a flat address ends in that of LDS
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform(at)), "v"(from));
+}
+
+// A pointer that is the same in the wave, in scalar registers.
+using mko::uniform;
+__device__ __forceinline__ const char* uniform(const void* p) {
+  const uint64_t a = reinterpret_cast<uintptr_t>(p);
+  const uint64_t lo = static_cast<uint32_t>(uniform(static_cast<int>(a))), hi = static_cast<uint32_t>(uniform(static_cast<int>(a >> 32)));
+  return reinterpret_cast<const char*>(hi << 32 | lo);
+}
+
+// The same from `base` (the same in the wave) + `off` bytes.
+__device__ __forceinline__ void direct_load(const void* base, uint32_t off, const void* to) {
+  const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform(at)), "v"(off),
+               "s"(uniform(base)));
 }
 
 // Every direct load of the workgroup has landed.
@@ -255,12 +272,48 @@ struct Tile {
   }
 };
 
-// What `scan` and `back` hold of a chunk in LDS: K, Q, a slice of V or dY, the tokens' factors, and the two
-// squares they multiply with where SQUARES.
+// A wave's share of the loads of whole-row tiles, with what is the same for every tile worked out once: a
+// lane's offsets repeat every 16 rows, and what differs between loads beyond that is the same in the wave.
+// Columns from `cols` on are left as they are.
+template <typename TM, int COLS, int WAVES>
+struct Lines {
+  typedef Tile<TM, COLS> T;
+  static constexpr int kRows = kWave / T::kUnits;                       // of a load
+  static constexpr int kLoads = kC * T::kUnits / kWave;                 // of a tile
+  static constexpr int kMine = (kLoads + WAVES - 1) / WAVES;            // of a wave, one for the first kLoads waves
+  static constexpr int kTurns = 16 / kRows / WAVES > 1 ? 16 / kRows / WAVES : 1;  // loads of a wave until offsets repeat
+  uint32_t off[kTurns];
+  bool in[kTurns];
+  int64_t bytes;  // from a load of the wave to the next
+
+  __device__ __forceinline__ Lines(int64_t stride, int cols, int wave) {
+    static_assert(kLoads % WAVES == 0 || kLoads < WAVES, "an equal share of the loads");
+    const int row = lane_id() / T::kUnits, unit = lane_id() % T::kUnits;
+#pragma unroll
+    for (int j = 0; j < kTurns; ++j) {
+      const int load = j * WAVES + wave, col = (unit ^ T::turn(load * kRows + row)) * T::kUnit;
+      off[j] = static_cast<uint32_t>((row * stride + col) * static_cast<int>(sizeof(TM)));
+      in[j] = col < cols && load < kLoads;
+    }
+    bytes = WAVES * kRows * stride * static_cast<int64_t>(sizeof(TM));
+  }
+  // All 64 rows at `base`, of the same stride.
+  __device__ __forceinline__ void issue(TM* tile, const TM* base, int wave) const {
+    const char* at = reinterpret_cast<const char*>(base) + wave * (bytes / WAVES);
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      if (in[j % kTurns]) direct_load(at, off[j % kTurns], tile + (j * WAVES + wave) * kWave * T::kUnit);
+      at += bytes;
+    }
+  }
+};
+
+// What `back` holds of a chunk in LDS: K, Q, a slice of dY, the tokens' factors, and the two squares it
+// multiplies with where SQUARES.
 template <typename TM, int KP, int BV, bool SQUARES>
 struct Chunk {
   TM k[Tile<TM, KP>::kElements], q[Tile<TM, KP>::kElements], v[Tile<TM, BV>::kElements];
-  float in[kC], out[kC], beta[kC];
+  float in[kC], write[kC];
   TM squares[SQUARES ? 12 * kFrag : 8];
 };
 
@@ -300,7 +353,7 @@ struct Feed {
       Tile<TM, KP>::template issue<W>(b.k, k + t0 * k_t, k_t, rows, key, wave, zeros);
       Tile<TM, KP>::template issue<W>(b.q, q + t0 * q_t, q_t, rows, key, wave, zeros);
       Tile<TM, BV>::template issue<W>(b.v, v + t0 * v_t, v_t, rows, value, wave, zeros);
-      if (wave == 0 && lane_id() < 3 * kC / 4) direct_load(from + 4 * lane_id(), b.in);
+      if (wave == 0 && lane_id() < 2 * kC / 4) direct_load(from + 4 * lane_id(), b.in);
       if constexpr (kSquares) {
         static_assert(12 % W == 0, "an equal share of the squares");
 #pragma unroll
@@ -313,7 +366,7 @@ struct Feed {
       Tile<TM, KP>::template copy<64 * W>(b.k, k + t0 * k_t, k_t, rows, key);
       Tile<TM, KP>::template copy<64 * W>(b.q, q + t0 * q_t, q_t, rows, key);
       Tile<TM, BV>::template copy<64 * W>(b.v, v + t0 * v_t, v_t, rows, value);
-      for (int i = static_cast<int>(threadIdx.x); i < 3 * kC; i += 64 * W) b.in[i] = from[i];
+      for (int i = static_cast<int>(threadIdx.x); i < 2 * kC; i += 64 * W) b.in[i] = from[i];
     }
   }
   // Chunk c is in its buffer, and the one after it (`next`, if there is one) on its way.
@@ -416,10 +469,10 @@ __device__ __forceinline__ void store_operands(TM* row, int n, const Frag<TM> (&
 
 // Bytes of the arrays that the forward leaves for the backward, and of the workspaces.
 struct Layout {
-  size_t tokens, lower, upper, states, e, total;
+  size_t tokens, lower, upper, w, states, e, total;
 };
 Layout saved_layout(const Geo& g);                // tokens, upper, states, e
-Layout forward_layout(const Geo& g, bool train);  // lower, and tokens unless they are saved
+Layout forward_layout(const Geo& g, bool train);  // lower and w, and tokens unless they are saved
 
 int make_geo(const mko_delta_params* prm, const char* what, Geo* g);
 Ptrs base_ptrs(const mko_delta_params* prm);

@@ -77,9 +77,8 @@ __global__ void __launch_bounds__(64 * W) back(Geo g, Ptrs p, int parts) {
       e[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) mma(e[i], KTile::rows(bf.k, 16 * i, 32 * kb), so[kb]);
-      const float4 d = *reinterpret_cast<const float4*>(bf.out + 16 * i + 4 * quad);
-      const float4 bt = *reinterpret_cast<const float4*>(bf.beta + 16 * i + 4 * quad);
-      e[i] = f32x4{e[i][0] * (d.x * bt.x), e[i][1] * (d.y * bt.y), e[i][2] * (d.z * bt.z), e[i][3] * (d.w * bt.w)};
+      const float4 d = *reinterpret_cast<const float4*>(bf.write + 16 * i + 4 * quad);
+      e[i] = f32x4{e[i][0] * d.x, e[i][1] * d.y, e[i][2] * d.z, e[i][3] * d.w};
 #pragma unroll
       for (int j = i / 2; j < 2; ++j) mma(e[i], square(1, i, j), yo[j]);
     }

@@ -46,7 +46,7 @@ CHUNK = 64
 MAX_KEY = 256
 """MKO_DELTA_MAX_KEY: the longest key."""
 
-_TOKENS = CHUNK * (8 + 3 * 4)  # bytes of a chunk's decays
+_TOKENS = CHUNK * (8 + 4 * 4)  # bytes of a chunk's decays
 _SQUARES = 2 * 6 * 512  # elements of its two triangular operands
 
 
