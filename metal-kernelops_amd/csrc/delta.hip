@@ -250,11 +250,6 @@ struct ScanLds {
   Hand hand[kHands][W];  // S and E of a chunk as operands, from the wave that carries to the one that follows
 };
 
-// Waves that fetch: a wave issues a direct load in about 75 cycles, so one alone brings 13.6 bytes a cycle to LDS,
-// two 25.7 and four, one on each SIMD, 44; eight no more (64 KB of rows of 256 bytes in L2, 256 workgroups).
-template <bool FAST>
-constexpr int kFetchers = FAST ? 4 : 0;
-
 template <typename TM>
 __device__ __forceinline__ void put_frag(TM* p, const Frag<TM>& f) {
   store_words(p + 8 * lane_id(), f.w);
@@ -263,8 +258,8 @@ __device__ __forceinline__ void put_frag(TM* p, const Frag<TM>& f) {
 // W waves carry 16 value columns each through the chunks, W follow, and four fetch.  Turn n: the first do chunk n,
 // the second finish chunk n - 1 and the last bring chunk n + 1.
 template <typename TM, int KB, int W, bool TRAIN, bool FAST>
-__global__ void __launch_bounds__(128 * W + 64 * kFetchers<FAST>) scan(Geo g, Ptrs p, int parts) {
-  constexpr int KP = 32 * KB, BV = 16 * W, kThreads = 128 * W + 64 * kFetchers<FAST>;
+__global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Geo g, Ptrs p, int parts) {
+  constexpr int KP = 32 * KB, BV = 16 * W, kThreads = 128 * W + 64 * (FAST ? kFetchers : 0);
   typedef ScanLds<TM, KB, W, FAST> Lds;
   typedef Tile<TM, KP> KTile;
   typedef Tile<TM, BV> VTile;
@@ -304,7 +299,7 @@ __global__ void __launch_bounds__(128 * W + 64 * kFetchers<FAST>) scan(Geo g, Pt
   }
   if constexpr (FAST) {
     if (wave >= 2 * W) {
-      constexpr int F = kFetchers<FAST>;
+      constexpr int F = kFetchers;
       const int part = wave - 2 * W;
       const Lines<TM, KP, F> w_lines(key, key, part), k_lines(g.k_t, key, part), q_lines(g.q_t, key, part);
       const Lines<TM, BV, F> v_lines(g.v_t, value - v0, part);
@@ -539,7 +534,7 @@ void launch(const Geo& g, const Ptrs& p, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(g.batch * g.heads * parts);
   if constexpr (KB * sizeof(TM) <= 16) {
     if (fast) {
-      MKO_TIMED("delta_scan", s, scan<TM, KB, W, TRAIN, true><<<grid, 128 * W + 64 * kFetchers<true>, 0, s>>>(g, p, parts));
+      MKO_TIMED("delta_scan", s, scan<TM, KB, W, TRAIN, true><<<grid, 128 * W + 64 * kFetchers, 0, s>>>(g, p, parts));
       return;
     }
   }

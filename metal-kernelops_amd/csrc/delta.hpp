@@ -330,13 +330,20 @@ __device__ __forceinline__ Frag<TM> frag_at(const TM* p) {
   return f;
 }
 
-// Chunks on their way to LDS for a workgroup of W waves.  FAST (rows of whole units at multiples of 16
-// bytes): two buffers, and the loads of the next chunk fly while one is worked on.  Otherwise one
-// buffer, filled between two barriers.
+// Waves that do nothing but fetch: a wave issues a direct load in about 75 cycles, so one alone brings 13.6
+// bytes a cycle to LDS, two 25.7 and four, one on each SIMD, 44; eight no more (64 KB of rows of 256 bytes in L2,
+// 256 workgroups).
+constexpr int kFetchers = 4;
+
+// Chunks on their way to LDS for `back`.  FAST (rows of whole units at multiples of 16 bytes): two buffers, and
+// the loads of the next chunk fly while one is worked on; kFetch: waves of their own issue them.  Otherwise
+// one buffer, filled between two barriers.
 template <typename TM, int KP, int BV, int W, bool FAST>
 struct Feed {
   static constexpr int kBufs = FAST ? 2 : 1;
-  static constexpr bool kSquares = FAST && KP <= 128;  // wider keys leave no room
+  static constexpr bool kFetch = FAST && KP * sizeof(TM) <= 256;  // wider keys leave no room for the squares,
+  static constexpr bool kSquares = kFetch;                        // and no registers for more waves
+  static constexpr int kWaves = kFetch ? kFetchers : W;           // that load
   typedef Chunk<TM, KP, BV, kSquares> Buf;
   const TM *k, *q, *v;
   int64_t k_t, q_t, v_t, length;
@@ -350,16 +357,17 @@ struct Feed {
     Buf& b = bufs[c & (kBufs - 1)];
     const float* from = tokens[c].in;
     if constexpr (FAST) {
-      Tile<TM, KP>::template issue<W>(b.k, k + t0 * k_t, k_t, rows, key, wave, zeros);
-      Tile<TM, KP>::template issue<W>(b.q, q + t0 * q_t, q_t, rows, key, wave, zeros);
-      Tile<TM, BV>::template issue<W>(b.v, v + t0 * v_t, v_t, rows, value, wave, zeros);
+      Tile<TM, KP>::template issue<kWaves>(b.k, k + t0 * k_t, k_t, rows, key, wave, zeros);
+      Tile<TM, KP>::template issue<kWaves>(b.q, q + t0 * q_t, q_t, rows, key, wave, zeros);
+      Tile<TM, BV>::template issue<kWaves>(b.v, v + t0 * v_t, v_t, rows, value, wave, zeros);
       if (wave == 0 && lane_id() < 2 * kC / 4) direct_load(from + 4 * lane_id(), b.in);
       if constexpr (kSquares) {
-        static_assert(12 % W == 0, "an equal share of the squares");
+        constexpr int kPer = 16 / static_cast<int>(sizeof(TM)) * kWave;  // elements of a load
+        static_assert(12 * kFrag / kPer % kWaves == 0, "an equal share of the squares");
 #pragma unroll
-        for (int j = 0; j < 12 / W; ++j) {
-          const int f = (j * W + wave) * kFrag;
-          direct_load(squares + c * 2 * kSquare + f + 8 * lane_id(), b.squares + f);
+        for (int j = 0; j < 12 * kFrag / kPer / kWaves; ++j) {
+          const int f = (j * kWaves + wave) * kPer;
+          direct_load(squares + c * 2 * kSquare + f, 16u * lane_id(), b.squares + f);
         }
       }
     } else {
@@ -371,7 +379,9 @@ struct Feed {
   }
   // Chunk c is in its buffer, and the one after it (`next`, if there is one) on its way.
   __device__ __forceinline__ const Buf& turn(Buf* bufs, int64_t c, int64_t next, bool more, int wave, const TM* zeros) const {
-    if constexpr (FAST) {
+    if constexpr (kFetch) {
+      __syncthreads();
+    } else if constexpr (FAST) {
       // every vector memory operation of this wave is done, loads to LDS among them; then everyone's
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();

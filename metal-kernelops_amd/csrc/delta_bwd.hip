@@ -24,8 +24,14 @@ namespace {
 
 __device__ uint4 zero_unit;  // where rows and columns outside come from
 
+// Waves of a workgroup of `back`: W that carry G, and those that fetch.
 template <typename TM, int KB, int W, bool FAST>
-__global__ void __launch_bounds__(64 * W) back(Geo g, Ptrs p, int parts) {
+constexpr int back_waves() {
+  return W + (Feed<TM, 32 * KB, 16 * W, W, FAST>::kFetch ? kFetchers : 0);
+}
+
+template <typename TM, int KB, int W, bool FAST>
+__global__ void __launch_bounds__((64 * back_waves<TM, KB, W, FAST>())) back(Geo g, Ptrs p, int parts) {
   constexpr int KP = 32 * KB, BV = 16 * W;
   typedef Feed<TM, KP, BV, W, FAST> Feeder;
   typedef Tile<TM, KP> KTile;
@@ -43,11 +49,22 @@ __global__ void __launch_bounds__(64 * W) back(Geo g, Ptrs p, int parts) {
                     static_cast<const TM*>(p.dy) + b * g.length * yrow + h * value + v0, g.k_t, g.q_t, yrow, g.length,
                     p.tokens + bh * g.chunks, static_cast<const TM*>(p.upper) + bh * g.chunks * 2 * kSquare, key, value - v0};
 
+  if constexpr (Feeder::kFetch) {
+    if (wave >= W) {
+      for (int64_t c = g.chunks - 1; c >= 0; --c) {
+        feed.fetch(bufs, c, wave - W, zeros);
+        // every vector memory operation of this wave is done, loads to LDS among them; then everyone's
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+      }
+      return;
+    }
+  }
   f32x4 s[2 * KB];  // G transposed: [key][value]
 #pragma unroll
   for (int i = 0; i < 2 * KB; ++i) s[i] = f32x4{0, 0, 0, 0};
   if (p.dfinal && vc < value) load_state<FAST>(s, p.dfinal, g.state_dtype, (bh * value + vc) * key, key);
-  if (FAST && g.chunks > 0) feed.fetch(bufs, g.chunks - 1, wave, zeros);
+  if (FAST && !Feeder::kFetch && g.chunks > 0) feed.fetch(bufs, g.chunks - 1, wave, zeros);
   for (int64_t c = g.chunks - 1; c >= 0; --c) {
     const int64_t at = bh * g.chunks + c, t0 = c * kC;
     Frag<TM> held[Feeder::kSquares ? 1 : 12];
@@ -437,15 +454,17 @@ void launch(const Geo& g, const Ptrs& p, hipStream_t s) {
   const int parts = static_cast<int>(cdiv(g.value, 16 * W));
   const unsigned grid = static_cast<unsigned>(g.batch * g.heads * parts);
   bool fast = false;
-  if constexpr (sizeof(TM) == 2) {
+  if constexpr (KB * sizeof(TM) <= 16) {
     fast = fast_rows(g, p);
-    if (fast) MKO_TIMED("delta_back", s, back<TM, KB, W, true><<<grid, 64 * W, 0, s>>>(g, p, parts));
+    if (fast) {
+      MKO_TIMED("delta_back", s, back<TM, KB, W, true><<<grid, 64 * back_waves<TM, KB, W, true>(), 0, s>>>(g, p, parts));
+      MKO_TIMED("delta_grads", s, grads<TM, KB, true><<<cells, 512, 0, s>>>(g, p));
+    }
   }
-  if (!fast) MKO_TIMED("delta_back", s, back<TM, KB, W, false><<<grid, 64 * W, 0, s>>>(g, p, parts));
-  if constexpr (sizeof(TM) == 2) {
-    if (fast) MKO_TIMED("delta_grads", s, grads<TM, KB, true><<<cells, 512, 0, s>>>(g, p));
+  if (!fast) {
+    MKO_TIMED("delta_back", s, back<TM, KB, W, false><<<grid, 64 * W, 0, s>>>(g, p, parts));
+    MKO_TIMED("delta_grads", s, grads<TM, KB, false><<<cells, 512, 0, s>>>(g, p));
   }
-  if (!fast) MKO_TIMED("delta_grads", s, grads<TM, KB, false><<<cells, 512, 0, s>>>(g, p));
   if (p.pq) {
     const int per = static_cast<int>(cdiv(g.key, 4));
     const int64_t groups = g.batch * g.length * g.key_heads * per;
