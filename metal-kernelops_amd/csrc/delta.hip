@@ -1,9 +1,9 @@
 // Gated delta rule, forward (delta.hpp has the formulas).
 //
-//   prep  per (batch, head, chunk): the decays' sums, T by blocked substitution in float32, the
-//         operands T and P (and their transposes, for the backward), and W
+//   prep  per (batch, head, chunk): the decays' sums, T by blocked substitution in float32, and the
+//         operands T and P (and their transposes, for the backward)
 //   scan  per (batch, head, 16 W value columns), sequential over the chunks.  W waves carry S in float32
-//         accumulators and do only what the next chunk waits for, E = T V - W S^T and S's update; W
+//         accumulators and do only what the next chunk waits for, E and S's update; W
 //         others follow a chunk behind with Y and the stores, and four fetch the chunk ahead.
 #include "delta.hpp"
 
@@ -189,18 +189,12 @@ __global__ void __launch_bounds__(256) prep(Geo g, Ptrs p, bool fast) {
   }
   __syncthreads();
   invert(a);
-  float te[4][4];  // -T exp(c), the lane's token's
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const bool in = j <= wave;
     const float4 v = *reinterpret_cast<const float4*>(a + tc * kPitch + 16 * j + 4 * lane_quad());
     const float f[4] = {in ? v.x : 0.0f, in ? v.y : 0.0f, in ? v.z : 0.0f, in ? v.w : 0.0f};
     if (j / 2 <= wave / 2) store_half<TM>(lp - kSquare + lower_at(wave, j / 2), j % 2, f);  // T's rows of tile `wave`
-    const float4 d = *reinterpret_cast<const float4*>(tok.in + 16 * j + 4 * lane_quad());
-    te[j][0] = -f[0] * d.x;
-    te[j][1] = -f[1] * d.y;
-    te[j][2] = -f[2] * d.z;
-    te[j][3] = -f[3] * d.w;
     if (TRAIN && j / 2 >= wave / 2) {  // its columns of tile `wave`, rows of tile j
       float f[4];
 #pragma unroll
@@ -208,36 +202,19 @@ __global__ void __launch_bounds__(256) prep(Geo g, Ptrs p, bool fast) {
       store_half<TM>(up - kSquare + upper_at(wave, j / 2), j % 2, f);
     }
   }
-  // -W of tile `wave`, [key][token], so that a lane stores eight keys of its token
-  Frag<TM> tf[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    tf[j] = frag_of<TM>(f32x4{te[2 * j][0], te[2 * j][1], te[2 * j][2], te[2 * j][3]},
-                        f32x4{te[2 * j + 1][0], te[2 * j + 1][1], te[2 * j + 1][2], te[2 * j + 1][3]});
-  TM* wp = static_cast<TM*>(p.w) + (at * kC + tc) * key;
-#pragma unroll
-  for (int i = 0; i < KB; ++i) {
-    f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      mma(x[n], KTile::keys_over_tokens(kt, 0, 2 * i + n), tf[0]);
-      if (wave >= 2) mma(x[n], KTile::keys_over_tokens(kt, 32, 2 * i + n), tf[1]);
-    }
-    const float f[8] = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
-    store_part<TM, 8>(wp, 32 * i + 8 * lane_quad(), key, f);
-  }
 }
 
-// What a workgroup of `scan` holds in LDS.  FAST (rows of whole units at multiples of 16 bytes): two buffers,
-// and the next chunk's loads fly while one is worked on.  Otherwise one buffer, filled between two barriers.
+// What a workgroup of `scan` holds in LDS.  FAST (rows of whole units at multiples of 16 bytes): two or three
+// buffers, and the loads of the next chunk or two fly while one is worked on.  Otherwise one buffer, filled
+// between two barriers.
 template <typename TM, int KB, int W, bool FAST>
 struct ScanLds {
-  static constexpr int kBufs = FAST ? 2 : 1;
   static constexpr bool kT = FAST && KB * sizeof(TM) <= 8;  // T too; wider keys leave no room
   static constexpr bool kQ = kT && sizeof(TM) == 2;         // and Q and P
+  static constexpr int kBufs = kQ ? 3 : FAST ? 2 : 1;
   typedef Tile<TM, 32 * KB> KTile;
   struct Buf {
-    TM w[KTile::kElements], k[KTile::kElements], v[Tile<TM, 16 * W>::kElements];
+    TM k[KTile::kElements], v[Tile<TM, 16 * W>::kElements];
     float in[kC], write[kC];
     TM t[kT ? 6 * kFrag : 8], p[kQ ? 6 * kFrag : 8], q[kQ ? KTile::kElements : 8];
   };
@@ -248,6 +225,7 @@ struct ScanLds {
   static constexpr int kHands = FAST && kBufs * sizeof(Buf) + 2 * W * sizeof(Hand) <= 160 * 1024 ? 2 : 1;
   Buf bufs[kBufs];
   Hand hand[kHands][W];  // S and E of a chunk as operands, from the wave that carries to the one that follows
+  __device__ __forceinline__ Buf& buf(int64_t c) { return bufs[kBufs == 1 ? 0 : static_cast<uint32_t>(c) % kBufs]; }
 };
 
 template <typename TM>
@@ -256,7 +234,7 @@ __device__ __forceinline__ void put_frag(TM* p, const Frag<TM>& f) {
 }
 
 // W waves carry 16 value columns each through the chunks, W follow, and four fetch.  Turn n: the first do chunk n,
-// the second finish chunk n - 1 and the last bring chunk n + 1.
+// the second finish chunk n - 1 and the last bring chunk n + 1, or n + 2 where three have room.
 template <typename TM, int KB, int W, bool TRAIN, bool FAST>
 __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Geo g, Ptrs p, int parts) {
   constexpr int KP = 32 * KB, BV = 16 * W, kThreads = 128 * W + 64 * (FAST ? kFetchers : 0);
@@ -274,13 +252,11 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
   const TM* k = static_cast<const TM*>(p.k) + b * g.k_b + h / g.rep * g.k_h;
   const TM* q = static_cast<const TM*>(p.q) + b * g.q_b + h / g.rep * g.q_h;
   const TM* v = static_cast<const TM*>(p.v) + b * g.v_b + h * g.v_h + v0;
-  const TM* w = static_cast<const TM*>(p.w) + bh * g.chunks * kC * key;
   const TM* squares = static_cast<const TM*>(p.lower) + bh * g.chunks * 2 * kSquare;
   const Tokens* tokens = p.tokens + bh * g.chunks;
   auto rows_of = [&](int64_t c) { return static_cast<int>(min(static_cast<int64_t>(kC), g.length - c * kC)); };
   auto copy = [&](int64_t c) {  // by all
-    typename Lds::Buf& bf = lds.bufs[0];
-    KTile::template copy<kThreads>(bf.w, w + c * kC * key, key, kC, key);
+    typename Lds::Buf& bf = lds.buf(c);
     KTile::template copy<kThreads>(bf.k, k + c * kC * g.k_t, g.k_t, rows_of(c), key);
     VTile::template copy<kThreads>(bf.v, v + c * kC * g.v_t, g.v_t, rows_of(c), value - v0);
     for (int i = static_cast<int>(threadIdx.x); i < 2 * kC; i += kThreads) bf.in[i] = tokens[c].in[i];
@@ -291,7 +267,6 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
       const uint32_t none[4] = {0, 0, 0, 0};
       typename Lds::Buf& bf = lds.bufs[i / (KTile::kElements / KTile::kUnit)];
       const int at = i % (KTile::kElements / KTile::kUnit) * KTile::kUnit;
-      store_words(bf.w + at, none);
       store_words(bf.k + at, none);
       if constexpr (Lds::kQ) store_words(bf.q + at, none);
     }
@@ -301,41 +276,56 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
     if (wave >= 2 * W) {
       constexpr int F = kFetchers;
       const int part = wave - 2 * W;
-      const Lines<TM, KP, F> w_lines(key, key, part), k_lines(g.k_t, key, part), q_lines(g.q_t, key, part);
-      const Lines<TM, BV, F> v_lines(g.v_t, value - v0, part);
-      for (int64_t c = 0; c <= g.chunks + 1; ++c) {  // turn c - 1
-        if (c < g.chunks) {
-          typename Lds::Buf& bf = lds.bufs[c & 1];
-          w_lines.issue(bf.w, w + c * kC * key, part);
-          if (Lds::kHands == 1 && c > 0) __syncthreads();  // where the others hand over
-          if (rows_of(c) == kC) {
-            k_lines.issue(bf.k, k + c * kC * g.k_t, part);
-            v_lines.issue(bf.v, v + c * kC * g.v_t, part);
-          } else {
-            KTile::template issue<F>(bf.k, k + c * kC * g.k_t, g.k_t, rows_of(c), key, part, zeros);
-            VTile::template issue<F>(bf.v, v + c * kC * g.v_t, g.v_t, rows_of(c), value - v0, part, zeros);
-          }
-          if (part == 0 && lane_id() < 2 * kC / 4) direct_load(tokens[c].in + 4 * lane_id(), bf.in);
-          if constexpr (Lds::kT) {  // P behind T in memory and in LDS
-            constexpr int kPer = 16 / static_cast<int>(sizeof(TM)) * kWave;  // elements of a load
-#pragma unroll
-            for (int i = 0; i < (Lds::kQ ? 2 : 1) * 6 * kFrag / kPer / F; ++i) {
-              const int f = (i * F + part) * kPer;
-              direct_load(squares + c * 2 * kSquare + f, 16u * lane_id(), bf.t + f);
-            }
-          }
-          if constexpr (Lds::kQ) {
-            if (rows_of(c) == kC)
-              q_lines.issue(bf.q, q + c * kC * g.q_t, part);
-            else
-              KTile::template issue<F>(bf.q, q + c * kC * g.q_t, g.q_t, rows_of(c), key, part, zeros);
-          }
-          // every vector memory operation of this wave is done, loads to LDS among them; then everyone's
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        } else if (Lds::kHands == 1 && c > 0) {
-          __syncthreads();
+      constexpr int kPer = 16 / static_cast<int>(sizeof(TM)) * kWave;  // elements of a load
+      constexpr int kSquareLoads = Lds::kT ? (Lds::kQ ? 2 : 1) * 6 * kFrag / kPer / F : 0;
+      typedef Lines<TM, KP, F> KLines;
+      typedef Lines<TM, BV, F> VLines;
+      const KLines k_lines(g.k_t, key, part), q_lines(g.q_t, key, part);
+      const VLines v_lines(g.v_t, value - v0, part);
+      // direct loads of a chunk, of each wave at least
+      constexpr int kLoads = (Lds::kQ ? 2 : 1) * KLines::kMine + (VLines::kLoads >= F ? VLines::kMine : 0) + kSquareLoads;
+      constexpr int kFly = Lds::kBufs - 2;  // chunks on their way beside the next
+      static_assert(kFly * kLoads < 64, "the count of loads on their way has six bits");
+      auto one_of_two = [&](int64_t c) {  // K
+        typename Lds::Buf& bf = lds.buf(c);
+        if (rows_of(c) == kC)
+          k_lines.issue(bf.k, k + c * kC * g.k_t, part);
+        else
+          KTile::template issue<F>(bf.k, k + c * kC * g.k_t, g.k_t, rows_of(c), key, part, zeros);
+      };
+      auto two_of_two = [&](int64_t c) {  // the rest
+        typename Lds::Buf& bf = lds.buf(c);
+        if (part == 0 && lane_id() < 2 * kC / 4) direct_load(tokens[c].in + 4 * lane_id(), bf.in);
+        if (rows_of(c) == kC) {
+          v_lines.issue(bf.v, v + c * kC * g.v_t, part);
+          if constexpr (Lds::kQ) q_lines.issue(bf.q, q + c * kC * g.q_t, part);
+        } else {
+          VTile::template issue<F>(bf.v, v + c * kC * g.v_t, g.v_t, rows_of(c), value - v0, part, zeros);
+          if constexpr (Lds::kQ)
+            KTile::template issue<F>(bf.q, q + c * kC * g.q_t, g.q_t, rows_of(c), key, part, zeros);
         }
-        if (c <= g.chunks) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSquareLoads; ++i) {  // P behind T in memory and in LDS
+          const int f = (i * F + part) * kPer;
+          direct_load(squares + c * 2 * kSquare + f, 16u * lane_id(), bf.t + f);
+        }
+      };
+      for (int64_t c = 0; c <= kFly && c < g.chunks; ++c) {
+        one_of_two(c);
+        two_of_two(c);
+      }
+      for (int64_t n = 0; n <= g.chunks; ++n) {
+        // Of this wave's vector memory operations, which end in their order, only the chunks' behind n are
+        // still on their way, and at the end none; then everyone's.
+        if (n + kFly < g.chunks)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kFly * kLoads) : "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const int64_t c = n + kFly + 1;
+        if (c < g.chunks) one_of_two(c);
+        if constexpr (Lds::kHands == 1) __syncthreads();  // where the others hand over
+        if (c < g.chunks) two_of_two(c);
       }
       return;
     }
@@ -359,24 +349,32 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
         copy(n);
         __syncthreads();
       }
-      const typename Lds::Buf& bf = lds.bufs[n & (Lds::kBufs - 1)];
+      const typename Lds::Buf& bf = lds.buf(n);
       f32x4 e[4];
       Frag<TM> so[KB];  // S as an operand over the keys
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) so[kb] = frag_of<TM>(s[2 * kb], s[2 * kb + 1]);
-      const Frag<TM> vo[2] = {VTile::over_tokens(bf.v, 0, 16 * mine), VTile::over_tokens(bf.v, 32, 16 * mine)};
+      // V - exp(c) K S0^T
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4 z = {0, 0, 0, 0};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) mma(z, KTile::rows(bf.k, 16 * i, 32 * kb), so[kb]);
+        const f32x4 vv = VTile::values(bf.v, 16 * i, 16 * mine);
+        const float4 d = *reinterpret_cast<const float4*>(bf.in + 16 * i + 4 * quad);
+        e[i] = f32x4{vv[0] - d.x * z[0], vv[1] - d.y * z[1], vv[2] - d.z * z[2], vv[3] - d.w * z[3]};
+      }
+      const Frag<TM> zo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         e[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j <= i / 2; ++j) {
           if constexpr (Lds::kT)
-            mma(e[i], frag_at(bf.t + lower_at(i, j)), vo[j]);
+            mma(e[i], frag_at(bf.t + lower_at(i, j)), zo[j]);
           else
-            mma(e[i], held[lower_at(i, j) / kFrag], vo[j]);
+            mma(e[i], held[lower_at(i, j) / kFrag], zo[j]);
         }
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) mma(e[i], KTile::rows(bf.w, 16 * i, 32 * kb), so[kb]);
       }
       const Frag<TM> eo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
       if (n + 1 < g.chunks) hold(n + 1);
@@ -493,7 +491,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
       }
     }
     if (n < g.chunks) {
-      const typename Lds::Buf& bf = lds.bufs[n & (Lds::kBufs - 1)];
+      const typename Lds::Buf& bf = lds.buf(n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         in[i] = g.scale * bf.in[16 * i + col];
@@ -520,13 +518,9 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
 
 // ------------------------------------------------------------------ the choice
 
-// Value tiles of a workgroup: two, and one where the LDS has no room for two.
-template <typename TM, int KB>
-constexpr int kTiles = sizeof(TM) == 4 && KB >= 4 ? 1 : 2;
-
 template <typename TM, int KB, bool TRAIN>
 void launch(const Geo& g, const Ptrs& p, hipStream_t s) {
-  constexpr int W = kTiles<TM, KB>;
+  constexpr int W = 2;
   const unsigned cells = static_cast<unsigned>(g.batch * g.heads * g.chunks);
   const int parts = static_cast<int>(cdiv(g.value, 16 * W));
   const bool fast = fast_rows(g, p);
@@ -636,7 +630,6 @@ Layout forward_layout(const Geo& g, bool train) {
   const size_t cells = static_cast<size_t>(g.batch * g.heads * g.chunks), el = element_size(g.dtype);
   size_t o = 0;
   l.lower = o; o = align256(o + cells * 2 * kSquare * el);
-  l.w = o; o = align256(o + cells * kC * g.key * el);
   l.tokens = o;
   if (!train) o = align256(o + cells * sizeof(Tokens));
   l.total = o;
@@ -683,7 +676,6 @@ extern "C" int mko_delta_fwd(const mko_delta_params* prm, void* stream) {
   Ptrs p = base_ptrs(prm);
   char* ws = static_cast<char*>(prm->workspace);
   p.lower = ws + w.lower;
-  p.w = ws + w.w;
   if (train) {
     const Layout l = saved_layout(g);
     char* sv = static_cast<char*>(prm->saved);

@@ -3,8 +3,8 @@
 // Per (batch, value head), with state S (value x key) and c the running sum of the log decay:
 //   e_t = v_t - exp(g_t) S_{t-1} k_t,  S_t = exp(g_t) S_{t-1} + beta_t e_t k_t^T,  y_t = scale S_t q_t
 // In a chunk of 64 tokens with entering state S0 the e of all tokens solve one triangular system:
-//   A[t][s] = exp(c_t - c_s) (k_t . k_s) beta_s for s < t,  T = (I + A)^-1,  W = T exp(c) K
-//   E = T V - W S0^T,  P[t][s] = scale exp(c_t - c_s) (q_t . k_s) beta_s for s <= t
+//   A[t][s] = exp(c_t - c_s) (k_t . k_s) beta_s for s < t,  T = (I + A)^-1
+//   E = T (V - exp(c) K S0^T),  P[t][s] = scale exp(c_t - c_s) (q_t . k_s) beta_s for s <= t
 //   Y = scale exp(c) Q S0^T + P E,  S' = exp(c_63) S0 + E^T (beta exp(c_63 - c) K)
 //
 // Everything runs on 16x16 tiles of the matrix cores, whose accumulator layout (lane l holds column
@@ -52,7 +52,6 @@ struct Ptrs {
   void *y, *final_state, *dq, *dk, *dv, *ddecay, *dbeta, *dinitial;
   Tokens* tokens;        // (batch, heads, chunks)
   void *lower, *upper;   // T and P as operands, and their transposes, (batch, heads, chunks, 2, kSquare)
-  void* w;               // -W, (batch, heads, chunks, kC, key)
   void *states, *grads;  // S0 and the gradient of S' of each chunk, (batch, heads, chunks, value, key)
   void* e;               // E, (batch, heads, chunks, kC, value)
   float *pq, *pk;        // dq and dk of each value head, where key heads are shared
@@ -479,10 +478,10 @@ __device__ __forceinline__ void store_operands(TM* row, int n, const Frag<TM> (&
 
 // Bytes of the arrays that the forward leaves for the backward, and of the workspaces.
 struct Layout {
-  size_t tokens, lower, upper, w, states, e, total;
+  size_t tokens, lower, upper, states, e, total;
 };
 Layout saved_layout(const Geo& g);                // tokens, upper, states, e
-Layout forward_layout(const Geo& g, bool train);  // lower and w, and tokens unless they are saved
+Layout forward_layout(const Geo& g, bool train);  // lower, and tokens unless they are saved
 
 int make_geo(const mko_delta_params* prm, const char* what, Geo* g);
 Ptrs base_ptrs(const mko_delta_params* prm);
