@@ -204,33 +204,87 @@ __global__ void __launch_bounds__(256) prep(Geo g, Ptrs p, bool fast) {
   }
 }
 
-// What a workgroup of `scan` holds in LDS.  FAST (rows of whole units at multiples of 16 bytes): two or three
-// buffers, and the loads of the next chunk or two fly while one is worked on.  Otherwise one buffer, filled
-// between two barriers.
+// LDS of `scan`.  FAST: rows of whole units at multiples of 16 bytes, which take direct loads.  T, Q and P are
+// there where they have room beside K, V and what is handed over; else T and P stay in registers.
 template <typename TM, int KB, int W, bool FAST>
-struct ScanLds {
-  static constexpr bool kT = FAST && KB * sizeof(TM) <= 8;  // T too; wider keys leave no room
-  static constexpr bool kQ = kT && sizeof(TM) == 2;         // and Q and P
-  static constexpr int kBufs = kQ ? 3 : FAST ? 2 : 1;
-  typedef Tile<TM, 32 * KB> KTile;
-  struct Buf {
-    TM k[KTile::kElements], v[Tile<TM, 16 * W>::kElements];
-    float in[kC], write[kC];
-    TM t[kT ? 6 * kFrag : 8], p[kQ ? 6 * kFrag : 8], q[kQ ? KTile::kElements : 8];
-  };
+struct ScanLds : Chunks<TM, KB, 16 * W, FAST ? (KB * sizeof(TM) <= 8 && sizeof(TM) == 2 ? 3 : 2) : 1,
+                        FAST && KB * sizeof(TM) <= 8 ? (sizeof(TM) == 2 ? 2 : 1) : 0,
+                        FAST && KB * sizeof(TM) <= 8 && sizeof(TM) == 2> {
   struct Hand {
     TM s[KB * kFrag], e[2 * kFrag];
   };
   // Two where there is room; one is read and written in one turn, on two sides of a barrier.
-  static constexpr int kHands = FAST && kBufs * sizeof(Buf) + 2 * W * sizeof(Hand) <= 160 * 1024 ? 2 : 1;
-  Buf bufs[kBufs];
+  static constexpr int kHands =
+      FAST && sizeof(Chunks<TM, KB, 16 * W, ScanLds::kBufs, ScanLds::kSquares, ScanLds::kQ>) + 2 * W * sizeof(Hand) <= 160 * 1024
+          ? 2 : 1;
   Hand hand[kHands][W];  // S and E of a chunk as operands, from the wave that carries to the one that follows
-  __device__ __forceinline__ Buf& buf(int64_t c) { return bufs[kBufs == 1 ? 0 : static_cast<uint32_t>(c) % kBufs]; }
 };
 
 template <typename TM>
 __device__ __forceinline__ void put_frag(TM* p, const Frag<TM>& f) {
   store_words(p + 8 * lane_id(), f.w);
+}
+
+// S of 16 value columns, carried through the chunks by one wave.
+template <typename TM, int KB>
+struct Carrier {
+  f32x4 s[2 * KB], e[4];  // S and E transposed: [key][value] and [token][value]
+  Frag<TM> so[KB];        // S as an operand over the keys
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i) s[i] = f32x4{0, 0, 0, 0};
+  }
+  // E = T (V - exp(c) K S0^T); `t` gives T's operands.
+  template <typename Lds, typename Square>
+  __device__ __forceinline__ void errors(const typename Lds::Buf& bf, int v0, bool no_values, Square t) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) so[kb] = frag_of<TM>(s[2 * kb], s[2 * kb + 1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 z = {0, 0, 0, 0};
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) mma(z, Lds::KTile::rows(bf.k, 16 * i, 32 * kb), so[kb]);
+      const f32x4 vv = no_values ? f32x4{0, 0, 0, 0} : Lds::VTile::values(bf.v, 16 * i, v0);
+      const float4 d = *reinterpret_cast<const float4*>(bf.in + 16 * i + 4 * lane_quad());
+      e[i] = f32x4{vv[0] - d.x * z[0], vv[1] - d.y * z[1], vv[2] - d.z * z[2], vv[3] - d.w * z[3]};
+    }
+    const Frag<TM> zo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      e[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j <= i / 2; ++j) mma(e[i], t(i, j), zo[j]);
+    }
+  }
+  // S' = exp(c_63) S0 + E^T (beta exp(c_63 - c) K)
+  template <typename Lds>
+  __device__ __forceinline__ void advance(const typename Lds::Buf& bf) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 d = *reinterpret_cast<const float4*>(bf.write + 16 * i + 4 * lane_quad());
+      e[i] = f32x4{e[i][0] * d.x, e[i][1] * d.y, e[i][2] * d.z, e[i][3] * d.w};
+    }
+    const Frag<TM> wo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
+    const float last = bf.in[kC - 1];
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[i][r] *= last;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) mma(s[i], Lds::KTile::keys_over_tokens(bf.k, 32 * j, i), wo[j]);
+    }
+  }
+};
+
+template <typename TM>
+__device__ __forceinline__ Source<TM> source(const Geo& g, const Ptrs& p, int64_t b, int64_t h, int v0) {
+  const int64_t bh = b * g.heads + h;
+  return Source<TM>{static_cast<const TM*>(p.k) + b * g.k_b + h / g.rep * g.k_h,
+                    static_cast<const TM*>(p.q) + b * g.q_b + h / g.rep * g.q_h,
+                    static_cast<const TM*>(p.v) + b * g.v_b + h * g.v_h + v0, g.k_t, g.q_t, g.v_t, g.length,
+                    p.tokens + bh * g.chunks, static_cast<const TM*>(p.lower) + bh * g.chunks * 2 * kSquare,
+                    static_cast<int>(g.key), static_cast<int>(g.value) - v0};
 }
 
 // W waves carry 16 value columns each through the chunks, W follow, and four fetch.  Turn n: the first do chunk n,
@@ -239,8 +293,8 @@ template <typename TM, int KB, int W, bool TRAIN, bool FAST>
 __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Geo g, Ptrs p, int parts) {
   constexpr int KP = 32 * KB, BV = 16 * W, kThreads = 128 * W + 64 * (FAST ? kFetchers : 0);
   typedef ScanLds<TM, KB, W, FAST> Lds;
-  typedef Tile<TM, KP> KTile;
-  typedef Tile<TM, BV> VTile;
+  typedef typename Lds::KTile KTile;
+  constexpr bool kMid = FAST && Lds::kHands == 1;
   __shared__ __align__(16) Lds lds;
   const WgId id = wg_id(parts, static_cast<int>(g.heads));
   const int64_t h = id.y, b = id.z, bh = b * g.heads + h;
@@ -248,161 +302,52 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
   const int mine = wave % W;  // of the value tiles
   const int v0 = id.x * BV, vt = v0 + 16 * mine, vc = vt + col;  // the lane's column of S and E
   const int key = static_cast<int>(g.key), value = static_cast<int>(g.value);
-  const TM* zeros = reinterpret_cast<const TM*>(&zero_unit);
-  const TM* k = static_cast<const TM*>(p.k) + b * g.k_b + h / g.rep * g.k_h;
-  const TM* q = static_cast<const TM*>(p.q) + b * g.q_b + h / g.rep * g.q_h;
-  const TM* v = static_cast<const TM*>(p.v) + b * g.v_b + h * g.v_h + v0;
-  const TM* squares = static_cast<const TM*>(p.lower) + bh * g.chunks * 2 * kSquare;
-  const Tokens* tokens = p.tokens + bh * g.chunks;
-  auto rows_of = [&](int64_t c) { return static_cast<int>(min(static_cast<int64_t>(kC), g.length - c * kC)); };
-  auto copy = [&](int64_t c) {  // by all
-    typename Lds::Buf& bf = lds.buf(c);
-    KTile::template copy<kThreads>(bf.k, k + c * kC * g.k_t, g.k_t, rows_of(c), key);
-    VTile::template copy<kThreads>(bf.v, v + c * kC * g.v_t, g.v_t, rows_of(c), value - v0);
-    for (int i = static_cast<int>(threadIdx.x); i < 2 * kC; i += kThreads) bf.in[i] = tokens[c].in[i];
-  };
+  const Source<TM> src = source<TM>(g, p, b, h, v0);
 
-  if (FAST && key < KP) {  // keys that no load fills
-    for (int i = static_cast<int>(threadIdx.x); i < Lds::kBufs * KTile::kElements / KTile::kUnit; i += kThreads) {
-      const uint32_t none[4] = {0, 0, 0, 0};
-      typename Lds::Buf& bf = lds.bufs[i / (KTile::kElements / KTile::kUnit)];
-      const int at = i % (KTile::kElements / KTile::kUnit) * KTile::kUnit;
-      store_words(bf.k + at, none);
-      if constexpr (Lds::kQ) store_words(bf.q + at, none);
-    }
-    __syncthreads();
-  }
+  if (FAST && key < KP) lds.clear(kThreads);
   if constexpr (FAST) {
     if (wave >= 2 * W) {
-      constexpr int F = kFetchers;
-      const int part = wave - 2 * W;
-      constexpr int kPer = 16 / static_cast<int>(sizeof(TM)) * kWave;  // elements of a load
-      constexpr int kSquareLoads = Lds::kT ? (Lds::kQ ? 2 : 1) * 6 * kFrag / kPer / F : 0;
-      typedef Lines<TM, KP, F> KLines;
-      typedef Lines<TM, BV, F> VLines;
-      const KLines k_lines(g.k_t, key, part), q_lines(g.q_t, key, part);
-      const VLines v_lines(g.v_t, value - v0, part);
-      // direct loads of a chunk, of each wave at least
-      constexpr int kLoads = (Lds::kQ ? 2 : 1) * KLines::kMine + (VLines::kLoads >= F ? VLines::kMine : 0) + kSquareLoads;
-      constexpr int kFly = Lds::kBufs - 2;  // chunks on their way beside the next
-      static_assert(kFly * kLoads < 64, "the count of loads on their way has six bits");
-      auto one_of_two = [&](int64_t c) {  // K
-        typename Lds::Buf& bf = lds.buf(c);
-        if (rows_of(c) == kC)
-          k_lines.issue(bf.k, k + c * kC * g.k_t, part);
-        else
-          KTile::template issue<F>(bf.k, k + c * kC * g.k_t, g.k_t, rows_of(c), key, part, zeros);
-      };
-      auto two_of_two = [&](int64_t c) {  // the rest
-        typename Lds::Buf& bf = lds.buf(c);
-        if (part == 0 && lane_id() < 2 * kC / 4) direct_load(tokens[c].in + 4 * lane_id(), bf.in);
-        if (rows_of(c) == kC) {
-          v_lines.issue(bf.v, v + c * kC * g.v_t, part);
-          if constexpr (Lds::kQ) q_lines.issue(bf.q, q + c * kC * g.q_t, part);
-        } else {
-          VTile::template issue<F>(bf.v, v + c * kC * g.v_t, g.v_t, rows_of(c), value - v0, part, zeros);
-          if constexpr (Lds::kQ)
-            KTile::template issue<F>(bf.q, q + c * kC * g.q_t, g.q_t, rows_of(c), key, part, zeros);
-        }
-#pragma unroll
-        for (int i = 0; i < kSquareLoads; ++i) {  // P behind T in memory and in LDS
-          const int f = (i * F + part) * kPer;
-          direct_load(squares + c * 2 * kSquare + f, 16u * lane_id(), bf.t + f);
-        }
-      };
-      for (int64_t c = 0; c <= kFly && c < g.chunks; ++c) {
-        one_of_two(c);
-        two_of_two(c);
-      }
-      for (int64_t n = 0; n <= g.chunks; ++n) {
-        // Of this wave's vector memory operations, which end in their order, only the chunks' behind n are
-        // still on their way, and at the end none; then everyone's.
-        if (n + kFly < g.chunks)
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kFly * kLoads) : "memory");
-        else
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        const int64_t c = n + kFly + 1;
-        if (c < g.chunks) one_of_two(c);
-        if constexpr (Lds::kHands == 1) __syncthreads();  // where the others hand over
-        if (c < g.chunks) two_of_two(c);
-      }
+      Fetcher<TM, KB, BV, Lds>(src, reinterpret_cast<const TM*>(&zero_unit), wave - 2 * W).template walk<kMid, 1>(lds, 0, 1, g.chunks);
       return;
     }
   }
   if (wave < W) {
-    f32x4 s[2 * KB];  // S transposed: [key][value]
-#pragma unroll
-    for (int i = 0; i < 2 * KB; ++i) s[i] = f32x4{0, 0, 0, 0};
-    if (p.initial && vc < value) load_state<FAST>(s, p.initial, g.state_dtype, (bh * value + vc) * key, key);
-    Frag<TM> held[Lds::kT ? 1 : 6];
+    Carrier<TM, KB> carrier;
+    carrier.clear();
+    if (p.initial && vc < value) load_state<FAST>(carrier.s, p.initial, g.state_dtype, (bh * value + vc) * key, key);
+    Frag<TM> held[Lds::kSquares ? 1 : 6];
     auto hold = [&](int64_t c) {
-      if constexpr (!Lds::kT) {
+      if constexpr (!Lds::kSquares) {
 #pragma unroll
-        for (int i = 0; i < 6; ++i) held[i] = frag_at(squares + c * 2 * kSquare + i * kFrag);
+        for (int i = 0; i < 6; ++i) held[i] = frag_at(src.squares + c * 2 * kSquare + i * kFrag);
       }
     };
     if (g.chunks > 0) hold(0);
     for (int64_t n = 0; n < g.chunks; ++n) {
       __syncthreads();
+      typename Lds::Buf& bf = lds.buf(n);
       if constexpr (!FAST) {
-        copy(n);
+        copy_chunk<kThreads, TM, Lds>(bf, src, n);
         __syncthreads();
       }
-      const typename Lds::Buf& bf = lds.buf(n);
-      f32x4 e[4];
-      Frag<TM> so[KB];  // S as an operand over the keys
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) so[kb] = frag_of<TM>(s[2 * kb], s[2 * kb + 1]);
-      // V - exp(c) K S0^T
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f32x4 z = {0, 0, 0, 0};
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) mma(z, KTile::rows(bf.k, 16 * i, 32 * kb), so[kb]);
-        const f32x4 vv = VTile::values(bf.v, 16 * i, 16 * mine);
-        const float4 d = *reinterpret_cast<const float4*>(bf.in + 16 * i + 4 * quad);
-        e[i] = f32x4{vv[0] - d.x * z[0], vv[1] - d.y * z[1], vv[2] - d.z * z[2], vv[3] - d.w * z[3]};
-      }
-      const Frag<TM> zo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e[i] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j <= i / 2; ++j) {
-          if constexpr (Lds::kT)
-            mma(e[i], frag_at(bf.t + lower_at(i, j)), zo[j]);
-          else
-            mma(e[i], held[lower_at(i, j) / kFrag], zo[j]);
-        }
-      }
-      const Frag<TM> eo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
+      carrier.template errors<Lds>(bf, 16 * mine, false, [&](int i, int j) {
+        if constexpr (Lds::kSquares > 0)
+          return frag_at(bf.squares + lower_at(i, j));
+        else
+          return held[lower_at(i, j) / kFrag];
+      });
       if (n + 1 < g.chunks) hold(n + 1);
-      if constexpr (FAST && Lds::kHands == 1) __syncthreads();  // what was handed over last has been read
+      if constexpr (kMid) __syncthreads();  // what was handed over last has been read
       typename Lds::Hand& hand = lds.hand[n & (Lds::kHands - 1)][mine];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) put_frag(hand.s + kb * kFrag, so[kb]);
-      put_frag(hand.e, eo[0]);
-      put_frag(hand.e + kFrag, eo[1]);
-      // S' = exp(c_63) S0 + E^T (beta exp(c_63 - c) K)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 d = *reinterpret_cast<const float4*>(bf.write + 16 * i + 4 * quad);
-        e[i] = f32x4{e[i][0] * d.x, e[i][1] * d.y, e[i][2] * d.z, e[i][3] * d.w};
-      }
-      const Frag<TM> wo[2] = {frag_of<TM>(e[0], e[1]), frag_of<TM>(e[2], e[3])};
-      const float last = bf.in[kC - 1];
-#pragma unroll
-      for (int i = 0; i < 2 * KB; ++i) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[i][r] *= last;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) mma(s[i], KTile::keys_over_tokens(bf.k, 32 * j, i), wo[j]);
-      }
+      for (int kb = 0; kb < KB; ++kb) put_frag(hand.s + kb * kFrag, carrier.so[kb]);
+      put_frag(hand.e, frag_of<TM>(carrier.e[0], carrier.e[1]));
+      put_frag(hand.e + kFrag, frag_of<TM>(carrier.e[2], carrier.e[3]));
+      carrier.template advance<Lds>(bf);
     }
     __syncthreads();  // the last turn of those that follow
-    if constexpr (FAST && Lds::kHands == 1) __syncthreads();
-    if (p.final_state && vc < value) store_state<FAST>(p.final_state, g.state_dtype, (bh * value + vc) * key, key, s);
+    if constexpr (kMid) __syncthreads();
+    if (p.final_state && vc < value) store_state<FAST>(p.final_state, g.state_dtype, (bh * value + vc) * key, key, carrier.s);
     return;
   }
 
@@ -426,20 +371,22 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
     __syncthreads();
     Frag<TM> so[KB], eo[2];
     if (n > 0) {
-      const typename Lds::Hand& hand = lds.hand[(n - 1) & (Lds::kHands - 1)][mine];
+      typename Lds::Hand& hand = lds.hand[(n - 1) & (Lds::kHands - 1)][mine];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) so[kb] = frag_at(hand.s + kb * kFrag);
       eo[0] = frag_at(hand.e);
       eo[1] = frag_at(hand.e + kFrag);
     }
-    if (!FAST && n < g.chunks) copy(n);
-    if (FAST ? Lds::kHands == 1 : n < g.chunks) __syncthreads();
+    if constexpr (!FAST) {
+      if (n < g.chunks) copy_chunk<kThreads, TM, Lds>(lds.buf(n), src, n);
+    }
+    if (FAST ? kMid : n < g.chunks) __syncthreads();
     // of tokens and keys that are not there, others' values: those tokens are not stored, and S has zeros at
     // those keys
     auto load_q = [&](int64_t c, int i, int kb) {
       if constexpr (FAST) {
-        const char* from = reinterpret_cast<const char*>(q + c * kC * g.q_t);
-        const uint32_t row = min(16 * i + col, rows_of(c) - 1) * static_cast<uint32_t>(g.q_t);
+        const char* from = reinterpret_cast<const char*>(src.q + c * kC * g.q_t);
+        const uint32_t row = min(16 * i + col, src.rows(c) - 1) * static_cast<uint32_t>(g.q_t);
         const uint32_t at = (row + (32 * kb + 8 * quad < key ? 32 * kb + 8 * quad : 0)) * static_cast<uint32_t>(sizeof(TM));
         Frag<TM> f;
 #pragma unroll
@@ -452,7 +399,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
         }
         return f;
       } else {
-        return frag_memory(q + c * kC * g.q_t, g.q_t, 16 * i, 32 * kb, rows_of(c), key);
+        return frag_memory(src.q + c * kC * g.q_t, g.q_t, 16 * i, 32 * kb, src.rows(c), key);
       }
     };
     if (n > 0) {
@@ -477,7 +424,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
         for (int r = 0; r < 4; ++r) y[r] *= in[i];
 #pragma unroll
         for (int j = 0; j <= i / 2; ++j) mma(y, eo[j], pf[lower_at(i, j) / kFrag]);
-        if (16 * i + col < rows_of(c))
+        if (16 * i + col < src.rows(c))
           store_four<TM, FAST>(yp + (16 * i + col) * y_row, vt + 4 * quad, value, y);
       }
       if constexpr (TRAIN) {
@@ -491,7 +438,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
       }
     }
     if (n < g.chunks) {
-      const typename Lds::Buf& bf = lds.buf(n);
+      typename Lds::Buf& bf = lds.buf(n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         in[i] = g.scale * bf.in[16 * i + col];
@@ -508,9 +455,9 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
 #pragma unroll
       for (int i = 0; i < 6; ++i) {
         if constexpr (Lds::kQ)
-          pf[i] = frag_at(bf.p + i * kFrag);
+          pf[i] = frag_at(bf.squares + kSquare + i * kFrag);
         else
-          pf[i] = frag_at(squares + (2 * n + 1) * kSquare + i * kFrag);
+          pf[i] = frag_at(src.squares + (2 * n + 1) * kSquare + i * kFrag);
       }
     }
   }

@@ -307,15 +307,6 @@ struct Lines {
   }
 };
 
-// What `back` holds of a chunk in LDS: K, Q, a slice of dY, the tokens' factors, and the two squares it
-// multiplies with where SQUARES.
-template <typename TM, int KP, int BV, bool SQUARES>
-struct Chunk {
-  TM k[Tile<TM, KP>::kElements], q[Tile<TM, KP>::kElements], v[Tile<TM, BV>::kElements];
-  float in[kC], write[kC];
-  TM squares[SQUARES ? 12 * kFrag : 8];
-};
-
 // Place of the operand of row tile i and contraction block j in a square: of the lower triangle
 // (j <= i / 2) or of its transpose (j >= i / 2).
 __host__ __device__ constexpr int lower_at(int i, int j) { return (i < 2 ? i : 2 * i - 2 + j) * kFrag; }
@@ -329,70 +320,133 @@ __device__ __forceinline__ Frag<TM> frag_at(const TM* p) {
   return f;
 }
 
-// Waves that do nothing but fetch: a wave issues a direct load in about 75 cycles, so one alone brings 13.6
-// bytes a cycle to LDS, two 25.7 and four, one on each SIMD, 44; eight no more (64 KB of rows of 256 bytes in L2,
-// 256 workgroups).
-constexpr int kFetchers = 4;
+// What a workgroup holds in LDS of the chunks it walks: K, a slice of V or dY, exp(c) and beta exp(c_63 - c);
+// SQUARES: one or two triangular squares, Q.  More than one buffer: the loads of the chunks ahead fly while
+// one is worked on.  One: it is filled between two barriers.
+template <typename TM, int KB, int BV, int BUFS, int SQUARES, bool Q>
+struct Chunks {
+  static constexpr int kBufs = BUFS, kSquares = SQUARES;
+  static constexpr bool kQ = Q;
+  typedef Tile<TM, 32 * KB> KTile;
+  typedef Tile<TM, BV> VTile;
+  struct Buf {
+    TM k[KTile::kElements], v[VTile::kElements];
+    float in[kC], write[kC];
+    TM squares[SQUARES > 0 ? SQUARES * kSquare : 8], q[Q ? KTile::kElements : 8];
+  };
+  Buf bufs[BUFS];
+  // That of the n-th chunk of the walk.
+  __device__ __forceinline__ Buf& buf(int64_t n) { return bufs[BUFS == 1 ? 0 : static_cast<uint32_t>(n) % BUFS]; }
 
-// Chunks on their way to LDS for `back`.  FAST (rows of whole units at multiples of 16 bytes): two buffers, and
-// the loads of the next chunk fly while one is worked on; kFetch: waves of their own issue them.  Otherwise
-// one buffer, filled between two barriers.
-template <typename TM, int KP, int BV, int W, bool FAST>
-struct Feed {
-  static constexpr int kBufs = FAST ? 2 : 1;
-  static constexpr bool kFetch = FAST && KP * sizeof(TM) <= 256;  // wider keys leave no room for the squares,
-  static constexpr bool kSquares = kFetch;                        // and no registers for more waves
-  static constexpr int kWaves = kFetch ? kFetchers : W;           // that load
-  typedef Chunk<TM, KP, BV, kSquares> Buf;
+  // Keys that no load fills become zero.
+  __device__ __forceinline__ void clear(int threads) {
+    constexpr int kUnits = KTile::kElements / KTile::kUnit;
+    for (int i = static_cast<int>(threadIdx.x); i < BUFS * kUnits; i += threads) {
+      const uint32_t none[4] = {0, 0, 0, 0};
+      const int at = i % kUnits * KTile::kUnit;
+      store_words(bufs[i / kUnits].k + at, none);
+      if constexpr (Q) store_words(bufs[i / kUnits].q + at, none);
+    }
+    __syncthreads();
+  }
+};
+
+// Where a head's chunks are.
+template <typename TM>
+struct Source {
   const TM *k, *q, *v;
   int64_t k_t, q_t, v_t, length;
   const Tokens* tokens;
   const TM* squares;  // two of a chunk
   int key, value;     // columns of K and Q, and of this slice
-
-  __device__ __forceinline__ void fetch(Buf* bufs, int64_t c, int wave, const TM* zeros) const {
-    const int64_t t0 = c * kC;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(kC), length - t0));
-    Buf& b = bufs[c & (kBufs - 1)];
-    const float* from = tokens[c].in;
-    if constexpr (FAST) {
-      Tile<TM, KP>::template issue<kWaves>(b.k, k + t0 * k_t, k_t, rows, key, wave, zeros);
-      Tile<TM, KP>::template issue<kWaves>(b.q, q + t0 * q_t, q_t, rows, key, wave, zeros);
-      Tile<TM, BV>::template issue<kWaves>(b.v, v + t0 * v_t, v_t, rows, value, wave, zeros);
-      if (wave == 0 && lane_id() < 2 * kC / 4) direct_load(from + 4 * lane_id(), b.in);
-      if constexpr (kSquares) {
-        constexpr int kPer = 16 / static_cast<int>(sizeof(TM)) * kWave;  // elements of a load
-        static_assert(12 * kFrag / kPer % kWaves == 0, "an equal share of the squares");
-#pragma unroll
-        for (int j = 0; j < 12 * kFrag / kPer / kWaves; ++j) {
-          const int f = (j * kWaves + wave) * kPer;
-          direct_load(squares + c * 2 * kSquare + f, 16u * lane_id(), b.squares + f);
-        }
-      }
-    } else {
-      Tile<TM, KP>::template copy<64 * W>(b.k, k + t0 * k_t, k_t, rows, key);
-      Tile<TM, KP>::template copy<64 * W>(b.q, q + t0 * q_t, q_t, rows, key);
-      Tile<TM, BV>::template copy<64 * W>(b.v, v + t0 * v_t, v_t, rows, value);
-      for (int i = static_cast<int>(threadIdx.x); i < 2 * kC; i += 64 * W) b.in[i] = from[i];
-    }
-  }
-  // Chunk c is in its buffer, and the one after it (`next`, if there is one) on its way.
-  __device__ __forceinline__ const Buf& turn(Buf* bufs, int64_t c, int64_t next, bool more, int wave, const TM* zeros) const {
-    if constexpr (kFetch) {
-      __syncthreads();
-    } else if constexpr (FAST) {
-      // every vector memory operation of this wave is done, loads to LDS among them; then everyone's
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (more) fetch(bufs, next, wave, zeros);
-    } else {
-      __syncthreads();
-      fetch(bufs, c, wave, zeros);
-      __syncthreads();
-    }
-    return bufs[c & (kBufs - 1)];
+  __device__ __forceinline__ int rows(int64_t c) const {
+    return static_cast<int>(min(static_cast<int64_t>(kC), length - c * kC));
   }
 };
+
+// Waves that do nothing but fetch: a wave issues a direct load in about 75 cycles, so one alone brings 13.6
+// bytes a cycle to LDS, two 25.7 and four, one on each SIMD, 44; eight no more (64 KB of rows of 256 bytes in L2,
+// 256 workgroups).
+constexpr int kFetchers = 4;
+
+template <typename TM, int KB, int BV, typename Lds>
+struct Fetcher {
+  static constexpr int F = kFetchers;
+  typedef Tile<TM, 32 * KB> KTile;
+  typedef Tile<TM, BV> VTile;
+  typedef Lines<TM, 32 * KB, F> KLines;
+  typedef Lines<TM, BV, F> VLines;
+  static constexpr int kPer = 16 / static_cast<int>(sizeof(TM)) * kWave;  // elements of a load
+  static constexpr int kSquareLoads = Lds::kSquares * kSquare / kPer / F;
+  static_assert(Lds::kSquares * kSquare % (kPer * F) == 0 || Lds::kSquares == 1, "an equal share of the squares");
+  // direct loads of a chunk, of each wave at least
+  static constexpr int kLoads =
+      (Lds::kQ ? 2 : 1) * KLines::kMine + (VLines::kLoads >= F ? VLines::kMine : 0) + kSquareLoads;
+  static constexpr int kFly = Lds::kBufs - 2;  // chunks on their way beside the next
+  static_assert(kFly * kLoads < 64, "the count of loads on their way has six bits");
+
+  const Source<TM>& src;
+  const TM* zeros;
+  int part;
+  KLines k_lines, q_lines;
+  VLines v_lines;
+  __device__ __forceinline__ Fetcher(const Source<TM>& s, const TM* z, int p)
+      : src(s), zeros(z), part(p), k_lines(s.k_t, s.key, p), q_lines(s.q_t, s.key, p), v_lines(s.v_t, s.value, p) {}
+
+  __device__ __forceinline__ void keys(typename Lds::Buf& b, int64_t c) const {
+    if (src.rows(c) == kC)
+      k_lines.issue(b.k, src.k + c * kC * src.k_t, part);
+    else
+      KTile::template issue<F>(b.k, src.k + c * kC * src.k_t, src.k_t, src.rows(c), src.key, part, zeros);
+  }
+  __device__ __forceinline__ void rest(typename Lds::Buf& b, int64_t c) const {
+    if (part == 0 && lane_id() < 2 * kC / 4) direct_load(src.tokens[c].in + 4 * lane_id(), b.in);
+    if (src.rows(c) == kC) {
+      v_lines.issue(b.v, src.v + c * kC * src.v_t, part);
+      if constexpr (Lds::kQ) q_lines.issue(b.q, src.q + c * kC * src.q_t, part);
+    } else {
+      VTile::template issue<F>(b.v, src.v + c * kC * src.v_t, src.v_t, src.rows(c), src.value, part, zeros);
+      if constexpr (Lds::kQ)
+        KTile::template issue<F>(b.q, src.q + c * kC * src.q_t, src.q_t, src.rows(c), src.key, part, zeros);
+    }
+#pragma unroll
+    for (int i = 0; i < (Lds::kSquares * kSquare + kPer * F - 1) / (kPer * F); ++i) {  // the second behind the first
+      const int f = (i * F + part) * kPer;
+      if (f < Lds::kSquares * kSquare) direct_load(src.squares + c * 2 * kSquare + f, 16u * lane_id(), b.squares + f);
+    }
+  }
+  // The chunks first, first + step, ..., n of them; a barrier each, MORE of them at the end, and MID: another
+  // within each turn.
+  template <bool MID, int MORE>
+  __device__ __forceinline__ void walk(Lds& lds, int64_t first, int64_t step, int64_t n) const {
+    for (int64_t i = 0; i <= kFly && i < n; ++i) {
+      keys(lds.buf(i), first + i * step);
+      rest(lds.buf(i), first + i * step);
+    }
+    for (int64_t i = 0; i < n + MORE; ++i) {
+      // Of this wave's vector memory operations, which end in their order, only the chunks' behind i are
+      // still on their way, and at the end none; then everyone's.
+      if (i + kFly < n)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kFly * kLoads) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      const int64_t j = i + kFly + 1, c = first + j * step;
+      if (j < n) keys(lds.buf(j), c);
+      if constexpr (MID) __syncthreads();
+      if (j < n) rest(lds.buf(j), c);
+    }
+  }
+};
+
+// A chunk through registers, by all THREADS.
+template <int THREADS, typename TM, typename Lds>
+__device__ __forceinline__ void copy_chunk(typename Lds::Buf& b, const Source<TM>& src, int64_t c) {
+  Lds::KTile::template copy<THREADS>(b.k, src.k + c * kC * src.k_t, src.k_t, src.rows(c), src.key);
+  if constexpr (Lds::kQ) Lds::KTile::template copy<THREADS>(b.q, src.q + c * kC * src.q_t, src.q_t, src.rows(c), src.key);
+  Lds::VTile::template copy<THREADS>(b.v, src.v + c * kC * src.v_t, src.v_t, src.rows(c), src.value);
+  for (int i = static_cast<int>(threadIdx.x); i < 2 * kC; i += THREADS) b.in[i] = src.tokens[c].in[i];
+}
 
 // N values at element i of a row of n, those below n; WHOLE: n is a multiple of N.
 template <typename T, bool WHOLE, int N>

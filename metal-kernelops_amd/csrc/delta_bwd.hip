@@ -24,18 +24,18 @@ namespace {
 
 __device__ uint4 zero_unit;  // where rows and columns outside come from
 
-// Waves of a workgroup of `back`: W that carry G, and those that fetch.
+// LDS of `back`; wider keys leave no room for the squares, which then stay in registers.
 template <typename TM, int KB, int W, bool FAST>
-constexpr int back_waves() {
-  return W + (Feed<TM, 32 * KB, 16 * W, W, FAST>::kFetch ? kFetchers : 0);
-}
+using BackLds = Chunks<TM, KB, 16 * W, FAST ? (KB * sizeof(TM) <= 8 && sizeof(TM) == 2 ? 3 : 2) : 1,
+                       FAST && KB * sizeof(TM) <= 8 ? 2 : 0, true>;
 
+// W waves carry 16 value columns of G each through the chunks, and four fetch.
 template <typename TM, int KB, int W, bool FAST>
-__global__ void __launch_bounds__((64 * back_waves<TM, KB, W, FAST>())) back(Geo g, Ptrs p, int parts) {
-  constexpr int KP = 32 * KB, BV = 16 * W;
-  typedef Feed<TM, KP, BV, W, FAST> Feeder;
+__global__ void __launch_bounds__(64 * W + 64 * (FAST ? kFetchers : 0)) back(Geo g, Ptrs p, int parts) {
+  constexpr int KP = 32 * KB, BV = 16 * W, kThreads = 64 * W + 64 * (FAST ? kFetchers : 0);
+  typedef BackLds<TM, KB, W, FAST> Lds;
   typedef Tile<TM, KP> KTile;
-  __shared__ __align__(16) typename Feeder::Buf bufs[Feeder::kBufs];
+  __shared__ __align__(16) Lds lds;
   const WgId id = wg_id(parts, static_cast<int>(g.heads));
   const int64_t h = id.y, b = id.z, bh = b * g.heads + h;
   const int wave = uniform(threadIdx.x >> 6), col = lane_col(), quad = lane_quad();
@@ -43,20 +43,15 @@ __global__ void __launch_bounds__((64 * back_waves<TM, KB, W, FAST>())) back(Geo
   const int key = static_cast<int>(g.key), value = static_cast<int>(g.value);
   const int64_t yrow = g.heads * g.value;  // dy and dv are dense
   TM* dv = static_cast<TM*>(p.dv) + b * g.length * yrow + h * value;
-  const TM* zeros = reinterpret_cast<const TM*>(&zero_unit);
-  const Feeder feed{static_cast<const TM*>(p.k) + b * g.k_b + h / g.rep * g.k_h,
-                    static_cast<const TM*>(p.q) + b * g.q_b + h / g.rep * g.q_h,
-                    static_cast<const TM*>(p.dy) + b * g.length * yrow + h * value + v0, g.k_t, g.q_t, yrow, g.length,
-                    p.tokens + bh * g.chunks, static_cast<const TM*>(p.upper) + bh * g.chunks * 2 * kSquare, key, value - v0};
+  const Source<TM> src{static_cast<const TM*>(p.k) + b * g.k_b + h / g.rep * g.k_h,
+                       static_cast<const TM*>(p.q) + b * g.q_b + h / g.rep * g.q_h,
+                       static_cast<const TM*>(p.dy) + b * g.length * yrow + h * value + v0, g.k_t, g.q_t, yrow, g.length,
+                       p.tokens + bh * g.chunks, static_cast<const TM*>(p.upper) + bh * g.chunks * 2 * kSquare, key, value - v0};
 
-  if constexpr (Feeder::kFetch) {
+  if (FAST && key < KP) lds.clear(kThreads);
+  if constexpr (FAST) {
     if (wave >= W) {
-      for (int64_t c = g.chunks - 1; c >= 0; --c) {
-        feed.fetch(bufs, c, wave - W, zeros);
-        // every vector memory operation of this wave is done, loads to LDS among them; then everyone's
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-      }
+      Fetcher<TM, KB, BV, Lds>(src, reinterpret_cast<const TM*>(&zero_unit), wave - W).template walk<false, 0>(lds, g.chunks - 1, -1, g.chunks);
       return;
     }
   }
@@ -64,17 +59,21 @@ __global__ void __launch_bounds__((64 * back_waves<TM, KB, W, FAST>())) back(Geo
 #pragma unroll
   for (int i = 0; i < 2 * KB; ++i) s[i] = f32x4{0, 0, 0, 0};
   if (p.dfinal && vc < value) load_state<FAST>(s, p.dfinal, g.state_dtype, (bh * value + vc) * key, key);
-  if (FAST && !Feeder::kFetch && g.chunks > 0) feed.fetch(bufs, g.chunks - 1, wave, zeros);
   for (int64_t c = g.chunks - 1; c >= 0; --c) {
     const int64_t at = bh * g.chunks + c, t0 = c * kC;
-    Frag<TM> held[Feeder::kSquares ? 1 : 12];
-    if constexpr (!Feeder::kSquares) {
+    Frag<TM> held[Lds::kSquares ? 1 : 12];
+    if constexpr (!Lds::kSquares) {
 #pragma unroll
-      for (int i = 0; i < 12; ++i) held[i] = frag_at(feed.squares + (12 * c + i) * kFrag);
+      for (int i = 0; i < 12; ++i) held[i] = frag_at(src.squares + (12 * c + i) * kFrag);
     }
-    const typename Feeder::Buf& bf = feed.turn(bufs, c, c - 1, c > 0, wave, zeros);
+    __syncthreads();
+    typename Lds::Buf& bf = lds.buf(g.chunks - 1 - c);
+    if constexpr (!FAST) {
+      copy_chunk<kThreads, TM, Lds>(bf, src, c);
+      __syncthreads();
+    }
     auto square = [&](int which, int i, int j) {  // the transposes of T and P
-      if constexpr (Feeder::kSquares)
+      if constexpr (Lds::kSquares > 0)
         return frag_at(bf.squares + which * kSquare + upper_at(i, j));
       else
         return held[6 * which + upper_at(i, j) / kFrag];
@@ -457,7 +456,7 @@ void launch(const Geo& g, const Ptrs& p, hipStream_t s) {
   if constexpr (KB * sizeof(TM) <= 16) {
     fast = fast_rows(g, p);
     if (fast) {
-      MKO_TIMED("delta_back", s, back<TM, KB, W, true><<<grid, 64 * back_waves<TM, KB, W, true>(), 0, s>>>(g, p, parts));
+      MKO_TIMED("delta_back", s, back<TM, KB, W, true><<<grid, 64 * (W + kFetchers), 0, s>>>(g, p, parts));
       MKO_TIMED("delta_grads", s, grads<TM, KB, true><<<cells, 512, 0, s>>>(g, p));
     }
   }
