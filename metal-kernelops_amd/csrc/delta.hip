@@ -5,6 +5,15 @@
 //   scan  per (batch, head, 16 W value columns), sequential over the chunks.  W waves carry S in float32
 //         accumulators and do only what the next chunk waits for, E and S's update; W
 //         others follow a chunk behind with Y and the stores, and four fetch the chunk ahead.
+//
+// Few long sequences leave most of the chip idle, so their chunks are cut into segments that are walked side
+// by side.  A segment makes S0 M + B of the state S0 before it:
+//   ends  per (batch, head, segment but the last, 64 columns): the chunks' walk without outputs, from zero (B) and
+//         from the unit matrix (M)
+//   join  per (batch, head, 16 value columns): S0 of each segment, in their order
+// and the scan starts each segment from its own S0.
+#include <algorithm>
+
 #include "delta.hpp"
 
 namespace mko {
@@ -287,6 +296,93 @@ __device__ __forceinline__ Source<TM> source(const Geo& g, const Ptrs& p, int64_
                     static_cast<int>(g.key), static_cast<int>(g.value) - v0};
 }
 
+// LDS of `ends`.
+template <typename TM, int KB, int W>
+using EndsLds = Chunks<TM, KB, 16 * W, sizeof(Chunks<TM, KB, 16 * W, 3, 1, false>) <= 160 * 1024 ? 3 : 2, 1, false>;
+constexpr int kEndsTiles = 4;
+
+template <typename TM, int KB>
+__global__ void __launch_bounds__(64 * (kEndsTiles + kFetchers)) ends(Geo g, Ptrs p, int value_parts, int parts) {
+  constexpr int W = kEndsTiles, BV = 16 * W;
+  typedef EndsLds<TM, KB, W> Lds;
+  __shared__ __align__(16) Lds lds;
+  const WgId id = wg_id(parts, static_cast<int>(g.heads));
+  const int64_t h = id.y, b = id.z / (g.segments - 1), seg = id.z % (g.segments - 1), bh = b * g.heads + h;
+  const bool unit = id.x >= value_parts;  // from the unit matrix, whose rows stand for values
+  if (unit && seg == 0) return;           // the state before it is known
+  const int wave = uniform(threadIdx.x >> 6), col = lane_col(), quad = lane_quad();
+  const int v0 = (unit ? id.x - value_parts : id.x) * BV, vc = v0 + 16 * wave + col;
+  const int key = static_cast<int>(g.key), value = static_cast<int>(g.value);
+  const Source<TM> src = source<TM>(g, p, b, h, unit ? 0 : v0);
+  const int64_t first = seg * g.span, at = bh * (g.segments - 1) + seg;
+
+  if (key < 32 * KB) lds.clear(64 * (W + kFetchers));
+  if (wave >= W) {
+    Fetcher<TM, KB, BV, Lds>(src, reinterpret_cast<const TM*>(&zero_unit), wave - W).template walk<false, 0>(lds, first, 1, g.span);
+    return;
+  }
+  Carrier<TM, KB> carrier;
+  carrier.clear();
+  if (unit) {
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) carrier.s[i][r] = 16 * (i & ~1) + 4 * (i & 1) + 8 * quad + r == vc ? 1.0f : 0.0f;
+    }
+  } else if (seg == 0 && p.initial && vc < value) {
+    load_state<true>(carrier.s, p.initial, g.state_dtype, (bh * value + vc) * key, key);
+  }
+  for (int64_t n = 0; n < g.span; ++n) {
+    __syncthreads();
+    typename Lds::Buf& bf = lds.buf(n);
+    carrier.template errors<Lds>(bf, 16 * wave, unit, [&](int i, int j) { return frag_at(bf.squares + lower_at(i, j)); });
+    carrier.template advance<Lds>(bf);
+  }
+  if (!unit) {
+    if (vc < value) store_row<float, true>(p.ends + (at * value + vc) * key, key, carrier.s);
+  } else if (vc < key) {  // transposed, as `join` reads it
+    TM* to = static_cast<TM*>(p.maps) + at * key * key + vc;
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = 16 * (i & ~1) + 4 * (i & 1) + 8 * quad + r;
+        if (k < key) to[k * key] = from_f32<TM>(carrier.s[i][r]);
+      }
+    }
+  }
+}
+
+// The state behind each segment from the one before it, in place of its B; a wave for 16 values.
+template <typename TM, int KB>
+__global__ void __launch_bounds__(64) join(Geo g, Ptrs p, int tiles) {
+  const int64_t bh = blockIdx.x / tiles;
+  const int col = lane_col(), quad = lane_quad(), key = static_cast<int>(g.key);
+  const int64_t vc = blockIdx.x % tiles * 16 + col;
+  const bool live = vc < g.value;
+  float* row = p.ends + (bh * (g.segments - 1) * g.value + (live ? vc : 0)) * key;
+  f32x4 s[2 * KB];
+  load_row<float, true>(s, row, key);
+  for (int64_t seg = 1; seg < g.segments - 1; ++seg) {
+    row += g.value * key;
+    const TM* map = static_cast<const TM*>(p.maps) + (bh * (g.segments - 1) + seg) * key * key;
+    Frag<TM> so[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) so[kb] = frag_of<TM>(s[2 * kb], s[2 * kb + 1]);
+    load_row<float, true>(s, row, key);
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i) {
+      const int k = 16 * (i & ~1) + 4 * (i & 1) + 8 * (col / 4) + col % 4;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const Words<TM, 8> w = load_part<TM, 8>(map + (k < key ? k * key : 0), 32 * kb + 8 * quad, k < key ? key : 0);
+        mma(s[i], __builtin_bit_cast(Frag<TM>, w), so[kb]);
+      }
+    }
+    if (live) store_row<float, true>(row, key, s);
+  }
+}
+
 // W waves carry 16 value columns each through the chunks, W follow, and four fetch.  Turn n: the first do chunk n,
 // the second finish chunk n - 1 and the last bring chunk n + 1, or n + 2 where three have room.
 template <typename TM, int KB, int W, bool TRAIN, bool FAST>
@@ -297,7 +393,8 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
   constexpr bool kMid = FAST && Lds::kHands == 1;
   __shared__ __align__(16) Lds lds;
   const WgId id = wg_id(parts, static_cast<int>(g.heads));
-  const int64_t h = id.y, b = id.z, bh = b * g.heads + h;
+  const int64_t h = id.y, b = id.z / g.segments, seg = id.z % g.segments, bh = b * g.heads + h;
+  const int64_t first = seg * g.span, chunks = min(g.span, g.chunks - first);  // of this segment
   const int wave = uniform(threadIdx.x >> 6), col = lane_col(), quad = lane_quad();
   const int mine = wave % W;  // of the value tiles
   const int v0 = id.x * BV, vt = v0 + 16 * mine, vc = vt + col;  // the lane's column of S and E
@@ -307,14 +404,19 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
   if (FAST && key < KP) lds.clear(kThreads);
   if constexpr (FAST) {
     if (wave >= 2 * W) {
-      Fetcher<TM, KB, BV, Lds>(src, reinterpret_cast<const TM*>(&zero_unit), wave - 2 * W).template walk<kMid, 1>(lds, 0, 1, g.chunks);
+      Fetcher<TM, KB, BV, Lds>(src, reinterpret_cast<const TM*>(&zero_unit), wave - 2 * W).template walk<kMid, 1>(lds, first, 1, chunks);
       return;
     }
   }
   if (wave < W) {
     Carrier<TM, KB> carrier;
     carrier.clear();
-    if (p.initial && vc < value) load_state<FAST>(carrier.s, p.initial, g.state_dtype, (bh * value + vc) * key, key);
+    if (seg > 0) {
+      if (vc < value)
+        load_row<float, FAST>(carrier.s, p.ends + ((bh * (g.segments - 1) + seg - 1) * value + vc) * key, key);
+    } else if (p.initial && vc < value) {
+      load_state<FAST>(carrier.s, p.initial, g.state_dtype, (bh * value + vc) * key, key);
+    }
     Frag<TM> held[Lds::kSquares ? 1 : 6];
     auto hold = [&](int64_t c) {
       if constexpr (!Lds::kSquares) {
@@ -322,12 +424,12 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
         for (int i = 0; i < 6; ++i) held[i] = frag_at(src.squares + c * 2 * kSquare + i * kFrag);
       }
     };
-    if (g.chunks > 0) hold(0);
-    for (int64_t n = 0; n < g.chunks; ++n) {
+    if (chunks > 0) hold(first);
+    for (int64_t n = 0; n < chunks; ++n) {
       __syncthreads();
       typename Lds::Buf& bf = lds.buf(n);
       if constexpr (!FAST) {
-        copy_chunk<kThreads, TM, Lds>(bf, src, n);
+        copy_chunk<kThreads, TM, Lds>(bf, src, first + n);
         __syncthreads();
       }
       carrier.template errors<Lds>(bf, 16 * mine, false, [&](int i, int j) {
@@ -336,7 +438,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
         else
           return held[lower_at(i, j) / kFrag];
       });
-      if (n + 1 < g.chunks) hold(n + 1);
+      if (n + 1 < chunks) hold(first + n + 1);
       if constexpr (kMid) __syncthreads();  // what was handed over last has been read
       typename Lds::Hand& hand = lds.hand[n & (Lds::kHands - 1)][mine];
 #pragma unroll
@@ -347,7 +449,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
     }
     __syncthreads();  // the last turn of those that follow
     if constexpr (kMid) __syncthreads();
-    if (p.final_state && vc < value) store_state<FAST>(p.final_state, g.state_dtype, (bh * value + vc) * key, key, carrier.s);
+    if (p.final_state && first + chunks == g.chunks && vc < value) store_state<FAST>(p.final_state, g.state_dtype, (bh * value + vc) * key, key, carrier.s);
     return;
   }
 
@@ -367,7 +469,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
     }
     one[i] = frag_of<TM>(x[0], x[1]);
   }
-  for (int64_t n = 0; n <= g.chunks; ++n) {
+  for (int64_t n = 0; n <= chunks; ++n) {
     __syncthreads();
     Frag<TM> so[KB], eo[2];
     if (n > 0) {
@@ -378,9 +480,9 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
       eo[1] = frag_at(hand.e + kFrag);
     }
     if constexpr (!FAST) {
-      if (n < g.chunks) copy_chunk<kThreads, TM, Lds>(lds.buf(n), src, n);
+      if (n < chunks) copy_chunk<kThreads, TM, Lds>(lds.buf(n), src, first + n);
     }
-    if (FAST ? kMid : n < g.chunks) __syncthreads();
+    if (FAST ? kMid : n < chunks) __syncthreads();
     // of tokens and keys that are not there, others' values: those tokens are not stored, and S has zeros at
     // those keys
     auto load_q = [&](int64_t c, int i, int kb) {
@@ -403,7 +505,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
       }
     };
     if (n > 0) {
-      const int64_t c = n - 1, at = bh * g.chunks + c;
+      const int64_t c = first + n - 1, at = bh * g.chunks + c;
       TM* yp = static_cast<TM*>(p.y) + ((b * g.length + c * kC) * g.heads + h) * value;
       const auto y_row = [&] {  // of FAST, 32 bits
         if constexpr (FAST) return static_cast<uint32_t>(g.heads * value);
@@ -437,7 +539,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
         if (vc < value) store_operands<TM, FAST>(static_cast<TM*>(p.states) + (at * value + vc) * key, key, so);
       }
     }
-    if (n < g.chunks) {
+    if (n < chunks) {
       typename Lds::Buf& bf = lds.buf(n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -448,7 +550,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
             if constexpr (Lds::kQ)
               qf[i][kb] = KTile::rows(bf.q, 16 * i, 32 * kb);
             else
-              qf[i][kb] = load_q(n, i, kb);
+              qf[i][kb] = load_q(first + n, i, kb);
           }
         }
       }
@@ -457,7 +559,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
         if constexpr (Lds::kQ)
           pf[i] = frag_at(bf.squares + kSquare + i * kFrag);
         else
-          pf[i] = frag_at(src.squares + (2 * n + 1) * kSquare + i * kFrag);
+          pf[i] = frag_at(src.squares + (2 * (first + n) + 1) * kSquare + i * kFrag);
       }
     }
   }
@@ -466,7 +568,7 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
 // ------------------------------------------------------------------ the choice
 
 template <typename TM, int KB, bool TRAIN>
-void launch(const Geo& g, const Ptrs& p, hipStream_t s) {
+void launch(Geo g, const Ptrs& p, hipStream_t s) {
   constexpr int W = 2;
   const unsigned cells = static_cast<unsigned>(g.batch * g.heads * g.chunks);
   const int parts = static_cast<int>(cdiv(g.value, 16 * W));
@@ -475,10 +577,21 @@ void launch(const Geo& g, const Ptrs& p, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(g.batch * g.heads * parts);
   if constexpr (KB * sizeof(TM) <= 16) {
     if (fast) {
+      if (g.segments > 1) {
+        const int values = static_cast<int>(cdiv(g.value, 16 * kEndsTiles)), all = values + static_cast<int>(cdiv(g.key, 16 * kEndsTiles));
+        const int tiles = static_cast<int>(cdiv(g.value, 16));
+        const unsigned cells = static_cast<unsigned>(g.batch * g.heads * (g.segments - 1) * all);
+        MKO_TIMED("delta_ends", s, ends<TM, KB><<<cells, 64 * (kEndsTiles + kFetchers), 0, s>>>(g, p, values, all));
+        if (g.segments > 2)
+          MKO_TIMED("delta_join_states", s, join<TM, KB><<<static_cast<unsigned>(g.batch * g.heads * tiles), 64, 0, s>>>(g, p, tiles));
+      }
+      const unsigned grid = static_cast<unsigned>(g.batch * g.heads * parts * g.segments);
       MKO_TIMED("delta_scan", s, scan<TM, KB, W, TRAIN, true><<<grid, 128 * W + 64 * kFetchers, 0, s>>>(g, p, parts));
       return;
     }
   }
+  g.segments = 1;
+  g.span = g.chunks;
   MKO_TIMED("delta_scan", s, scan<TM, KB, W, TRAIN, false><<<grid, 128 * W, 0, s>>>(g, p, parts));
 }
 
@@ -498,6 +611,17 @@ void launch(const Geo& g, const Ptrs& p, bool train, hipStream_t s) {
 }  // namespace
 
 // ------------------------------------------------------------------ sizes
+
+// Segments that a sequence is cut into: where its workgroups leave more than two thirds of the 256 CUs without
+// work, as many as give each CU one, of 8 chunks or more, and no more than the square root of the chunks, since
+// `join` walks them one by one.  Walking the chunks twice pays from three segments on.
+int64_t segments_of(const mko_delta_params* prm, int64_t chunks) {
+  const int64_t groups = prm->batch * prm->heads * cdiv(prm->value, 32);
+  if (prm->key % 8 || prm->value % 8 || groups < 1 || 3 * groups > 256) return 1;
+  int64_t n = std::min<int64_t>(256 / groups, chunks / 8);
+  while (n > 1 && n * n > chunks) --n;
+  return n < 3 ? 1 : cdiv(chunks, cdiv(chunks, n));
+}
 
 int make_geo(const mko_delta_params* prm, const char* what, Geo* g) {
   if (!prm || prm->batch < 0 || prm->length < 0 || prm->key_heads < 0 || prm->heads < 0 || prm->key < 0 || prm->value < 0) {
@@ -526,8 +650,10 @@ int make_geo(const mko_delta_params* prm, const char* what, Geo* g) {
   }
   *g = Geo{prm->batch, prm->length, prm->key_heads, prm->heads, prm->key, prm->value,
            prm->q_stride_b, prm->q_stride_t, prm->q_stride_h, prm->k_stride_b, prm->k_stride_t, prm->k_stride_h,
-           prm->v_stride_b, prm->v_stride_t, prm->v_stride_h, chunks, static_cast<int>(prm->heads / prm->key_heads),
+           prm->v_stride_b, prm->v_stride_t, prm->v_stride_h, chunks, segments_of(prm, chunks), 0,
+           static_cast<int>(prm->heads / prm->key_heads),
            prm->scale, prm->dtype, prm->decay_dtype, prm->beta_dtype, prm->state_dtype};
+  g->span = cdiv(chunks, g->segments);
   return MKO_OK;
 }
 
@@ -579,6 +705,9 @@ Layout forward_layout(const Geo& g, bool train) {
   l.lower = o; o = align256(o + cells * 2 * kSquare * el);
   l.tokens = o;
   if (!train) o = align256(o + cells * sizeof(Tokens));
+  const size_t ends = static_cast<size_t>(g.batch * g.heads * (g.segments - 1));
+  l.ends = o; o = align256(o + ends * g.value * g.key * sizeof(float));
+  l.maps = o; o = align256(o + ends * g.key * g.key * el);
   l.total = o;
   return l;
 }
@@ -623,6 +752,8 @@ extern "C" int mko_delta_fwd(const mko_delta_params* prm, void* stream) {
   Ptrs p = base_ptrs(prm);
   char* ws = static_cast<char*>(prm->workspace);
   p.lower = ws + w.lower;
+  p.ends = reinterpret_cast<float*>(ws + w.ends);
+  p.maps = ws + w.maps;
   if (train) {
     const Layout l = saved_layout(g);
     char* sv = static_cast<char*>(prm->saved);

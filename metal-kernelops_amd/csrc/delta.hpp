@@ -34,7 +34,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 struct Geo {
   int64_t batch, length, key_heads, heads, key, value;
   int64_t q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h;
-  int64_t chunks;  // of a sequence
+  int64_t chunks;    // of a sequence
+  int64_t segments;  // that the forward walks side by side
+  int64_t span;      // chunks of a segment, the last one's at most
   int rep;         // value heads of a key head
   float scale;
   int dtype, decay_dtype, beta_dtype, state_dtype;
@@ -55,6 +57,8 @@ struct Ptrs {
   void *states, *grads;  // S0 and the gradient of S' of each chunk, (batch, heads, chunks, value, key)
   void* e;               // E, (batch, heads, chunks, kC, value)
   float *pq, *pk;        // dq and dk of each value head, where key heads are shared
+  float* ends;           // states behind the segments but the last, (batch, heads, segments - 1, value, key)
+  void* maps;            // what a segment makes of the state before it, (batch, heads, segments - 1, key, key)
 };
 
 // A lane's share of a 16 x 32 operand: row (or column) l % 16.  Over tokens element 4 h + r is index
@@ -532,10 +536,10 @@ __device__ __forceinline__ void store_operands(TM* row, int n, const Frag<TM> (&
 
 // Bytes of the arrays that the forward leaves for the backward, and of the workspaces.
 struct Layout {
-  size_t tokens, lower, upper, states, e, total;
+  size_t tokens, lower, upper, states, e, ends, maps, total;
 };
 Layout saved_layout(const Geo& g);                // tokens, upper, states, e
-Layout forward_layout(const Geo& g, bool train);  // lower, and tokens unless they are saved
+Layout forward_layout(const Geo& g, bool train);  // lower, ends and maps, and tokens unless they are saved
 
 int make_geo(const mko_delta_params* prm, const char* what, Geo* g);
 Ptrs base_ptrs(const mko_delta_params* prm);
