@@ -213,6 +213,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
   f32x4 dp[4], da[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) dp[i] = da[i] = f32x4{0, 0, 0, 0};
+  // tiles above the diagonal; the two waves of a SIMD, `tile` of each half, have five of eight together
+  auto outside = [&](int i) { return half ? i < tile : i > tile; };
   float gs = 0.0f;  // <G, S0>
   for (int v0 = 0; v0 < value; v0 += NV) {
     const int n = value - v0;
@@ -247,10 +249,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
         mma(ak[i], fs, mx);
         mma(aw[i], STile::keys_over_values(lds.gr, v, half * KT + i, lane), me);
       }
-      // without a branch on the triangle: what lies outside is dropped later
       const Frag<TM> b1 = half ? me : my, b2 = half ? me : mx;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        if (outside(i)) continue;
         mma(dp[i], VTile::rows(half ? lds.dy : lds.e, 16 * i, v, lane), b1);
         mma(da[i], VTile::rows(half ? lds.x : lds.e, 16 * i, v, lane), b2);
       }
@@ -302,6 +304,12 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     // first half: [s of tile i][its t]; second: [t of tile i][its s]
+    if (outside(i)) {
+      const uint32_t none[kWordsOf<TM, 4>] = {};
+      store_words(lds.squares[2 * half][tile][i / 2] + 8 * lane_id() + 4 * (i % 2), none);
+      store_words(lds.squares[2 * half + 1][tile][i / 2] + 8 * lane_id() + 4 * (i % 2), none);
+      continue;
+    }
     f32x4 qk = {0, 0, 0, 0}, kk = {0, 0, 0, 0};
     const int lane = lane_again();  // its own rows are read again for every tile: kept, they would spill
 #pragma unroll
