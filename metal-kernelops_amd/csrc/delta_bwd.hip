@@ -14,8 +14,9 @@
 //
 //   back   per (batch, head, 16 W value columns), sequential from the last chunk: G stays in float32
 //          accumulators; writes dV and each chunk's G
-//   grads  per (batch, head, chunk): everything else
-//   join   dq and dk summed over the value heads of a key head, in their order
+//   grads  per (batch, head, chunk): everything else.  Where value heads share a key head, a workgroup takes them
+//          one after the other, with dq and dk summed in registers in their order
+//   join   that sum where there are few such workgroups, or no room for it in LDS
 #include "delta.hpp"
 
 namespace mko {
@@ -153,57 +154,96 @@ __device__ __forceinline__ float quad_sum(float v) {
 // half of the keys, w / 4.  Of the 64 x 64 products dY E^T and X E^T the waves of the first half make
 // the columns of their t, those of the second the columns of their s, and hand them over through LDS.
 template <typename TM, int KB>
-struct GradsLds {
+struct GradsTiles {
   // values at a time; and whether K and Q are in LDS together
   static constexpr int kValues = sizeof(TM) == 2 && KB <= 4 ? 64 : 32;
   static constexpr bool kBoth = sizeof(TM) == 2 || KB <= 4;
   typedef Tile<TM, 32 * KB> KTile;
   typedef Tile<TM, 32 * KB, kValues> STile;
   typedef Tile<TM, kValues> VTile;
-  union {
-    struct {
-      TM s0[STile::kElements], gr[STile::kElements], dy[VTile::kElements], x[VTile::kElements], e[VTile::kElements];
-    };
-    struct {
-      TM k[KTile::kElements], q[kBoth ? KTile::kElements : 8];
-      TM squares[4][4][2][kFrag];  // dP and dA as operands: [reader, writer] x [dP, dA], token tile, block of 32
-    };
+  struct Values {
+    TM s0[STile::kElements], gr[STile::kElements], dy[VTile::kElements], x[VTile::kElements], e[VTile::kElements];
   };
-  Tokens tok;
-  float dc[kC], dots[4][3][16], rows[4][16], cols[4][16], gs[8], wrote[4];
+  struct Keys {
+    TM k[KTile::kElements], q[kBoth ? KTile::kElements : 8];
+    TM squares[4][4][2][kFrag];  // dP and dA as operands: [reader, writer] x [dP, dA], token tile, block of 32
+  };
+  struct Sums {
+    Tokens tok;
+    float dc[kC], dots[4][3][16], rows[4][16], cols[4][16], gs[8], wrote[4];
+  };
 };
+// GROUP: of a key head, whose K and Q stay while the first values of the next value head fly; otherwise the two
+// take turns in one place.
+template <typename TM, int KB, bool GROUP>
+struct GradsLds : GradsTiles<TM, KB>::Sums {
+  union {
+    typename GradsTiles<TM, KB>::Values values;
+    typename GradsTiles<TM, KB>::Keys keys;
+  };
+};
+template <typename TM, int KB>
+struct GradsLds<TM, KB, true> : GradsTiles<TM, KB>::Sums {
+  typename GradsTiles<TM, KB>::Values values;
+  typename GradsTiles<TM, KB>::Keys keys;
+};
+// Whether the value heads of a key head may be summed in registers: where K, Q, the squares and the values have
+// room in LDS side by side.
+template <typename TM, int KB>
+constexpr bool kGroups = sizeof(TM) == 2 || KB <= 2;
 
-template <typename TM, int KB, bool FAST>
-__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof(TM) == 2 && KB <= 4 ? 4 : 2))) grads(Geo g, Ptrs p) {
+template <typename TM, int KB, bool FAST, bool GROUP>
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof(TM) == 2 && KB <= 4 && !GROUP ? 4 : 2)))
+grads(Geo g, Ptrs p) {
   constexpr int KT = KB;  // key tiles of a wave
-  typedef GradsLds<TM, KB> Lds;
-  typedef typename Lds::KTile KTile;
-  typedef typename Lds::STile STile;
-  typedef typename Lds::VTile VTile;
-  constexpr int NV = Lds::kValues;
-  constexpr bool kBoth = Lds::kBoth;
-  __shared__ __align__(16) Lds lds;
-  const WgId id = wg_id(static_cast<int>(g.heads), static_cast<int>(g.chunks));
-  const int64_t h = id.x, c = id.y, b = id.z;
-  const int64_t at = (b * g.heads + h) * g.chunks + c, t0 = c * kC;
+  typedef GradsTiles<TM, KB> Tiles;
+  typedef typename Tiles::KTile KTile;
+  typedef typename Tiles::STile STile;
+  typedef typename Tiles::VTile VTile;
+  constexpr int NV = Tiles::kValues;
+  constexpr bool kBoth = Tiles::kBoth;
+  __shared__ __align__(16) GradsLds<TM, KB, GROUP> lds;
+  typename Tiles::Values& lv = lds.values;
+  typename Tiles::Keys& lk = lds.keys;
+  const WgId id = wg_id(static_cast<int>(GROUP ? g.key_heads : g.heads), static_cast<int>(g.chunks));
+  const int64_t h0 = GROUP ? id.x * g.rep : id.x, c = id.y, b = id.z, t0 = c * kC;
   const int rows = static_cast<int>(min(static_cast<int64_t>(kC), g.length - t0));
   const int wave = uniform(threadIdx.x >> 6), tile = wave & 3, half = wave >> 2, col = lane_col(), quad = lane_quad();
   const int key = static_cast<int>(g.key), value = static_cast<int>(g.value);
-  const TM* q = static_cast<const TM*>(p.q) + b * g.q_b + t0 * g.q_t + h / g.rep * g.q_h;
-  const TM* k = static_cast<const TM*>(p.k) + b * g.k_b + t0 * g.k_t + h / g.rep * g.k_h;
-  const int64_t yrow = g.heads * g.value, y0 = (b * g.length + t0) * yrow + h * value;
-  const TM *dy = static_cast<const TM*>(p.dy) + y0, *x = static_cast<const TM*>(p.dv) + y0;
-  const TM* e = static_cast<const TM*>(p.e) + at * kC * value;
-  const TM* s0 = static_cast<const TM*>(p.states) + at * value * key;
-  const TM* gr = static_cast<const TM*>(p.grads) + at * value * key;
+  const TM* q = static_cast<const TM*>(p.q) + b * g.q_b + t0 * g.q_t + h0 / g.rep * g.q_h;
+  const TM* k = static_cast<const TM*>(p.k) + b * g.k_b + t0 * g.k_t + h0 / g.rep * g.k_h;
+  const int64_t yrow = g.heads * g.value;
   const TM* zeros = reinterpret_cast<const TM*>(&zero_unit);
   const Tokens& tok = lds.tok;
+  auto load_values = [&](int64_t h, int v0) {
+    const int64_t at = (b * g.heads + h) * g.chunks + c, y0 = (b * g.length + t0) * yrow + h * value + v0;
+    const int64_t s0 = (at * value + v0) * key;
+    const int n = value - v0;
+    STile::template load<8, FAST>(lv.s0, static_cast<const TM*>(p.states) + s0, key, n, key, wave, zeros);
+    STile::template load<8, FAST>(lv.gr, static_cast<const TM*>(p.grads) + s0, key, n, key, wave, zeros);
+    VTile::template load<8, FAST>(lv.dy, static_cast<const TM*>(p.dy) + y0, yrow, rows, n, wave, zeros);
+    VTile::template load<8, FAST>(lv.x, static_cast<const TM*>(p.dv) + y0, yrow, rows, n, wave, zeros);
+    VTile::template load<8, FAST>(lv.e, static_cast<const TM*>(p.e) + at * kC * value + v0, value, kC, n, wave, zeros);
+  };
+  auto load_keys = [&] {
+    KTile::template load<8, FAST>(lk.k, k, g.k_t, rows, key, wave, zeros);
+    if constexpr (kBoth) KTile::template load<8, FAST>(lk.q, q, g.q_t, rows, key, wave, zeros);
+  };
+  const int tc = 16 * tile + col;  // the lane's token
+  const bool live = tc < rows;
+  f32x4 sq[GROUP ? KT : 1], sk[GROUP ? KT : 1];  // dq and dk of the key head
+  if constexpr (GROUP) {
+#pragma unroll
+    for (int i = 0; i < KT; ++i) sq[i] = sk[i] = f32x4{0, 0, 0, 0};
+    load_keys();
+  }
+  load_values(h0, 0);
+  for (int64_t h = h0; h < h0 + (GROUP ? g.rep : 1); ++h) {
   {
-    const uint32_t* from = reinterpret_cast<const uint32_t*>(p.tokens + at);
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(p.tokens + (b * g.heads + h) * g.chunks + c);
     uint32_t* to = reinterpret_cast<uint32_t*>(&lds.tok);
     for (int i = threadIdx.x; i < static_cast<int>(sizeof(Tokens) / 4); i += 512) to[i] = from[i];
   }
-  const int tc = 16 * tile + col;  // the lane's token
 
   // ---- over the values: the products with the states, and dY E^T and X E^T
   f32x4 aq[KT], ak[KT], aw[KT];  // [key][token]: dY S0, X S0, E G
@@ -217,21 +257,18 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
   auto outside = [&](int i) { return half ? i < tile : i > tile; };
   float gs = 0.0f;  // <G, S0>
   for (int v0 = 0; v0 < value; v0 += NV) {
-    const int n = value - v0;
-    if (v0) __syncthreads();
-    STile::template load<8, FAST>(lds.s0, s0 + static_cast<int64_t>(v0) * key, key, n, key, wave, zeros);
-    STile::template load<8, FAST>(lds.gr, gr + static_cast<int64_t>(v0) * key, key, n, key, wave, zeros);
-    VTile::template load<8, FAST>(lds.dy, dy + v0, yrow, rows, n, wave, zeros);
-    VTile::template load<8, FAST>(lds.x, x + v0, yrow, rows, n, wave, zeros);
-    VTile::template load<8, FAST>(lds.e, e + v0, value, kC, n, wave, zeros);
+    if (v0) {
+      __syncthreads();
+      load_values(h, v0);
+    }
     direct_wait();
 #pragma unroll 1
     for (int o = 8 * threadIdx.x; o < STile::kElements; o += 8 * 512) {
       uint32_t w[kWordsOf<TM, 8>];
       float fa[8], fb[8];
-      load_words(lds.s0 + o, w);
+      load_words(lv.s0 + o, w);
       unpack_words<TM, 8>(w, fa);
-      load_words(lds.gr + o, w);
+      load_words(lv.gr + o, w);
       unpack_words<TM, 8>(w, fb);
 #pragma unroll
       for (int j = 0; j < 8; ++j) gs += fa[j] * fb[j];
@@ -240,44 +277,46 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
     for (int vb = 0; vb < NV / 32; ++vb) {
       const int v = 32 * vb, lane = lane_again();
       if (v0 + v >= value) break;
-      const Frag<TM> my = VTile::rows(lds.dy, 16 * tile, v, lane), mx = VTile::rows(lds.x, 16 * tile, v, lane),
-                     me = VTile::rows(lds.e, 16 * tile, v, lane);
+      const Frag<TM> my = VTile::rows(lv.dy, 16 * tile, v, lane), mx = VTile::rows(lv.x, 16 * tile, v, lane),
+                     me = VTile::rows(lv.e, 16 * tile, v, lane);
 #pragma unroll
       for (int i = 0; i < KT; ++i) {
-        const Frag<TM> fs = STile::keys_over_values(lds.s0, v, half * KT + i, lane);
+        const Frag<TM> fs = STile::keys_over_values(lv.s0, v, half * KT + i, lane);
         mma(aq[i], fs, my);
         mma(ak[i], fs, mx);
-        mma(aw[i], STile::keys_over_values(lds.gr, v, half * KT + i, lane), me);
+        mma(aw[i], STile::keys_over_values(lv.gr, v, half * KT + i, lane), me);
       }
       const Frag<TM> b1 = half ? me : my, b2 = half ? me : mx;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (outside(i)) continue;
-        mma(dp[i], VTile::rows(half ? lds.dy : lds.e, 16 * i, v, lane), b1);
-        mma(da[i], VTile::rows(half ? lds.x : lds.e, 16 * i, v, lane), b2);
+        mma(dp[i], VTile::rows(half ? lv.dy : lv.e, 16 * i, v, lane), b1);
+        mma(da[i], VTile::rows(half ? lv.x : lv.e, 16 * i, v, lane), b2);
       }
     }
   }
   __syncthreads();
-  KTile::template load<8, FAST>(lds.k, k, g.k_t, rows, key, wave, zeros);
-  if constexpr (kBoth) KTile::template load<8, FAST>(lds.q, q, g.q_t, rows, key, wave, zeros);
   gs = wave_sum(gs);
   if (lane_id() == 0) lds.gs[wave] = gs;
-  direct_wait();
+  if constexpr (GROUP) {
+    if (h + 1 < h0 + g.rep) load_values(h + 1, 0);  // K and Q came with the first head's
+  } else {
+    load_keys();
+    direct_wait();
+  }
 
   // ---- the states' parts of dq and dk, [key][token] in place
   const float in = tok.in[tc], out = tok.out[tc], beta = tok.beta[tc];
-  const bool live = tc < rows;
   float dot[3] = {0.0f, 0.0f, 0.0f};  // q . state part of dq, k . that of dk, k . E G
 #pragma unroll
   for (int i = 0; i < KT; ++i) {
     const int n = half * KT + i, k0 = 32 * (n / 2) + 8 * quad + 4 * (n % 2);
     float kv[4], qv[4];
     uint32_t w[kWordsOf<TM, 4>];
-    load_words(lds.k + KTile::at(tc, k0), w);
+    load_words(lk.k + KTile::at(tc, k0), w);
     unpack_words<TM, 4>(w, kv);
     if constexpr (kBoth) {
-      load_words(lds.q + KTile::at(tc, k0), w);
+      load_words(lk.q + KTile::at(tc, k0), w);
       unpack_words<TM, 4>(w, qv);
     } else {
       unpack_words<TM, 4>(load_part<TM, 4>(q + (live ? tc * g.q_t : 0), k0, live ? key : 0).w, qv);
@@ -306,19 +345,19 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
     // first half: [s of tile i][its t]; second: [t of tile i][its s]
     if (outside(i)) {
       const uint32_t none[kWordsOf<TM, 4>] = {};
-      store_words(lds.squares[2 * half][tile][i / 2] + 8 * lane_id() + 4 * (i % 2), none);
-      store_words(lds.squares[2 * half + 1][tile][i / 2] + 8 * lane_id() + 4 * (i % 2), none);
+      store_words(lk.squares[2 * half][tile][i / 2] + 8 * lane_id() + 4 * (i % 2), none);
+      store_words(lk.squares[2 * half + 1][tile][i / 2] + 8 * lane_id() + 4 * (i % 2), none);
       continue;
     }
     f32x4 qk = {0, 0, 0, 0}, kk = {0, 0, 0, 0};
     const int lane = lane_again();  // its own rows are read again for every tile: kept, they would spill
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const Frag<TM> other = KTile::rows(lds.k, 16 * i, 32 * kb, lane), mine = KTile::rows(lds.k, 16 * tile, 32 * kb, lane);
+      const Frag<TM> other = KTile::rows(lk.k, 16 * i, 32 * kb, lane), mine = KTile::rows(lk.k, 16 * tile, 32 * kb, lane);
       mma(kk, other, mine);
       if constexpr (kBoth) {
-        mma(qk, KTile::rows(half ? lds.q : lds.k, 16 * i, 32 * kb, lane),
-            KTile::rows(half ? lds.k : lds.q, 16 * tile, 32 * kb, lane));
+        mma(qk, KTile::rows(half ? lk.q : lk.k, 16 * i, 32 * kb, lane),
+            KTile::rows(half ? lk.k : lk.q, 16 * tile, 32 * kb, lane));
       } else {
         const Frag<TM> f = frag_memory(q, g.q_t, 16 * (half ? i : tile), 32 * kb, rows, key);
         mma(qk, half ? f : other, half ? mine : f);
@@ -342,9 +381,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
     }
     uint32_t w[kWordsOf<TM, 4>];
     pack_words<TM, 4>(vp, w);
-    store_words(lds.squares[2 * half][tile][i / 2] + 8 * lane + 4 * (i % 2), w);
+    store_words(lk.squares[2 * half][tile][i / 2] + 8 * lane + 4 * (i % 2), w);
     pack_words<TM, 4>(va, w);
-    store_words(lds.squares[2 * half + 1][tile][i / 2] + 8 * lane + 4 * (i % 2), w);
+    store_words(lk.squares[2 * half + 1][tile][i / 2] + 8 * lane + 4 * (i % 2), w);
     asm volatile("" : "+v"(sum));  // a tile at a time, for the registers
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -356,29 +395,35 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
   const int last = lane_again();
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const Frag<TM> pr = frag_at(lds.squares[0][tile][j]), ar = frag_at(lds.squares[1][tile][j]),
-                   pw = frag_at(lds.squares[2][tile][j]), aw2 = frag_at(lds.squares[3][tile][j]);
+    const Frag<TM> pr = frag_at(lk.squares[0][tile][j]), ar = frag_at(lk.squares[1][tile][j]),
+                   pw = frag_at(lk.squares[2][tile][j]), aw2 = frag_at(lk.squares[3][tile][j]);
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
-      const Frag<TM> ok = KTile::keys_over_tokens(lds.k, 32 * j, half * KT + i, last);
+      const Frag<TM> ok = KTile::keys_over_tokens(lk.k, 32 * j, half * KT + i, last);
       mma(aq[i], ok, pr);
       mma(ak[i], ok, ar);
       mma(ak[i], ok, aw2);
-      if constexpr (kBoth) mma(ak[i], KTile::keys_over_tokens(lds.q, 32 * j, half * KT + i, last), pw);
+      if constexpr (kBoth) mma(ak[i], KTile::keys_over_tokens(lk.q, 32 * j, half * KT + i, last), pw);
     }
   }
   if constexpr (!kBoth) {
     __syncthreads();
-    KTile::template load<8, FAST>(lds.k, q, g.q_t, rows, key, wave, zeros);
+    KTile::template load<8, FAST>(lk.k, q, g.q_t, rows, key, wave, zeros);
     direct_wait();
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const Frag<TM> pw = frag_at(lds.squares[2][tile][j]);
+      const Frag<TM> pw = frag_at(lk.squares[2][tile][j]);
 #pragma unroll
-      for (int i = 0; i < KT; ++i) mma(ak[i], KTile::keys_over_tokens(lds.k, 32 * j, half * KT + i, last), pw);
+      for (int i = 0; i < KT; ++i) mma(ak[i], KTile::keys_over_tokens(lk.k, 32 * j, half * KT + i, last), pw);
     }
   }
-  if (live) {
+  if constexpr (GROUP) {
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+      sq[i] += aq[i];
+      sk[i] += ak[i];
+    }
+  } else if (live) {
     const int64_t row = ((b * g.length + t0 + tc) * g.heads + h) * key;
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
@@ -418,6 +463,19 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
     }
     if (lane < rows) store_one(p.ddecay, g.decay_dtype, (b * g.length + t0 + lane) * g.heads + h, d);
   }
+  if constexpr (GROUP) __syncthreads();  // before the next head's tokens
+  }
+  if constexpr (GROUP) {
+    if (live) {
+      const int64_t row = ((b * g.length + t0 + tc) * g.key_heads + id.x) * key;
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+        const int n = half * KT + i, k0 = 32 * (n / 2) + 8 * quad + 4 * (n % 2);
+        store_four<TM, FAST>(static_cast<TM*>(p.dq) + row, k0, key, sq[i]);
+        store_four<TM, FAST>(static_cast<TM*>(p.dk) + row, k0, key, sk[i]);
+      }
+    }
+  }
 }
 
 // dq and dk of a key head: the sum over its value heads, four elements a thread.
@@ -439,13 +497,19 @@ __global__ void __launch_bounds__(256) join(Geo g, Ptrs p, int64_t groups, int p
   store_part<TM, 4>(to + row * key, at, key, s);
 }
 
+// Whether they are: with a workgroup or more for each of the 256 CUs (bf16, 2048 of them, four heads each: 344 us, and
+// 519 with partial sums in memory).  Fewer leave CUs idle (float32, 128 of two heads: 52 us, and 35).
+bool grouped(const Geo& g) {
+  return g.rep > 1 && (g.dtype != MKO_F32 || g.key <= 64) && g.batch * g.key_heads * g.chunks >= 256;
+}
+
 struct Space {
   size_t grads, pq, pk, total;
 };
 Space backward_layout(const Geo& g) {
   Space l{};
   const size_t cells = static_cast<size_t>(g.batch * g.heads * g.chunks), el = element_size(g.dtype);
-  const size_t part = g.rep > 1 ? static_cast<size_t>(g.batch * g.length * g.heads * g.key) * 4 : 0;
+  const size_t part = g.rep > 1 && !grouped(g) ? static_cast<size_t>(g.batch * g.length * g.heads * g.key) * 4 : 0;
   size_t o = 0;
   l.grads = o; o = align256(o + cells * g.value * g.key * el);
   l.pq = o; o = align256(o + part);
@@ -460,22 +524,29 @@ void launch(const Geo& g, const Ptrs& p, hipStream_t s) {
   const unsigned cells = static_cast<unsigned>(g.batch * g.heads * g.chunks);
   const int parts = static_cast<int>(cdiv(g.value, 16 * W));
   const unsigned grid = static_cast<unsigned>(g.batch * g.heads * parts);
+  const unsigned groups = static_cast<unsigned>(g.batch * g.key_heads * g.chunks);
   bool fast = false;
   if constexpr (KB * sizeof(TM) <= 16) {
     fast = fast_rows(g, p);
     if (fast) {
       MKO_TIMED("delta_back", s, back<TM, KB, W, true><<<grid, 64 * (W + kFetchers), 0, s>>>(g, p, parts));
-      MKO_TIMED("delta_grads", s, grads<TM, KB, true><<<cells, 512, 0, s>>>(g, p));
+      if constexpr (kGroups<TM, KB>) {
+        if (grouped(g)) MKO_TIMED("delta_grads", s, grads<TM, KB, true, true><<<groups, 512, 0, s>>>(g, p));
+      }
+      if (!grouped(g)) MKO_TIMED("delta_grads", s, grads<TM, KB, true, false><<<cells, 512, 0, s>>>(g, p));
     }
   }
   if (!fast) {
     MKO_TIMED("delta_back", s, back<TM, KB, W, false><<<grid, 64 * W, 0, s>>>(g, p, parts));
-    MKO_TIMED("delta_grads", s, grads<TM, KB, false><<<cells, 512, 0, s>>>(g, p));
+    if constexpr (kGroups<TM, KB>) {
+      if (grouped(g)) MKO_TIMED("delta_grads", s, grads<TM, KB, false, true><<<groups, 512, 0, s>>>(g, p));
+    }
+    if (!grouped(g)) MKO_TIMED("delta_grads", s, grads<TM, KB, false, false><<<cells, 512, 0, s>>>(g, p));
   }
   if (p.pq) {
     const int per = static_cast<int>(cdiv(g.key, 4));
-    const int64_t groups = g.batch * g.length * g.key_heads * per;
-    MKO_TIMED("delta_join", s, join<TM><<<dim3(static_cast<unsigned>(cdiv(groups, 256)), 2), 256, 0, s>>>(g, p, groups, per));
+    const int64_t fours = g.batch * g.length * g.key_heads * per;
+    MKO_TIMED("delta_join", s, join<TM><<<dim3(static_cast<unsigned>(cdiv(fours, 256)), 2), 256, 0, s>>>(g, p, fours, per));
   }
 }
 
@@ -526,7 +597,7 @@ extern "C" int mko_delta_bwd(const mko_delta_params* prm, void* stream) {
   p.states = sv + l.states;
   p.e = sv + l.e;
   p.grads = ws + w.grads;
-  if (g.rep > 1) {
+  if (g.rep > 1 && !grouped(g)) {
     p.pq = reinterpret_cast<float*>(ws + w.pq);
     p.pk = reinterpret_cast<float*>(ws + w.pk);
   }

@@ -9,6 +9,8 @@
 // that of the differences from the mean, in a second pass over the registers.  The backward's teams
 // walk rows, with the next row's loads in flight, and keep dweight and dbias of their columns in
 // registers; a workgroup adds its teams' in order and writes one row of partial sums.
+#include <algorithm>
+
 #include "common.hpp"
 #include "io.hpp"
 #include "rows.hpp"
@@ -20,7 +22,7 @@ namespace {
 constexpr int kThreads = 256;       // workgroup of teams of up to four waves, forward
 constexpr int kMostWaves = 16;      // waves of a team
 constexpr int kMostVectors = 8;     // vectors a lane holds, forward
-constexpr int kBwdThreads = 512;
+constexpr int kBwdThreads = 512;    // workgroup of teams of up to eight waves, backward
 constexpr int kBwdMostVectors = 3;  // three arrays a vector, twice
 constexpr int kBwdBlocks = 512;     // two workgroups a CU; more only add partial sums
 
@@ -55,8 +57,8 @@ __device__ __forceinline__ float team_sum(float v, float* slots, int team, int t
 
 // ------------------------------------------------------------------ forward
 
-template <typename T, typename S, int SUB, int NV>
-__global__ void __launch_bounds__(kMostWaves * kWave) forward(mko_layernorm_params p, Geo g) {
+template <typename T, typename S, int SUB, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS) forward(mko_layernorm_params p, Geo g) {
   constexpr int VEC = kVecOf<T>;
   __shared__ float slots[2][kMostWaves];
   const int threads = SUB < kWave ? SUB : g.team;
@@ -76,6 +78,10 @@ __global__ void __launch_bounds__(kMostWaves * kWave) forward(mko_layernorm_para
     xr[k] = load_part<T, VEC>(x, i, n);
     if (p.residual) rr[k] = load_part<S, VEC>(res, i, n);
   }
+  float w[NV][VEC];  // on its way while the sums meet
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    load_param_part<VEC>(p.weight, p.wdtype, static_cast<int64_t>(lt + k * threads) * VEC, p.features, w[k]);
   float v[NV][VEC], sum = 0.0f;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -112,11 +118,10 @@ __global__ void __launch_bounds__(kMostWaves * kWave) forward(mko_layernorm_para
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int64_t i = static_cast<int64_t>(lt + k * threads) * VEC;
-    float w[VEC], b[VEC], o[VEC];
-    load_param_part<VEC>(p.weight, p.wdtype, i, p.features, w);
+    float b[VEC], o[VEC];
     if (p.bias) load_param_part<VEC>(p.bias, p.bdtype, i, p.features, b);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = v[k][e] * r * w[e] + (p.bias ? b[e] : 0.0f);
+    for (int e = 0; e < VEC; ++e) o[e] = v[k][e] * r * w[k][e] + (p.bias ? b[e] : 0.0f);
     store_part<T, VEC>(static_cast<T*>(p.out) + row * p.features, i, n, o);
   }
 }
@@ -176,10 +181,10 @@ struct Row {
   float mu, r;
 };
 
-template <typename T, typename S, int SUB, int NV>
-__global__ void __launch_bounds__(kBwdThreads) backward(mko_layernorm_params p, Geo g, float* part) {
+template <typename T, typename S, int SUB, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS) backward(mko_layernorm_params p, Geo g, float* part) {
   constexpr int VEC = kVecOf<T>;
-  __shared__ float slots[2][2][kBwdThreads / kWave];
+  __shared__ float slots[2][2][THREADS / kWave];
   extern __shared__ float columns[];  // a team's dweight and dbias
   const int threads = SUB < kWave ? SUB : g.team;
   const int teams = blockDim.x / threads;
@@ -416,7 +421,11 @@ template <typename T, typename S, int SUB, int NV>
 void launch_fwd_n(const mko_layernorm_params& p, const Geo& g, hipStream_t s) {
   const int threads = g.team > kThreads ? g.team : kThreads / g.team * g.team;
   const unsigned grid = static_cast<unsigned>(cdiv(p.rows, threads / g.team));
-  MKO_TIMED("layernorm_fwd", s, forward<T, S, SUB, NV><<<grid, threads, 0, s>>>(p, g));
+  // up to four waves may take more registers than sixteen: five vectors a lane would spill
+  if (threads <= kThreads)
+    MKO_TIMED("layernorm_fwd", s, forward<T, S, SUB, NV, kThreads><<<grid, threads, 0, s>>>(p, g));
+  else
+    MKO_TIMED("layernorm_fwd", s, forward<T, S, SUB, NV, kMostWaves * kWave><<<grid, threads, 0, s>>>(p, g));
 }
 
 // Rows of up to 16 or 32 vectors: four or two to a wave.  Wider ones: for few rows a vector a lane, for
@@ -443,25 +452,32 @@ void launch_fwd(const mko_layernorm_params& p, hipStream_t s) {
 }
 
 struct BwdPlan {
-  int nv;  // 0: the row is too wide for registers
+  int nv;  // vectors a lane holds; 0: the row is too wide for registers
   Geo g;
   int teams;
   size_t lds;
 };
 
+// One vector a lane as far as a team of sixteen waves goes: it leaves registers for more waves, which hide the
+// loads better than more vectors do (8192 x 2560 bf16 42 us, 63 with two a lane and 68 with three; 1003 x 5120 beside
+// a float32 stream 26, 28 and 56).  Wider rows take three in teams of up to eight.
 BwdPlan bwd_plan(const mko_layernorm_params* p) {
   BwdPlan b{};
   const int64_t vectors = vectors_of(p), waves = cdiv(vectors, kWave);
   constexpr int kWaves = kBwdThreads / kWave;
-  int team = 1;
-  while (team < kWaves && depth(waves, team, kBwdMostVectors) == 0) ++team;
-  b.nv = depth(waves, team, kBwdMostVectors);
-  if (b.nv == 0) {
+  int team = static_cast<int>(std::min<int64_t>(waves, kMostWaves));
+  b.nv = 1;
+  if (waves > kMostWaves) {
+    b.nv = kBwdMostVectors;
+    team = static_cast<int>(cdiv(waves, kBwdMostVectors));
+  }
+  if (team > (b.nv == 1 ? kMostWaves : kWaves)) {
+    b.nv = 0;
     b.g.blocks = cdiv(p->rows, kWideRows);
     return b;
   }
   b.g.team = vectors <= 16 ? 16 : vectors <= 32 ? 32 : team * kWave;
-  b.teams = kWaves / team * (team * kWave / b.g.team);
+  b.teams = team > kWaves ? 1 : kWaves / team * (team * kWave / b.g.team);
   b.lds = b.teams > 1 ? static_cast<size_t>(p->features) * 2 * sizeof(float) : 0;
   b.g.rows_of = cdiv(cdiv(p->rows, b.teams), kBwdBlocks);
   b.g.blocks = cdiv(p->rows, b.teams * b.g.rows_of);
@@ -479,15 +495,15 @@ void launch_bwd(const mko_layernorm_params& p, const BwdPlan& b, hipStream_t s) 
       MKO_TIMED("layernorm_bwd_params_wide", s, params_wide<T, S><<<wide, kThreads, 0, s>>>(p, part));
     }
   } else if (b.g.team == 16) {
-    MKO_TIMED("layernorm_bwd", s, backward<T, S, 16, 1><<<grid, threads, b.lds, s>>>(p, b.g, part));
+    MKO_TIMED("layernorm_bwd", s, backward<T, S, 16, 1, kBwdThreads><<<grid, threads, b.lds, s>>>(p, b.g, part));
   } else if (b.g.team == 32) {
-    MKO_TIMED("layernorm_bwd", s, backward<T, S, 32, 1><<<grid, threads, b.lds, s>>>(p, b.g, part));
+    MKO_TIMED("layernorm_bwd", s, backward<T, S, 32, 1, kBwdThreads><<<grid, threads, b.lds, s>>>(p, b.g, part));
+  } else if (b.nv == 1 && threads <= kBwdThreads) {
+    MKO_TIMED("layernorm_bwd", s, backward<T, S, 64, 1, kBwdThreads><<<grid, threads, b.lds, s>>>(p, b.g, part));
   } else if (b.nv == 1) {
-    MKO_TIMED("layernorm_bwd", s, backward<T, S, 64, 1><<<grid, threads, b.lds, s>>>(p, b.g, part));
-  } else if (b.nv == 2) {
-    MKO_TIMED("layernorm_bwd", s, backward<T, S, 64, 2><<<grid, threads, b.lds, s>>>(p, b.g, part));
+    MKO_TIMED("layernorm_bwd", s, backward<T, S, 64, 1, kMostWaves * kWave><<<grid, threads, b.lds, s>>>(p, b.g, part));
   } else {
-    MKO_TIMED("layernorm_bwd", s, backward<T, S, 64, 3><<<grid, threads, b.lds, s>>>(p, b.g, part));
+    MKO_TIMED("layernorm_bwd", s, backward<T, S, 64, kBwdMostVectors, kBwdThreads><<<grid, threads, b.lds, s>>>(p, b.g, part));
   }
   if (part)
     MKO_TIMED("layernorm_bwd_finish", s,
