@@ -4,7 +4,7 @@
 //         operands T and P (and their transposes, for the backward)
 //   scan  per (batch, head, 16 W value columns), sequential over the chunks.  W waves carry S in float32
 //         accumulators and do only what the next chunk waits for, E and S's update; W
-//         others follow a chunk behind with Y and the stores, and four fetch the chunk ahead.
+//         others follow a chunk behind with Y, and four fetch the chunk ahead and store what the backward reads.
 //
 // Few long sequences leave most of the chip idle, so their chunks are cut into segments that are walked side
 // by side.  A segment makes S0 M + B of the state S0 before it:
@@ -219,20 +219,12 @@ template <typename TM, int KB, int W, bool FAST>
 struct ScanLds : Chunks<TM, KB, 16 * W, FAST ? (KB * sizeof(TM) <= 8 && sizeof(TM) == 2 ? 3 : 2) : 1,
                         FAST && KB * sizeof(TM) <= 8 ? (sizeof(TM) == 2 ? 2 : 1) : 0,
                         FAST && KB * sizeof(TM) <= 8 && sizeof(TM) == 2> {
-  struct Hand {
-    TM s[KB * kFrag], e[2 * kFrag];
-  };
   // Two where there is room; one is read and written in one turn, on two sides of a barrier.
   static constexpr int kHands =
-      FAST && sizeof(Chunks<TM, KB, 16 * W, ScanLds::kBufs, ScanLds::kSquares, ScanLds::kQ>) + 2 * W * sizeof(Hand) <= 160 * 1024
+      FAST && sizeof(Chunks<TM, KB, 16 * W, ScanLds::kBufs, ScanLds::kSquares, ScanLds::kQ>) + 2 * W * sizeof(Hand<TM, KB>) <= 160 * 1024
           ? 2 : 1;
-  Hand hand[kHands][W];  // S and E of a chunk as operands, from the wave that carries to the one that follows
+  Hand<TM, KB> hand[kHands][W];  // S and E of a chunk
 };
-
-template <typename TM>
-__device__ __forceinline__ void put_frag(TM* p, const Frag<TM>& f) {
-  store_words(p + 8 * lane_id(), f.w);
-}
 
 // S of 16 value columns, carried through the chunks by one wave.
 template <typename TM, int KB>
@@ -318,7 +310,8 @@ __global__ void __launch_bounds__(64 * (kEndsTiles + kFetchers)) ends(Geo g, Ptr
 
   if (key < 32 * KB) lds.clear(64 * (W + kFetchers));
   if (wave >= W) {
-    Fetcher<TM, KB, BV, Lds>(src, reinterpret_cast<const TM*>(&zero_unit), wave - W).template walk<false, 0>(lds, first, 1, g.span);
+    Fetcher<TM, KB, BV, Lds>(src, reinterpret_cast<const TM*>(&zero_unit), wave - W).template walk<false, 0>(
+        lds, first, 1, g.span, [](int64_t) {}, [](int64_t) {});
     return;
   }
   Carrier<TM, KB> carrier;
@@ -404,7 +397,21 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
   if (FAST && key < KP) lds.clear(kThreads);
   if constexpr (FAST) {
     if (wave >= 2 * W) {
-      Fetcher<TM, KB, BV, Lds>(src, reinterpret_cast<const TM*>(&zero_unit), wave - 2 * W).template walk<kMid, 1>(lds, first, 1, chunks);
+      Storer<TM, KB> storer(wave - 2 * W);
+      Fetcher<TM, KB, BV, Lds>(src, reinterpret_cast<const TM*>(&zero_unit), wave - 2 * W).template walk<kMid, 1>(
+          lds, first, 1, chunks,
+          [&](int64_t n) {
+            if (TRAIN && n > 0) storer.take(lds.hand[(n - 1) & (Lds::kHands - 1)][storer.tile]);
+          },
+          [&](int64_t n) {
+            if (!TRAIN || n == 0) return;
+            const int64_t at = bh * g.chunks + first + n - 1;
+            const int t = v0 + 16 * storer.tile;
+            if (storer.rows)
+              store_rows<TM, true>(static_cast<TM*>(p.e) + at * kC * value, static_cast<uint32_t>(value), t, value, kC, storer.f, storer.one);
+            else if (t + col < value)
+              store_operands<TM, true, KB>(static_cast<TM*>(p.states) + (at * value + t + col) * key, key, storer.f);
+          });
       return;
     }
   }
@@ -440,11 +447,8 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
       });
       if (n + 1 < chunks) hold(first + n + 1);
       if constexpr (kMid) __syncthreads();  // what was handed over last has been read
-      typename Lds::Hand& hand = lds.hand[n & (Lds::kHands - 1)][mine];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) put_frag(hand.s + kb * kFrag, carrier.so[kb]);
-      put_frag(hand.e, frag_of<TM>(carrier.e[0], carrier.e[1]));
-      put_frag(hand.e + kFrag, frag_of<TM>(carrier.e[2], carrier.e[3]));
+      const Frag<TM> eo[2] = {frag_of<TM>(carrier.e[0], carrier.e[1]), frag_of<TM>(carrier.e[2], carrier.e[3])};
+      hand_over(lds.hand[n & (Lds::kHands - 1)][mine], carrier.so, eo);
       carrier.template advance<Lds>(bf);
     }
     __syncthreads();  // the last turn of those that follow
@@ -458,22 +462,12 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
   constexpr bool kAhead = KB * sizeof(TM) <= 8;
   Frag<TM> qf[4][kAhead ? KB : 1], pf[6], one[2];
   float in[4];
-  // a half of the unit matrix as an operand, which transposes E exactly
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    f32x4 x[2];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      x[0][r] = i == 0 && 4 * quad + r == col ? 1.0f : 0.0f;
-      x[1][r] = i == 1 && 4 * quad + r == col ? 1.0f : 0.0f;
-    }
-    one[i] = frag_of<TM>(x[0], x[1]);
-  }
+  unit_halves<TM>(one);
   for (int64_t n = 0; n <= chunks; ++n) {
     __syncthreads();
     Frag<TM> so[KB], eo[2];
     if (n > 0) {
-      typename Lds::Hand& hand = lds.hand[(n - 1) & (Lds::kHands - 1)][mine];
+      const Hand<TM, KB>& hand = lds.hand[(n - 1) & (Lds::kHands - 1)][mine];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) so[kb] = frag_at(hand.s + kb * kFrag);
       eo[0] = frag_at(hand.e);
@@ -529,14 +523,9 @@ __global__ void __launch_bounds__(128 * W + 64 * (FAST ? kFetchers : 0)) scan(Ge
         if (16 * i + col < src.rows(c))
           store_four<TM, FAST>(yp + (16 * i + col) * y_row, vt + 4 * quad, value, y);
       }
-      if constexpr (TRAIN) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f32x4 et = {0, 0, 0, 0};
-          mma(et, eo[i / 2], one[i % 2]);
-          store_four<TM, FAST>(static_cast<TM*>(p.e) + (at * kC + 16 * i + col) * value, vt + 4 * quad, value, et);
-        }
-        if (vc < value) store_operands<TM, FAST>(static_cast<TM*>(p.states) + (at * value + vc) * key, key, so);
+      if constexpr (TRAIN && !FAST) {
+        store_rows<TM, false>(static_cast<TM*>(p.e) + at * kC * value, static_cast<int64_t>(value), vt, value, kC, eo, one);
+        if (vc < value) store_operands<TM, false, KB>(static_cast<TM*>(p.states) + (at * value + vc) * key, key, so);
       }
     }
     if (n < chunks) {

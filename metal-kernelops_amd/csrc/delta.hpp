@@ -420,9 +420,10 @@ struct Fetcher {
     }
   }
   // The chunks first, first + step, ..., n of them; a barrier each, MORE of them at the end, and MID: another
-  // within each turn.
-  template <bool MID, int MORE>
-  __device__ __forceinline__ void walk(Lds& lds, int64_t first, int64_t step, int64_t n) const {
+  // within each turn.  `take(i)` and `put(i)` are what else the wave does in turn i, ahead of and after that; vector
+  // memory operations of theirs only make the waits here longer.
+  template <bool MID, int MORE, typename Take, typename Put>
+  __device__ __forceinline__ void walk(Lds& lds, int64_t first, int64_t step, int64_t n, Take take, Put put) const {
     for (int64_t i = 0; i <= kFly && i < n; ++i) {
       keys(lds.buf(i), first + i * step);
       rest(lds.buf(i), first + i * step);
@@ -435,13 +436,33 @@ struct Fetcher {
       else
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
+      take(i);
       const int64_t j = i + kFly + 1, c = first + j * step;
       if (j < n) keys(lds.buf(j), c);
       if constexpr (MID) __syncthreads();
       if (j < n) rest(lds.buf(j), c);
+      put(i);
     }
   }
 };
+
+// A state over the keys and a chunk's rows over the tokens as operands, from the wave that carries to those that
+// store them.
+template <typename TM, int KB>
+struct Hand {
+  TM s[KB * kFrag], e[2 * kFrag];
+};
+template <typename TM>
+__device__ __forceinline__ void put_frag(TM* p, const Frag<TM>& f) {
+  store_words(p + 8 * lane_id(), f.w);
+}
+template <typename TM, int KB>
+__device__ __forceinline__ void hand_over(Hand<TM, KB>& hand, const Frag<TM> (&s)[KB], const Frag<TM> (&e)[2]) {
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) put_frag(hand.s + kb * kFrag, s[kb]);
+  put_frag(hand.e, e[0]);
+  put_frag(hand.e + kFrag, e[1]);
+}
 
 // A chunk through registers, by all THREADS.
 template <int THREADS, typename TM, typename Lds>
@@ -520,7 +541,7 @@ __device__ __forceinline__ void store_state(void* p, int dtype, int64_t row, int
 
 // The same of a state as operands, in TM.
 template <typename TM, bool WHOLE, int KB>
-__device__ __forceinline__ void store_operands(TM* row, int n, const Frag<TM> (&s)[KB]) {
+__device__ __forceinline__ void store_operands(TM* row, int n, const Frag<TM>* s) {
 #pragma unroll
   for (int j = 0; j < KB; ++j) {
     const int at = 32 * j + 8 * lane_quad();
@@ -533,6 +554,48 @@ __device__ __forceinline__ void store_operands(TM* row, int n, const Frag<TM> (&
     }
   }
 }
+
+// Halves of the unit matrix as operands, which transpose rows over tokens exactly.
+template <typename TM>
+__device__ __forceinline__ void unit_halves(Frag<TM> (&one)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f32x4 x[2];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[0][r] = i == 0 && 4 * lane_quad() + r == lane_col() ? 1.0f : 0.0f;
+      x[1][r] = i == 1 && 4 * lane_quad() + r == lane_col() ? 1.0f : 0.0f;
+    }
+    one[i] = frag_of<TM>(x[0], x[1]);
+  }
+}
+// Rows over tokens to memory: token t's at to + t stride, its values from v on, of the first `rows` tokens.
+template <typename TM, bool WHOLE, typename Stride>
+__device__ __forceinline__ void store_rows(TM* to, Stride stride, int v, int value, int rows, const Frag<TM>* e,
+                                           const Frag<TM> (&one)[2]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f32x4 et = {0, 0, 0, 0};  // [value][token], whose lanes hold four values of a token
+    mma(et, e[i / 2], one[i % 2]);
+    if (16 * i + lane_col() < rows) store_four<TM, WHOLE>(to + (16 * i + lane_col()) * stride, v + 4 * lane_quad(), value, et);
+  }
+}
+
+// What the waves that fetch do beside: two tiles of 16 values, for each of them one wave stores the states and another
+// the rows that were handed over in the turn before.
+template <typename TM, int KB>
+struct Storer {
+  Frag<TM> f[KB > 2 ? KB : 2], one[2];
+  int tile;
+  bool rows;
+  __device__ __forceinline__ explicit Storer(int part) : tile(part & 1), rows(part >> 1) { unit_halves<TM>(one); }
+  __device__ __forceinline__ void take(const Hand<TM, KB>& hand) {
+#pragma unroll
+    for (int i = 0; i < (KB > 2 ? KB : 2); ++i) {
+      if (rows ? i < 2 : i < KB) f[i] = frag_at((rows ? hand.e : hand.s) + i * kFrag);
+    }
+  }
+};
 
 // Bytes of the arrays that the forward leaves for the backward, and of the workspaces.
 struct Layout {

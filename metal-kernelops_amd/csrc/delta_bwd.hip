@@ -27,15 +27,21 @@ __device__ uint4 zero_unit;  // where rows and columns outside come from
 
 // LDS of `back`; wider keys leave no room for the squares, which then stay in registers.
 template <typename TM, int KB, int W, bool FAST>
-using BackLds = Chunks<TM, KB, 16 * W, FAST ? (KB * sizeof(TM) <= 8 && sizeof(TM) == 2 ? 3 : 2) : 1,
-                       FAST && KB * sizeof(TM) <= 8 ? 2 : 0, true>;
+struct BackLds : Chunks<TM, KB, 16 * W, FAST ? (KB * sizeof(TM) <= 8 && sizeof(TM) == 2 ? 3 : 2) : 1,
+                        FAST && KB * sizeof(TM) <= 8 ? 2 : 0, true> {
+  // G and X go to the waves that store them where these have room.
+  static constexpr bool kHand = FAST && KB * sizeof(TM) <= 8;
+  Hand<TM, kHand ? KB : 1> hand[kHand ? W : 1];
+};
 
-// W waves carry 16 value columns of G each through the chunks, and four fetch.
+// W waves carry 16 value columns of G each through the chunks, and four fetch the chunk ahead and store G and dV of
+// the chunk before.
 template <typename TM, int KB, int W, bool FAST>
 __global__ void __launch_bounds__(64 * W + 64 * (FAST ? kFetchers : 0)) back(Geo g, Ptrs p, int parts) {
   constexpr int KP = 32 * KB, BV = 16 * W, kThreads = 64 * W + 64 * (FAST ? kFetchers : 0);
   typedef BackLds<TM, KB, W, FAST> Lds;
   typedef Tile<TM, KP> KTile;
+  constexpr bool kHand = Lds::kHand;
   __shared__ __align__(16) Lds lds;
   const WgId id = wg_id(parts, static_cast<int>(g.heads));
   const int64_t h = id.y, b = id.z, bh = b * g.heads + h;
@@ -52,7 +58,26 @@ __global__ void __launch_bounds__(64 * W + 64 * (FAST ? kFetchers : 0)) back(Geo
   if (FAST && key < KP) lds.clear(kThreads);
   if constexpr (FAST) {
     if (wave >= W) {
-      Fetcher<TM, KB, BV, Lds>(src, reinterpret_cast<const TM*>(&zero_unit), wave - W).template walk<false, 0>(lds, g.chunks - 1, -1, g.chunks);
+      const Fetcher<TM, KB, BV, Lds> fetcher(src, reinterpret_cast<const TM*>(&zero_unit), wave - W);
+      if constexpr (kHand) {
+        Storer<TM, KB> storer(wave - W);
+        fetcher.template walk<true, 1>(
+            lds, g.chunks - 1, -1, g.chunks,
+            [&](int64_t n) {
+              if (n > 0) storer.take(lds.hand[storer.tile]);
+            },
+            [&](int64_t n) {
+              if (n == 0) return;
+              const int64_t c = g.chunks - n;
+              const int t = v0 + 16 * storer.tile;
+              if (storer.rows)
+                store_rows<TM, true>(dv + c * kC * yrow, static_cast<uint32_t>(yrow), t, value, src.rows(c), storer.f, storer.one);
+              else if (t + col < value)
+                store_operands<TM, true, KB>(static_cast<TM*>(p.grads) + ((bh * g.chunks + c) * value + t + col) * key, key, storer.f);
+            });
+      } else {
+        fetcher.template walk<false, 0>(lds, g.chunks - 1, -1, g.chunks, [](int64_t) {}, [](int64_t) {});
+      }
       return;
     }
   }
@@ -83,8 +108,8 @@ __global__ void __launch_bounds__(64 * W + 64 * (FAST ? kFetchers : 0)) back(Geo
     Frag<TM> so[KB];  // G as an operand over the keys
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) so[kb] = frag_of<TM>(s[2 * kb], s[2 * kb + 1]);
-    if (vc < value)
-      store_operands<TM, FAST>(static_cast<TM*>(p.grads) + (at * value + vc) * key, key, so);
+    if (!kHand && vc < value)
+      store_operands<TM, FAST, KB>(static_cast<TM*>(p.grads) + (at * value + vc) * key, key, so);
     Frag<TM> yo[2];  // dY as an operand over the tokens
 #pragma unroll
     for (int j = 0; j < 2; ++j) yo[j] = Tile<TM, BV>::over_tokens(bf.v, 32 * j, 16 * wave);
@@ -109,10 +134,15 @@ __global__ void __launch_bounds__(64 * W + 64 * (FAST ? kFetchers : 0)) back(Geo
       for (int j = i / 2; j < 2; ++j) {
         const Frag<TM> t = square(0, i, j);
         mma(x[i], t, eo[j]);
-        mma(xt, eo[j], t);
+        if (!kHand) mma(xt, eo[j], t);
       }
       const int64_t t = t0 + 16 * i + col;
-      if (t < g.length) store_four<TM, FAST>(dv + t * yrow, v0 + 16 * wave + 4 * quad, value, xt);
+      if (!kHand && t < g.length) store_four<TM, FAST>(dv + t * yrow, v0 + 16 * wave + 4 * quad, value, xt);
+    }
+    if constexpr (kHand) {
+      __syncthreads();  // what was handed over last has been read
+      const Frag<TM> dx[2] = {frag_of<TM>(x[0], x[1]), frag_of<TM>(x[2], x[3])};
+      hand_over(lds.hand[wave], so, dx);
     }
     // G of the chunk before
 #pragma unroll
@@ -140,6 +170,10 @@ __global__ void __launch_bounds__(64 * W + 64 * (FAST ? kFetchers : 0)) back(Geo
         mma(s[i], KTile::keys_over_tokens(bf.k, 32 * j, i), xo[j]);
       }
     }
+  }
+  if constexpr (kHand) {  // the last turn of those that store
+    __syncthreads();
+    __syncthreads();
   }
   if (p.dinitial && vc < value) store_state<FAST>(p.dinitial, g.state_dtype, (bh * value + vc) * key, key, s);
 }
