@@ -18,7 +18,9 @@ log decay of ``-inf`` drops the state before it, so documents packed in one row 
 Kernels (``libmko.so``): chunks of 64 tokens on the matrix cores, their operands rounded to the
 activations' type (float32 products for float32), with the state, the decays and all sums in float32
 and the triangular systems of the chunks solved in float32.  The gradients are analytic,
-once-differentiable and summed in a fixed order, so repeated runs give the same bits.  A value that is
+once-differentiable and summed in a fixed order, so repeated runs give the same bits.  Few long sequences
+are cut into segments that run side by side; whether goes by the sizes of the call, so a sequence alone and
+the same one in a batch may differ by roundings.  A value that is
 not finite reaches its whole chunk and what follows it.  There is no counterpart in dbydd/metal-kernelops.
 """
 

@@ -23,7 +23,7 @@ TOL = {F32: F32_TOL, F16: F32_TOL + 2.0 ** -11, BF16: F32_TOL + 2.0 ** -8}
 PAIRS = [(F32, F32), (F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)]
 # one feature, around a quarter, a half and whole wavefronts' vectors, odd widths, several vectors a lane,
 # and beyond what a team of lanes holds
-FEATURES = [2, 7, 64, 77, 96, 128, 129, 256, 260, 512, 520, 1001, 1536, 2560, 4099, 5120, 8192, 13000, 40000]
+FEATURES = [2, 7, 64, 77, 96, 128, 129, 256, 260, 512, 520, 1001, 1536, 2560, 4099, 5120, 8192, 10240, 13000, 40000]
 NAMES = ("x", "weight", "bias", "residual")
 
 
