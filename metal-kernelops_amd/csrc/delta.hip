@@ -6,12 +6,19 @@
 //         accumulators and do only what the next chunk waits for, E and S's update; W
 //         others follow a chunk behind with Y, and four fetch the chunk ahead and store what the backward reads.
 //
+// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: prep 69 us, scan 169.  Prep moves 56 KB a chunk and
+// head, 3.3 TB/s, behind the latency of its substitution.  A turn of the scan takes 2.6 us: its chain of products
+// about 1.0 (2400 cycles), fetching 48 KB and storing 16 KB for the backward on every CU at once the rest; without
+// gradients a turn takes 1.6.  With the chain's waves fetching and storing for themselves the scan took 254 us, with
+// the fetches in waves of their own and two buffers 232, with three 163 to 173.
+//
 // Few long sequences leave most of the chip idle, so their chunks are cut into segments that are walked side
 // by side.  A segment makes S0 M + B of the state S0 before it:
 //   ends  per (batch, head, segment but the last, 64 columns): the chunks' walk without outputs, from zero (B) and
 //         from the unit matrix (M)
 //   join  per (batch, head, 16 value columns): S0 of each segment, in their order
-// and the scan starts each segment from its own S0.
+// and the scan starts each segment from its own S0.  One sequence of 32768 tokens with 16 such heads: 108 + 147 + 19 + 200
+// us in four segments; uncut, prep and scan took 107 + 659.
 #include <algorithm>
 
 #include "delta.hpp"
@@ -601,7 +608,7 @@ void launch(const Geo& g, const Ptrs& p, bool train, hipStream_t s) {
 
 // ------------------------------------------------------------------ sizes
 
-// Segments that a sequence is cut into: where its workgroups leave more than two thirds of the 256 CUs without
+// Segments that a sequence is cut into (the figures are above): where its workgroups leave more than two thirds of the 256 CUs without
 // work, as many as give each CU one, of 8 chunks or more, and no more than the square root of the chunks, since
 // `join` walks them one by one.  Walking the chunks twice pays from three segments on.
 int64_t segments_of(const mko_delta_params* prm, int64_t chunks) {

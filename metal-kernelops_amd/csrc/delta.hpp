@@ -606,7 +606,7 @@ Layout forward_layout(const Geo& g, bool train);  // lower, ends and maps, and t
 
 int make_geo(const mko_delta_params* prm, const char* what, Geo* g);
 Ptrs base_ptrs(const mko_delta_params* prm);
-// Whether q, k, v and dy, in 16 bits, can be loaded to LDS directly: rows of whole 16-byte units at multiples of 16 bytes.
+// Whether q, k, v and dy can be loaded to LDS directly: rows of whole 16-byte units at multiples of 16 bytes.
 bool fast_rows(const Geo& g, const Ptrs& p);
 
 inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }

@@ -104,6 +104,8 @@ void launch_n(const mko_delta_update_params& p, hipStream_t s) {
     MKO_TIMED("delta_update", s, step<S, LANES, NR, false><<<grid, 256, 0, s>>>(p, waves, per_head));
 }
 
+// Eight groups of rows a wave where that leaves 4096 waves, four a SIMD, or more: 256 sequences of 32 heads of
+// 128 x 128 take 193 us (5.6 TB/s), with two groups 203.  One sequence of 16 heads takes 4.8 us with two, 7.5 with eight.
 template <typename S, int LANES>
 void launch(const mko_delta_update_params& p, hipStream_t s) {
   if (p.batch * p.heads * p.value * LANES / kWave >= 8 * 4096)

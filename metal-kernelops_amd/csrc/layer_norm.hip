@@ -429,8 +429,9 @@ void launch_fwd_n(const mko_layernorm_params& p, const Geo& g, hipStream_t s) {
 }
 
 // Rows of up to 16 or 32 vectors: four or two to a wave.  Wider ones: for few rows a vector a lane, for
-// the shortest way from load to store; for many fewer waves to a row, down to one, where nothing has
-// to meet, as long as 2048 waves, two a SIMD, have work.
+// the shortest way from load to store (7 x 4096: 4.0 us, 10.1 with one wave a row); for many fewer waves
+// to a row, down to one, where nothing has to meet, as long as 2048 waves, two a SIMD, have work (8192 x 2560
+// bf16: 37 us, 4.5 TB/s, with five vectors a lane, 37 with two or three, 42 with one).
 template <typename T, typename S>
 void launch_fwd(const mko_layernorm_params& p, hipStream_t s) {
   const int64_t vectors = vectors_of(&p), waves = cdiv(vectors, kWave);
