@@ -6,8 +6,8 @@
 //         accumulators and do only what the next chunk waits for, E and S's update; W
 //         others follow a chunk behind with Y, and four fetch the chunk ahead and store what the backward reads.
 //
-// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: prep 69 us, scan 169.  Prep moves 56 KB a chunk and
-// head, 3.3 TB/s, behind the latency of its substitution.  A turn of the scan takes 2.6 us: its chain of products
+// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: prep 67 us, scan 169.  Prep moves 56 KB a chunk and
+// head, 3.4 TB/s, behind the latency of its substitution.  A turn of the scan takes 2.6 us: its chain of products
 // about 1.0 (2400 cycles), fetching 48 KB and storing 16 KB for the backward on every CU at once the rest; without
 // gradients a turn takes 1.6.  With the chain's waves fetching and storing for themselves the scan took 254 us, with
 // the fetches in waves of their own and two buffers 232, with three 163 to 173.
@@ -17,7 +17,7 @@
 //   ends  per (batch, head, segment but the last, 64 columns): the chunks' walk without outputs, from zero (B) and
 //         from the unit matrix (M)
 //   join  per (batch, head, 16 value columns): S0 of each segment, in their order
-// and the scan starts each segment from its own S0.  One sequence of 32768 tokens with 16 such heads: 108 + 147 + 19 + 200
+// and the scan starts each segment from its own S0.  One sequence of 32768 tokens with 16 such heads: 101 + 147 + 19 + 200
 // us in four segments; uncut, prep and scan took 107 + 659.
 #include <algorithm>
 
@@ -122,13 +122,18 @@ __device__ __forceinline__ void store_half(TM* p, int h, const float (&f)[4]) {
   store_words(p + 8 * lane_id() + 4 * h, w);
 }
 
-// Wave w owns the row tile w of A and P.
+// Wave w owns the row tile w of A and P.  Six waves a SIMD, for whose registers and LDS K and A share a place, hide more of
+// the substitution than four did: 72 -> 67 us (the sizes above), 111 -> 101 without the transposes.
 template <typename TM, int KB, bool TRAIN>
-__global__ void __launch_bounds__(256) prep(Geo g, Ptrs p, bool fast) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KB * sizeof(TM) <= 8 ? 6 : 1))) prep(Geo g, Ptrs p, bool fast) {
   typedef Tile<TM, 32 * KB> KTile;
   __shared__ Tokens tok;
-  __shared__ __align__(16) float a[kC * kPitch];
-  __shared__ __align__(16) TM kt[KTile::kElements];
+  __shared__ __align__(16) union {  // K until its products are there, then A and T: room for more workgroups
+    TM kt[KTile::kElements];
+    float a[kC * kPitch];
+  } lds;
+  TM* kt = lds.kt;
+  float* a = lds.a;
   const WgId id = wg_id(static_cast<int>(g.heads), static_cast<int>(g.chunks));
   const int64_t h = id.x, c = id.y, b = id.z;
   const int64_t at = (b * g.heads + h) * g.chunks + c, t0 = c * kC;
@@ -176,7 +181,10 @@ __global__ void __launch_bounds__(256) prep(Geo g, Ptrs p, bool fast) {
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) kf[kb] = KTile::rows(kt, 16 * wave, 32 * kb);
   const int tr = 16 * wave + 4 * lane_quad(), tc = 16 * wave + lane_col();  // this tile's tokens as rows and columns
-  for (int j = 0; j <= wave; ++j) {
+  float av[4][4];  // A's rows of tile `wave`
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j > wave) continue;
     f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0}, kq = {0, 0, 0, 0};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -191,7 +199,7 @@ __global__ void __launch_bounds__(256) prep(Geo g, Ptrs p, bool fast) {
     for (int r = 0; r < 4; ++r) {
       const int t = tr + r, s = sr + r;
       const float m = t >= sc ? fast_exp2(static_cast<float>(tok.c[t] - tok.c[sc])) * tok.beta[sc] : 0.0f;
-      a[t * kPitch + sc] = t > sc ? kk[r] * m : 0.0f;
+      av[j][r] = t > sc ? kk[r] * m : 0.0f;
       if (TRAIN) pt[r] = t >= sc ? g.scale * qk[r] * m : 0.0f;
       pp[r] = tc >= s ? g.scale * kq[r] * fast_exp2(static_cast<float>(tok.c[tc] - tok.c[s])) * tok.beta[s] : 0.0f;
     }
@@ -202,6 +210,13 @@ __global__ void __launch_bounds__(256) prep(Geo g, Ptrs p, bool fast) {
     const float none[4] = {0, 0, 0, 0};
     store_half<TM>(lp + lower_at(wave, wave / 2), 1, none);
     if (TRAIN) store_half<TM>(up + upper_at(wave + 1, wave / 2), 0, none);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j > wave) continue;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a[(tr + r) * kPitch + 16 * j + lane_col()] = av[j][r];
   }
   __syncthreads();
   invert(a);

@@ -122,7 +122,8 @@ __device__ __forceinline__ Frag<TM> frag_memory(const TM* base, int64_t stride, 
 // 16 bytes a lane from memory to LDS, to `to` + 16 lane bytes (`to` the same in the wave), in flight until
 // the wave waits for its vector memory operations.  In assembly because the compiler would wait for all
 // of them ahead of the next LDS read, whatever it reads; it counts fewer operations than there are,
-// so its own waits only last longer.  One idle state from the write of m0 to its use by the load.
+// so its own waits only last longer.  One idle state from the write of m0 to its use by the load; nothing else in
+// these kernels uses m0, which cannot be named as overwritten.
 __device__ __forceinline__ void direct_load(const void* from, void* to) {
   const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to));  // a flat address ends in that of LDS
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform(at)), "v"(from));
@@ -338,6 +339,7 @@ struct Chunks {
     float in[kC], write[kC];
     TM squares[SQUARES > 0 ? SQUARES * kSquare : 8], q[Q ? KTile::kElements : 8];
   };
+  static_assert(sizeof(Buf) % 16 == 0, "every tile starts at a multiple of 16 bytes");
   Buf bufs[BUFS];
   // That of the n-th chunk of the walk.
   __device__ __forceinline__ Buf& buf(int64_t n) { return bufs[BUFS == 1 ? 0 : static_cast<uint32_t>(n) % BUFS]; }

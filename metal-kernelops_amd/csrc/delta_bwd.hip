@@ -210,6 +210,7 @@ struct GradsTiles {
     Tokens tok;
     float dc[kC], dots[4][3][16], rows[4][16], cols[4][16], gs[8], wrote[4];
   };
+  static_assert(sizeof(Sums) % 16 == 0, "the tiles behind it start at multiples of 16 bytes");
 };
 // GROUP: of a key head, whose K and Q stay while the first values of the next value head fly; otherwise the two
 // take turns in one place.
