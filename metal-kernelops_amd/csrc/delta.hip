@@ -6,7 +6,7 @@
 //         accumulators and do only what the next chunk waits for, E and S's update; W
 //         others follow a chunk behind with Y, and four fetch the chunk ahead and store what the backward reads.
 //
-// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: prep 67 us, scan 169.  Prep moves 56 KB a chunk and
+// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: prep 65 us, scan 172.  Prep moves 56 KB a chunk and
 // head, 3.4 TB/s, behind the latency of its substitution.  A turn of the scan takes 2.6 us: its chain of products
 // about 1.0 (2400 cycles), fetching 48 KB and storing 16 KB for the backward on every CU at once the rest; without
 // gradients a turn takes 1.6.  With the chain's waves fetching and storing for themselves the scan took 254 us, with
@@ -17,7 +17,7 @@
 //   ends  per (batch, head, segment but the last, 64 columns): the chunks' walk without outputs, from zero (B) and
 //         from the unit matrix (M)
 //   join  per (batch, head, 16 value columns): S0 of each segment, in their order
-// and the scan starts each segment from its own S0.  One sequence of 32768 tokens with 16 such heads: 101 + 147 + 19 + 200
+// and the scan starts each segment from its own S0.  One sequence of 32768 tokens with 16 such heads: 99 + 152 + 19 + 202
 // us in four segments; uncut, prep and scan took 107 + 659.
 #include <algorithm>
 

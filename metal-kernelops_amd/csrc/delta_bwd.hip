@@ -18,7 +18,7 @@
 //          one after the other, with dq and dk summed in registers in their order
 //   join   that sum where there are few such workgroups, or no room for it in LDS
 //
-// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: back 142 us, grads 197.  A turn of `back` is 2.2 us of
+// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: back 142 us, grads 194.  A turn of `back` is 2.2 us of
 // 60 products that follow from one another, with their reads of LDS.  `grads` moves 176 KB a chunk and head, 3.7 TB/s;
 // two workgroups a CU overlap one's loads and the other's products.
 #include "delta.hpp"
