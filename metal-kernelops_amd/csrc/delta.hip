@@ -13,11 +13,12 @@
 // the fetches in waves of their own and two buffers 232, with three 163 to 173.
 //
 // Few long sequences leave most of the chip idle, so their chunks are cut into segments that are walked side
-// by side.  A segment makes S0 M + B of the state S0 before it:
+// by side.  A segment makes d S0 + S0 N + B of the state S0 before it, d its decay:
 //   ends  per (batch, head, segment but the last, 64 columns): the chunks' walk without outputs, from zero (B) and
-//         from the unit matrix (M)
-//   join  per (batch, head, 16 value columns): S0 of each segment, in their order
-// and the scan starts each segment from its own S0.  One sequence of 32768 tokens with 16 such heads: 99 + 152 + 19 + 202
+//         from the unit matrix (d I + N)
+//   join  per (batch, head, 16 value columns): S0 of each segment, in their order.  What a state only keeps, d S0,
+//         is a float32 product, as in the uncut walk
+// and the scan starts each segment from its own S0.  One sequence of 32768 tokens with 16 such heads: 99 + 149 + 10 + 199
 // us in four segments; uncut, prep and scan took 107 + 659.
 #include <algorithm>
 
@@ -347,54 +348,101 @@ __global__ void __launch_bounds__(64 * (kEndsTiles + kFetchers)) ends(Geo g, Ptr
   } else if (seg == 0 && p.initial && vc < value) {
     load_state<true>(carrier.s, p.initial, g.state_dtype, (bh * value + vc) * key, key);
   }
+  float left = 1.0f;  // of the state, rounded as the walk rounds it
   for (int64_t n = 0; n < g.span; ++n) {
     __syncthreads();
     typename Lds::Buf& bf = lds.buf(n);
     carrier.template errors<Lds>(bf, 16 * wave, unit, [&](int i, int j) { return frag_at(bf.squares + lower_at(i, j)); });
+    left *= bf.in[kC - 1];
     carrier.template advance<Lds>(bf);
   }
   if (!unit) {
     if (vc < value) store_row<float, true>(p.ends + (at * value + vc) * key, key, carrier.s);
-  } else if (vc < key) {  // transposed, as `join` reads it
-    TM* to = static_cast<TM*>(p.maps) + at * key * key + vc;
+    return;
+  }
+  if (vc == 0 && quad == 0) p.kept[at] = left;
+  if (vc < key) {  // transposed, as `join` reads it
+    float* to = p.maps + at * key * key + vc;
 #pragma unroll
     for (int i = 0; i < 2 * KB; ++i) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int k = 16 * (i & ~1) + 4 * (i & 1) + 8 * quad + r;
-        if (k < key) to[k * key] = from_f32<TM>(carrier.s[i][r]);
+        if (k < key) to[k * key] = carrier.s[i][r] - (k == vc ? left : 0.0f);
       }
     }
   }
 }
 
-// The state behind each segment from the one before it, in place of its B; a wave for 16 values.
+// f as TM, and what that leaves of it as TM.
+template <typename TM, int N>
+__device__ __forceinline__ void split(const float (&f)[N], uint32_t (&hi)[kWordsOf<TM, N>], uint32_t (&lo)[kWordsOf<TM, N>]) {
+  float h[N], l[N];
+  pack_words<TM, N>(f, hi);
+  unpack_words<TM, N>(hi, h);
+#pragma unroll
+  for (int i = 0; i < N; ++i) l[i] = f[i] - h[i];
+  pack_words<TM, N>(l, lo);
+}
+
+// The state behind each segment from the one before it, in place of its B: wave i has 16 values of the key tile i and
+// takes S0 as an operand from the others.  In 16 bits N and S0 are two operands each, whose products leave
+// 2^-16 (bfloat16) of N S0: one rounding of a state for a whole segment would stay where N takes all of it away.
 template <typename TM, int KB>
-__global__ void __launch_bounds__(64) join(Geo g, Ptrs p, int tiles) {
+__global__ void __launch_bounds__(128 * KB) join(Geo g, Ptrs p, int tiles) {
+  constexpr bool kSplit = sizeof(TM) == 2;
+  __shared__ __align__(16) TM lds[2][kSplit ? 2 : 1][KB * kFrag];  // one is read while the next is written
   const int64_t bh = blockIdx.x / tiles;
-  const int col = lane_col(), quad = lane_quad(), key = static_cast<int>(g.key);
+  const int wave = uniform(threadIdx.x >> 6), col = lane_col(), quad = lane_quad(), key = static_cast<int>(g.key);
   const int64_t vc = blockIdx.x % tiles * 16 + col;
   const bool live = vc < g.value;
+  const int k0 = 32 * (wave / 2) + 8 * quad + 4 * (wave % 2);           // the lane's keys of S
+  const int kr = 32 * (wave / 2) + 8 * (col / 4) + 4 * (wave % 2) + col % 4;  // and its row of N
   float* row = p.ends + (bh * (g.segments - 1) * g.value + (live ? vc : 0)) * key;
-  f32x4 s[2 * KB];
-  load_row<float, true>(s, row, key);
+  float s[4];
+  unpack_words<float, 4>(load_part<float, 4>(row, k0, key).w, s);
   for (int64_t seg = 1; seg < g.segments - 1; ++seg) {
     row += g.value * key;
-    const TM* map = static_cast<const TM*>(p.maps) + (bh * (g.segments - 1) + seg) * key * key;
-    Frag<TM> so[KB];
+    const int64_t at = bh * (g.segments - 1) + seg;
+    const float* map = p.maps + at * key * key + (kr < key ? kr * key : 0);
+    Words<float, 8> n[KB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) so[kb] = frag_of<TM>(s[2 * kb], s[2 * kb + 1]);
-    load_row<float, true>(s, row, key);
+    for (int kb = 0; kb < KB; ++kb) n[kb] = load_part<float, 8>(map, 32 * kb + 8 * quad, kr < key ? key : 0);
+    float b[4];
+    unpack_words<float, 4>(load_part<float, 4>(row, k0, key).w, b);
+    const float left = p.kept[at];
+    TM(&so)[kSplit ? 2 : 1][KB * kFrag] = lds[seg & 1];
+    const int to = wave / 2 * kFrag + 8 * lane_id() + 4 * (wave % 2);
+    if constexpr (kSplit) {
+      uint32_t hi[kWordsOf<TM, 4>], lo[kWordsOf<TM, 4>];
+      split<TM, 4>(s, hi, lo);
+      store_words(so[0] + to, hi);
+      store_words(so[1] + to, lo);
+    } else {
+      uint32_t w[kWordsOf<TM, 4>];
+      pack_words<TM, 4>(s, w);
+      store_words(so[0] + to, w);
+    }
+    __syncthreads();
+    f32x4 acc = {b[0] + left * s[0], b[1] + left * s[1], b[2] + left * s[2], b[3] + left * s[3]};
 #pragma unroll
-    for (int i = 0; i < 2 * KB; ++i) {
-      const int k = 16 * (i & ~1) + 4 * (i & 1) + 8 * (col / 4) + col % 4;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const Words<TM, 8> w = load_part<TM, 8>(map + (k < key ? k * key : 0), 32 * kb + 8 * quad, k < key ? key : 0);
-        mma(s[i], __builtin_bit_cast(Frag<TM>, w), so[kb]);
+    for (int kb = 0; kb < KB; ++kb) {
+      const Frag<TM> x = frag_at(so[0] + kb * kFrag);
+      if constexpr (kSplit) {
+        Frag<TM> hi, lo;
+        float f[8];
+        unpack_words<float, 8>(n[kb].w, f);
+        split<TM, 8>(f, hi.w, lo.w);
+        mma(acc, lo, x);
+        mma(acc, hi, frag_at(so[1] + kb * kFrag));
+        mma(acc, hi, x);
+      } else {
+        mma(acc, __builtin_bit_cast(Frag<TM>, n[kb]), x);
       }
     }
-    if (live) store_row<float, true>(row, key, s);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] = acc[r];
+    if (live) store_part<float, 4>(row, k0, key, s);
   }
 }
 
@@ -594,7 +642,7 @@ void launch(Geo g, const Ptrs& p, hipStream_t s) {
         const unsigned cells = static_cast<unsigned>(g.batch * g.heads * (g.segments - 1) * all);
         MKO_TIMED("delta_ends", s, ends<TM, KB><<<cells, 64 * (kEndsTiles + kFetchers), 0, s>>>(g, p, values, all));
         if (g.segments > 2)
-          MKO_TIMED("delta_join_states", s, join<TM, KB><<<static_cast<unsigned>(g.batch * g.heads * tiles), 64, 0, s>>>(g, p, tiles));
+          MKO_TIMED("delta_join_states", s, join<TM, KB><<<static_cast<unsigned>(g.batch * g.heads * tiles), 128 * KB, 0, s>>>(g, p, tiles));
       }
       const unsigned grid = static_cast<unsigned>(g.batch * g.heads * parts * g.segments);
       MKO_TIMED("delta_scan", s, scan<TM, KB, W, TRAIN, true><<<grid, 128 * W + 64 * kFetchers, 0, s>>>(g, p, parts));
@@ -718,7 +766,8 @@ Layout forward_layout(const Geo& g, bool train) {
   if (!train) o = align256(o + cells * sizeof(Tokens));
   const size_t ends = static_cast<size_t>(g.batch * g.heads * (g.segments - 1));
   l.ends = o; o = align256(o + ends * g.value * g.key * sizeof(float));
-  l.maps = o; o = align256(o + ends * g.key * g.key * el);
+  l.maps = o; o = align256(o + ends * g.key * g.key * sizeof(float));
+  l.kept = o; o = align256(o + ends * sizeof(float));
   l.total = o;
   return l;
 }
@@ -764,7 +813,8 @@ extern "C" int mko_delta_fwd(const mko_delta_params* prm, void* stream) {
   char* ws = static_cast<char*>(prm->workspace);
   p.lower = ws + w.lower;
   p.ends = reinterpret_cast<float*>(ws + w.ends);
-  p.maps = ws + w.maps;
+  p.maps = reinterpret_cast<float*>(ws + w.maps);
+  p.kept = reinterpret_cast<float*>(ws + w.kept);
   if (train) {
     const Layout l = saved_layout(g);
     char* sv = static_cast<char*>(prm->saved);

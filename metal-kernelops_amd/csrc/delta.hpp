@@ -58,7 +58,9 @@ struct Ptrs {
   void* e;               // E, (batch, heads, chunks, kC, value)
   float *pq, *pk;        // dq and dk of each value head, where key heads are shared
   float* ends;           // states behind the segments but the last, (batch, heads, segments - 1, value, key)
-  void* maps;            // what a segment makes of the state before it, (batch, heads, segments - 1, key, key)
+  // What a segment makes of the state before it, but for its decay: (batch, heads, segments - 1, key, key), and the
+  // decay, (batch, heads, segments - 1)
+  float *maps, *kept;
 };
 
 // A lane's share of a 16 x 32 operand: row (or column) l % 16.  Over tokens element 4 h + r is index
@@ -601,10 +603,10 @@ struct Storer {
 
 // Bytes of the arrays that the forward leaves for the backward, and of the workspaces.
 struct Layout {
-  size_t tokens, lower, upper, states, e, ends, maps, total;
+  size_t tokens, lower, upper, states, e, ends, maps, kept, total;
 };
 Layout saved_layout(const Geo& g);                // tokens, upper, states, e
-Layout forward_layout(const Geo& g, bool train);  // lower, ends and maps, and tokens unless they are saved
+Layout forward_layout(const Geo& g, bool train);  // lower, ends, maps and kept, and tokens unless they are saved
 
 int make_geo(const mko_delta_params* prm, const char* what, Geo* g);
 Ptrs base_ptrs(const mko_delta_params* prm);

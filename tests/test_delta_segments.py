@@ -1,0 +1,98 @@
+"""The gated delta rule on sequences that run in segments side by side, where the state outlives a segment: what is
+kept passes in float32, and every chunk is compared by itself.
+
+Tolerances, with u half a unit in the last place of the activations (2^-8 for bfloat16, 2^-11 for float16).  The part of
+the state that is only kept is a product of one factor a chunk: a float32 exponential (one unit, at most 2^-24 of a
+number just below one) and a float32 product (2^-24), and two more products a segment, of which there is at most one for
+eight chunks: 3 * 2^-24 a chunk.  What corrections have written or taken away carries eight 16-bit roundings: 8 u of its
+norm, as the rule's own tests count them.  Compared by chunks, where a fault of one chunk is as large as the output, the
+roundings of different operands are independent and add by their squares: the forward's eight to sqrt(8) u, the
+backward's sixteen to 4 u, and u for storing a gradient.  Float32: 1e-5, and the same a chunk for what is kept.
+"""
+
+import math
+
+import pytest
+import torch
+
+from oracle import delta_rule as oracle
+from test_gated_delta import BF16, DEV, F16, F32, NAMES, U, call, gradients, problem, to_dev
+
+FWD = {F32: 1e-5, F16: math.sqrt(8) * U[F16], BF16: math.sqrt(8) * U[BF16]}
+BWD = {F32: 1e-5, F16: 5 * U[F16], BF16: 5 * U[BF16]}
+CORRECTED = {F32: 1e-5, F16: 8 * U[F16], BF16: 8 * U[BF16]}
+
+
+def kept(length):
+    return 3 * 2.0 ** -24 * -(-length // 64)
+
+
+def slow(batch, length, key_heads, heads, key, value, dtype, decay, beta, seed=0):
+    """A problem whose tokens forget ``exp(decay)`` and correct by ``beta``, each varied by half, with gates and
+    states in float32."""
+    p = problem(batch, length, key_heads, heads, key, value, dtype, seed=seed, gates=F32, state=F32)
+    g = torch.Generator().manual_seed(length + seed)
+    for name, mean in (("log_decay", decay), ("beta", beta)):
+        p[name] = mean * (0.5 + torch.rand(p[name].shape, generator=g))
+    return p
+
+
+def exact(p):
+    return oracle.gated_delta_rule(*(p[n] for n in NAMES[:5]), initial=p["initial"])
+
+
+def by_chunks(got, want):
+    """The largest relative error of a chunk of 64 tokens of a head of a sequence."""
+    got, want = got.detach().double().cpu(), want.detach().double()
+    return max(((a - b).norm(dim=(1, 3)) / b.norm(dim=(1, 3))).max().item()
+               for a, b in zip(got.split(64, 1), want.split(64, 1)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("sizes", [(1, 2048, 1, 1, 64, 64), (1, 4001, 1, 2, 128, 40), (2, 1600, 1, 1, 24, 8)])
+def test_a_state_that_nothing_changes_comes_back_bit_for_bit(sizes, dtype):
+    """No forgetting and no correction: every output reads the initial state."""
+    p = slow(*sizes, dtype, 0.0, 0.0)
+    with torch.no_grad():
+        y, final = call(to_dev(p))
+    assert torch.equal(final.cpu(), p["initial"])
+    assert by_chunks(y, exact(p)[0]) <= FWD[dtype]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("length,decay,beta", [(16384, -1e-5, 5e-4), (16384, -1e-6, 5e-5), (32768, -1.2e-6, 0.0),
+                                               (5000, -1e-3, 1e-4), (5000, 0.0, 1e-2)])
+def test_a_state_that_forgets_slowly(length, decay, beta, dtype):
+    p = slow(1, length, 1, 1, 64, 64, dtype, decay, beta)
+    want, last = exact(p)
+    with torch.no_grad():
+        y, final = call(to_dev(p))
+    start = p["initial"].double()
+    left = p["log_decay"].double().sum(1).exp()[..., None, None] * start
+    bound = kept(length) * left.norm().item() + CORRECTED[dtype] * (last - left).norm().item()
+    assert (final.cpu().double() - last).norm().item() <= bound
+    # the state's error reaches an output beside the output's own roundings
+    assert by_chunks(y, want) <= FWD[dtype] + bound / min(last.norm().item(), start.norm().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("length", [24 * 64 - 1, 24 * 64, 24 * 64 + 1, 25 * 64, 1727, 3001])
+def test_chunks_and_gradients_at_the_seams(length, dtype):
+    """States that reach across several segments: outputs and gradients chunk by chunk, the last one's single token
+    among them, and the whole gradient of the initial state."""
+    p = slow(1, length, 1, 2, 64, 48, dtype, -5e-4, 0.02)
+    args = [p[n] for n in NAMES[:5]]
+    want, last = exact(p)
+    outs, grads = gradients(to_dev(p))
+    assert by_chunks(outs["y"], want) <= FWD[dtype]
+    assert (outs["final"].detach().cpu().double() - last).norm().item() <= FWD[dtype] * last.norm().item()
+    exact_grads = dict(zip(NAMES, oracle.gated_delta_rule_bwd(p["dy"], p["dfinal"], *args, initial=p["initial"])))
+    for name in ("q", "k", "v"):
+        assert by_chunks(grads[name], exact_grads[name]) <= BWD[dtype], name
+    for name in ("beta", "initial"):  # a number a token, and one gradient
+        w = exact_grads[name]
+        assert w.norm().item() > 0.1  # it is there
+        assert (grads[name].cpu().double() - w).norm().item() <= BWD[dtype] * w.norm().item(), name
