@@ -700,11 +700,17 @@ int make_geo(const mko_delta_params* prm, const char* what, Geo* g) {
     mko_set_error("%s: the key axis has at most %d elements", what, MKO_DELTA_MAX_KEY);
     return MKO_EUNSUPPORTED;
   }
-  // workgroups of 256 threads, counted in 32 bits; each factor is bounded before the product
-  const int64_t most = int64_t(1) << 24, chunks = cdiv(prm->length, kC), parts = cdiv(prm->value, 16);
-  if (prm->length >= int64_t(1) << 30 || prm->value >= int64_t(1) << 20 || prm->batch >= most || prm->heads >= most ||
+  if (prm->value >= int64_t(1) << 20) {
+    mko_set_error("%s: the value axis is below 2^20", what);
+    return MKO_EUNSUPPORTED;
+  }
+  // a launch counts its threads in 32 bits, and `scan` and `grads` have 512 in a workgroup; each factor is bounded before
+  // the product
+  const int64_t most = int64_t(1) << 23, chunks = cdiv(prm->length, kC), parts = cdiv(prm->value, 16);
+  if (prm->length >= int64_t(1) << 30 || prm->batch >= most || prm->heads >= most ||
       prm->batch * prm->heads >= most || prm->batch * prm->heads * (chunks > parts ? chunks : parts) >= most) {
-    mko_set_error("%s: batch * heads * (chunks of %d tokens, or tiles of 16 values) must be below 2^24", what, kC);
+    mko_set_error("%s: batch * heads * (chunks of %d tokens, or tiles of 16 values) must be below 2^23 (of 512 threads; 2^24 of 256 fill a "
+                  "launch)", what, kC);
     return MKO_EUNSUPPORTED;
   }
   *g = Geo{prm->batch, prm->length, prm->key_heads, prm->heads, prm->key, prm->value,

@@ -249,9 +249,9 @@ def _check(op, q, k, v, log_decay, beta, scale, lead):
     return rules, key ** -0.5 if scale is None else float(scale)
 
 
-def _limit(rules, cells, text):
-    if cells >= 1 << 24:
-        rules.fail(f"{text} should be below 2^24 (got {cells})")
+def _limit(rules, n, bits, text):
+    if n >= 1 << bits:
+        rules.fail(f"{text} should be below 2^{bits} (got {n})")
 
 
 def gated_delta_rule(q, k, v, log_decay, beta, scale=None, initial_state=None, return_final_state=False):
@@ -260,7 +260,8 @@ def gated_delta_rule(q, k, v, log_decay, beta, scale=None, initial_state=None, r
     Args:
         q, k: ``(batch, length, key_heads, key)``, float32, float16 or bfloat16 on the ROCm GPU, ``key``
             up to 256.  Keys are used as they are; normalise them first.
-        v: ``(batch, length, heads, value)`` in their dtype; ``heads`` is a multiple of ``key_heads``.
+        v: ``(batch, length, heads, value)`` in their dtype; ``heads`` is a multiple of ``key_heads``, and
+            ``batch * heads`` times the chunks of 64 tokens, or the tiles of 16 values, is below 2^23.
         log_decay: ``(batch, length, heads)`` logarithm of what the state keeps at a step, at most 0, in
             one of those dtypes.  Below ``-1e4`` it counts as ``-1e4``, which clears the state.
         beta: ``(batch, length, heads)`` strength of the correction, in one of those dtypes.
@@ -279,7 +280,8 @@ def gated_delta_rule(q, k, v, log_decay, beta, scale=None, initial_state=None, r
         rules.shape("initial_state", initial_state, (batch, heads, value, q.shape[3]))
         rules.same_device(q.device, initial_state=initial_state)
         rules.dtype_in(_FLOATS, initial_state=initial_state)
-    _limit(rules, batch * heads * max(-(-length // CHUNK), -(-value // 16)),
+    _limit(rules, value, 20, "the value axis")
+    _limit(rules, batch * heads * max(-(-length // CHUNK), -(-value // 16)), 23,
            "batch * heads * (chunks of 64 tokens, or tiles of 16 values)")
     initial, want_final = nat.dense(initial_state), bool(return_final_state)
     log_decay, beta = nat.dense(log_decay), nat.dense(beta)
@@ -321,7 +323,7 @@ def gated_delta_rule_update(state, q, k, v, log_decay, beta, scale=None, out_sta
             rules.fail("out_state should be contiguous")
         if out_state.requires_grad:
             rules.fail("out_state is overwritten in place, so it may not require grad")
-    _limit(rules, shape[0] * shape[1] * -(-shape[2] // 8), "batch * heads * (groups of 8 values)")
+    _limit(rules, shape[0] * shape[1] * -(-shape[2] // 8), 24, "batch * heads * (groups of 8 values)")
     if nat.wants_grad(state, q, k, v, log_decay, beta):
         if out_state is not None and out_state.untyped_storage()._cdata == state.untyped_storage()._cdata:
             state = state.clone()  # the backward reads the entering state, which its destination overwrites
