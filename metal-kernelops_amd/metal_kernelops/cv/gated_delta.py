@@ -162,7 +162,7 @@ def _(q, k, v, log_decay, beta, initial, scale, want_final, save):
     kept = sum(-(-cells * n // 256) * 256 for n in (_TOKENS, _SQUARES * size, value * key * size, CHUNK * value * size))
     return (v.new_empty(v.shape),
             (v if initial is None else initial).new_empty((batch, heads, value, key) if want_final else 0),
-            v.new_empty(kept if save else 0, dtype=torch.uint8))
+            v.new_empty(kept if save and value else 0, dtype=torch.uint8))  # without values nothing is launched
 
 
 def _delta_bwd_op(dy: Optional[Tensor], dfinal: Optional[Tensor], q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor,

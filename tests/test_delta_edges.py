@@ -46,3 +46,29 @@ def test_calls_refuse_what_the_launches_do_not_take(monkeypatch):
         q, v, gate = (one.expand(s) for s in ((batch, length, 1, 1), (batch, length, heads, value), (batch, length, heads)))
         with pytest.raises(ValueError, match=text):
             gated_delta_rule(q, q, v, gate, gate)
+
+
+# --------------------------------------------------------------------------- CPU: what a trace is told
+
+
+@pytest.mark.parametrize("sizes", [(0, 5, 1, 2, 8, 8), (2, 0, 1, 2, 8, 8), (2, 5, 1, 2, 8, 0), (2, 5, 1, 0, 8, 8)])
+@pytest.mark.parametrize("carried", [False, True])
+def test_fakes_of_empty_calls_have_the_shapes_of_the_ops(sizes, carried):
+    """Calls without outputs launch nothing, so what the ops return can be seen here."""
+    from metal_kernelops.cv import gated_delta
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    b, l, hk, h, k, v = sizes
+
+    def inputs(device):
+        shapes = ((b, l, hk, k), (b, l, hk, k), (b, l, h, v), (b, l, h), (b, l, h), (b, h, v, k))
+        return [torch.zeros(s, device=device) for s in shapes[:5]] + [torch.zeros(shapes[5], device=device) if carried else None]
+
+    args = inputs("cpu")
+    outs = gated_delta._delta_fwd_op(*args, 1.0, True, True)
+    grads = gated_delta._delta_bwd_op(outs[0], outs[1], *args, outs[2], 1.0, carried)
+    with FakeTensorMode():
+        args = inputs(DEV)
+        fakes = torch.ops.mko.delta_fwd(*args, 1.0, True, True)
+        fake_grads = torch.ops.mko.delta_bwd(fakes[0], fakes[1], *args, fakes[2], 1.0, carried)
+    assert [(t.shape, t.dtype) for t in fakes] == [(t.shape, t.dtype) for t in outs]
+    assert [(t.shape, t.dtype) for t in fake_grads] == [(t.shape, t.dtype) for t in grads]
