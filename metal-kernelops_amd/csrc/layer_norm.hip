@@ -326,10 +326,12 @@ __global__ void __launch_bounds__(THREADS) backward(mko_layernorm_params p, Geo 
   }
 }
 
-// Sums of the workgroups' rows of 2 * features partial sums.
+// Sums of the workgroups' rows of 2 * features partial sums, on a grid of two axes: 2^32 threads, the most that one
+// has, are 2^26 features.
+constexpr int64_t kFinishColumns = 1 << 16;  // workgroups of 32 sums in a row of the grid
 __global__ void __launch_bounds__(kColumnThreads) finish(const float* part, int64_t blocks, int64_t features, float* dweight,
                                                          float* dbias) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
+  const int64_t i = (blockIdx.y * kFinishColumns + blockIdx.x) * 32 + (threadIdx.x & 31);
   const float s = column_sum(part, blocks, 2 * features, i);
   if (threadIdx.x >= 32 || i >= 2 * features) return;
   if (i < features) {
@@ -506,10 +508,11 @@ void launch_bwd(const mko_layernorm_params& p, const BwdPlan& b, hipStream_t s) 
   } else {
     MKO_TIMED("layernorm_bwd", s, backward<T, S, 64, kBwdMostVectors, kBwdThreads><<<grid, threads, b.lds, s>>>(p, b.g, part));
   }
-  if (part)
-    MKO_TIMED("layernorm_bwd_finish", s,
-              finish<<<static_cast<unsigned>(cdiv(2 * p.features, 32)), kColumnThreads, 0, s>>>(part, b.g.blocks, p.features,
-                                                                                                p.dweight, p.dbias));
+  if (part) {
+    const int64_t groups = cdiv(2 * p.features, 32);
+    const dim3 columns(static_cast<unsigned>(std::min(groups, kFinishColumns)), static_cast<unsigned>(cdiv(groups, kFinishColumns)));
+    MKO_TIMED("layernorm_bwd_finish", s, finish<<<columns, kColumnThreads, 0, s>>>(part, b.g.blocks, p.features, p.dweight, p.dbias));
+  }
 }
 
 }  // namespace

@@ -72,3 +72,25 @@ def test_fakes_of_empty_calls_have_the_shapes_of_the_ops(sizes, carried):
         fake_grads = torch.ops.mko.delta_bwd(fakes[0], fakes[1], *args, fakes[2], 1.0, carried)
     assert [(t.shape, t.dtype) for t in fakes] == [(t.shape, t.dtype) for t in outs]
     assert [(t.shape, t.dtype) for t in fake_grads] == [(t.shape, t.dtype) for t in grads]
+
+
+# --------------------------------------------------------------------------- GPU
+
+
+@pytest.mark.gpu
+def test_gradients_of_a_norm_of_67_million_features():
+    """The sums of the parameters' gradients have more columns than one axis of a launch has room for.  One row: dbias is
+    dout, and dweight's error is that of the variance, whose threads add 65537 squares each: at most 65537 * 2^-24 of it,
+    and half of that of its root."""
+    from metal_kernelops.cv import layernorm_residual
+    g = torch.Generator(device=DEV).manual_seed(0)
+    n = (1 << 26) + 100
+    x = torch.randn(1, n, generator=g, device=DEV).half()
+    dout = torch.randn(1, n, generator=g, device=DEV).half()
+    w, b = (torch.ones(n, device=DEV, requires_grad=True) for _ in range(2))
+    dw, db = torch.autograd.grad(layernorm_residual(x, w, b)[0], (w, b), dout)
+    assert torch.equal(db, dout[0].float())
+    wide = x[0].double()
+    wide = (wide - wide.mean()) / wide.std(correction=0)
+    wide *= dout[0].double()
+    assert (dw.double() - wide).norm() <= 65537 * 2.0 ** -25 * wide.norm()
