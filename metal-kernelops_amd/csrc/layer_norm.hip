@@ -228,11 +228,12 @@ __global__ void __launch_bounds__(THREADS) backward(mko_layernorm_params p, Geo 
       float dy[VEC], s[VEC];
       unpack_words<T, VEC>(a.g[k].w, dy);
       unpack_words<S, VEC>(a.s[k].w, s);
+      const int count = static_cast<int>(p.features) - (lt + k * threads) * VEC;  // features from this vector on
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float xh = (s[e] - a.mu) * a.r, gw = dy[e] * w[k][e];
         c1 += gw;
-        c2 += gw * xh;
+        c2 += e < count ? gw * xh : 0.0f;  // beyond the row gw is zero, but -mu r may be infinite
         dw[k][e] += dy[e] * xh;
         db[k][e] += dy[e];
       }

@@ -94,3 +94,21 @@ def test_gradients_of_a_norm_of_67_million_features():
     wide = (wide - wide.mean()) / wide.std(correction=0)
     wide *= dout[0].double()
     assert (dw.double() - wide).norm() <= 65537 * 2.0 ** -25 * wide.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("features", [96, 100, 1000])
+def test_a_norm_of_large_equal_features_has_finite_gradients(features, dtype):
+    """mu / sqrt(eps) passes float32's largest number, and so does the zero of a lane without features normalised.  The
+    sums are exact: the row's differences from its mean are zero, and dx is (gw - mean(gw)) / sqrt(eps)."""
+    from metal_kernelops.cv import layernorm_residual
+    g = torch.Generator().manual_seed(features)
+    x = torch.full((3, features), 2.0 ** (120 if features < 128 else 117), dtype=dtype, device=DEV, requires_grad=True)
+    w = torch.ones(features, device=DEV, requires_grad=True)
+    dout = torch.randn(3, features, generator=g).to(dtype)
+    eps = 1e-5 if features < 128 else 1e-8
+    dx, dw = torch.autograd.grad(layernorm_residual(x, w, eps=eps)[0], (x, w), dout.to(DEV))
+    want = (dout.double() - dout.double().mean(-1, keepdim=True)) * eps ** -0.5
+    assert (dw == 0).all()
+    assert (dx.cpu().double() - want).norm() <= (1e-6 + torch.finfo(dtype).eps / 2) * want.norm()
