@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from test_gated_delta import DEV, _params
+from test_gated_delta import DEV, _params, gradients, problem, to_dev
 
 
 # --------------------------------------------------------------------------- CPU: the largest calls
@@ -112,3 +112,18 @@ def test_a_norm_of_large_equal_features_has_finite_gradients(features, dtype):
     want = (dout.double() - dout.double().mean(-1, keepdim=True)) * eps ** -0.5
     assert (dw == 0).all()
     assert (dx.cpu().double() - want).norm() <= (1e-6 + torch.finfo(dtype).eps / 2) * want.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cleared", [-float("inf"), -2e4, -1e4, -150.0])
+@pytest.mark.parametrize("heads", [1, 4])
+def test_a_decay_that_clears_the_state_has_a_gradient_of_zero(cleared, dtype, heads):
+    """It is exp(log_decay) times something, and float32 has no number for exp(-104) and below."""
+    p = problem(2, 150, 1, heads, 32, 24, dtype, gates=torch.float32)
+    at = [0, 1, 63, 64, 100, 149]
+    p["log_decay"][:, at] = cleared
+    _, grads = gradients(to_dev(p))
+    assert (grads["log_decay"][:, at] == 0).all()
+    rest = [t for t in range(150) if t not in at]
+    assert (grads["log_decay"][:, rest] != 0).all()
