@@ -305,10 +305,12 @@ def gated_delta_rule_update(state, q, k, v, log_decay, beta, scale=None, out_sta
     and ``v`` ``(batch, heads, value)`` in one of those dtypes, ``log_decay`` and ``beta``
     ``(batch, heads)``, and ``y`` is ``(batch, heads, value)`` in ``v.dtype``.  With ``out_state``
     (contiguous, the state's shape and dtype, not requiring grad) the new state is written there and
-    returned as that tensor, outside the autograd graph; the state may be its own destination.  The step
-    is computed in float32; ``new_state`` and ``y`` are each rounded once.
+    returned as that tensor, outside the autograd graph; the state may be its own destination.
 
-    Where a gradient is wanted the step is a :func:`gated_delta_rule` of length one.
+    Without a gradient the step is computed in float32; ``new_state`` and ``y`` are each rounded once.  Where
+    one is wanted it is a :func:`gated_delta_rule` of length one, whose operands (the state that it reads, the
+    error, the correction) are rounded to the activations' type: 16-bit calls differ by those roundings, float32 ones
+    by the order of their sums.
     """
     rules, scale = _check("gated_delta_rule_update", q, k, v, log_decay, beta, scale, "batch")
     shape = (*v.shape, q.shape[2])

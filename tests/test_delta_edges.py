@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from test_gated_delta import DEV, _params, gradients, problem, to_dev
+from test_gated_delta import DEV, NAMES, U, _params, gradients, problem, rel, to_dev
 
 
 # --------------------------------------------------------------------------- CPU: the largest calls
@@ -127,3 +127,20 @@ def test_a_decay_that_clears_the_state_has_a_gradient_of_zero(cleared, dtype, he
     assert (grads["log_decay"][:, at] == 0).all()
     rest = [t for t in range(150) if t not in at]
     assert (grads["log_decay"][:, rest] != 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_an_update_with_a_gradient_is_a_rule_of_length_one(dtype):
+    """Its values are the rule's, to the bit, and beside the update's without a gradient off by the rule's eight roundings
+    to the activations' type, which the update does not make, and by the stored output's of both: 10 u."""
+    from metal_kernelops.cv import gated_delta_rule, gated_delta_rule_update
+    d = to_dev(problem(2, 1, 2, 4, 64, 48, dtype, state=torch.float32))
+    args = [d[n] for n in NAMES[:5]]
+    one = [t[:, 0] for t in args]
+    plain = gated_delta_rule_update(d["initial"], *one)
+    recorded = gated_delta_rule_update(d["initial"].clone().requires_grad_(True), *one)
+    y, final = gated_delta_rule(*args, initial_state=d["initial"], return_final_state=True)
+    assert torch.equal(recorded[0], y[:, 0]) and torch.equal(recorded[1], final)
+    for a, b in zip(recorded, plain):
+        assert rel(a, b) <= (1e-5 if dtype == torch.float32 else 10 * U[dtype])
