@@ -96,3 +96,45 @@ def test_chunks_and_gradients_at_the_seams(length, dtype):
         w = exact_grads[name]
         assert w.norm().item() > 0.1  # it is there
         assert (grads[name].cpu().double() - w).norm().item() <= BWD[dtype] * w.norm().item(), name
+
+
+def check_chunks(p, fwd, bwd):
+    """Outputs and the gradients of q, k and v chunk by chunk, the others whole."""
+    args = [p[n] for n in NAMES[:5]]
+    want, last = exact(p)
+    outs, grads = gradients(to_dev(p))
+    assert by_chunks(outs["y"], want) <= fwd
+    assert (outs["final"].detach().cpu().double() - last).norm().item() <= (fwd + U[p["dfinal"].dtype]) * last.norm().item()
+    exact_grads = dict(zip(NAMES, oracle.gated_delta_rule_bwd(p["dy"], p["dfinal"], *args, initial=p["initial"])))
+    for name in ("q", "k", "v"):
+        assert by_chunks(grads[name], exact_grads[name]) <= bwd, name
+    for name in ("beta", "initial"):
+        w = exact_grads[name]
+        assert (grads[name].cpu().double() - w).norm().item() <= bwd * w.norm().item(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("sizes", [(2, 1, 1, 2, 64, 48), (2, 129, 1, 2, 64, 48), (1, 200, 2, 2, 128, 128), (1, 131, 1, 2, 256, 64),
+                                   (1, 131, 1, 2, 33, 31), (2, 150, 1, 4, 128, 64), (3, 64 * 43 + 1, 2, 4, 32, 40)])
+def test_every_chunk_is_as_near_as_its_roundings(sizes, dtype):
+    """Sequences that are not cut: one token, whole and ragged chunks, wide and odd rows, shared key heads."""
+    check_chunks(problem(*sizes, dtype), FWD[dtype], BWD[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_equal_keys_in_every_type(dtype):
+    """One key throughout and no forgetting: a state is a telescoping sum of the chunk's 64 corrections, whose
+    roundings are independent and add to sqrt(64) times one of them."""
+    p = problem(1, 150, 1, 2, 32, 32, dtype)
+    p["k"] = p["k"][:, :1].expand_as(p["k"]).contiguous()
+    p["log_decay"] = torch.zeros_like(p["log_decay"])
+    p["beta"][:, ::3], p["beta"][:, 1::3] = 0.0, 1.0
+    times = 1 if dtype == F32 else 8
+    y, _ = exact(p)
+    outs, grads = gradients(to_dev(p))
+    assert (outs["y"].detach().cpu().double() - y).norm().item() <= times * FWD[dtype] * y.norm().item()
+    want = oracle.gated_delta_rule_bwd(p["dy"], p["dfinal"], *(p[n] for n in NAMES[:5]), initial=p["initial"])
+    for name, w in zip(NAMES, want):
+        assert (grads[name].cpu().double() - w).norm().item() <= times * BWD[dtype] * w.norm().item(), name
