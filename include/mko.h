@@ -581,14 +581,15 @@ int mko_int8_linear(const mko_int8_linear_params* p, void* stream);
  * beta (batch, length, heads) of their own dtypes; states (batch, heads, value, key) of
  * `state_dtype`.  These and all outputs and gradients are contiguous; a gradient has its
  * input's dtype.  The recurrence runs over chunks of MKO_DELTA_CHUNK tokens in float32, its
- * operands rounded to `dtype`; a value that is not finite reaches its whole chunk. */
+ * operands rounded to `dtype`; a value that is not finite reaches its whole chunk.
+ * batch * heads * (chunks, or tiles of 16 values) is below 2^23 and value below 2^20. */
 typedef struct mko_delta_params {
   const void* q;
   const void* k;
   const void* v;
   const void* log_decay;
   const void* beta;
-  const void* initial;     /* or NULL */
+  const void* initial;     /* or NULL, the same in forward and backward */
   void* y;                 /* forward */
   void* final_state;       /* forward, or NULL */
   void* saved;             /* mko_delta_saved_size() bytes at a multiple of 16, which the forward

@@ -500,8 +500,10 @@ grads(Geo g, Ptrs p) {
       const float u = __shfl_down(d, o);
       if (lane + o < kC) d += u;
     }
-    // d is exp(log decay) times something: of a decay that clears the state only the roundings of what cancels are left
-    if (fast_exp2(static_cast<float>(tok.c[lane] - (lane ? tok.c[lane - 1] : 0.0))) == 0.0f) d = 0.0f;
+    // d is exp(log decay) <G, S>: of a decay that clears the state, and of one that meets none, only the roundings of
+    // what cancels are left
+    const bool none = !p.initial && t0 + lane == 0;
+    if (none || fast_exp2(static_cast<float>(tok.c[lane] - (lane ? tok.c[lane - 1] : 0.0))) == 0.0f) d = 0.0f;
     if (lane < rows) store_one(p.ddecay, g.decay_dtype, (b * g.length + t0 + lane) * g.heads + h, d);
   }
   if constexpr (GROUP) __syncthreads();  // before the next head's tokens

@@ -144,3 +144,16 @@ def test_an_update_with_a_gradient_is_a_rule_of_length_one(dtype):
     assert torch.equal(recorded[0], y[:, 0]) and torch.equal(recorded[1], final)
     for a, b in zip(recorded, plain):
         assert rel(a, b) <= (1e-5 if dtype == torch.float32 else 10 * U[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("length", [1, 2, 65])
+@pytest.mark.parametrize("heads", [1, 3])
+def test_a_decay_that_meets_no_state_has_a_gradient_of_zero(length, heads, dtype):
+    """The first token's without an initial state."""
+    for carried in (False, True):
+        p = problem(2, length, 1, heads, 32, 24, dtype, initial=carried)
+        _, grads = gradients(to_dev(p), use=("y",))
+        assert ((grads["log_decay"][:, 0] != 0) == carried).all()
+        assert (grads["log_decay"][:, 1:] != 0).all()
