@@ -70,14 +70,6 @@ struct Frag {
   uint32_t w[kWordsOf<TM, 8>];
 };
 
-template <typename TM>
-__device__ __forceinline__ Frag<TM> frag_zero() {
-  Frag<TM> f;
-#pragma unroll
-  for (int i = 0; i < kWordsOf<TM, 8>; ++i) f.w[i] = 0u;
-  return f;
-}
-
 // acc += a b over the 32 indices.
 template <typename TM>
 __device__ __forceinline__ void mma(f32x4& acc, const Frag<TM>& a, const Frag<TM>& b) {
