@@ -671,15 +671,24 @@ void launch(const Geo& g, const Ptrs& p, bool train, hipStream_t s) {
 
 // ------------------------------------------------------------------ sizes
 
-// Segments that a sequence is cut into (the figures are above): where its workgroups leave more than two thirds of the 256 CUs without
+// Segments that a sequence is cut into: where its workgroups leave more than two thirds of the 256 CUs without
 // work, as many as give each CU one, of 8 chunks or more, and no more than the square root of the chunks, since
-// `join` walks them one by one.  Walking the chunks twice pays from three segments on.
+// `join` walks them one by one.  The chunks are walked twice, in two turns a chunk of a segment for one of the uncut walk,
+// with two launches more.  Where a turn is long that pays from three segments on (kernels but prep, uncut and cut, in
+// us: 24 chunks in three, keys of 256 in bfloat16 76 and 65, of 64 in float32 81 and 69; 64 chunks of 84 workgroups 316
+// and 176, 205 and 160), for float32 keys of up to 32 from four (40 chunks in five 96 and 57, 64 in three 150 and 181).  Where
+// it is short, from 32 turns fewer on (keys of 128 in bfloat16: 50 chunks in six, 32 fewer, 50.3 and 49.3; 64
+// in four, 32 fewer, 67 and 63; 64 in three, 20 fewer, 66 and 72; 24 in three 29 and 38; keys of 64: 36 and 35, 54 and 49,
+// 47 and 55, 21 and 30).
 int64_t segments_of(const mko_delta_params* prm, int64_t chunks) {
   const int64_t groups = prm->batch * prm->heads * cdiv(prm->value, 32);
   if (prm->key % 8 || prm->value % 8 || groups < 1 || 3 * groups > 256) return 1;
   int64_t n = std::min<int64_t>(256 / groups, chunks / 8);
   while (n > 1 && n * n > chunks) --n;
-  return n < 3 ? 1 : cdiv(chunks, cdiv(chunks, n));
+  if (n < (prm->dtype == MKO_F32 && prm->key <= 32 ? 4 : 3)) return 1;
+  const int64_t span = cdiv(chunks, n);
+  if (prm->dtype != MKO_F32 && prm->key <= 128 && chunks - 2 * span < 32) return 1;
+  return cdiv(chunks, span);
 }
 
 int make_geo(const mko_delta_params* prm, const char* what, Geo* g) {

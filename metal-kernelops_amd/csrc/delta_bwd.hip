@@ -540,8 +540,10 @@ __global__ void __launch_bounds__(256) join(Geo g, Ptrs p, int64_t groups, int p
   store_part<TM, 4>(to + row * key, at, key, s);
 }
 
-// Whether they are: with a workgroup or more for each of the 256 CUs (bf16, 2048 of them, four heads each: 344 us, and
-// 519 with partial sums in memory).  Fewer leave CUs idle (float32, 128 of two heads: 52 us, and 35).
+// Whether they are: with a workgroup or more for each of the 256 CUs.  In us, summed in registers and with partial
+// sums in memory: 256 workgroups of two heads in bfloat16 28 and 36 (keys of 128) and 22 and 26 (of 64), in float32
+// 49 and 59, of four heads 46 and 60, 35 and 41, 88 and 103; 2048 186 and 217, 137 and 131, 373 and 418, and 318 and
+// 423, 240 and 238, 699 and 804.  128 leave CUs idle: 25 and 26, 20 and 21, 46 and 35, and 41 and 35, 33 and 26, 83 and 58.
 bool grouped(const Geo& g) {
   return g.rep > 1 && (g.dtype != MKO_F32 || g.key <= 64) && g.batch * g.key_heads * g.chunks >= 256;
 }

@@ -10,6 +10,7 @@ roundings of different operands are independent and add by their squares: the fo
 backward's sixteen to 4 u, and u for storing a gradient.  Float32: 1e-5, and the same a chunk for what is kept.
 """
 
+import ctypes
 import math
 
 import pytest
@@ -48,9 +49,31 @@ def by_chunks(got, want):
                for a, b in zip(got.split(64, 1), want.split(64, 1)))
 
 
+def segments(length, heads, key, value, dtype):
+    """Of one sequence, from the workspace that the library asks for: T and P, the decays, and beside them what the
+    segments but the last one leave."""
+    from metal_kernelops import _native as nat
+    p = nat.DeltaParams(batch=1, length=length, key_heads=1, heads=heads, key=key, value=value, dtype=nat.code(dtype))
+    size, cells = 4 if dtype == F32 else 2, heads * -(-length // 64)
+    more = nat.lib().mko_delta_fwd_workspace_size(ctypes.byref(p)) - cells * (2 * 6 * 512 * size + 64 * 24)
+    each = heads * 4 * (value * key + key * key + 1)
+    return 1 + round(more / each)  # whole, but for the alignment of the arrays
+
+
+@pytest.mark.parametrize("dtype,key,value,chunks,heads,want", [
+    (BF16, 128, 128, 24, 1, 1), (BF16, 64, 64, 40, 2, 1), (BF16, 128, 128, 64, 21, 1), (F16, 32, 32, 80, 84, 1),
+    (BF16, 128, 128, 48, 1, 6), (BF16, 64, 64, 50, 2, 6), (BF16, 128, 128, 64, 16, 4), (BF16, 128, 128, 512, 16, 4),
+    (F16, 64, 64, 512, 1, 22), (BF16, 256, 128, 24, 1, 3), (BF16, 256, 128, 64, 21, 3), (F32, 64, 64, 24, 2, 3),
+    (F32, 64, 64, 64, 42, 3), (F32, 32, 32, 24, 4, 1), (F32, 32, 32, 40, 4, 5), (F32, 32, 32, 160, 84, 1),
+    (BF16, 128, 128, 512, 22, 1), (BF16, 60, 64, 512, 2, 1)])
+def test_sequences_are_cut_where_it_pays(dtype, key, value, chunks, heads, want):
+    """The sizes that the rule was measured at, on both of its sides."""
+    assert segments(chunks * 64, heads, key, value, dtype) == want
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("sizes", [(1, 2048, 1, 1, 64, 64), (1, 4001, 1, 2, 128, 40), (2, 1600, 1, 1, 24, 8)])
+@pytest.mark.parametrize("sizes", [(1, 4096, 1, 1, 64, 64), (1, 4001, 1, 2, 128, 40), (2, 3300, 1, 1, 24, 8), (1, 1600, 1, 1, 256, 16)])
 def test_a_state_that_nothing_changes_comes_back_bit_for_bit(sizes, dtype):
     """No forgetting and no correction: every output reads the initial state."""
     p = slow(*sizes, dtype, 0.0, 0.0)
@@ -79,10 +102,11 @@ def test_a_state_that_forgets_slowly(length, decay, beta, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("length", [24 * 64 - 1, 24 * 64, 24 * 64 + 1, 25 * 64, 1727, 3001])
+@pytest.mark.parametrize("length", [24 * 64 - 1, 24 * 64 + 1, 47 * 64 + 1, 50 * 64, 50 * 64 + 1])
 def test_chunks_and_gradients_at_the_seams(length, dtype):
-    """States that reach across several segments: outputs and gradients chunk by chunk, the last one's single token
-    among them, and the whole gradient of the initial state."""
+    """States that reach across several segments (the shorter sequences are cut in float32, the longer in every type):
+    outputs and gradients chunk by chunk, the last one's single token among them, and the whole gradient of the initial
+    state."""
     p = slow(1, length, 1, 2, 64, 48, dtype, -5e-4, 0.02)
     args = [p[n] for n in NAMES[:5]]
     want, last = exact(p)
@@ -138,3 +162,28 @@ def test_equal_keys_in_every_type(dtype):
     want = oracle.gated_delta_rule_bwd(p["dy"], p["dfinal"], *(p[n] for n in NAMES[:5]), initial=p["initial"])
     for name, w in zip(NAMES, want):
         assert (grads[name].cpu().double() - w).norm().item() <= times * BWD[dtype] * w.norm().item(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_two_captured_cut_sequences_replay(dtype):
+    """Each graph has segments of its own, and a replay with other values those values' results."""
+    ds = [to_dev(slow(1, 3200, 1, 2, 64, 48, dtype, -5e-4, 0.02, seed=i)) for i in range(2)]
+    with torch.no_grad():
+        graphs = []
+        for d in ds:
+            call(d)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                held = call(d)
+            graphs.append((graph, held))
+        for k in range(3):
+            for d in ds:
+                d["v"].copy_(torch.randn(d["v"].shape, generator=torch.Generator().manual_seed(k)))
+            want = [call(d) for d in ds]
+            for graph, _ in graphs:
+                graph.replay()
+            torch.cuda.synchronize()
+            for (_, held), w in zip(graphs, want):
+                assert all(torch.equal(a, b) for a, b in zip(held, w))
