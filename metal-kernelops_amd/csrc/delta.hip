@@ -6,11 +6,11 @@
 //         accumulators and do only what the next chunk waits for, E and S's update; W
 //         others follow a chunk behind with Y, and four fetch the chunk ahead and store what the backward reads.
 //
-// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: prep 65 us, scan 172.  Prep moves 56 KB a chunk and
+// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: prep 65 us, scan 170.  Prep moves 56 KB a chunk and
 // head, 3.4 TB/s, behind the latency of its substitution.  A turn of the scan takes 2.6 us: its chain of products
 // about 1.0 (2400 cycles), fetching 48 KB and storing 16 KB for the backward on every CU at once the rest; without
 // gradients a turn takes 1.6.  With the chain's waves fetching and storing for themselves the scan took 254 us, with
-// the fetches in waves of their own and two buffers 232, with three 163 to 173.
+// the fetches in waves of their own and two buffers 232, with three 163, and 170 with the backward's states stored by them.
 //
 // Few long sequences leave most of the chip idle, so their chunks are cut into segments that are walked side
 // by side.  A segment makes d S0 + S0 N + B of the state S0 before it, d its decay:
@@ -18,8 +18,8 @@
 //         from the unit matrix (d I + N)
 //   join  per (batch, head, 16 value columns): S0 of each segment, in their order.  What a state only keeps, d S0,
 //         is a float32 product, as in the uncut walk
-// and the scan starts each segment from its own S0.  One sequence of 32768 tokens with 16 such heads: 99 + 149 + 10 + 199
-// us in four segments; uncut, prep and scan took 107 + 659.
+// and the scan starts each segment from its own S0.  One sequence of 32768 tokens with 16 such heads: 98 + 154 + 8 + 200
+// us in four segments; uncut, prep and scan take 100 + 649.
 #include <algorithm>
 
 #include "delta.hpp"
@@ -124,7 +124,8 @@ __device__ __forceinline__ void store_half(TM* p, int h, const float (&f)[4]) {
 }
 
 // Wave w owns the row tile w of A and P.  Six waves a SIMD, for whose registers and LDS K and A share a place, hide more of
-// the substitution than four did: 72 -> 67 us (the sizes above), 111 -> 101 without the transposes.
+// the substitution than four did, for three or four registers that spill: 72 -> 67 us (the sizes above), 111 -> 101
+// without the transposes.
 template <typename TM, int KB, bool TRAIN>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KB * sizeof(TM) <= 8 ? 6 : 1))) prep(Geo g, Ptrs p, bool fast) {
   typedef Tile<TM, 32 * KB> KTile;

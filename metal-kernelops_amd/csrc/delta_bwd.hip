@@ -18,7 +18,7 @@
 //          one after the other, with dq and dk summed in registers in their order
 //   join   that sum where there are few such workgroups, or no room for it in LDS
 //
-// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: back 142 us, grads 194.  A turn of `back` is 2.2 us of
+// Four sequences of 4096 tokens with 16 heads of 128 x 128 in bf16: back 143 us, grads 201.  A turn of `back` is 2.2 us of
 // 60 products that follow from one another, with their reads of LDS.  `grads` moves 176 KB a chunk and head, 3.7 TB/s;
 // two workgroups a CU overlap one's loads and the other's products.
 #include "delta.hpp"
@@ -39,7 +39,8 @@ struct BackLds : Chunks<TM, KB, 16 * W, FAST ? (KB * sizeof(TM) <= 8 && sizeof(T
 };
 
 // W waves carry 16 value columns of G each through the chunks, and four fetch the chunk ahead and store G and dV of
-// the chunk before.
+// the chunk before.  In float32 keys of more than 64 spill 20 registers and of more than 128, where nothing is
+// fetched ahead, 170: 763 us for two sequences of 1024 tokens with 8 heads of 256 x 128.
 template <typename TM, int KB, int W, bool FAST>
 __global__ void __launch_bounds__(64 * W + 64 * (FAST ? kFetchers : 0)) back(Geo g, Ptrs p, int parts) {
   constexpr int KP = 32 * KB, BV = 16 * W, kThreads = 64 * W + 64 * (FAST ? kFetchers : 0);
@@ -231,6 +232,8 @@ struct GradsLds<TM, KB, true> : GradsTiles<TM, KB>::Sums {
 template <typename TM, int KB>
 constexpr bool kGroups = sizeof(TM) == 2 || KB <= 2;
 
+// Two workgroups a CU, or one of a GROUP or of wide keys, set the registers.  For two in 16 bits with keys of more than 64
+// 7 or 8 spill, 28 to 30 with rows that are copied; of a GROUP with keys of more than 128 29 to 51.
 template <typename TM, int KB, bool FAST, bool GROUP>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof(TM) == 2 && KB <= 4 && !GROUP ? 4 : 2)))
 grads(Geo g, Ptrs p) {

@@ -424,7 +424,9 @@ template <typename T, typename S, int SUB, int NV>
 void launch_fwd_n(const mko_layernorm_params& p, const Geo& g, hipStream_t s) {
   const int threads = g.team > kThreads ? g.team : kThreads / g.team * g.team;
   const unsigned grid = static_cast<unsigned>(cdiv(p.rows, threads / g.team));
-  // up to four waves may take more registers than sixteen: five vectors a lane would spill
+  // Up to four waves may take more registers than sixteen, where four vectors a lane spill 14 to 17 registers, five 78 to 112
+  // and eight 146 to 331.  Rows of more than 8192 features take those when a few hundred of them come: 400 x 10240 bf16
+  // 15 us, 300 x 16384 23, and 25 beside a float32 stream.
   if (threads <= kThreads)
     MKO_TIMED("layernorm_fwd", s, forward<T, S, SUB, NV, kThreads><<<grid, threads, 0, s>>>(p, g));
   else
@@ -464,7 +466,9 @@ struct BwdPlan {
 
 // One vector a lane as far as a team of sixteen waves goes: it leaves registers for more waves, which hide the
 // loads better than more vectors do (8192 x 2560 bf16 42 us, 63 with two a lane and 68 with three; 1003 x 5120 beside
-// a float32 stream 26, 28 and 56).  Wider rows take three in teams of up to eight.
+// a float32 stream 26, 28 and 56).  Wider rows take three in teams of up to eight, and
+// spill 28 registers, beside a float32 stream 63 (float16) or 127: 8192 x 10240 bf16 187 us, 1003 x 12288 beside a float32
+// stream 83.
 BwdPlan bwd_plan(const mko_layernorm_params* p) {
   BwdPlan b{};
   const int64_t vectors = vectors_of(p), waves = cdiv(vectors, kWave);
